@@ -51,6 +51,11 @@ SIGNATURES = {
                       _p, _i32, _f32, _p, _i32, _f32, _i32, _i32, _p, _p, _i64, _p],
     "dfs_adaln_modulate": [_p, _i64, _i64, _i32, _p, _p, _p, _p, _f32, _p, _p],
     "dfs_gated_residual": [_p, _p, _p, _i64, _i64, _i32, _p, _p],
+    "dfs_linear_workspace_size": [_i64, _i64, _i64],
+    "dfs_linear": [_p, _i64, _p, _i64, _i64, _i64, _i64, _i32, _p, _i32, _i32, _p, _p, _i64, _p, _i64, _p, _i64, _p],
+    "dfs_window_attention_workspace_size": [_p],
+    "dfs_window_attention": [_p, _p],
+    "dfs_qkv_cache": [_p, _p],
 }
 
 class CallArgs(ctypes.Structure):
@@ -66,10 +71,36 @@ class CallArgs(ctypes.Structure):
             "workspace")]
 
 
+class WindowArgs(ctypes.Structure):
+    """dfs_window_args, field by field."""
+
+    _fields_ = [(n, _i64) for n in (
+        "batch", "q_heads", "kv_heads", "q_rows", "slots", "head_dim", "dtype", "left", "right", "sinks", "rolling",
+        "q_batch_stride", "q_head_stride", "q_row_stride", "k_batch_stride", "k_head_stride", "k_row_stride",
+        "v_batch_stride", "v_head_stride", "v_row_stride", "out_batch_stride", "out_head_stride", "out_row_stride",
+        "workspace_bytes")] + [("scale", ctypes.c_double)] + [(n, _p) for n in (
+            "q", "k", "v", "out", "lse", "q_lens", "kv_lens", "workspace")]
+
+
+class CacheArgs(ctypes.Structure):
+    """dfs_cache_args, field by field."""
+
+    _fields_ = [(n, _i64) for n in (
+        "batch", "tokens", "q_heads", "kv_heads", "head_dim", "slots", "dtype", "sinks", "rolling", "table_rows",
+        "q_weight_dtype", "q_norm_all", "k_weight_dtype", "k_norm_all",
+        "q_batch_stride", "q_token_stride", "q_head_stride", "k_batch_stride", "k_token_stride", "k_head_stride",
+        "v_batch_stride", "v_token_stride", "v_head_stride", "q_out_batch_stride", "q_out_token_stride",
+        "q_out_head_stride", "k_cache_batch_stride", "k_cache_slot_stride", "k_cache_head_stride",
+        "v_cache_batch_stride", "v_cache_slot_stride", "v_cache_head_stride")] + [("eps", ctypes.c_double)] + [
+        (n, _p) for n in ("q", "k", "v", "q_out", "k_cache", "v_cache", "q_weight", "k_weight", "cos_table",
+                          "sin_table", "lens", "new_lens")]
+
+
 _RESTYPES = {"dfs_last_error": ctypes.c_char_p, "dfs_block_score_topk_workspace_size": ctypes.c_int64,
              "dfs_block_score_topk_split_size": ctypes.c_int64, "dfs_bsa_fwd_workspace_size": ctypes.c_int64,
-             "dfs_call_workspace_size": ctypes.c_int64}
-ABI_VERSION = 5
+             "dfs_call_workspace_size": ctypes.c_int64, "dfs_linear_workspace_size": ctypes.c_int64,
+             "dfs_window_attention_workspace_size": ctypes.c_int64}
+ABI_VERSION = 6
 
 _lock = threading.Lock()
 _lib = None

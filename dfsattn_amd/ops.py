@@ -698,3 +698,318 @@ def gated_residual(x: torch.Tensor, y: torch.Tensor, gate: torch.Tensor,
     _lib.call("dfs_gated_residual", _ptr(xc), _ptr(yc), _ptr(g), xc.numel() // C, C, DTYPE_CODE[x.dtype],
               _ptr(out), _stream(xc))
     return out
+
+
+# --------------------------------------------------------------------------
+# Products with their epilogue, windowed attention and its cache
+# --------------------------------------------------------------------------
+
+ACTIVATION_CODE = {None: 0, "gelu_tanh": 1, "gelu": 2, "silu": 3}
+HALF = (torch.bfloat16, torch.float16)
+
+
+def _refuse_grad(entry: str, *tensors: Optional[torch.Tensor]) -> None:
+    """These operators have no backward pass: a graph would lose it silently."""
+    if torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in tensors):
+        raise RuntimeError(f"{entry} has no backward pass: call it under torch.no_grad() or inference_mode()")
+
+
+def _call_on(t: torch.Tensor, entry: str, *args) -> None:
+    """An entry point on t's device and that device's current stream (the
+    last argument), whichever device the caller has current."""
+    if t.device.index == torch.cuda.current_device():
+        _lib.call(entry, *args, _stream(t))
+    else:
+        with torch.cuda.device(t.device):
+            _lib.call(entry, *args, _stream(t))
+
+
+def _span(t: torch.Tensor) -> Tuple[int, int]:
+    """First byte and the byte behind the last one that t's elements touch."""
+    last = sum((n - 1) * s for n, s in zip(t.shape, t.stride()))
+    return t.data_ptr(), t.data_ptr() + (last + 1) * t.element_size()
+
+
+def _refuse_overlap(entry: str, name: str, out: torch.Tensor, *tensors: Optional[torch.Tensor]) -> None:
+    if out.numel() == 0:
+        return
+    lo, hi = _span(out)
+    for t in tensors:
+        if t is not None and t.numel():
+            a, b = _span(t)
+            if a < hi and lo < b:
+                raise ValueError(f"{entry}: {name} overlaps an input")
+
+
+def _axis_strides(t: torch.Tensor) -> Tuple[int, ...]:
+    """Strides with 0 for axes of one, which have none."""
+    return tuple(s if n > 1 else 0 for n, s in zip(t.shape, t.stride()))
+
+
+def _chunk_rows(t: torch.Tensor) -> bool:
+    """Whether rows of the last axis lie on 16-byte boundaries (16-bit elements)."""
+    strides = _axis_strides(t)
+    return strides[-1] in (0, 1) and t.data_ptr() % 16 == 0 and all(s % 8 == 0 for s in strides[:-1])
+
+
+def _own_rows(t: torch.Tensor) -> bool:
+    """Rows to write to: on 16-byte boundaries, none of them shared."""
+    return _chunk_rows(t) and not any(n > 1 and s == 0 for n, s in zip(t.shape, t.stride()))
+
+
+def _matrix(t: torch.Tensor) -> Tuple[torch.Tensor, int]:
+    """(t as [rows, channels] with channel stride 1, row stride); a copy where
+    t's axes do not join."""
+    m = t.reshape(-1, t.shape[-1])
+    if m.stride(1) != 1 and m.shape[1] > 1:
+        m = m.contiguous()
+    return m, (m.stride(0) if m.shape[0] > 1 else m.shape[1])
+
+
+@functools.lru_cache(maxsize=1024)
+def _linear_workspace(rows: int, n: int, k: int) -> int:
+    return int(_lib.lib().dfs_linear_workspace_size(rows, n, k))
+
+
+def linear(x: torch.Tensor, weight: torch.Tensor, bias: Optional[torch.Tensor] = None,
+           activation: Optional[str] = None, gate: Optional[torch.Tensor] = None,
+           residual: Optional[torch.Tensor] = None, out: Optional[torch.Tensor] = None) -> torch.Tensor:
+    """residual + gate * act(x @ weight.T + bias) in one call: x [..., K],
+    weight [N, K] (as nn.Linear holds it), bias [N] in their dtype or fp32,
+    gate N fp32 values, residual [..., N]; activation None, "gelu_tanh",
+    "gelu" (erf form) or "silu". Sums and the epilogue are fp32, rounded once
+    to x's dtype (bf16 or f16). ``out`` may be the residual itself. No
+    backward pass."""
+    _refuse_grad("linear", x, weight, bias, gate, residual)
+    if x.dtype not in HALF or weight.dtype != x.dtype:
+        raise ValueError(f"linear: x and weight must both be bf16 or f16, got {x.dtype} and {weight.dtype}")
+    if x.dim() < 1 or weight.dim() != 2 or weight.shape[1] != x.shape[-1]:
+        raise ValueError(f"linear: weight must be [N, K] for x [..., K], got {tuple(weight.shape)} and {tuple(x.shape)}")
+    n, k = weight.shape
+    if n == 0 or k == 0:
+        raise ValueError(f"linear: weight {tuple(weight.shape)} has no elements")
+    if activation not in ACTIVATION_CODE:
+        raise ValueError(f"linear: activation must be one of {list(ACTIVATION_CODE)}, got {activation!r}")
+    b_code = 0
+    if bias is not None:
+        if bias.dim() != 1 or bias.numel() != n or bias.dtype not in (x.dtype, torch.float32):
+            raise ValueError(f"linear: bias must hold {n} values of x's dtype or float32, got {bias.dtype} "
+                             f"{tuple(bias.shape)}")
+        bias, b_code = bias.contiguous(), DTYPE_CODE[bias.dtype]
+    gate = _vec(gate, n, "linear: gate")
+    shape = (*x.shape[:-1], n)
+    for name, t in (("residual", residual), ("out", out)):
+        if t is not None and (tuple(t.shape) != shape or t.dtype != x.dtype):
+            raise ValueError(f"linear: {name} must be {x.dtype} {shape}, got {t.dtype} {tuple(t.shape)}")
+    _require_device(x, weight, bias, gate, residual, out)
+    if out is None:
+        out = torch.empty(shape, dtype=x.dtype, device=x.device)
+    elif not out.is_contiguous():
+        raise ValueError("linear: out must be contiguous")
+    else:
+        same = residual is not None and residual.data_ptr() == out.data_ptr() and residual.is_contiguous()
+        _refuse_overlap("linear", "out", out, x, weight, bias, gate, None if same else residual)
+    if out.numel() == 0:
+        return out
+    x2, ldx = _matrix(x)
+    w2, ldw = _matrix(weight)
+    r2, ldr = _matrix(residual) if residual is not None else (None, 0)
+    rows = x2.shape[0]
+    ws_bytes = _linear_workspace(rows, n, k)
+    ws = torch.empty(ws_bytes, dtype=torch.uint8, device=x.device) if ws_bytes else None
+    _call_on(x, "dfs_linear", _ptr(x2), ldx, _ptr(w2), ldw, rows, n, k, DTYPE_CODE[x.dtype], _ptr(bias), b_code,
+             ACTIVATION_CODE[activation], _ptr(gate), _ptr(r2), ldr, _ptr(out), n, _ptr(ws), ws_bytes)
+    return out
+
+
+def _check_lens(entry: str, name: str, t: Optional[torch.Tensor], batch: int) -> None:
+    if t is not None and (t.dtype != torch.int32 or tuple(t.shape) != (batch,) or not t.is_contiguous()):
+        raise ValueError(f"{entry}: {name} must be a contiguous int32 [{batch}] vector, got {t.dtype} "
+                         f"{tuple(t.shape)}")
+
+
+def _limit(entry: str, name: str, n: Optional[int]) -> int:
+    if n is None:
+        return -1
+    if int(n) < 0:
+        raise ValueError(f"{entry}: {name} must be None (no limit) or not negative, got {n}")
+    return int(n)
+
+
+def window_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, left: Optional[int] = None,
+                     right: Optional[int] = None, sinks: int = 0, q_lens: Optional[torch.Tensor] = None,
+                     kv_lens: Optional[torch.Tensor] = None, rolling: bool = False, scale: Optional[float] = None,
+                     out: Optional[torch.Tensor] = None, want_lse: bool = False):
+    """Attention of q [B, H, L, D] over k and v [B, G, S, D] (H a multiple of
+    G: query head h reads head h // (H // G)) with a sliding window: a query
+    at position p sees the keys from p - left to p + right (None: no limit)
+    and, up to p + right, the first ``sinks`` ones. A sequence's queries are
+    its last tokens: query i of q_lens[b] (default L) stands at position
+    kv_lens[b] - q_lens[b] + i of kv_lens[b] (default S) keys. right=0 is
+    causal attention; L=1 a token over its cache. The lengths are device int32
+    vectors and are never read back.
+
+    ``rolling``: k and v are caches that keep the sinks and the newest tokens
+    (``qkv_cache``); kv_lens counts every token so far and S must be at least
+    sinks + left + L.
+
+    bf16 or f16, D 64 or 128, fp32 softmax; returns out in q's dtype (and
+    storage order) and with ``want_lse`` the fp32 log-sum-exp [B, H, L]. Rows
+    that see no key (rows from q_lens[b] on among them) are 0, their lse -inf.
+    Keys behind kv_lens may hold anything; values a query does not see inside
+    the sequence must be finite. No backward pass."""
+    entry = "window_attention"
+    _refuse_grad(entry, q, k, v)
+    if q.dtype not in HALF or k.dtype != q.dtype or v.dtype != q.dtype:
+        raise ValueError(f"{entry}: q, k and v must all be bf16 or f16, got {q.dtype}, {k.dtype}, {v.dtype}")
+    if q.dim() != 4 or k.dim() != 4 or v.shape != k.shape or k.shape[0] != q.shape[0] or k.shape[3] != q.shape[3]:
+        raise ValueError(f"{entry}: q must be [B, H, L, D] and k and v [B, G, S, D], got {tuple(q.shape)}, "
+                         f"{tuple(k.shape)}, {tuple(v.shape)}")
+    batch, heads, rows, dim = q.shape
+    groups, slots = k.shape[1], k.shape[2]
+    if dim not in (64, 128):
+        raise ValueError(f"{entry}: head dim {dim} (supported: 64, 128)")
+    if groups == 0 or heads % groups:
+        raise ValueError(f"{entry}: {heads} query heads over {groups} key heads")
+    lo, hi, sinks = _limit(entry, "left", left), _limit(entry, "right", right), int(sinks)
+    if sinks < 0:
+        raise ValueError(f"{entry}: sinks must not be negative, got {sinks}")
+    _check_lens(entry, "q_lens", q_lens, batch)
+    _check_lens(entry, "kv_lens", kv_lens, batch)
+    if rolling and (kv_lens is None or lo < 0 or slots < sinks + lo + rows):
+        raise ValueError(f"{entry}: a rolling cache needs kv_lens, left and at least sinks + left + L slots, got "
+                         f"{slots} for sinks={sinks}, left={left}, L={rows}")
+    scale = 1.0 / math.sqrt(dim) if scale is None else float(scale)
+    if not 0.0 < scale < 1e30:
+        raise ValueError(f"{entry}: scale must be positive and finite, got {scale}")
+    _require_device(q, k, v, q_lens, kv_lens, out)
+    if out is None:
+        out = torch.empty_like(q)  # q's storage order
+        if not _chunk_rows(out):
+            out = torch.empty(q.shape, dtype=q.dtype, device=q.device)
+    else:
+        if out.shape != q.shape or out.dtype != q.dtype or not _own_rows(out):
+            raise ValueError(f"{entry}: out must be {q.dtype} {tuple(q.shape)} with rows of its own on 16-byte "
+                             "boundaries")
+        _refuse_overlap(entry, "out", out, q, k, v)
+    lse = torch.empty((batch, heads, rows), dtype=torch.float32, device=q.device) if want_lse else None
+    if out.numel() == 0 or slots == 0:
+        out.zero_()
+        if want_lse:
+            lse.fill_(-math.inf)
+        return (out, lse) if want_lse else out
+    q, k, v = (t if _chunk_rows(t) else t.clone(memory_format=torch.contiguous_format) for t in (q, k, v))
+    a = _lib.WindowArgs()
+    a.batch, a.q_heads, a.kv_heads, a.q_rows, a.slots, a.head_dim = batch, heads, groups, rows, slots, dim
+    a.dtype, a.left, a.right, a.sinks, a.rolling = DTYPE_CODE[q.dtype], lo, hi, sinks, int(rolling)
+    a.q_batch_stride, a.q_head_stride, a.q_row_stride, _ = _axis_strides(q)
+    a.k_batch_stride, a.k_head_stride, a.k_row_stride, _ = _axis_strides(k)
+    a.v_batch_stride, a.v_head_stride, a.v_row_stride, _ = _axis_strides(v)
+    a.out_batch_stride, a.out_head_stride, a.out_row_stride, _ = _axis_strides(out)
+    a.scale = scale
+    a.q, a.k, a.v, a.out = q.data_ptr(), k.data_ptr(), v.data_ptr(), out.data_ptr()
+    a.lse, a.q_lens, a.kv_lens = _ptr(lse), _ptr(q_lens), _ptr(kv_lens)
+    size = int(_lib.lib().dfs_window_attention_workspace_size(ctypes.byref(a)))
+    ws = torch.empty(size, dtype=torch.uint8, device=q.device) if size > 0 else None
+    a.workspace, a.workspace_bytes = _ptr(ws), max(size, 0)
+    _call_on(q, "dfs_window_attention", ctypes.byref(a))
+    return (out, lse) if want_lse else out
+
+
+def qkv_cache(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tensor,
+              lens: torch.Tensor, q_weight: Optional[torch.Tensor] = None, k_weight: Optional[torch.Tensor] = None,
+              eps: float = 1e-6, table: Optional[Tuple[torch.Tensor, torch.Tensor]] = None,
+              new_lens: Optional[torch.Tensor] = None, sinks: int = 0, rolling: bool = False) -> torch.Tensor:
+    """New tokens' q [B, T, H, D] and k, v [B, T, G, D] on their way into
+    ``window_attention``: the heads of q and k are RMS-normalised (weight [D]:
+    each by itself; weight [H * D] or [G * D]: all together; None: not at all)
+    and rotated by the row of their position in ``table`` (fp32 cos and sin
+    [P, D/2], adjacent channels a pair), in fp32 and rounded once; k and v are
+    appended to the caches [B, G, S, D] in place. Returns the new q as a
+    [B, H, T, D] view of token-major storage.
+
+    Token t of sequence b stands at position lens[b] + t (lens: the device
+    int32 counts before this call, left as they are; the attention's kv_lens is
+    lens + T) and takes that slot, or in a ``rolling`` cache, whose first
+    ``sinks`` tokens stay, the oldest one's. new_lens (device int32 [B]): how
+    many of the T tokens each sequence has; behind them q is 0 and the caches
+    keep what they hold. Nothing is read back: a token past the last slot is
+    dropped, and a position past the table makes its rows NaN. No backward
+    pass."""
+    entry = "qkv_cache"
+    cos, sin = table if table is not None else (None, None)
+    _refuse_grad(entry, q, k, v, q_weight, k_weight)
+    if q.dtype not in HALF or any(t.dtype != q.dtype for t in (k, v, k_cache, v_cache)):
+        raise ValueError(f"{entry}: q, k, v and the caches must share bf16 or f16")
+    if q.dim() != 4 or k.dim() != 4 or v.shape != k.shape or k.shape[:2] != q.shape[:2] or k.shape[3] != q.shape[3]:
+        raise ValueError(f"{entry}: q must be [B, T, H, D] and k and v [B, T, G, D], got {tuple(q.shape)}, "
+                         f"{tuple(k.shape)}, {tuple(v.shape)}")
+    batch, tokens, heads, dim = q.shape
+    groups = k.shape[2]
+    if dim < 16 or dim > 512 or dim & (dim - 1):
+        raise ValueError(f"{entry}: head dim {dim} must be a power of two from 16 to 512")
+    if heads == 0 or groups == 0 or max(heads, groups) * dim > 8192:
+        raise ValueError(f"{entry}: {max(heads, groups)} heads of {dim} channels (supported: up to 8192 channels)")
+    if k_cache.dim() != 4 or v_cache.shape != k_cache.shape or (
+            k_cache.shape[0], k_cache.shape[1], k_cache.shape[3]) != (batch, groups, dim):
+        raise ValueError(f"{entry}: caches must be [{batch}, {groups}, S, {dim}], got {tuple(k_cache.shape)} and "
+                         f"{tuple(v_cache.shape)}")
+    slots, sinks = k_cache.shape[2], int(sinks)
+    if sinks < 0:
+        raise ValueError(f"{entry}: sinks must not be negative, got {sinks}")
+    if tokens > slots - (sinks if rolling else 0):
+        raise ValueError(f"{entry}: {tokens} new tokens do not fit a cache of {slots} slots"
+                         + (f" with {sinks} sinks" if rolling else ""))
+    for name, t in (("k_cache", k_cache), ("v_cache", v_cache)):
+        if not _own_rows(t):
+            raise ValueError(f"{entry}: {name} must have rows of its own on 16-byte boundaries")
+    for name, t in (("k_cache", k_cache), ("v_cache", v_cache)):
+        _refuse_overlap(entry, name, t, q, k, v)
+    if k_cache.data_ptr() == v_cache.data_ptr() and k_cache.numel():  # their rows may alternate in one tensor
+        raise ValueError(f"{entry}: k_cache and v_cache are the same memory")
+    if lens is None:
+        raise ValueError(f"{entry}: lens is needed")
+    _check_lens(entry, "lens", lens, batch)
+    _check_lens(entry, "new_lens", new_lens, batch)
+    if not eps >= 0.0:
+        raise ValueError(f"{entry}: eps must not be negative, got {eps}")
+    a = _lib.CacheArgs()
+    refs = []
+    for side, w, count in (("q", q_weight, heads), ("k", k_weight, groups)):
+        if w is None:
+            continue
+        if w.dim() != 1 or w.numel() not in (dim, count * dim) or w.dtype not in DTYPE_CODE:
+            raise ValueError(f"{entry}: {side}_weight must be a [{dim}] or [{count * dim}] vector, got {w.dtype} "
+                             f"{tuple(w.shape)}")
+        if not w.is_contiguous() or w.data_ptr() % 16:
+            w = w.clone(memory_format=torch.contiguous_format)
+        refs.append(w)
+        setattr(a, f"{side}_weight", w.data_ptr())
+        setattr(a, f"{side}_weight_dtype", DTYPE_CODE[w.dtype])
+        setattr(a, f"{side}_norm_all", int(w.numel() != dim))
+    if (cos is None) != (sin is None):
+        raise ValueError(f"{entry}: pass both cos and sin or neither")
+    if cos is not None:
+        for t in (cos, sin):
+            if t.dtype != torch.float32 or t.dim() != 2 or t.shape != cos.shape or t.shape[1] != dim // 2 or (
+                    not t.is_contiguous()) or t.shape[0] == 0:
+                raise ValueError(f"{entry}: tables must be contiguous float32 [P, {dim // 2}], got {t.dtype} "
+                                 f"{tuple(t.shape)}")
+        a.cos_table, a.sin_table, a.table_rows = cos.data_ptr(), sin.data_ptr(), cos.shape[0]
+    _require_device(q, k, v, k_cache, v_cache, lens, q_weight, k_weight, cos, sin, new_lens)
+    out = torch.empty((batch, tokens, heads, dim), dtype=q.dtype, device=q.device)
+    if out.numel() == 0:
+        return out.transpose(1, 2)
+    q, k, v = (t if _chunk_rows(t) else t.clone(memory_format=torch.contiguous_format) for t in (q, k, v))
+    a.batch, a.tokens, a.q_heads, a.kv_heads, a.head_dim, a.slots = batch, tokens, heads, groups, dim, slots
+    a.dtype, a.sinks, a.rolling, a.eps = DTYPE_CODE[q.dtype], sinks, int(rolling), float(eps)
+    a.q_batch_stride, a.q_token_stride, a.q_head_stride, _ = _axis_strides(q)
+    a.k_batch_stride, a.k_token_stride, a.k_head_stride, _ = _axis_strides(k)
+    a.v_batch_stride, a.v_token_stride, a.v_head_stride, _ = _axis_strides(v)
+    a.q_out_batch_stride, a.q_out_token_stride, a.q_out_head_stride, _ = _axis_strides(out)
+    a.k_cache_batch_stride, a.k_cache_head_stride, a.k_cache_slot_stride, _ = _axis_strides(k_cache)
+    a.v_cache_batch_stride, a.v_cache_head_stride, a.v_cache_slot_stride, _ = _axis_strides(v_cache)
+    a.q, a.k, a.v, a.q_out = q.data_ptr(), k.data_ptr(), v.data_ptr(), out.data_ptr()
+    a.k_cache, a.v_cache, a.lens, a.new_lens = k_cache.data_ptr(), v_cache.data_ptr(), lens.data_ptr(), _ptr(new_lens)
+    _call_on(q, "dfs_qkv_cache", ctypes.byref(a))
+    return out.transpose(1, 2)

@@ -42,7 +42,7 @@ const char* dfs_last_error(void);
 /* ABI version; bumped whenever a signature below changes (2: scoring workspace; 3: device cu_seqlens
  * and per-head operand exponents in the attention call, per-head overflow flags and dfs_prepare_fixup;
  * 4: separate query and key tile sizes in preparation and scoring; 5: Q read from the input by
- * the attention kernel, q_perm optional). */
+ * the attention kernel, q_perm optional; 6: dfs_linear, dfs_window_attention and dfs_qkv_cache). */
 int dfs_abi_version(void);
 
 /*
@@ -477,6 +477,91 @@ int dfs_adaln_modulate(const void* x, int64_t rows, int64_t channels,
 int dfs_gated_residual(const void* x, const void* y, const float* gate,
                        int64_t rows, int64_t channels, int dtype, void* out,
                        dfs_stream_t stream);
+
+/*
+ * Matrix product with bias, activation, gate and residual:
+ *   out = residual + gate * act(x W^T + bias)
+ * x [rows][k], w [n][k] (row strides x_stride, w_stride), residual and out
+ * [rows][n], all bf16 or f16; bias [n] (bf16, f16 or f32), gate fp32 [n],
+ * each of bias, gate and residual optional (NULL). Sums and everything behind
+ * them are fp32, rounded once. activation: 0 none, 1 GELU (tanh form), 2 GELU
+ * (erf form), 3 SiLU. Any sizes and strides (operands on 16-byte rows run
+ * faster); out may be the residual itself, but overlap nothing else. The
+ * workspace is the caller's, dfs_linear_workspace_size bytes (0: none).
+ */
+enum { DFS_ACT_NONE = 0, DFS_ACT_GELU_TANH = 1, DFS_ACT_GELU = 2, DFS_ACT_SILU = 3 };
+int64_t dfs_linear_workspace_size(int64_t rows, int64_t n, int64_t k);
+int dfs_linear(const void* x, int64_t x_stride, const void* w, int64_t w_stride,
+               int64_t rows, int64_t n, int64_t k, int dtype, const void* bias,
+               int bias_dtype, int activation, const float* gate,
+               const void* residual, int64_t r_stride, void* out,
+               int64_t o_stride, void* workspace, int64_t workspace_bytes,
+               dfs_stream_t stream);
+
+/*
+ * Attention with a sliding window and sinks. q [B][q_heads][q_rows][D], k and
+ * v [B][kv_heads][slots][D] (q head h reads kv head h / (q_heads / kv_heads)),
+ * out like q, with any strides that are multiples of 8 elements; D 64 or 128,
+ * bf16 or f16. A sequence of nq = q_lens[b] queries (q_rows without q_lens) and
+ * nk = kv_lens[b] keys (slots without kv_lens; device int32, clamped to the
+ * tensors): query i stands at position p = nk - nq + i and sees key j where
+ * j < nk, j <= p + right and (j >= p - left or j < sinks); left and right -1:
+ * no limit. Rows that see no key, rows from nq on among them, are 0 and their
+ * lse (fp32 [B][q_heads][q_rows], optional) is -inf.
+ * rolling: key j lies in slot j < sinks ? j : sinks + (j - sinks) mod
+ * (slots - sinks); kv_lens counts all keys ever written and slots - sinks must
+ * be at least left + q_rows. The workspace is the caller's,
+ * dfs_window_attention_workspace_size bytes (0: none).
+ */
+typedef struct dfs_window_args {
+  int64_t batch, q_heads, kv_heads, q_rows, slots, head_dim, dtype;
+  int64_t left, right, sinks, rolling;
+  int64_t q_batch_stride, q_head_stride, q_row_stride;
+  int64_t k_batch_stride, k_head_stride, k_row_stride;
+  int64_t v_batch_stride, v_head_stride, v_row_stride;
+  int64_t out_batch_stride, out_head_stride, out_row_stride;
+  int64_t workspace_bytes;
+  double scale;
+  const void *q, *k, *v;
+  void* out;
+  float* lse;
+  const int32_t *q_lens, *kv_lens;
+  void* workspace;
+} dfs_window_args;
+int64_t dfs_window_attention_workspace_size(const dfs_window_args* args);
+int dfs_window_attention(const dfs_window_args* args, dfs_stream_t stream);
+
+/*
+ * New tokens on their way into attention over a cache: q [B][tokens][q_heads][D]
+ * and k, v [B][tokens][kv_heads][D] (channel stride 1, other strides multiples
+ * of 8 elements). q and k are RMS-normalised (weight [D]: each head, or with
+ * norm_all weight [heads * D]: all heads together; NULL: no norm) and rotated
+ * by row lens[b] + t of the fp32 tables [table_rows][D/2] (adjacent channels
+ * are a pair; NULL: no rotation), all in fp32 and rounded once. q goes to
+ * q_out, k and v to slot lens[b] + t of the caches, or with rolling to slot
+ * pos < sinks ? pos : sinks + (pos - sinks) mod (slots - sinks). new_lens
+ * (optional): tokens of each sequence; behind them q_out is 0 and the caches
+ * stay as they are. A token past the last slot is not kept, and a position
+ * past the table gives NaN.
+ */
+typedef struct dfs_cache_args {
+  int64_t batch, tokens, q_heads, kv_heads, head_dim, slots, dtype;
+  int64_t sinks, rolling, table_rows;
+  int64_t q_weight_dtype, q_norm_all, k_weight_dtype, k_norm_all;
+  int64_t q_batch_stride, q_token_stride, q_head_stride;
+  int64_t k_batch_stride, k_token_stride, k_head_stride;
+  int64_t v_batch_stride, v_token_stride, v_head_stride;
+  int64_t q_out_batch_stride, q_out_token_stride, q_out_head_stride;
+  int64_t k_cache_batch_stride, k_cache_slot_stride, k_cache_head_stride;
+  int64_t v_cache_batch_stride, v_cache_slot_stride, v_cache_head_stride;
+  double eps;
+  const void *q, *k, *v;
+  void *q_out, *k_cache, *v_cache;
+  const void *q_weight, *k_weight;
+  const float *cos_table, *sin_table;
+  const int32_t *lens, *new_lens;
+} dfs_cache_args;
+int dfs_qkv_cache(const dfs_cache_args* args, dfs_stream_t stream);
 
 #ifdef __cplusplus
 }

@@ -1,0 +1,361 @@
+"""GPU parity of ops.linear, ops.window_attention and ops.qkv_cache against
+their 64-bit definitions (operator_refs), within the bounds that their
+roundings allow."""
+import math
+
+import pytest
+import torch
+
+import operator_refs as refs
+from dfsattn_amd import ops
+
+pytestmark = pytest.mark.gpu
+BF, HF = torch.bfloat16, torch.float16
+
+
+def _randn(gen, *shape, dtype, std=1.0):
+    return (torch.randn(*shape, generator=gen) * std).to(dtype)
+
+
+def _within(got, ref, tol, what=""):
+    got = got.detach().cpu().double()
+    assert got.shape == ref.shape
+    assert bool(torch.isfinite(got).all()), f"{what}: not finite"
+    off = (got - ref).abs() - tol
+    worst = int(off.argmax())
+    assert float(off.max()) <= 0, (f"{what}: at {worst} got {float(got.flatten()[worst])}, want "
+                                   f"{float(ref.flatten()[worst])} within {float(tol.flatten()[worst])}")
+
+
+# --------------------------------------------------------------------------
+# linear
+# --------------------------------------------------------------------------
+
+LINEAR = [
+    # M, N, K, dtype, bias dtype, act, gate, residual
+    (1, 64, 64, BF, BF, None, False, False),
+    (1, 1, 1, BF, None, None, False, True),
+    (1, 2048, 1024, BF, torch.float32, "silu", False, False),
+    (3, 257, 2500, HF, HF, "gelu_tanh", True, True),
+    (2, 200, 8200, BF, BF, None, False, False),
+    (16, 640, 256, BF, BF, "gelu", False, True),
+    (17, 96, 2048, HF, None, None, True, False),
+    (33, 1000, 1032, BF, BF, "gelu_tanh", False, False),
+    (64, 520, 4096, BF, None, None, False, True),
+    (65, 129, 63, BF, BF, "silu", True, True),
+    (100, 128, 65, HF, torch.float32, None, False, False),
+    (127, 255, 511, HF, HF, "gelu", True, True),
+    (128, 128, 128, BF, BF, None, False, False),
+    (200, 384, 640, BF, BF, "gelu_tanh", True, True),
+    (256, 256, 64, BF, None, None, False, False),
+    (257, 513, 72, HF, HF, None, False, True),
+    (300, 1025, 1000, BF, BF, "silu", False, False),
+    (513, 1024, 1024, BF, BF, "gelu_tanh", False, True),
+    (1000, 776, 136, HF, None, None, True, True),
+    (2100, 2056, 192, BF, BF, None, True, True),
+    (2049, 2304, 328, HF, HF, "gelu_tanh", False, False),
+    (4099, 1100, 70, BF, torch.float32, "gelu_tanh", False, True),
+]
+
+
+@pytest.mark.parametrize("m,n,k,dtype,bias,act,gate,residual", LINEAR)
+def test_linear_matches_definition(dev, m, n, k, dtype, bias, act, gate, residual):
+    print(f"linear {m} x {n} x {k} {dtype} bias={bias} act={act} gate={gate} residual={residual}", flush=True)
+    g = torch.Generator().manual_seed(m * 7 + n * 3 + k)
+    x, w = _randn(g, m, k, dtype=dtype), _randn(g, n, k, dtype=dtype, std=2 / math.sqrt(k))
+    b = None if bias is None else _randn(g, n, dtype=bias)
+    gt = torch.randn(n, generator=g) if gate else None
+    r = _randn(g, m, n, dtype=dtype) if residual else None
+    ref, tol = refs.linear(x, w, b, act, gt, r)
+    d = [None if t is None else t.to(dev) for t in (x, w, b, gt, r)]
+    got = ops.linear(d[0], d[1], d[2], activation=act, gate=d[3], residual=d[4])
+    assert got.dtype == dtype
+    _within(got, ref, tol, "linear")
+    again = ops.linear(d[0], d[1], d[2], activation=act, gate=d[3], residual=d[4])
+    assert torch.equal(got, again)
+    if residual:  # in place of the residual
+        d[4] = ops.linear(d[0], d[1], d[2], activation=act, gate=d[3], residual=d[4], out=d[4])
+        assert torch.equal(got, d[4])
+
+
+@pytest.mark.parametrize("m", [1, 5, 40, 130, 700])
+def test_linear_strided_rows_and_batches(dev, m):
+    """x inside wider rows (channels 8 and 3 in), weight inside wider rows, a
+    batch axis, a residual that is a transposed view."""
+    g = torch.Generator().manual_seed(m)
+    k, n = 264, 136
+    wide = _randn(g, 2, m, k + 24, dtype=BF)
+    ww = _randn(g, n, k + 16, dtype=BF, std=0.1)
+    r = _randn(g, n, 2, m, dtype=BF)
+    wide_d, ww_d, r_d = wide.to(dev), ww.to(dev), r.to(dev).permute(1, 2, 0)
+    for off in (8, 3):
+        print(f"linear strided m={m} offset={off}", flush=True)
+        x = wide[:, :, off:off + k]
+        ref, tol = refs.linear(x.reshape(-1, k), ww[:, 8:8 + k], None, None, None,
+                               r.permute(1, 2, 0).reshape(-1, n))
+        got = ops.linear(wide_d[:, :, off:off + k], ww_d[:, 8:8 + k], residual=r_d)
+        assert got.shape == (2, m, n)
+        _within(got.reshape(-1, n), ref, tol, "linear strided")
+
+
+def test_linear_leaves_what_surrounds_out(dev):
+    """Every tile form's stores end at out's last row and column."""
+    for m, n, k, dtype in ((1, 72, 64, BF), (20, 40, 64, BF), (130, 264, 72, HF), (2100, 2056, 64, BF),
+                           (300, 77, 65, BF)):
+        print(f"linear guard {m} x {n} x {k}", flush=True)
+        g = torch.Generator().manual_seed(n)
+        x, w = _randn(g, m, k, dtype=dtype).to(dev), _randn(g, n, k, dtype=dtype).to(dev)
+        room = torch.full((m * n + 1024,), 7.0, dtype=dtype, device=dev)
+        out = room[512:512 + m * n].view(m, n)
+        ops.linear(x, w, out=out)
+        assert bool((room[:512] == 7).all()) and bool((room[512 + m * n:] == 7).all())
+        assert torch.equal(out, ops.linear(x, w))
+
+
+def test_linear_infinities_and_nan_stay_in_their_rows(dev):
+    for m, n, k in ((4, 128, 512), (300, 300, 136), (2048, 2304, 128)):
+        print(f"linear inf {m} x {n} x {k}", flush=True)
+        g = torch.Generator().manual_seed(m)
+        x, w = _randn(g, m, k, dtype=BF), _randn(g, n, k, dtype=BF)
+        x[1, 3], x[2, k - 1] = math.inf, math.nan
+        got = ops.linear(x.to(dev), w.to(dev)).cpu()
+        ref = (x.double() @ w.double().t())
+        keep = [i for i in range(m) if i not in (1, 2)]
+        assert bool(torch.isnan(got[2]).all())
+        assert torch.equal(got[1].double(), ref[1])  # plus or minus infinity by the weight's sign
+        assert bool(torch.isfinite(got[keep]).all())
+
+
+def test_linear_empty_batch(dev):
+    w = torch.zeros(8, 16, dtype=BF, device=dev)
+    assert ops.linear(torch.zeros(0, 16, dtype=BF, device=dev), w).shape == (0, 8)
+
+
+# --------------------------------------------------------------------------
+# window_attention
+# --------------------------------------------------------------------------
+
+ATTENTION = [
+    # B, H, G, L, S, D, dtype, left, right, sinks, q_lens, kv_lens, rolling
+    (1, 2, 2, 1, 1, 128, BF, None, 0, 0, None, None, False),
+    (1, 2, 1, 1, 300, 64, HF, None, 0, 0, None, None, False),
+    (2, 8, 2, 1, 700, 128, BF, 100, 0, 5, None, [700, 33], False),
+    (3, 4, 4, 1, 257, 128, HF, 64, 0, 0, None, [1, 0, 200], False),
+    (2, 20, 4, 1, 130, 64, BF, 97, 0, 4, None, [1000, 57], True),
+    (1, 16, 1, 1, 515, 128, BF, 500, 0, 10, None, [2000], True),
+    (2, 6, 2, 3, 140, 64, HF, 50, 0, 3, None, [140, 2], False),
+    (1, 12, 3, 7, 400, 128, BF, 130, 2, 130, None, None, False),
+    (1, 4, 2, 17, 17, 64, BF, None, 0, 0, None, None, False),
+    (2, 4, 1, 40, 40, 128, HF, 9, 0, 2, [40, 13], [40, 13], False),
+    (1, 2, 2, 129, 129, 128, BF, 20, 20, 30, None, None, False),
+    (1, 3, 1, 200, 200, 64, HF, 70, 0, 4, None, None, False),
+    (1, 2, 1, 130, 77, 128, BF, None, None, 0, None, [50], False),
+    (1, 2, 2, 150, 77, 128, HF, None, 0, 0, None, None, False),  # the first rows stand before the first key
+    (1, 2, 1, 100, 420, 128, BF, 200, None, 60, None, [777], True),
+    (2, 2, 2, 90, 310, 64, HF, 150, 0, 64, [90, 31], [1234, 200], True),
+    (1, 1, 1, 64, 500, 128, BF, 0, 0, 0, None, None, False),
+    (1, 1, 1, 140, 300, 128, BF, 0, 0, 200, None, None, False),
+    (2, 2, 1, 33, 90, 128, BF, 40, 3, 7, [0, 33], [90, 0], False),
+    (1, 5, 5, 260, 260, 64, BF, 128, 128, 128, None, None, False),
+]
+
+
+@pytest.mark.parametrize("B,H,G,L,S,D,dtype,left,right,sinks,q_lens,kv_lens,rolling", ATTENTION)
+def test_window_attention_matches_definition(dev, B, H, G, L, S, D, dtype, left, right, sinks, q_lens, kv_lens,
+                                             rolling):
+    print(f"window B={B} H={H} G={G} L={L} S={S} D={D} {dtype} left={left} right={right} sinks={sinks} "
+          f"q={q_lens} kv={kv_lens} rolling={rolling}", flush=True)
+    g = torch.Generator().manual_seed(L * S + H)
+    q = _randn(g, B, L, H, D, dtype=dtype).transpose(1, 2)
+    k, v = _randn(g, B, G, S, D, dtype=dtype), _randn(g, B, G, S, D, dtype=dtype)
+    ref, lse_ref, tol, lse_tol = refs.window_attention(q, k, v, left, right, sinks, q_lens, kv_lens, rolling)
+    if kv_lens is not None and not rolling:  # keys behind a sequence may hold anything
+        for b, n in enumerate(kv_lens):
+            k[b, :, n:], v[b, :, n:] = math.nan, math.inf
+    lens = [None if t is None else torch.tensor(t, dtype=torch.int32, device=dev) for t in (q_lens, kv_lens)]
+    qd, kd, vd = q.to(dev), k.to(dev), v.to(dev)
+    out, lse = ops.window_attention(qd, kd, vd, left, right, sinks, *lens, rolling=rolling, want_lse=True)
+    assert out.dtype == dtype and out.stride() == qd.stride()
+    _within(out, ref, tol, "window out")
+    lse = lse.cpu().double()
+    empty = lse_ref == -math.inf
+    assert torch.equal(lse == -math.inf, empty)
+    assert bool((out.cpu()[empty] == 0).all())
+    _within(lse.masked_fill(empty, 0), lse_ref.masked_fill(empty, 0), lse_tol, "window lse")
+    for _ in range(2):
+        assert torch.equal(out, ops.window_attention(qd, kd, vd, left, right, sinks, *lens, rolling=rolling))
+
+
+@pytest.mark.parametrize("L,S", [(1, 400), (6, 200), (150, 150)])
+def test_window_attention_strides_scale_and_out(dev, L, S):
+    """Token-major keys of a joint projection, another scale, out between
+    guards, unaligned rows (copied)."""
+    print(f"window strides L={L} S={S}", flush=True)
+    g = torch.Generator().manual_seed(L)
+    H, G, D = 4, 2, 64
+    q = _randn(g, 2, L, H, D, dtype=BF).transpose(1, 2)
+    kv = _randn(g, 2, S, 2, G, D, dtype=BF)
+    k, v = kv[:, :, 0].transpose(1, 2), kv[:, :, 1].transpose(1, 2)
+    ref, _, tol, _ = refs.window_attention(q, k, v, 90, 0, 3, scale=0.3)
+    kvd, qd = kv.to(dev), q.to(dev)
+    room = torch.full((2, H, L + 2, D), 5.0, dtype=BF, device=dev)
+    out = ops.window_attention(qd, kvd[:, :, 0].transpose(1, 2), kvd[:, :, 1].transpose(1, 2), 90, 0, 3, scale=0.3,
+                               out=room[:, :, 1:-1])
+    _within(out, ref, tol, "window strided")
+    assert bool((room[:, :, 0] == 5).all()) and bool((room[:, :, -1] == 5).all())
+    odd = torch.empty(2, H, L, D + 2, dtype=BF, device=dev)[..., :D]
+    odd.copy_(qd)
+    assert torch.equal(out, ops.window_attention(odd, k.to(dev), v.to(dev), 90, 0, 3, scale=0.3))
+
+
+@pytest.mark.parametrize("L", [1, 200])
+def test_window_attention_large_scores_and_infinities(dev, L):
+    """Scores far beyond the exponent's range, a key of minus infinite scores
+    and one of plus infinite values that only some rows see."""
+    print(f"window extremes L={L}", flush=True)
+    g = torch.Generator().manual_seed(3)
+    q, k, v = (_randn(g, 1, 2, n, 128, dtype=BF) for n in (L, 300, 300))
+    q, k = q * 30, k * 30
+    ref, _, tol, _ = refs.window_attention(q, k, v, 100, 0, 4)
+    out = ops.window_attention(q.to(dev), k.to(dev), v.to(dev), 100, 0, 4)
+    _within(out, ref, tol, "large scores")
+
+
+def test_window_attention_empty_sizes(dev):
+    q = torch.ones(1, 2, 3, 64, dtype=BF, device=dev)
+    k = torch.ones(1, 2, 0, 64, dtype=BF, device=dev)
+    out, lse = ops.window_attention(q, k, k, want_lse=True)
+    assert bool((out == 0).all()) and bool((lse == -math.inf).all())
+    assert ops.window_attention(q[:, :, :0], q, q).shape == (1, 2, 0, 64)
+
+
+# --------------------------------------------------------------------------
+# qkv_cache
+# --------------------------------------------------------------------------
+
+CACHE = [
+    # B, T, H, G, D, S, dtype, norm ("head", "all", None), weight dtype, rotation, sinks, rolling, lens, new_lens
+    (1, 1, 2, 2, 128, 4, BF, "head", BF, True, 0, False, [3], None),
+    (3, 1, 8, 2, 64, 40, HF, "head", torch.float32, True, 0, False, [0, 39, 7], None),
+    (2, 5, 6, 3, 128, 16, BF, "all", BF, True, 4, True, [50, 0], None),
+    (2, 9, 4, 1, 64, 30, HF, "all", HF, False, 0, False, [2, 5], [9, 4]),
+    (1, 13, 40, 40, 128, 64, BF, "all", BF, True, 16, True, [40], None),
+    (2, 3, 1, 1, 32, 8, BF, None, None, True, 2, True, [7, 1], [0, 3]),
+    (1, 7, 3, 3, 256, 9, HF, "head", BF, True, 0, False, [2], None),
+    (1, 4, 16, 2, 512, 6, BF, "head", HF, False, 0, False, [1], [3]),
+    (2, 2, 12, 4, 16, 5, BF, None, None, False, 0, False, [3, 2], None),
+]
+
+
+def _cache_inputs(B, T, H, G, D, S, dtype, norm, wdt, rotate, lens):
+    g = torch.Generator().manual_seed(B * T + H * D)
+    x = [_randn(g, B, T, n, D, dtype=dtype, std=3) for n in (H, G, G)]
+    caches = [_randn(g, B, G, S, D, dtype=dtype) for _ in range(2)]
+    w = [None if norm is None else (torch.rand(D if norm == "head" else n * D, generator=g) + 0.5).to(wdt)
+         for n in (H, G)]
+    ang = torch.rand(max(lens) + T, D // 2, generator=g, dtype=torch.float64) * 50
+    table = (torch.cos(ang).float(), torch.sin(ang).float()) if rotate else None
+    return x, caches, w, table
+
+
+@pytest.mark.parametrize("B,T,H,G,D,S,dtype,norm,wdt,rotate,sinks,rolling,lens,new_lens", CACHE)
+def test_qkv_cache_matches_definition(dev, B, T, H, G, D, S, dtype, norm, wdt, rotate, sinks, rolling, lens, new_lens):
+    print(f"qkv_cache B={B} T={T} H={H} G={G} D={D} S={S} {dtype} norm={norm} rolling={rolling}", flush=True)
+    x, caches, w, table = _cache_inputs(B, T, H, G, D, S, dtype, norm, wdt, rotate, lens)
+    ref = refs.qkv_cache(*x, *caches, lens, *w, table=table, new_lens=new_lens, sinks=sinks, rolling=rolling)
+    xd, cd = [t.to(dev) for t in x], [t.to(dev) for t in caches]
+    wd = [None if t is None else t.to(dev) for t in w]
+    td = None if table is None else tuple(t.to(dev) for t in table)
+    ld = torch.tensor(lens, dtype=torch.int32, device=dev)
+    nd = None if new_lens is None else torch.tensor(new_lens, dtype=torch.int32, device=dev)
+    q = ops.qkv_cache(*xd, *cd, ld, *wd, table=td, new_lens=nd, sinks=sinks, rolling=rolling)
+    assert q.shape == (B, H, T, D) and q.dtype == dtype
+    _within(q, ref[0], ref[3], "q")
+    _within(cd[0], ref[1], ref[4], "k_cache")
+    assert torch.equal(cd[1].cpu().double(), ref[2])
+    assert ld.tolist() == lens
+
+
+def test_qkv_cache_views_and_ends(dev):
+    """A joint projection's slices, caches whose rows alternate in one tensor;
+    tokens past the last slot are dropped, positions past the table NaN."""
+    g = torch.Generator().manual_seed(1)
+    B, T, H, G, D, S = 2, 3, 4, 2, 64, 8
+    qkv = _randn(g, B, T, H + 2 * G, D, dtype=BF)
+    kv = torch.full((B, G, S + 1, 2, D), 9.0, dtype=BF)
+    lens = [6, 2]
+    ang = torch.rand(8, D // 2, generator=g, dtype=torch.float64)
+    table = (torch.cos(ang).float(), torch.sin(ang).float())
+    d, kvd = qkv.to(dev), kv.to(dev)
+    q = ops.qkv_cache(d[:, :, :H], d[:, :, H:H + G], d[:, :, H + G:], kvd[:, :, :S, 0], kvd[:, :, :S, 1],
+                      torch.tensor(lens, dtype=torch.int32, device=dev), table=tuple(t.to(dev) for t in table)).cpu()
+    got = kvd.cpu()
+    assert bool(torch.isnan(q[0, :, 2].float()).all())  # position 8 of 8
+    assert bool((got[:, :, S] == 9).all())  # nothing behind the last slot
+    wide = tuple(torch.cat([t, t[:1]]) for t in table)
+    ref = refs.qkv_cache(qkv[:, :, :H], qkv[:, :, H:H + G], qkv[:, :, H + G:], kv[:, :, :S, 0], kv[:, :, :S, 1], lens,
+                         table=wide)
+    _within(q[:, :, :2], ref[0][:, :, :2], ref[3][:, :, :2], "q")
+    _within(got[:, :, :S, 0], ref[1], ref[4], "k_cache")
+    assert torch.equal(got[:, :, :S, 1].double(), ref[2])
+
+
+# --------------------------------------------------------------------------
+# together
+# --------------------------------------------------------------------------
+
+def test_operators_on_another_stream(dev):
+    g = torch.Generator().manual_seed(5)
+    x, w = _randn(g, 300, 256, dtype=BF).to(dev), _randn(g, 512, 256, dtype=BF).to(dev)
+    k = _randn(g, 1, 4, 300, 128, dtype=BF).to(dev)
+    want = ops.linear(x, w)
+    att = ops.window_attention(want.view(1, 300, 4, 128).transpose(1, 2), k, k, left=50, right=0)
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        got = ops.linear(x, w)
+        att2 = ops.window_attention(got.view(1, 300, 4, 128).transpose(1, 2), k, k, left=50, right=0)
+    side.synchronize()
+    assert torch.equal(want, got) and torch.equal(att, att2)
+
+
+def test_operators_in_a_graph(dev):
+    """A layer's token over its cache (products, append, attention) captured
+    once and replayed with other inputs, each replay against the eager run."""
+    g = torch.Generator().manual_seed(6)
+    B, H, G, D, S, C = 3, 8, 2, 64, 600, 512
+    w_qkv = _randn(g, (H + 2 * G) * D, C, dtype=BF, std=0.05).to(dev)
+    w_out = _randn(g, C, H * D, dtype=BF, std=0.05).to(dev)
+    w_up, w_down = (_randn(g, *s, dtype=BF, std=0.05).to(dev) for s in ((1100, C), (C, 1100)))
+    norm = torch.ones(D, dtype=BF, device=dev)
+    ang = torch.rand(900, D // 2, generator=g)
+    table = (torch.cos(ang).to(dev), torch.sin(ang).to(dev))
+    x = torch.zeros(B, 1, C, dtype=BF, device=dev)
+    lens = torch.zeros(B, dtype=torch.int32, device=dev)
+    kc, vc = (torch.zeros(B, G, S, D, dtype=BF, device=dev) for _ in range(2))
+
+    def layer():
+        qkv = ops.linear(x, w_qkv).view(B, 1, H + 2 * G, D)
+        q = ops.qkv_cache(qkv[:, :, :H], qkv[:, :, H:H + G], qkv[:, :, H + G:], kc, vc, lens, norm, norm, table=table,
+                          sinks=4, rolling=True)
+        o = ops.window_attention(q, kc, vc, left=500, right=0, sinks=4, kv_lens=lens + 1, rolling=True)
+        y = ops.linear(o.transpose(1, 2).reshape(B, 1, H * D), w_out, residual=x)
+        return ops.linear(ops.linear(y, w_up, activation="gelu_tanh"), w_down, residual=y)
+
+    layer()
+    torch.cuda.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        out = layer()
+    for i in range(4):
+        xi = _randn(g, B, 1, C, dtype=BF).to(dev)
+        li = torch.tensor([i, 590 + i, 700 + 3 * i], dtype=torch.int32, device=dev)
+        ki, vi = (_randn(g, B, G, S, D, dtype=BF).to(dev) for _ in range(2))
+        x.copy_(xi), lens.copy_(li), kc.copy_(ki), vc.copy_(vi)
+        graph.replay()
+        torch.cuda.synchronize()
+        got, gk, gv = out.clone(), kc.clone(), vc.clone()
+        x.copy_(xi), lens.copy_(li), kc.copy_(ki), vc.copy_(vi)
+        want = layer()
+        assert torch.equal(got, want) and torch.equal(gk, kc) and torch.equal(gv, vc)
+        assert bool(torch.isfinite(got).all())

@@ -1,0 +1,137 @@
+"""What ops.linear, ops.window_attention and ops.qkv_cache refuse, before any
+device is touched, and the rolling cache's slots."""
+import pytest
+import torch
+
+import operator_refs as refs
+from dfsattn_amd import ops
+
+BF = torch.bfloat16
+
+
+def _t(*shape, dtype=BF):
+    return torch.zeros(*shape, dtype=dtype)
+
+
+@pytest.mark.parametrize("change", [
+    {"x": _t(4, 16, dtype=torch.float32)},
+    {"weight": _t(8, 16, dtype=torch.float16)},
+    {"weight": _t(8, 15)},
+    {"weight": _t(8, 2, 8)},
+    {"weight": _t(0, 16)},
+    {"x": _t(4, 0), "weight": _t(8, 0)},
+    {"bias": _t(7)},
+    {"bias": _t(8, dtype=torch.float16)},
+    {"bias": _t(8, 1)},
+    {"activation": "relu"},
+    {"gate": _t(8)},
+    {"gate": _t(4, dtype=torch.float32)},
+    {"residual": _t(4, 7)},
+    {"residual": _t(4, 8, dtype=torch.float32)},
+    {"out": _t(5, 8)},
+    {"out": _t(4, 8, dtype=torch.float16)},
+])
+def test_linear_refuses(change):
+    args = {"x": _t(4, 16), "weight": _t(8, 16), **change}
+    with pytest.raises(ValueError):
+        ops.linear(**args)
+
+
+ATT = dict(q=_t(2, 4, 3, 64), k=_t(2, 2, 9, 64), v=_t(2, 2, 9, 64))
+
+
+@pytest.mark.parametrize("change", [
+    {"q": _t(2, 4, 3, 64, dtype=torch.float32)},
+    {"v": _t(2, 2, 9, 64, dtype=torch.float16)},
+    {"q": _t(4, 3, 64)},
+    {"v": _t(2, 2, 8, 64)},
+    {"k": _t(1, 2, 9, 64), "v": _t(1, 2, 9, 64)},
+    {"k": _t(2, 3, 9, 64), "v": _t(2, 3, 9, 64)},
+    {"q": _t(2, 4, 3, 96), "k": _t(2, 2, 9, 96), "v": _t(2, 2, 9, 96)},
+    {"left": -1},
+    {"right": -2},
+    {"sinks": -1},
+    {"q_lens": torch.zeros(2, dtype=torch.int64)},
+    {"kv_lens": torch.zeros(3, dtype=torch.int32)},
+    {"kv_lens": torch.zeros(4, dtype=torch.int32)[::2]},
+    {"rolling": True, "left": 2},
+    {"rolling": True, "kv_lens": torch.zeros(2, dtype=torch.int32)},
+    {"rolling": True, "left": 5, "sinks": 2, "kv_lens": torch.zeros(2, dtype=torch.int32)},
+    {"scale": 0.0},
+    {"scale": float("nan")},
+])
+def test_window_attention_refuses(change):
+    with pytest.raises(ValueError):
+        ops.window_attention(**{**ATT, **change})
+
+
+CACHE = dict(q=_t(2, 3, 4, 64), k=_t(2, 3, 2, 64), v=_t(2, 3, 2, 64), k_cache=_t(2, 2, 9, 64), v_cache=_t(2, 2, 9, 64),
+             lens=torch.zeros(2, dtype=torch.int32))
+SHARED = _t(2, 2, 9, 64)
+
+
+@pytest.mark.parametrize("change", [
+    {"q": _t(2, 3, 4, 64, dtype=torch.float16)},
+    {"q": _t(2, 4, 64)},
+    {"k": _t(2, 4, 2, 64)},
+    {"v": _t(2, 3, 1, 64)},
+    {"k_cache": _t(2, 2, 9, 128)},
+    {"v_cache": _t(2, 2, 8, 64)},
+    {"k_cache": _t(2, 2, 2, 64), "v_cache": _t(2, 2, 2, 64)},
+    {"sinks": -1},
+    {"sinks": 7, "rolling": True},
+    {"k_cache": SHARED, "v_cache": SHARED},
+    {"k_cache": _t(2, 1, 9, 64).expand(2, 2, 9, 64)},
+    {"k_cache": _t(2, 2, 9, 65)[..., 1:]},
+    {"lens": torch.zeros(3, dtype=torch.int32)},
+    {"lens": None},
+    {"lens": torch.zeros(2)},
+    {"new_lens": torch.zeros(1, dtype=torch.int32)},
+    {"eps": -1.0},
+    {"eps": float("nan")},
+    {"q_weight": _t(128)},
+    {"k_weight": _t(64, 1)},
+    {"table": (torch.zeros(9, 64), torch.zeros(9, 64))},
+    {"table": (torch.zeros(9, 32), torch.zeros(8, 32))},
+    {"table": (torch.zeros(9, 32, dtype=torch.float64), torch.zeros(9, 32, dtype=torch.float64))},
+    {"table": (torch.zeros(9, 32), None)},
+])
+def test_qkv_cache_refuses(change):
+    with pytest.raises(ValueError):
+        ops.qkv_cache(**{**CACHE, **change})
+
+
+def test_head_dims_that_do_not_fit_are_refused():
+    for d in (8, 48, 1024):
+        with pytest.raises(ValueError):
+            ops.qkv_cache(_t(1, 1, 1, d), _t(1, 1, 1, d), _t(1, 1, 1, d), _t(1, 1, 4, d), _t(1, 1, 4, d),
+                          torch.zeros(1, dtype=torch.int32))
+    with pytest.raises(ValueError):  # more channels than a wave holds
+        ops.qkv_cache(_t(1, 1, 65, 128), _t(1, 1, 1, 128), _t(1, 1, 1, 128), _t(1, 1, 4, 128), _t(1, 1, 4, 128),
+                      torch.zeros(1, dtype=torch.int32))
+
+
+def test_operators_refuse_the_cpu_and_gradients():
+    with pytest.raises(RuntimeError, match="ROCm GPU"):
+        ops.linear(_t(4, 16), _t(8, 16))
+    with pytest.raises(RuntimeError, match="ROCm GPU"):
+        ops.window_attention(**ATT)
+    with pytest.raises(RuntimeError, match="ROCm GPU"):
+        ops.qkv_cache(**CACHE)
+    with pytest.raises(RuntimeError, match="no backward"):
+        ops.linear(_t(4, 16), _t(8, 16).requires_grad_())
+    with pytest.raises(RuntimeError, match="no backward"):
+        ops.window_attention(**{**ATT, "v": _t(2, 2, 9, 64).requires_grad_()})
+    with pytest.raises(RuntimeError, match="no backward"):
+        ops.qkv_cache(**{**CACHE, "q_weight": _t(64).requires_grad_()})
+
+
+def test_rolling_slots_hold_the_sinks_and_the_newest_tokens():
+    for slots, sinks in ((7, 2), (9, 0), (5, 4)):
+        held = {}
+        for pos in range(40):
+            held[refs.slot_of(pos, slots, sinks, True)] = pos
+            kept = sorted(held.values())
+            ring = slots - sinks
+            want = [p for p in range(pos + 1) if p < sinks or p > pos - ring]
+            assert kept == want
