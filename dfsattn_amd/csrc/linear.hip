@@ -10,6 +10,8 @@
 // groups cover 4 consecutive n; the A operand's rows are dealt to the tiles so
 // that the groups of a wave's tiles join into 8 or 16 consecutive n and leave
 // as 16-byte stores (TileRows).
+#include <type_traits>
+
 #include "common.h"
 #include "lds_copy.h"
 
@@ -53,20 +55,30 @@ struct Half<true> {
   static __device__ __forceinline__ uint32_t from_f32(float v) { return f32_to_f16_bits(v); }
 };
 
-__device__ __forceinline__ float activate(float z, int act) {
+template <int ACT>
+__device__ __forceinline__ float activate(float z) {
   // sigmoid(t) = 1 / (1 + e^-t); 0.5 (1 + tanh u) = sigmoid(2 u). e^-t may
-  // overflow to infinity: the quotient is 0 then.
+  // overflow to infinity: its reciprocal is 0 then.
+  if constexpr (ACT == kActGeluTanh) {
+    const float u = 1.5957691216057308f * (z + 0.044715f * z * z * z);
+    return z * __builtin_amdgcn_rcpf(1.f + exp2_fast(-1.4426950408889634f * u));
+  } else if constexpr (ACT == kActGelu) {
+    return 0.5f * z * erfcf(-0.70710678118654752f * z);
+  } else if constexpr (ACT == kActSilu) {
+    return z * __builtin_amdgcn_rcpf(1.f + exp2_fast(-1.4426950408889634f * z));
+  } else {
+    return z;
+  }
+}
+
+// f(integral_constant<ACT>) with the call's activation.
+template <typename F>
+__device__ __forceinline__ void with_activation(int act, F&& f) {
   switch (act) {
-    case kActGeluTanh: {
-      const float u = 1.5957691216057308f * (z + 0.044715f * z * z * z);
-      return z / (1.f + exp2_fast(-1.4426950408889634f * u));
-    }
-    case kActGelu:
-      return 0.5f * z * erfcf(-0.70710678118654752f * z);
-    case kActSilu:
-      return z / (1.f + exp2_fast(-1.4426950408889634f * z));
-    default:
-      return z;
+    case kActGeluTanh: return f(std::integral_constant<int, kActGeluTanh>{});
+    case kActGelu: return f(std::integral_constant<int, kActGelu>{});
+    case kActSilu: return f(std::integral_constant<int, kActSilu>{});
+    default: return f(std::integral_constant<int, kActNone>{});
   }
 }
 
@@ -77,9 +89,20 @@ __device__ __forceinline__ float bias_at(const LinearParams& p, int n) {
   return p.bias_dtype == DFS_DTYPE_BF16 ? bf16_bits_to_f32(b) : f16_bits_to_f32(b);
 }
 
+// Bias and gate of eight consecutive outputs n.. (any values past N).
+__device__ __forceinline__ void load_columns8(const LinearParams& p, int n, float* bias, float* gate) {
+#pragma unroll
+  for (int i = 0; i < 8; ++i) {
+    const int c = min(n + i, p.N - 1);
+    bias[i] = bias_at(p, c);
+    gate[i] = p.gate ? p.gate[c] : 1.f;
+  }
+}
+
 // Eight consecutive outputs n.. of row m from their sums.
-template <bool F16>
-__device__ __forceinline__ void finish8(const LinearParams& p, int m, int n, const float* z) {
+template <bool F16, int ACT>
+__device__ __forceinline__ void finish8(const LinearParams& p, int m, int n, const float* z, const float* bias,
+                                        const float* gate) {
   if (m >= p.M || n >= p.N) return;
   const uint16_t* r = p.residual ? p.residual + m * p.ldr + n : nullptr;
   uint16_t* o = p.out + m * p.ldo + n;
@@ -89,8 +112,8 @@ __device__ __forceinline__ void finish8(const LinearParams& p, int m, int n, con
     uint32_t packed[4];
 #pragma unroll
     for (int i = 0; i < 8; ++i) {
-      float y = activate(z[i] + bias_at(p, n + i), p.act);
-      if (p.gate) y *= p.gate[n + i];
+      float y = activate<ACT>(z[i] + bias[i]);
+      if (p.gate) y *= gate[i];
       if (r) y += Half<F16>::to_f32(u16_at(rv, i));
       const uint32_t h = Half<F16>::from_f32(y);
       packed[i / 2] = i & 1 ? packed[i / 2] | h << 16 : h;
@@ -101,8 +124,8 @@ __device__ __forceinline__ void finish8(const LinearParams& p, int m, int n, con
 #pragma unroll
   for (int i = 0; i < 8; ++i) {
     if (n + i >= p.N) break;
-    float y = activate(z[i] + bias_at(p, n + i), p.act);
-    if (p.gate) y *= p.gate[n + i];
+    float y = activate<ACT>(z[i] + bias[i]);
+    if (p.gate) y *= gate[i];
     if (r) y += Half<F16>::to_f32(r[i]);
     o[i] = static_cast<uint16_t>(Half<F16>::from_f32(y));
   }
@@ -163,7 +186,9 @@ __global__ void __launch_bounds__(256) linear_any_kernel(LinearParams p) {
   const int m = m0 + (w >> 1) * 32 + l32;
 #pragma unroll
   for (int g = 0; g < 2; ++g) {
-    float z[8];
+    float z[8], bias[8], gate[8];
+    const int n = n0 + (w & 1) * 32 + g * 16 + hl * 8;
+    load_columns8(p, n, bias, gate);
 #pragma unroll
     for (int i = 0; i < 4; ++i) {
       const auto t = __builtin_amdgcn_permlane32_swap(__float_as_uint(acc[g * 8 + i]),
@@ -171,8 +196,213 @@ __global__ void __launch_bounds__(256) linear_any_kernel(LinearParams p) {
       z[i] = __uint_as_float(t[0]);
       z[4 + i] = __uint_as_float(t[1]);
     }
-    finish8<F16>(p, m, n0 + (w & 1) * 32 + g * 16 + hl * 8, z);
+    with_activation(p.act, [&](auto act) { finish8<F16, decltype(act)::value>(p, m, n, z, bias, gate); });
   }
+}
+
+// Tiles of BN = 32 NI WN outputs by BM = 32 MI WM rows, a workgroup of WN x WM
+// = 4 waves with NI x MI products of 32 x 32 each, 64 channels a step through
+// two LDS buffers that the loads fill directly. For operands on 16-byte rows.
+//
+// A step's 128-byte rows hold eight 16-byte chunks; chunk c of row r lies at
+// c ^ f(r) with f such that any 16 rows that one quarter of a wave reads
+// together fall on all 64 banks. Row i of the A operand of tile ni is output
+// (i >> 2) * 4 NI + ni * 4 + (i & 3), so a lane ends with 4 NI consecutive
+// outputs.
+//
+// Order of a step: the fragments of a quarter (16 channels) are read while the
+// quarter before is multiplied; before the last quarter's products, the next
+// step's data is waited for and, behind the barrier, its successor's loads go
+// into the buffer just read. So there is one barrier a step, the products of a
+// quarter are there on both sides of it, and a load has a whole step to land.
+constexpr uint32_t kOutside = 0x80000000u;  // byte offset past every buffer's records
+
+template <int NI, int MI, int WN, int WM, bool F16>
+struct Tile {
+  static constexpr int BN = 32 * NI * WN, BM = 32 * MI * WM;
+  static constexpr int kShift = NI == 1 ? 2 : NI == 2 ? 3 : 4;
+  typedef typename Half<F16>::vec vec;
+  static __device__ __forceinline__ int swz_w(int n) { return ((n >> 1) & 1) | ((n >> kShift) & 3) << 1; }
+  static __device__ __forceinline__ int swz_x(int m) { return (m >> 1) & 7; }
+};
+
+// Tile of a workgroup: XCD i takes the i-th eighth of the tile list, which
+// walks bands of 8 tile rows, so the 32 tiles an XCD has in flight share 8
+// slices of x and 4 of w in its L2.
+__device__ __forceinline__ void tile_of(int id, int mt, int nt, int& tm, int& tn) {
+  const int total = mt * nt, x = id & 7, i = id >> 3;
+  const int lin = x * (total >> 3) + min(x, total & 7) + i;
+  const int band = lin / (8 * nt), rows = min(8, mt - band * 8), at = lin - band * 8 * nt;
+  tn = at / rows;
+  tm = band * 8 + at - tn * rows;
+}
+
+template <int NI, int MI, int WN, int WM, bool F16>
+__global__ void __launch_bounds__(256, NI * MI == 16 ? 1 : 2) linear_tile_kernel(LinearParams p) {
+  typedef Tile<NI, MI, WN, WM, F16> T;
+  typedef typename T::vec vec;
+  constexpr int JW = T::BN / 32, JX = T::BM / 32;  // loads of 1 KB a wave and step
+  __shared__ __attribute__((aligned(16))) uint16_t w0[T::BN * 64];
+  __shared__ __attribute__((aligned(16))) uint16_t x0[T::BM * 64];
+  __shared__ __attribute__((aligned(16))) uint16_t w1[T::BN * 64];
+  __shared__ __attribute__((aligned(16))) uint16_t x1[T::BM * 64];
+  const int lane = threadIdx.x & 63, w = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  const int l32 = lane & 31, hl = lane >> 5;
+  int tm, tn;
+  tile_of(blockIdx.x, (p.M + T::BM - 1) / T::BM, (p.N + T::BN - 1) / T::BN, tm, tn);
+  const int n0 = tn * T::BN, m0 = tm * T::BM;
+  const auto wrs = make_rsrc(p.w + static_cast<int64_t>(n0) * p.ldw, kOutside);
+  const auto xrs = make_rsrc(p.x + static_cast<int64_t>(m0) * p.ldx, kOutside);
+  // Byte offsets of this lane's chunks in step 0; rows past the matrix repeat
+  // its last one.
+  uint32_t wv[JW], xv[JX];
+  const int r8 = w * 8 + (lane >> 3), c8 = lane & 7;
+#pragma unroll
+  for (int j = 0; j < JW; ++j) {
+    const int r = j * 32 + r8;
+    wv[j] = static_cast<uint32_t>(min(n0 + r, p.N - 1) - n0) * static_cast<uint32_t>(p.ldw * 2) +
+            (c8 ^ T::swz_w(r)) * 16;
+  }
+#pragma unroll
+  for (int j = 0; j < JX; ++j) {
+    const int r = j * 32 + r8;
+    xv[j] = static_cast<uint32_t>(min(m0 + r, p.M - 1) - m0) * static_cast<uint32_t>(p.ldx * 2) +
+            (c8 ^ T::swz_x(r)) * 16;
+  }
+  const int steps = (p.K + 127) >> 7 << 1;  // an even number: the last may be all zeros
+  auto issue = [&](int t, uint16_t* wb, uint16_t* xb) {
+    const int left = p.K - t * 64;
+    if (left < 64) {  // the last steps: chunks past K come as zeros
+#pragma unroll
+      for (int j = 0; j < JX; ++j)
+        if ((c8 ^ T::swz_x(j * 32 + r8)) * 8 >= left) xv[j] = kOutside;
+#pragma unroll
+      for (int j = 0; j < JW; ++j)
+        if ((c8 ^ T::swz_w(j * 32 + r8)) * 8 >= left) wv[j] = kOutside;
+    }
+#pragma unroll
+    for (int j = 0; j < JX; ++j)
+      load_lds16(xrs, xb + (j * 4 + w) * 512, xv[j], t * 128);
+#pragma unroll
+    for (int j = 0; j < JW; ++j)
+      load_lds16(wrs, wb + (j * 4 + w) * 512, wv[j], t * 128);
+  };
+  // Fragment addresses (elements): row part, then the chunk of quarter s.
+  const int wn = w % WN, wm = w / WN;
+  const int arow = (wn * 32 * NI + (l32 >> 2) * 4 * NI + (l32 & 3)) * 64;
+  const int brow = (wm * 32 * MI + l32) * 64;
+  const int fa = T::swz_w((l32 >> 2) * 4 * NI + (l32 & 3)), fb = T::swz_x(l32);
+  f32x16 acc[NI][MI];
+#pragma unroll
+  for (int i = 0; i < NI; ++i)
+#pragma unroll
+    for (int j = 0; j < MI; ++j) acc[i][j] = f32x16{};
+  auto fetch = [&](const uint16_t* wb, const uint16_t* xb, int s, uint4* a, uint4* b) {
+#pragma unroll
+    for (int i = 0; i < NI; ++i)
+      a[i] = *reinterpret_cast<const uint4*>(wb + arow + i * 256 + ((2 * s + hl) ^ fa) * 8);
+#pragma unroll
+    for (int j = 0; j < MI; ++j)
+      b[j] = *reinterpret_cast<const uint4*>(xb + brow + j * 2048 + ((2 * s + hl) ^ fb) * 8);
+  };
+  auto multiply = [&](const uint4* a, const uint4* b) {
+#pragma unroll
+    for (int j = 0; j < MI; ++j)
+#pragma unroll
+      for (int i = 0; i < NI; ++i)
+        acc[i][j] = Half<F16>::mfma(__builtin_bit_cast(vec, a[i]), __builtin_bit_cast(vec, b[j]), acc[i][j]);
+  };
+  constexpr int kMfma = 0x008, kDsRead = 0x100, kVmem = 0x020;
+  constexpr int PER = NI * MI / (NI + MI) > 0 ? NI * MI / (NI + MI) : 1;
+  auto pin = [&](bool loads) {
+#pragma unroll
+    for (int i = 0; i < NI + MI; ++i) {
+      __builtin_amdgcn_sched_group_barrier(kDsRead, 1, 0);
+      if (loads) __builtin_amdgcn_sched_group_barrier(kVmem, (JW + JX) / (NI + MI), 0);
+      __builtin_amdgcn_sched_group_barrier(kMfma, PER, 0);
+    }
+  };
+  uint4 a0[NI], b0[MI], a1[NI], b1[MI];
+  auto step = [&](int t, uint16_t* wc, uint16_t* xc, const uint16_t* wnext, const uint16_t* xnext) {
+    fetch(wc, xc, 1, a1, b1);
+    multiply(a0, b0);
+    pin(false);
+    __builtin_amdgcn_sched_barrier(0);
+    fetch(wc, xc, 2, a0, b0);
+    multiply(a1, b1);
+    pin(false);
+    __builtin_amdgcn_sched_barrier(0);
+    fetch(wc, xc, 3, a1, b1);
+    multiply(a0, b0);
+    pin(false);
+    __builtin_amdgcn_sched_barrier(0);
+    wait_vmcnt_0();
+    block_barrier();
+    issue(t + 2, wc, xc);  // past the last step: zeros, without a memory access
+    fetch(wnext, xnext, 0, a0, b0);  // past the last step: read and not used
+    multiply(a1, b1);
+    pin(true);
+    __builtin_amdgcn_sched_barrier(0);
+  };
+  issue(0, w0, x0);
+  issue(1, w1, x1);
+  wait_vmcnt<JW + JX>();
+  block_barrier();
+  fetch(w0, x0, 0, a0, b0);
+  for (int t = 0; t < steps; t += 2) {
+    step(t, w0, x0, w1, x1);
+    step(t + 1, w1, x1, w0, x0);
+  }
+  wait_vmcnt_0();  // the trailing loads have landed before the workgroup's LDS is released
+  const int nb = n0 + wn * 32 * NI + hl * 4 * NI, mb = m0 + wm * 32 * MI + l32;
+  with_activation(p.act, [&](auto act) {
+    if constexpr (NI == 1) {
+#pragma unroll
+      for (int g = 0; g < 2; ++g) {
+        float bias[8], gate[8];
+        const int n = n0 + wn * 32 + g * 16 + hl * 8;
+        load_columns8(p, n, bias, gate);
+#pragma unroll
+        for (int j = 0; j < MI; ++j) {
+          float z[8];
+#pragma unroll
+          for (int i = 0; i < 4; ++i) {
+            const auto u = __builtin_amdgcn_permlane32_swap(__float_as_uint(acc[0][j][g * 8 + i]),
+                                                            __float_as_uint(acc[0][j][g * 8 + 4 + i]), false, false);
+            z[i] = __uint_as_float(u[0]);
+            z[4 + i] = __uint_as_float(u[1]);
+          }
+          finish8<F16, decltype(act)::value>(p, mb + j * 32, n, z, bias, gate);
+        }
+      }
+    } else {
+#pragma unroll
+      for (int g = 0; g < 4; ++g)
+#pragma unroll
+        for (int q = 0; q < NI / 2; ++q) {
+          float bias[8], gate[8];
+          const int n = nb + g * 8 * NI + q * 8;
+          load_columns8(p, n, bias, gate);
+#pragma unroll
+          for (int j = 0; j < MI; ++j) {
+            float z[8];
+#pragma unroll
+            for (int i = 0; i < 8; ++i) z[i] = acc[2 * q + (i >> 2)][j][g * 4 + (i & 3)];
+            finish8<F16, decltype(act)::value>(p, mb + j * 32, n, z, bias, gate);
+          }
+        }
+    }
+  });
+}
+
+template <int NI, int MI, int WN, int WM>
+void launch_tile(const LinearParams& p, bool f16, hipStream_t st) {
+  const int64_t mt = (p.M + 32 * MI * WM - 1) / (32 * MI * WM), nt = (p.N + 32 * NI * WN - 1) / (32 * NI * WN);
+  const dim3 grid(static_cast<unsigned>(mt * nt));
+  if (f16)
+    linear_tile_kernel<NI, MI, WN, WM, true><<<grid, 256, 0, st>>>(p);
+  else
+    linear_tile_kernel<NI, MI, WN, WM, false><<<grid, 256, 0, st>>>(p);
 }
 
 }  // namespace
@@ -231,6 +461,20 @@ extern "C" int dfs_linear(const void* x, int64_t x_stride, const void* w, int64_
   p.out = static_cast<uint16_t*>(out);
   p.wide = o_stride % 8 == 0 && addr(out) % 16 == 0 && (!residual || (r_stride % 8 == 0 && addr(residual) % 16 == 0));
   hipStream_t st = reinterpret_cast<hipStream_t>(stream);
+  const bool chunks = k % 8 == 0 && x_stride % 8 == 0 && w_stride % 8 == 0 && addr(x) % 16 == 0 && addr(w) % 16 == 0 &&
+                      x_stride < (1 << 21) && w_stride < (1 << 21);
+  if (chunks) {
+    const int64_t big = ((rows + 255) / 256) * ((n + 255) / 256);
+    const int64_t mid = ((rows + 127) / 128) * ((n + 127) / 128);
+    const bool f16 = dtype == DFS_DTYPE_F16;
+    if (big >= 256)
+      launch_tile<4, 4, 2, 2>(p, f16, st);
+    else if (mid >= 256)
+      launch_tile<2, 2, 2, 2>(p, f16, st);
+    else
+      launch_tile<1, 1, 2, 2>(p, f16, st);
+    return check_launch(name);
+  }
   const int64_t mt = (rows + 63) / 64, nt = (n + 63) / 64;
   DFS_REQUIRE(mt < 65536, "%s: too many rows", name);
   const dim3 grid(static_cast<unsigned>(nt), static_cast<unsigned>(mt));
