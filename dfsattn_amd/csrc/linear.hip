@@ -34,6 +34,8 @@ struct LinearParams {
   int wide;  // rows of out and residual allow 16-byte accesses at multiples of 8
 };
 
+typedef float f32x2_t __attribute__((ext_vector_type(2)));
+
 template <bool F16>
 struct Half;
 template <>
@@ -44,6 +46,10 @@ struct Half<false> {
   }
   static __device__ __forceinline__ float to_f32(uint32_t bits) { return bf16_bits_to_f32(bits); }
   static __device__ __forceinline__ uint32_t from_f32(float v) { return f32_to_bf16_bits(v); }
+  static __device__ __forceinline__ uint32_t pack(float a, float b) {  // one v_cvt_pk, a in the low half
+    typedef __bf16 pair __attribute__((ext_vector_type(2)));
+    return __builtin_bit_cast(uint32_t, __builtin_convertvector((f32x2_t){a, b}, pair));
+  }
 };
 template <>
 struct Half<true> {
@@ -53,6 +59,10 @@ struct Half<true> {
   }
   static __device__ __forceinline__ float to_f32(uint32_t bits) { return f16_bits_to_f32(bits); }
   static __device__ __forceinline__ uint32_t from_f32(float v) { return f32_to_f16_bits(v); }
+  static __device__ __forceinline__ uint32_t pack(float a, float b) {
+    typedef _Float16 pair __attribute__((ext_vector_type(2)));
+    return __builtin_bit_cast(uint32_t, __builtin_convertvector((f32x2_t){a, b}, pair));
+  }
 };
 
 template <int ACT>
@@ -73,7 +83,7 @@ __device__ __forceinline__ float activate(float z) {
 
 // f(integral_constant<ACT>) with the call's activation.
 template <typename F>
-__device__ __forceinline__ void with_activation(int act, F&& f) {
+__host__ __device__ __forceinline__ void with_activation(int act, F&& f) {
   switch (act) {
     case kActGeluTanh: return f(std::integral_constant<int, kActGeluTanh>{});
     case kActGelu: return f(std::integral_constant<int, kActGelu>{});
@@ -99,36 +109,51 @@ __device__ __forceinline__ void load_columns8(const LinearParams& p, int n, floa
   }
 }
 
-// Eight consecutive outputs n.. of row m from their sums.
+// Eight consecutive outputs n.. of row m from their sums, all of them inside
+// the matrix and on a 16-byte boundary.
+template <bool F16, int ACT>
+__device__ __forceinline__ void finish8_wide(const LinearParams& p, int m, int n, const float* z, const float* bias,
+                                             const float* gate) {
+  float y[8];
+#pragma unroll
+  for (int i = 0; i < 8; ++i) y[i] = activate<ACT>(z[i] + bias[i]);
+  if (p.gate) {
+#pragma unroll
+    for (int i = 0; i < 8; ++i) y[i] *= gate[i];
+  }
+  if (p.residual) {
+    const uint4 rv = *reinterpret_cast<const uint4*>(p.residual + m * p.ldr + n);
+#pragma unroll
+    for (int i = 0; i < 8; ++i) y[i] += Half<F16>::to_f32(u16_at(rv, i));
+  }
+  *reinterpret_cast<uint4*>(p.out + m * p.ldo + n) =
+      make_uint4(Half<F16>::pack(y[0], y[1]), Half<F16>::pack(y[2], y[3]), Half<F16>::pack(y[4], y[5]),
+                 Half<F16>::pack(y[6], y[7]));
+}
+
+// The same at the matrix's edge, or for rows on no 16-byte boundary.
+template <bool F16, int ACT>
+__device__ __forceinline__ void finish8_edge(const LinearParams& p, int m, int n, const float* z, const float* bias,
+                                             const float* gate) {
+  if (m >= p.M) return;
+#pragma unroll
+  for (int i = 0; i < 8; ++i) {
+    float y = activate<ACT>(z[i] + bias[i]) * gate[i];
+    if (n + i < p.N) {
+      if (p.residual) y += Half<F16>::to_f32(p.residual[m * p.ldr + n + i]);
+      p.out[m * p.ldo + n + i] = static_cast<uint16_t>(Half<F16>::from_f32(y));
+    }
+  }
+}
+
 template <bool F16, int ACT>
 __device__ __forceinline__ void finish8(const LinearParams& p, int m, int n, const float* z, const float* bias,
                                         const float* gate) {
   if (m >= p.M || n >= p.N) return;
-  const uint16_t* r = p.residual ? p.residual + m * p.ldr + n : nullptr;
-  uint16_t* o = p.out + m * p.ldo + n;
-  if (p.wide && n + 8 <= p.N) {
-    uint4 rv = make_uint4(0, 0, 0, 0);
-    if (r) rv = *reinterpret_cast<const uint4*>(r);
-    uint32_t packed[4];
-#pragma unroll
-    for (int i = 0; i < 8; ++i) {
-      float y = activate<ACT>(z[i] + bias[i]);
-      if (p.gate) y *= gate[i];
-      if (r) y += Half<F16>::to_f32(u16_at(rv, i));
-      const uint32_t h = Half<F16>::from_f32(y);
-      packed[i / 2] = i & 1 ? packed[i / 2] | h << 16 : h;
-    }
-    *reinterpret_cast<uint4*>(o) = make_uint4(packed[0], packed[1], packed[2], packed[3]);
-    return;
-  }
-#pragma unroll
-  for (int i = 0; i < 8; ++i) {
-    if (n + i >= p.N) break;
-    float y = activate<ACT>(z[i] + bias[i]);
-    if (p.gate) y *= gate[i];
-    if (r) y += Half<F16>::to_f32(r[i]);
-    o[i] = static_cast<uint16_t>(Half<F16>::from_f32(y));
-  }
+  if (p.wide && n + 8 <= p.N)
+    finish8_wide<F16, ACT>(p, m, n, z, bias, gate);
+  else
+    finish8_edge<F16, ACT>(p, m, n, z, bias, gate);
 }
 
 // Eight elements k..k+7 of a row of K that may start at any 2-byte address;
@@ -395,6 +420,201 @@ __global__ void __launch_bounds__(256, NI * MI == 16 ? 1 : 2) linear_tile_kernel
   });
 }
 
+// 256 x 256 outputs a workgroup, four waves of 128 x 128, 64 channels a step.
+// Each operand's slice of a step is two halves of 128 rows (64 of each wave
+// row's 128), and a step is four phases of one quadrant each, 16 products:
+//   (A0, B0) (A1, B0) (A1, B1) (A0, B1)
+// A phase reads one half into registers for the next (A1, B1, then the next
+// step's B0 and A0: the registers just left), and loads the half read in the
+// phase before, two steps on. So all phases are alike: one half read, one
+// loaded seven phases before it is read, one barrier that says both that the
+// half to be read has landed and that the half to be loaded was read by all.
+template <bool F16, int ACT>
+__global__ void __launch_bounds__(256, 1) linear_big_kernel(LinearParams p) {
+  typedef typename Half<F16>::vec vec;
+  typedef Tile<2, 2, 2, 2, F16> T;  // swizzles of a half
+  __shared__ __attribute__((aligned(16))) uint16_t a00[128 * 64], a01[128 * 64], a10[128 * 64], a11[128 * 64];
+  __shared__ __attribute__((aligned(16))) uint16_t b00[128 * 64], b01[128 * 64], b10[128 * 64], b11[128 * 64];
+  __shared__ __attribute__((aligned(16))) float stage[4 * 2048];
+  const int lane = threadIdx.x & 63, w = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  const int l32 = lane & 31, hl = lane >> 5;
+  int tm, tn;
+  tile_of(blockIdx.x, (p.M + 255) / 256, (p.N + 255) / 256, tm, tn);
+  const int n0 = tn * 256, m0 = tm * 256;
+  const auto wrs = make_rsrc(p.w + static_cast<int64_t>(n0) * p.ldw, kOutside);
+  const auto xrs = make_rsrc(p.x + static_cast<int64_t>(m0) * p.ldx, kOutside);
+  // Byte offsets of this lane's chunks in step 0, [half][load]; rows past the
+  // matrix repeat its last one. Row q of wave row r's 64 in half h is output
+  // r * 128 + (q >> 3) * 16 + h * 8 + (q & 7), so that a lane ends with 16
+  // consecutive outputs, or row r * 128 + h * 64 + q of x.
+  uint32_t wv[2][4], xv[2][4];
+  const int r8 = w * 8 + (lane >> 3), c8 = lane & 7;
+#pragma unroll
+  for (int h = 0; h < 2; ++h)
+#pragma unroll
+    for (int j = 0; j < 4; ++j) {
+      const int r = j * 32 + r8, q = r & 63, base = (r >> 6) * 128;
+      const int n = min(n0 + base + (q >> 3) * 16 + h * 8 + (q & 7), p.N - 1) - n0;
+      const int m = min(m0 + base + h * 64 + q, p.M - 1) - m0;
+      wv[h][j] = static_cast<uint32_t>(n) * static_cast<uint32_t>(p.ldw * 2) + (c8 ^ T::swz_w(q)) * 16;
+      xv[h][j] = static_cast<uint32_t>(m) * static_cast<uint32_t>(p.ldx * 2) + (c8 ^ T::swz_x(q)) * 16;
+    }
+  const int steps = (p.K + 127) >> 7 << 1;  // an even number: the last may be all zeros
+  auto load_w = [&](int t, int h, uint16_t* buf) {
+    const int left = p.K - t * 64;
+    if (left < 64) {  // the last steps: chunks past K come as zeros, without a memory access
+#pragma unroll
+      for (int j = 0; j < 4; ++j)
+        if ((c8 ^ T::swz_w((j * 32 + r8) & 63)) * 8 >= left) wv[h][j] = kOutside;
+    }
+#pragma unroll
+    for (int j = 0; j < 4; ++j) load_lds16(wrs, buf + (j * 4 + w) * 512, wv[h][j], t * 128);
+  };
+  auto load_x = [&](int t, int h, uint16_t* buf) {
+    const int left = p.K - t * 64;
+    if (left < 64) {
+#pragma unroll
+      for (int j = 0; j < 4; ++j)
+        if ((c8 ^ T::swz_x((j * 32 + r8) & 63)) * 8 >= left) xv[h][j] = kOutside;
+    }
+#pragma unroll
+    for (int j = 0; j < 4; ++j) load_lds16(xrs, buf + (j * 4 + w) * 512, xv[h][j], t * 128);
+  };
+  const int wn = w & 1, wm = w >> 1;
+  const int arow = (wn * 64 + (l32 >> 2) * 8 + (l32 & 3)) * 64, brow = (wm * 64 + l32) * 64;
+  const int fa = T::swz_w((l32 >> 2) * 8 + (l32 & 3)), fb = T::swz_x(l32);
+  f32x16 acc[4][4];
+#pragma unroll
+  for (int i = 0; i < 4; ++i)
+#pragma unroll
+    for (int j = 0; j < 4; ++j) acc[i][j] = f32x16{};
+  typedef uint4 Frag[8];  // [quarter][tile]
+  auto read_w = [&](const uint16_t* buf, Frag& f) {
+#pragma unroll
+    for (int s = 0; s < 4; ++s)
+#pragma unroll
+      for (int i = 0; i < 2; ++i)
+        f[2 * s + i] = *reinterpret_cast<const uint4*>(buf + arow + i * 256 + ((2 * s + hl) ^ fa) * 8);
+  };
+  auto read_x = [&](const uint16_t* buf, Frag& f) {
+#pragma unroll
+    for (int s = 0; s < 4; ++s)
+#pragma unroll
+      for (int i = 0; i < 2; ++i)
+        f[2 * s + i] = *reinterpret_cast<const uint4*>(buf + brow + i * 2048 + ((2 * s + hl) ^ fb) * 8);
+  };
+  auto quadrant = [&](const Frag& a, const Frag& b, int ha, int hb) {
+#pragma unroll
+    for (int s = 0; s < 4; ++s)
+#pragma unroll
+      for (int j = 0; j < 2; ++j)
+#pragma unroll
+        for (int i = 0; i < 2; ++i)
+          acc[2 * ha + i][2 * hb + j] = Half<F16>::mfma(__builtin_bit_cast(vec, a[2 * s + i]),
+                                                        __builtin_bit_cast(vec, b[2 * s + j]),
+                                                        acc[2 * ha + i][2 * hb + j]);
+    constexpr int kMfma = 0x008, kDsRead = 0x100, kVmem = 0x020;
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      __builtin_amdgcn_sched_group_barrier(kDsRead, 2, 0);
+      __builtin_amdgcn_sched_group_barrier(kMfma, 2, 0);
+      __builtin_amdgcn_sched_group_barrier(kVmem, 1, 0);
+      __builtin_amdgcn_sched_group_barrier(kMfma, 2, 0);
+    }
+    __builtin_amdgcn_sched_barrier(0);
+  };
+  auto landed = [&] {  // the half loaded seven phases ago; six phases' loads are behind it
+    wait_vmcnt<24>();
+    block_barrier();
+  };
+  Frag fa0, fa1, fb0, fb1;
+  // One step with its A0 in c0, the other A registers c1; ends with the next
+  // step's A0 in c1. *c: this step's buffers, *n: the next step's.
+  auto step = [&](int t, Frag& c0, Frag& c1, uint16_t* a0c, uint16_t* a1c, uint16_t* b0c, uint16_t* b1c, uint16_t* a0n,
+                  uint16_t* b0n) {
+    landed();
+    read_w(a1c, c1);
+    load_w(t + 2, 0, a0c);
+    quadrant(c0, fb0, 0, 0);
+    landed();
+    read_x(b1c, fb1);
+    load_w(t + 2, 1, a1c);
+    quadrant(c1, fb0, 1, 0);
+    landed();
+    read_x(b0n, fb0);
+    load_x(t + 2, 1, b1c);
+    quadrant(c1, fb1, 1, 1);
+    landed();
+    read_w(a0n, c1);
+    load_x(t + 3, 0, b0n);
+    quadrant(c0, fb1, 0, 1);
+  };
+  load_x(0, 0, b00);
+  load_w(0, 0, a00);
+  load_w(0, 1, a10);
+  load_x(0, 1, b10);
+  load_x(1, 0, b01);
+  load_w(1, 0, a01);
+  load_w(1, 1, a11);
+  load_x(1, 1, b11);
+  wait_vmcnt<28>();
+  block_barrier();
+  read_x(b00, fb0);
+  landed();
+  read_w(a00, fa0);
+  load_x(2, 0, b00);
+  for (int t = 0; t < steps; t += 2) {
+    step(t, fa0, fa1, a00, a10, b00, b10, a01, b01);
+    step(t + 1, fa1, fa0, a01, a11, b01, b11, a00, b00);
+  }
+  wait_vmcnt_0();  // the trailing loads have landed before the workgroup's LDS is released
+  // A lane's 16 outputs of a row lie 64 rows apart from its neighbour's, so the
+  // sums go through LDS, 32 rows x 64 outputs at a time, in the wave's own part
+  // of it: whole rows of 128 bytes leave (and come, for the residual).
+  float* const st = stage + w * 2048;
+  const bool inside = p.wide && m0 + 256 <= p.M && n0 + 256 <= p.N;
+#pragma unroll
+  for (int gp = 0; gp < 2; ++gp) {
+    const int n = n0 + wn * 128 + gp * 64 + (lane & 7) * 8, c = (lane & 7) * 2;
+    float bias[8], gate[8];
+    load_columns8(p, n, bias, gate);
+#pragma unroll
+    for (int j = 0; j < 4; ++j) {
+#pragma unroll
+      for (int g = 0; g < 2; ++g)
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {  // outputs g * 32 + hl * 16 + 4 i .. + 3 of row l32
+          const f32x16& z = acc[i][j];
+          *reinterpret_cast<float4*>(st + l32 * 64 + ((g * 8 + hl * 4 + i) ^ (l32 & 15)) * 4) =
+              make_float4(z[gp * 8 + g * 4], z[gp * 8 + g * 4 + 1], z[gp * 8 + g * 4 + 2], z[gp * 8 + g * 4 + 3]);
+        }
+      auto row = [&](int i, float* z) {
+        const int r = i * 8 + (lane >> 3);
+        const float4 lo = *reinterpret_cast<const float4*>(st + r * 64 + (c ^ (r & 15)) * 4);
+        const float4 hi = *reinterpret_cast<const float4*>(st + r * 64 + ((c + 1) ^ (r & 15)) * 4);
+        z[0] = lo.x; z[1] = lo.y; z[2] = lo.z; z[3] = lo.w;
+        z[4] = hi.x; z[5] = hi.y; z[6] = hi.z; z[7] = hi.w;
+        return m0 + wm * 128 + j * 32 + r;
+      };
+      if (inside) {
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+          float z[8];
+          const int m = row(i, z);
+          finish8_wide<F16, ACT>(p, m, n, z, bias, gate);
+        }
+      } else {
+#pragma unroll 1
+        for (int i = 0; i < 4; ++i) {
+          float z[8];
+          const int m = row(i, z);
+          finish8_edge<F16, ACT>(p, m, n, z, bias, gate);
+        }
+      }
+    }
+  }
+}
+
 template <int NI, int MI, int WN, int WM>
 void launch_tile(const LinearParams& p, bool f16, hipStream_t st) {
   const int64_t mt = (p.M + 32 * MI * WM - 1) / (32 * MI * WM), nt = (p.N + 32 * NI * WN - 1) / (32 * NI * WN);
@@ -467,9 +687,15 @@ extern "C" int dfs_linear(const void* x, int64_t x_stride, const void* w, int64_
     const int64_t big = ((rows + 255) / 256) * ((n + 255) / 256);
     const int64_t mid = ((rows + 127) / 128) * ((n + 127) / 128);
     const bool f16 = dtype == DFS_DTYPE_F16;
-    if (big >= 256)
-      launch_tile<4, 4, 2, 2>(p, f16, st);
-    else if (mid >= 256)
+    if (big >= 256) {
+      const dim3 grid(static_cast<unsigned>(big));
+      with_activation(p.act, [&](auto act) {
+        if (f16)
+          linear_big_kernel<true, decltype(act)::value><<<grid, 256, 0, st>>>(p);
+        else
+          linear_big_kernel<false, decltype(act)::value><<<grid, 256, 0, st>>>(p);
+      });
+    } else if (mid >= 256)
       launch_tile<2, 2, 2, 2>(p, f16, st);
     else
       launch_tile<1, 1, 2, 2>(p, f16, st);
