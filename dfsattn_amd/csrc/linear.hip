@@ -460,9 +460,10 @@ __global__ void __launch_bounds__(256, 1) linear_big_kernel(LinearParams p) {
       xv[h][j] = static_cast<uint32_t>(m) * static_cast<uint32_t>(p.ldx * 2) + (c8 ^ T::swz_x(q)) * 16;
     }
   const int steps = (p.K + 127) >> 7 << 1;  // an even number: the last may be all zeros
-  auto load_w = [&](int t, int h, uint16_t* buf) {
+  // The last steps' chunks past K (tail) come as zeros, without a memory access.
+  auto load_w = [&](auto tail, int t, int h, uint16_t* buf) {
     const int left = p.K - t * 64;
-    if (left < 64) {  // the last steps: chunks past K come as zeros, without a memory access
+    if (tail.value && left < 64) {
 #pragma unroll
       for (int j = 0; j < 4; ++j)
         if ((c8 ^ T::swz_w((j * 32 + r8) & 63)) * 8 >= left) wv[h][j] = kOutside;
@@ -470,9 +471,9 @@ __global__ void __launch_bounds__(256, 1) linear_big_kernel(LinearParams p) {
 #pragma unroll
     for (int j = 0; j < 4; ++j) load_lds16(wrs, buf + (j * 4 + w) * 512, wv[h][j], t * 128);
   };
-  auto load_x = [&](int t, int h, uint16_t* buf) {
+  auto load_x = [&](auto tail, int t, int h, uint16_t* buf) {
     const int left = p.K - t * 64;
-    if (left < 64) {
+    if (tail.value && left < 64) {
 #pragma unroll
       for (int j = 0; j < 4; ++j)
         if ((c8 ^ T::swz_x((j * 32 + r8) & 63)) * 8 >= left) xv[h][j] = kOutside;
@@ -515,11 +516,15 @@ __global__ void __launch_bounds__(256, 1) linear_big_kernel(LinearParams p) {
                                                         acc[2 * ha + i][2 * hb + j]);
     constexpr int kMfma = 0x008, kDsRead = 0x100, kVmem = 0x020;
 #pragma unroll
+    for (int i = 0; i < 8; ++i) {
+      __builtin_amdgcn_sched_group_barrier(kMfma, 1, 0);
+      __builtin_amdgcn_sched_group_barrier(kDsRead, 1, 0);
+    }
+#pragma unroll
     for (int i = 0; i < 4; ++i) {
-      __builtin_amdgcn_sched_group_barrier(kDsRead, 2, 0);
-      __builtin_amdgcn_sched_group_barrier(kMfma, 2, 0);
+      __builtin_amdgcn_sched_group_barrier(kMfma, 1, 0);
       __builtin_amdgcn_sched_group_barrier(kVmem, 1, 0);
-      __builtin_amdgcn_sched_group_barrier(kMfma, 2, 0);
+      __builtin_amdgcn_sched_group_barrier(kMfma, 1, 0);
     }
     __builtin_amdgcn_sched_barrier(0);
   };
@@ -530,42 +535,50 @@ __global__ void __launch_bounds__(256, 1) linear_big_kernel(LinearParams p) {
   Frag fa0, fa1, fb0, fb1;
   // One step with its A0 in c0, the other A registers c1; ends with the next
   // step's A0 in c1. *c: this step's buffers, *n: the next step's.
-  auto step = [&](int t, Frag& c0, Frag& c1, uint16_t* a0c, uint16_t* a1c, uint16_t* b0c, uint16_t* b1c, uint16_t* a0n,
+  constexpr std::true_type may_end{};
+  constexpr std::false_type whole{};
+  auto step = [&](auto tail, int t, Frag& c0, Frag& c1, uint16_t* a0c, uint16_t* a1c, uint16_t* b0c, uint16_t* b1c, uint16_t* a0n,
                   uint16_t* b0n) {
     landed();
     read_w(a1c, c1);
-    load_w(t + 2, 0, a0c);
+    load_w(tail, t + 2, 0, a0c);
     quadrant(c0, fb0, 0, 0);
     landed();
     read_x(b1c, fb1);
-    load_w(t + 2, 1, a1c);
+    load_w(tail, t + 2, 1, a1c);
     quadrant(c1, fb0, 1, 0);
     landed();
     read_x(b0n, fb0);
-    load_x(t + 2, 1, b1c);
+    load_x(tail, t + 2, 1, b1c);
     quadrant(c1, fb1, 1, 1);
     landed();
     read_w(a0n, c1);
-    load_x(t + 3, 0, b0n);
+    load_x(tail, t + 3, 0, b0n);
     quadrant(c0, fb1, 0, 1);
   };
-  load_x(0, 0, b00);
-  load_w(0, 0, a00);
-  load_w(0, 1, a10);
-  load_x(0, 1, b10);
-  load_x(1, 0, b01);
-  load_w(1, 0, a01);
-  load_w(1, 1, a11);
-  load_x(1, 1, b11);
+  load_x(may_end, 0, 0, b00);
+  load_w(may_end, 0, 0, a00);
+  load_w(may_end, 0, 1, a10);
+  load_x(may_end, 0, 1, b10);
+  load_x(may_end, 1, 0, b01);
+  load_w(may_end, 1, 0, a01);
+  load_w(may_end, 1, 1, a11);
+  load_x(may_end, 1, 1, b11);
   wait_vmcnt<28>();
   block_barrier();
   read_x(b00, fb0);
   landed();
   read_w(a00, fa0);
-  load_x(2, 0, b00);
-  for (int t = 0; t < steps; t += 2) {
-    step(t, fa0, fa1, a00, a10, b00, b10, a01, b01);
-    step(t + 1, fa1, fa0, a01, a11, b01, b11, a00, b00);
+  load_x(may_end, 2, 0, b00);
+  int t = 0;
+  for (; (t + 5) * 64 <= p.K; t += 2) {  // nothing past K is loaded
+    step(whole, t, fa0, fa1, a00, a10, b00, b10, a01, b01);
+    step(whole, t + 1, fa1, fa0, a01, a11, b01, b11, a00, b00);
+  }
+#pragma unroll 1
+  for (; t < steps; t += 2) {
+    step(may_end, t, fa0, fa1, a00, a10, b00, b10, a01, b01);
+    step(may_end, t + 1, fa1, fa0, a01, a11, b01, b11, a00, b00);
   }
   wait_vmcnt_0();  // the trailing loads have landed before the workgroup's LDS is released
   // A lane's 16 outputs of a row lie 64 rows apart from its neighbour's, so the
