@@ -6,7 +6,10 @@
 // sees none), lse_i the log of the softmax's denominator (-inf there).
 // Key j lies in slot j of the sequence's rows, or, in a rolling cache of S
 // slots, in slot j < sinks ? j : sinks + (j - sinks) mod (S - sinks).
+#include <algorithm>
+
 #include "common.h"
+#include "lds_copy.h"
 
 namespace dfs {
 namespace {
@@ -23,71 +26,643 @@ struct WindowParams {
   int left, right, sinks;  // kNoLimit for no limit
   int rolling;
   float scale_log2;
+  // How the call is cut (plan).
+  int group;   // query heads of a key head
+  int few;     // window_few_kernel
+  int blocks;  // of 128 rows of a (sequence, key head)
+  int chunks, whole, split, parts;
+  float *part_o, *part_ml;  // O [row][D] and (m, l) [row][2] of the parts
 };
 
+__device__ __forceinline__ int slot_of(const WindowParams& p, int pos) {
+  if (pos < p.sinks) return pos;
+  return p.sinks + static_cast<int>(static_cast<uint32_t>(pos - p.sinks) % static_cast<uint32_t>(p.S - p.sinks));
+}
+
 template <bool F16>
-__device__ __forceinline__ float half_to_f32(uint32_t bits) {
-  return F16 ? f16_bits_to_f32(bits) : bf16_bits_to_f32(bits);
+struct Half;
+template <>
+struct Half<false> {
+  typedef bf16x8 vec;
+  typedef __bf16 pair __attribute__((ext_vector_type(2)));
+  static __device__ __forceinline__ f32x16 mfma(vec a, vec b, f32x16 c) {
+    return __builtin_amdgcn_mfma_f32_32x32x16_bf16(a, b, c, 0, 0, 0);
+  }
+  // acc + x.lo + x.hi in fp32.
+  static __device__ __forceinline__ float sum2(pair x, float acc) {
+    return __builtin_amdgcn_fdot2_f32_bf16(x, (pair){(__bf16)1.0f, (__bf16)1.0f}, acc, false);
+  }
+};
+template <>
+struct Half<true> {
+  typedef f16x8 vec;
+  typedef _Float16 pair __attribute__((ext_vector_type(2)));
+  static __device__ __forceinline__ f32x16 mfma(vec a, vec b, f32x16 c) {
+    return __builtin_amdgcn_mfma_f32_32x32x16_f16(a, b, c, 0, 0, 0);
+  }
+  static __device__ __forceinline__ float sum2(pair x, float acc) {
+    return __builtin_amdgcn_fdot2(x, (pair){(_Float16)1.0f, (_Float16)1.0f}, acc, false);
+  }
+};
+typedef float f32x2 __attribute__((ext_vector_type(2)));
+
+// Two values rounded to the storage type, the first in the low half.
+template <bool F16>
+__device__ __forceinline__ uint32_t pack2(float a, float b) {
+  return __builtin_bit_cast(uint32_t, __builtin_convertvector((f32x2){a, b}, typename Half<F16>::pair));
 }
 
-__device__ __forceinline__ int slot_of(const WindowParams& p, int64_t pos) {
-  if (!p.rolling || pos < p.sinks) return static_cast<int>(pos);
-  return p.sinks + static_cast<int>((pos - p.sinks) % (p.S - p.sinks));
+// This lane's value with the other lane half's (lane ^ 32).
+__device__ __forceinline__ float xhalf_max(float v) {
+  const auto r = __builtin_amdgcn_permlane32_swap(__float_as_uint(v), __float_as_uint(v), false, false);
+  return fmaxf(__uint_as_float(r[0]), __uint_as_float(r[1]));
+}
+__device__ __forceinline__ float xhalf_sum(float v) {
+  const auto r = __builtin_amdgcn_permlane32_swap(__float_as_uint(v), __float_as_uint(v), false, false);
+  return __uint_as_float(r[0]) + __uint_as_float(r[1]);
 }
 
-// One wave a query: its D channels over the lanes, the keys one at a time with
-// the running maximum and sum.
-template <int D, bool F16>
-__global__ void __launch_bounds__(256) window_simple_kernel(WindowParams p) {
-  constexpr int E = D / 64;
-  const int lane = threadIdx.x & 63;
-  const int64_t row = static_cast<int64_t>(blockIdx.x) * 4 + (threadIdx.x >> 6);
-  if (row >= static_cast<int64_t>(p.B) * p.Hq * p.Lq) return;
-  const int i = static_cast<int>(row % p.Lq), h = static_cast<int>(row / p.Lq % p.Hq);
-  const int b = static_cast<int>(row / p.Lq / p.Hq), g = h / (p.Hq / p.Hkv);
-  const int nq = p.q_lens ? min(max(p.q_lens[b], 0), p.Lq) : p.Lq;
-  int nk = p.kv_lens ? max(p.kv_lens[b], 0) : p.S;
-  if (!p.rolling) nk = min(nk, p.S);
-  const uint16_t* q = p.q + b * p.q_sb + h * p.q_sh + i * p.q_sl;
-  const uint16_t* k = p.k + b * p.k_sb + g * p.k_sh;
-  const uint16_t* v = p.v + b * p.v_sb + g * p.v_sh;
-  float qv[E], o[E] = {};
+// Queries and keys of sequence b.
+struct Seq {
+  int nq;
+  int64_t nk;
+};
+__device__ __forceinline__ Seq seq_of(const WindowParams& p, int b) {
+  Seq s;
+  s.nq = p.q_lens ? min(max(p.q_lens[b], 0), p.Lq) : p.Lq;
+  s.nk = p.kv_lens ? max(p.kv_lens[b], 0) : p.S;
+  s.nk = min(s.nk, static_cast<int64_t>(p.rolling ? 0x7fffff00 : p.S));  // tile ends stay within 32 bits
+  return s;
+}
+// Last key and first key behind the sinks that query i sees.
+__device__ __forceinline__ int last_key(const WindowParams& p, const Seq& s, int i) {
+  return static_cast<int>(max(min(s.nk - s.nq + i + p.right, s.nk - 1), int64_t(-1)));
+}
+__device__ __forceinline__ int first_key(const WindowParams& p, const Seq& s, int i) {
+  return static_cast<int>(max(s.nk - s.nq + i - p.left, int64_t(0)));
+}
+
+// The key tiles of T keys that queries q0..q1 see: `sink` tiles from 0 on,
+// then those from `low` on, `n` in all.
+struct Tiles {
+  int sink, low, n;
+  __device__ __forceinline__ int at(int i) const { return i < sink ? i : low + i - sink; }
+};
+template <int T>
+__device__ __forceinline__ Tiles tiles_of(const WindowParams& p, const Seq& s, int q0, int q1) {
+  Tiles t{0, 0, 0};
+  if (q1 < q0) return t;
+  const int hi = last_key(p, s, q1) + 1, lo = first_key(p, s, q0);
+  t.low = lo / T;
+  t.sink = min((min(p.sinks, hi) + T - 1) / T, t.low);
+  t.n = t.sink + max((hi + T - 1) / T - t.low, 0);
+  return t;
+}
+
+// Copies of a key tile into LDS by NW waves, rows of D channels straight from
+// the sequence's slab: load j of wave w fills 1 KB. Rows past the sequence come
+// as zeros.
+template <int D, int T, int NW>
+struct KeyTile {
+  static constexpr int CPR = D / 8, RPI = 64 / CPR, LOADS = T * D * 2 / (NW * 1024);
+  bool value;
+  int row0;      // this lane's row in load 0
+  uint32_t col;  // byte of its chunk within that row
+  __device__ __forceinline__ KeyTile(int w, int lane, bool value_) : value(value_) {
+    row0 = w * RPI + lane / CPR;
+    const int c = lane % CPR;
+    col = (value ? c ^ swz_v(row0) : c ^ swz_k(row0)) * 16;
+  }
+  // ... and in load j, whose rows lie j * NW * RPI further.
+  __device__ __forceinline__ uint32_t col_of(int j) const {
+    return col ^ (value ? swz_v(j * NW * RPI) : swz_k(j * NW * RPI)) * 16;
+  }
+  // Chunk c of row r lies at c ^ swz(r): 16 keys read one chunk each, or 4 keys
+  // four chunks each (the transposing reads of V), without a bank conflict.
+  static __device__ __forceinline__ int swz_k(int r) { return D == 128 ? r & 15 : (r >> 1) & 7; }
+  static __device__ __forceinline__ int swz_v(int r) { return D == 128 ? (r & 3) << 2 : ((r >> 1) & 1) << 2; }
+
+  template <bool ROLL>
+  __device__ __forceinline__ void issue(const WindowParams& p, const uint16_t* slab, int64_t stride, int64_t nk,
+                                        int tile, uint16_t* lds, int w) const {
+    const int first = tile * T;
+    const uint32_t bytes = static_cast<uint32_t>(stride * 2);
+    if (!ROLL) {
+      const int rows = static_cast<int>(max(min(nk - first, static_cast<int64_t>(T)), int64_t(0)));
+      const auto rs = make_rsrc(slab + first * stride, rows ? (rows - 1) * bytes + D * 2 : 0);
 #pragma unroll
-  for (int e = 0; e < E; ++e) qv[e] = half_to_f32<F16>(q[lane * E + e]) * p.scale_log2;
-  float m = -INFINITY, l = 0.f;
-  const int64_t pos = static_cast<int64_t>(nk) - nq + i;
-  const int64_t hi = i < nq ? min(static_cast<int64_t>(nk), pos + p.right + 1) : 0;
-  const int64_t lo = max(int64_t(0), pos - p.left);
-  for (int64_t j = 0; j < hi; ++j) {
-    if (j >= p.sinks && j < lo) j = lo;
-    if (j >= hi) break;
-    const int64_t slot = slot_of(p, j);
-    float s = 0.f;
+      for (int j = 0; j < LOADS; ++j)
+        load_lds16(rs, lds + (j * NW + w) * 512, (row0 + j * NW * RPI) * bytes + col_of(j), 0);
+      return;
+    }
+    const auto rs = make_rsrc(slab, (p.S - 1) * bytes + D * 2);
+    const int s0 = slot_of(p, first);
+    uint32_t off[LOADS];
+    if (first + T <= nk && s0 + T <= p.S) {  // one stretch of slots
 #pragma unroll
-    for (int e = 0; e < E; ++e) s += qv[e] * half_to_f32<F16>(k[slot * p.k_sl + lane * E + e]);
+      for (int j = 0; j < LOADS; ++j) off[j] = (s0 + row0 + j * NW * RPI) * bytes + col_of(j);
+    } else {
 #pragma unroll
-    for (int off = 32; off >= 1; off >>= 1) s += __shfl_xor(s, off, 64);
-    const float mn = fmaxf(m, s), ref = mn == -INFINITY ? 0.f : mn;
-    const float alpha = exp2f(m - ref), w = exp2f(s - ref);
-    l = l * alpha + w;
+      for (int j = 0; j < LOADS; ++j) {
+        const int r = row0 + j * NW * RPI;
+        const int slot = s0 + r < p.S ? s0 + r : slot_of(p, s0 + r);
+        off[j] = first + r < nk ? slot * bytes + col_of(j) : 0xfffffff0u;
+      }
+    }
 #pragma unroll
-    for (int e = 0; e < E; ++e) o[e] = o[e] * alpha + w * half_to_f32<F16>(v[slot * p.v_sl + lane * E + e]);
+    for (int j = 0; j < LOADS; ++j) load_lds16(rs, lds + (j * NW + w) * 512, off[j], 0);
+  }
+};
+
+// S^T of 32 keys (LDS rows k0..) and the wave's 32 queries.
+template <int D, bool F16, int T>
+__device__ __forceinline__ f32x16 scores32(const uint16_t* keys, int k0, const typename Half<F16>::vec* q, int l32,
+                                           int hl) {
+  typedef KeyTile<D, T, 1> KT;
+  f32x16 s = f32x16{};
+#pragma unroll
+  for (int i = 0; i < D / 16; ++i) {
+    const uint4 a =
+        *reinterpret_cast<const uint4*>(keys + (k0 + l32) * D + ((2 * i + hl) ^ KT::swz_k(l32)) * 8);
+    s = Half<F16>::mfma(__builtin_bit_cast(typename Half<F16>::vec, a), q[i], s);
+  }
+  return s;
+}
+
+// V^T operand of 16 keys (LDS rows k0..) and channels dc * 32..: two
+// transposing reads, which give a lane 4 keys of one channel each, in the order
+// in which its scores hold them (k0 + hl * 4 + 0..3, then 8 further).
+template <int D, bool F16, int T>
+__device__ __forceinline__ typename Half<F16>::vec values16(const uint16_t* vals, int k0, int dc, int lane) {
+  typedef short s16x4 __attribute__((ext_vector_type(4)));
+  typedef short s16x8 __attribute__((ext_vector_type(8)));
+  typedef __attribute__((address_space(3))) s16x4 lds_s16x4;
+  const int i = lane & 15, key = (lane >> 5) * 4 + (i >> 2);
+  const int chunk = dc * 4 + ((lane >> 4) & 1) * 2 + ((i >> 1) & 1);
+  const uint16_t* at = vals + (k0 + key) * D + (chunk ^ KeyTile<D, T, 1>::swz_v(key)) * 8 + (i & 1) * 4;
+  const s16x4 lo = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s16x4*)at);
+  const s16x4 hi = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s16x4*)(at + 8 * D));
+  const s16x8 v = {lo[0], lo[1], lo[2], lo[3], hi[0], hi[1], hi[2], hi[3]};
+  return __builtin_bit_cast(typename Half<F16>::vec, v);
+}
+
+// Running maximum, in log2 units, of the scores s[0..N) times c; O and l follow
+// it when some row's maximum has grown by more than 2^kSlack (P then stays
+// below 2^kSlack, which costs neither its relative precision nor fp32's range,
+// and most tiles leave O alone).
+constexpr float kSlack = 8.f;
+template <int N, int DCH>
+__device__ __forceinline__ float follow_max(const f32x16* s, float c, float& m, float& l, f32x16* o) {
+  float mx = -INFINITY;
+#pragma unroll
+  for (int k = 0; k < N; ++k)
+#pragma unroll
+    for (int r = 0; r < 16; ++r) mx = fmaxf(mx, s[k][r]);
+  mx = xhalf_max(mx) * c;
+  if (__any(mx > m + kSlack)) {
+    const float mn = fmaxf(m, mx);
+    const float alpha = exp2_fast(m - (mn == -INFINITY ? 0.f : mn));
+    l *= alpha;
+#pragma unroll
+    for (int i = 0; i < DCH; ++i)
+#pragma unroll
+      for (int r = 0; r < 16; ++r) o[i][r] *= alpha;
     m = mn;
   }
-  uint16_t* out = p.out + b * p.o_sb + h * p.o_sh + i * p.o_sl;
+  return m == -INFINITY ? 0.f : m;  // rows without a key so far: P = 2^(-inf)
+}
+
+// P = 2^(s c - m) of 32 keys as two PV operands; their rounded values are added
+// to l.
+template <bool F16>
+__device__ __forceinline__ void weights32(const f32x16& s, float c, float m, typename Half<F16>::vec* pf, float& l) {
 #pragma unroll
-  for (int e = 0; e < E; ++e) {
-    const float y = l > 0.f ? o[e] / l : (l == 0.f ? 0.f : l);
-    out[lane * E + e] = static_cast<uint16_t>(F16 ? f32_to_f16_bits(y) : f32_to_bf16_bits(y));
+  for (int h = 0; h < 2; ++h) {
+    uint32_t w[4];
+#pragma unroll
+    for (int j = 0; j < 4; ++j) {
+      w[j] = pack2<F16>(exp2_fast(fmaf(s[h * 8 + 2 * j], c, -m)), exp2_fast(fmaf(s[h * 8 + 2 * j + 1], c, -m)));
+      l = Half<F16>::sum2(__builtin_bit_cast(typename Half<F16>::pair, w[j]), l);
+    }
+    pf[h] = __builtin_bit_cast(typename Half<F16>::vec, make_uint4(w[0], w[1], w[2], w[3]));
   }
-  if (p.lse && lane == 0)
-    p.lse[row] = l == 0.f ? -INFINITY : (m + log2f(l)) * 0.69314718055994531f;
+}
+
+// Keys first.. of the scores that the row does not see get -inf.
+__device__ __forceinline__ void mask32(f32x16& s, int first, int hl, int klo, int khi, int sinks) {
+#pragma unroll
+  for (int r = 0; r < 16; ++r) {
+    const int key = first + (r >> 2) * 8 + hl * 4 + (r & 3);
+    if (key > khi || (key < klo && key >= sinks)) s[r] = -INFINITY;
+  }
+}
+
+__device__ __forceinline__ float lse_of(float m, float l) {
+  return l == 0.f ? -INFINITY : (m + log2f(l)) * 0.69314718055994531f;
+}
+
+// O^T / l of a lane's row: the halves of a lane pair are joined into 8
+// consecutive channels, 16-byte stores.
+template <int D, bool F16>
+__device__ __forceinline__ void store_row(uint16_t* out, const f32x16* o, float inv, bool live, int hl) {
+#pragma unroll
+  for (int dc = 0; dc < D / 32; ++dc)
+#pragma unroll
+    for (int g = 0; g < 2; ++g) {
+      uint32_t a[2], b[2];
+#pragma unroll
+      for (int i = 0; i < 2; ++i) {
+        a[i] = pack2<F16>(o[dc][g * 8 + 2 * i] * inv, o[dc][g * 8 + 2 * i + 1] * inv);
+        b[i] = pack2<F16>(o[dc][g * 8 + 4 + 2 * i] * inv, o[dc][g * 8 + 5 + 2 * i] * inv);
+      }
+      const auto x = __builtin_amdgcn_permlane32_swap(a[0], b[0], false, false);
+      const auto y = __builtin_amdgcn_permlane32_swap(a[1], b[1], false, false);
+      if (live) *reinterpret_cast<uint4*>(out + dc * 32 + g * 16 + hl * 8) = make_uint4(x[0], y[0], x[1], y[1]);
+    }
+}
+
+// A part's O and (m, l) of a lane's row as they are.
+template <int D>
+__device__ __forceinline__ void store_part(float* po, float* pml, const f32x16* o, float m, float l, int hl) {
+#pragma unroll
+  for (int dc = 0; dc < D / 32; ++dc)
+#pragma unroll
+    for (int g = 0; g < 4; ++g)
+      *reinterpret_cast<float4*>(po + dc * 32 + g * 8 + hl * 4) =
+          make_float4(o[dc][g * 4], o[dc][g * 4 + 1], o[dc][g * 4 + 2], o[dc][g * 4 + 3]);
+  if (hl == 0) *reinterpret_cast<float2*>(pml) = make_float2(m, l);
+}
+
+// Rows of a (sequence, key head): query i of query head g of the group is row
+// i * group + g, so that a block's rows share their keys and stand at few
+// positions.
+struct Row {
+  int i, g;
+};
+__device__ __forceinline__ Row row_of(const WindowParams& p, int r) {
+  Row x;
+  x.i = r / p.group;
+  x.g = r - x.i * p.group;
+  return x;
+}
+
+// Work item of a workgroup: block `blk` of (sequence, key head) `bh`, part
+// `piece` of `pieces`, whose result goes to `slot`.
+struct Item {
+  int bh, blk, piece, pieces, slot;
+};
+
+// Hardware deals workgroup i to XCD i % 8. The blocks of a (sequence, key
+// head) are cut into p.chunks ranges and range u of them all belongs to XCD
+// u % 8, so neighbouring blocks, which share keys, run on one XCD's L2 and
+// sequences of different lengths spread evenly. Of an XCD's list the first
+// p.whole blocks are one workgroup each, the rest p.parts, joined by
+// window_join_kernel. Late blocks, which see most keys where left has no limit,
+// are started first.
+__device__ __forceinline__ bool item_of(const WindowParams& p, Item& it) {
+  const int x = blockIdx.x & 7, j = blockIdx.x >> 3;
+  int i = j;
+  it.piece = 0;
+  it.pieces = 1;
+  it.slot = 0;
+  if (j >= p.whole && p.parts > 1) {
+    const int t = (j - p.whole) / p.parts;
+    it.piece = j - p.whole - t * p.parts;
+    it.pieces = p.parts;
+    it.slot = (t * 8 + x) * p.parts + it.piece;
+    i = p.whole + t;
+  }
+  const int per = (p.blocks + p.chunks - 1) / p.chunks;  // blocks of a range
+  const int u = i / per * 8 + x;
+  it.bh = u / p.chunks;
+  it.blk = p.blocks - 1 - (u % p.chunks * per + i % per);
+  return it.bh < p.B * p.Hkv && it.blk >= 0;
+}
+
+// 128 rows a workgroup, four waves of 32, tiles of 128 keys; the framework's
+// block-sparse schedule: two workgroups a CU, one K and one V buffer each, the
+// next K copied under the softmax and P V, the next V under Q K^T. S^T = K Q^T
+// leaves a lane with one query, whose P is the second operand of
+// O^T += V^T P^T as it lies in the registers.
+template <int D, bool F16, bool ROLL>
+__global__ void __launch_bounds__(256, 2) window_tile_kernel(WindowParams p) {
+  constexpr int DCH = D / 32, T = 128;
+  typedef KeyTile<D, T, 4> KT;
+  typedef typename Half<F16>::vec vec;
+  __shared__ __attribute__((aligned(16))) uint16_t k_lds[T * D];
+  __shared__ __attribute__((aligned(16))) uint16_t v_lds[T * D];
+  Item it;
+  if (!item_of(p, it)) return;
+  const int lane = threadIdx.x & 63, w = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  const int l32 = lane & 31, hl = lane >> 5;
+  const int b = it.bh / p.Hkv, g = it.bh - b * p.Hkv;
+  const Seq seq = seq_of(p, b);
+  const int rows = p.Lq * p.group, r0 = it.blk * 128;
+  const Tiles tiles = tiles_of<T>(p, seq, r0 / p.group, min(min(r0 + 127, rows - 1) / p.group, seq.nq - 1));
+  const int t0 = static_cast<int64_t>(tiles.n) * it.piece / it.pieces;
+  const int t1 = static_cast<int64_t>(tiles.n) * (it.piece + 1) / it.pieces;
+  // This wave's rows, and its lane's.
+  const int wr = r0 + w * 32;
+  const int wq0 = min(wr, rows - 1) / p.group, wq1 = min(min(wr + 31, rows - 1) / p.group, seq.nq - 1);
+  const int wlo0 = first_key(p, seq, wq0), wlo1 = first_key(p, seq, wq1);
+  const int whi0 = last_key(p, seq, wq0), whi1 = wq1 < wq0 ? -1 : last_key(p, seq, wq1);
+  const bool in = wr + l32 < rows;
+  const Row row = row_of(p, min(wr + l32, rows - 1));
+  const int klo = first_key(p, seq, row.i), khi = last_key(p, seq, row.i);
+  const int head = g * p.group + row.g;
+  f32x16 o[DCH];
+#pragma unroll
+  for (int i = 0; i < DCH; ++i) o[i] = f32x16{};
+  float m = -INFINITY, l = 0.f;
+  if (t0 < t1) {
+    const uint16_t* const ks = p.k + b * p.k_sb + g * p.k_sh;
+    const uint16_t* const vs = p.v + b * p.v_sb + g * p.v_sh;
+    const KT kc(w, lane, false), vc(w, lane, true);
+    int tile = tiles.at(t0);
+    kc.template issue<ROLL>(p, ks, p.k_sl, seq.nk, tile, k_lds, w);
+    vc.template issue<ROLL>(p, vs, p.v_sl, seq.nk, tile, v_lds, w);
+    vec qf[D / 16];
+    {
+      const uint16_t* q = p.q + b * p.q_sb + head * p.q_sh + row.i * p.q_sl;
+#pragma unroll
+      for (int i = 0; i < D / 16; ++i)
+        qf[i] = __builtin_bit_cast(vec, *reinterpret_cast<const uint4*>(q + (2 * i + hl) * 8));
+#pragma unroll
+      for (int i = 0; i < D / 16; ++i) asm volatile("" ::"v"(qf[i]));  // arrived: no wait for them in the loop
+    }
+    for (int t = t0; t < t1; ++t) {
+      // The last tile's copies are repeated, unread, so that every turn waits
+      // for the same number of loads.
+      const int next = t + 1 < t1 ? tiles.at(t + 1) : tile;
+      const int first = tile * T;
+      const bool seen = first <= whi1 && (first + T > wlo0 || first < p.sinks);
+      f32x16 s[4];
+      vec pf[8];
+      wait_vmcnt<KT::LOADS>();  // this wave's part of K has landed
+      block_barrier();          // ... and everybody else's
+      if (seen) {
+        __builtin_amdgcn_s_setprio(1);
+#pragma unroll
+        for (int kb = 0; kb < 4; ++kb) s[kb] = scores32<D, F16, T>(k_lds, kb * 32, qf, l32, hl);
+        __builtin_amdgcn_s_setprio(0);
+      }
+      block_barrier();  // K has been read by all
+      kc.template issue<ROLL>(p, ks, p.k_sl, seq.nk, next, k_lds, w);
+      if (seen) {
+        if (first + T - 1 > whi0 || (first < wlo1 && first + T > p.sinks)) {
+#pragma unroll
+          for (int kb = 0; kb < 4; ++kb) mask32(s[kb], first + kb * 32, hl, klo, khi, p.sinks);
+        }
+        const float ref = follow_max<4, DCH>(s, p.scale_log2, m, l, o);
+#pragma unroll
+        for (int kb = 0; kb < 4; ++kb) weights32<F16>(s[kb], p.scale_log2, ref, pf + 2 * kb, l);
+      }
+      wait_vmcnt<KT::LOADS>();  // V has landed
+      block_barrier();
+      if (seen) {
+#pragma unroll
+        for (int kg = 0; kg < 8; ++kg)
+#pragma unroll
+          for (int dc = 0; dc < DCH; ++dc)
+            o[dc] = Half<F16>::mfma(values16<D, F16, T>(v_lds, kg * 16, dc, lane), pf[kg], o[dc]);
+      }
+      block_barrier();  // V has been read by all
+      vc.template issue<ROLL>(p, vs, p.v_sl, seq.nk, next, v_lds, w);
+      tile = next;
+    }
+    wait_vmcnt_0();  // the trailing copies have landed before the workgroup's LDS is released
+  }
+  l = xhalf_sum(l);
+  const bool dead = row.i >= seq.nq;
+  if (it.pieces > 1) {
+    const int64_t at = static_cast<int64_t>(it.slot) * 128 + w * 32 + l32;
+    if (in) store_part<D>(p.part_o + at * D, p.part_ml + at * 2, o, dead ? -INFINITY : m, dead ? 0.f : l, hl);
+    return;
+  }
+  const float inv = dead || l == 0.f ? 0.f : 1.f / l;
+  if (dead) {
+#pragma unroll
+    for (int i = 0; i < DCH; ++i) o[i] = f32x16{};
+  }
+  store_row<D, F16>(p.out + b * p.o_sb + head * p.o_sh + row.i * p.o_sl, o, inv, in, hl);
+  if (p.lse && in && hl == 0)
+    p.lse[(static_cast<int64_t>(b) * p.Hq + head) * p.Lq + row.i] = dead ? -INFINITY : lse_of(m, l);
+}
+
+// At most 32 rows (a token, or a few, of a group's heads) over many keys: a
+// wave a workgroup, tiles of 32 keys through two LDS buffers of its own that
+// the loads fill directly; no barrier, five waves a CU keep 80 KB in flight.
+// The keys are dealt over p.parts waves; reading them is all that counts.
+template <int D, bool F16, bool ROLL>
+__global__ void __launch_bounds__(64, 2) window_few_kernel(WindowParams p) {
+  constexpr int DCH = D / 32, T = 32;
+  typedef KeyTile<D, T, 1> KT;
+  typedef typename Half<F16>::vec vec;
+  __shared__ __attribute__((aligned(16))) uint16_t k0[T * D], v0[T * D], k1[T * D], v1[T * D];
+  const int bh = blockIdx.x / p.parts, piece = blockIdx.x - bh * p.parts;
+  const int lane = threadIdx.x, l32 = lane & 31, hl = lane >> 5;
+  const int b = bh / p.Hkv, g = bh - b * p.Hkv;
+  const Seq seq = seq_of(p, b);
+  const int rows = p.Lq * p.group;
+  const Tiles tiles = tiles_of<T>(p, seq, 0, seq.nq - 1);
+  const int t0 = static_cast<int64_t>(tiles.n) * piece / p.parts;
+  const int t1 = static_cast<int64_t>(tiles.n) * (piece + 1) / p.parts;
+  const bool in = l32 < rows;
+  const Row row = row_of(p, min(l32, rows - 1));
+  const int klo = first_key(p, seq, row.i), khi = last_key(p, seq, row.i);
+  const int head = g * p.group + row.g;
+  f32x16 o[DCH];
+#pragma unroll
+  for (int i = 0; i < DCH; ++i) o[i] = f32x16{};
+  float m = -INFINITY, l = 0.f;
+  if (t0 < t1) {
+    const uint16_t* const ks = p.k + b * p.k_sb + g * p.k_sh;
+    const uint16_t* const vs = p.v + b * p.v_sb + g * p.v_sh;
+    const KT kc(0, lane, false), vc(0, lane, true);
+    auto load = [&](int t, uint16_t* kb, uint16_t* vb) {
+      const int tile = tiles.at(min(t, t1 - 1));  // past the last one: that again, unread
+      kc.template issue<ROLL>(p, ks, p.k_sl, seq.nk, tile, kb, 0);
+      vc.template issue<ROLL>(p, vs, p.v_sl, seq.nk, tile, vb, 0);
+    };
+    vec qf[D / 16];
+    const uint16_t* q = p.q + b * p.q_sb + head * p.q_sh + row.i * p.q_sl;
+#pragma unroll
+    for (int i = 0; i < D / 16; ++i)
+      qf[i] = __builtin_bit_cast(vec, *reinterpret_cast<const uint4*>(q + (2 * i + hl) * 8));
+#pragma unroll
+    for (int i = 0; i < D / 16; ++i) asm volatile("" ::"v"(qf[i]));
+    load(t0, k0, v0);
+    load(t0 + 1, k1, v1);
+    auto step = [&](int t, uint16_t* kb, uint16_t* vb) {
+      wait_vmcnt<2 * KT::LOADS>();  // this tile has landed, the next may be in flight
+      const int first = tiles.at(t) * T;
+      f32x16 s = scores32<D, F16, T>(kb, 0, qf, l32, hl);
+      mask32(s, first, hl, klo, khi, p.sinks);
+      const float ref = follow_max<1, DCH>(&s, p.scale_log2, m, l, o);
+      vec pf[2];
+      weights32<F16>(s, p.scale_log2, ref, pf, l);
+#pragma unroll
+      for (int kg = 0; kg < 2; ++kg)
+#pragma unroll
+        for (int dc = 0; dc < DCH; ++dc)
+          o[dc] = Half<F16>::mfma(values16<D, F16, T>(vb, kg * 16, dc, lane), pf[kg], o[dc]);
+      wait_lgkm_0();  // the buffers have been read
+      load(t + 2, kb, vb);
+    };
+    for (int t = t0; t < t1; t += 2) {
+      step(t, k0, v0);
+      if (t + 1 >= t1) break;
+      step(t + 1, k1, v1);
+    }
+    wait_vmcnt_0();
+  }
+  l = xhalf_sum(l);
+  const bool dead = row.i >= seq.nq;
+  if (p.parts > 1) {
+    const int64_t at = static_cast<int64_t>(blockIdx.x) * rows + l32;
+    if (in) store_part<D>(p.part_o + at * D, p.part_ml + at * 2, o, dead ? -INFINITY : m, dead ? 0.f : l, hl);
+    return;
+  }
+  const float inv = dead || l == 0.f ? 0.f : 1.f / l;
+  if (dead) {
+#pragma unroll
+    for (int i = 0; i < DCH; ++i) o[i] = f32x16{};
+  }
+  store_row<D, F16>(p.out + b * p.o_sb + head * p.o_sh + row.i * p.o_sl, o, inv, in, hl);
+  if (p.lse && in && hl == 0)
+    p.lse[(static_cast<int64_t>(b) * p.Hq + head) * p.Lq + row.i] = dead ? -INFINITY : lse_of(m, l);
+}
+
+// Joins the parts of a row: O = sum 2^(m_i - M) O_i over the same sum of l_i.
+// A part without keys (l = 0) has no weight; NaN reaches its row. D / 4 lanes a
+// row.
+template <int D, bool F16, bool FEW>
+__global__ void __launch_bounds__(256) window_join_kernel(WindowParams p) {
+  constexpr int LANES = D / 4;
+  const int lane = threadIdx.x % LANES;
+  const int64_t id = static_cast<int64_t>(blockIdx.x) * (256 / LANES) + threadIdx.x / LANES;
+  const int rows = p.Lq * p.group;
+  int bh, r;
+  int64_t first, step;  // row of the first part, rows between parts
+  if (FEW) {
+    bh = static_cast<int>(id / rows);
+    r = static_cast<int>(id - static_cast<int64_t>(bh) * rows);
+    if (bh >= p.B * p.Hkv) return;
+    first = static_cast<int64_t>(bh) * p.parts * rows + r;
+    step = rows;
+  } else {
+    const int block = static_cast<int>(id >> 7), x = block & 7, i = p.whole + (block >> 3);
+    const int per = (p.blocks + p.chunks - 1) / p.chunks;
+    if (block >= p.split * 8) return;
+    const int u = i / per * 8 + x;
+    bh = u / p.chunks;
+    const int blk = p.blocks - 1 - (u % p.chunks * per + i % per);
+    r = blk * 128 + static_cast<int>(id & 127);
+    if (bh >= p.B * p.Hkv || blk < 0 || r >= rows) return;
+    first = static_cast<int64_t>(block) * p.parts * 128 + (id & 127);
+    step = 128;
+  }
+  float M = -INFINITY;
+  for (int i = 0; i < p.parts; ++i) M = fmaxf(M, p.part_ml[(first + i * step) * 2]);
+  const float ref = M == -INFINITY ? 0.f : M;
+  float l = 0.f, o[4] = {};
+  for (int i = 0; i < p.parts; ++i) {
+    const float2 ml = *reinterpret_cast<const float2*>(p.part_ml + (first + i * step) * 2);
+    const float4 v = *reinterpret_cast<const float4*>(p.part_o + (first + i * step) * D + lane * 4);
+    const float a = exp2_fast(ml.x - ref);
+    if (ml.y == 0.f) continue;  // rows of a dead or keyless part hold no O
+    l += a * ml.y;
+    o[0] += a * v.x; o[1] += a * v.y; o[2] += a * v.z; o[3] += a * v.w;
+  }
+  const float inv = l == 0.f ? 0.f : 1.f / l;
+  const int b = bh / p.Hkv, g = bh - b * p.Hkv;
+  const Row row = row_of(p, r);
+  const int head = g * p.group + row.g;
+  *reinterpret_cast<uint2*>(p.out + b * p.o_sb + head * p.o_sh + row.i * p.o_sl + lane * 4) =
+      make_uint2(pack2<F16>(o[0] * inv, o[1] * inv), pack2<F16>(o[2] * inv, o[3] * inv));
+  if (p.lse && lane == 0) p.lse[(static_cast<int64_t>(b) * p.Hq + head) * p.Lq + row.i] = lse_of(M, l);
+}
+
+// How a call is cut. Slots for two workgroups on each of 256 CUs; the blocks
+// left over behind full rounds of an XCD's 64 slots are cut into parts so that
+// the last round fills the chip too, each part at least two tiles.
+void plan(const dfs_window_args* a, WindowParams& p) {
+  constexpr int kSlots = 64;  // of an XCD
+  p.group = static_cast<int>(a->q_heads / a->kv_heads);
+  const int64_t rows = a->q_rows * p.group, heads = a->batch * a->kv_heads;
+  auto limit = [](int64_t n) { return n < 0 || n > kNoLimit ? int64_t(kNoLimit) : n; };
+  const int64_t keys_all = a->rolling ? a->sinks + limit(a->left) + a->q_rows : a->slots;  // some query may see
+  p.few = rows <= 32;
+  if (p.few) {
+    const int64_t keys = std::min(keys_all, std::min(limit(a->sinks), a->slots) + limit(a->left) + a->q_rows + limit(a->right));
+    // Five waves of 32 KB a CU; at least four tiles a wave.
+    p.parts = static_cast<int>(std::max(int64_t(1), std::min(1280 / heads, (keys + 127) / 128)));
+    p.split = 0;
+    return;
+  }
+  p.blocks = static_cast<int>((rows + 127) / 128);
+  int64_t g = heads, e = 8;
+  while (e) { const int64_t t = g % e; g = e; e = t; }
+  p.chunks = static_cast<int>(8 / g);
+  const int64_t per = (p.blocks + p.chunks - 1) / p.chunks;  // blocks of a range
+  const int64_t list = (heads * p.chunks + 7) / 8 * per;     // of an XCD
+  const int64_t near = limit(a->left) + limit(a->right) + 128 / p.group + 128;
+  const int64_t tiles = std::min((keys_all + 127) / 128,
+                                 (near + 127) / 128 + (std::min(limit(a->sinks), a->slots) + 127) / 128);
+  p.whole = static_cast<int>(list);
+  p.parts = 1;
+  p.split = 0;
+  const int64_t rest = list % kSlots;
+  if (rest == 0 || list >= 16 * kSlots || tiles < 4) return;
+  // Time of the last round in whole blocks: rounds / parts, and a part's own
+  // start and store, worth about a tile.
+  double best = 1.0;
+  for (int64_t n = 2; n <= std::min<int64_t>(tiles / 2, 32); ++n) {
+    const double cost = static_cast<double>((rest * n + kSlots - 1) / kSlots) *
+                        (1.0 / static_cast<double>(n) + 1.0 / static_cast<double>(tiles));
+    if (cost < best * 0.95) {
+      best = cost;
+      p.parts = static_cast<int>(n);
+    }
+  }
+  if (p.parts > 1) {
+    p.whole = static_cast<int>(list - rest);
+    p.split = static_cast<int>(rest);
+  }
+}
+
+int64_t part_rows(const dfs_window_args* a, const WindowParams& p) {
+  if (p.parts <= 1) return 0;
+  return p.few ? a->batch * a->kv_heads * p.parts * a->q_rows * p.group : int64_t(8) * p.split * p.parts * 128;
+}
+
+template <int D, bool F16, bool ROLL>
+void launch(const WindowParams& p, hipStream_t st) {
+  const unsigned heads = static_cast<unsigned>(p.B * p.Hkv);
+  if (p.few) {
+    window_few_kernel<D, F16, ROLL><<<heads * p.parts, 64, 0, st>>>(p);
+    const int64_t rows = static_cast<int64_t>(heads) * p.Lq * p.group;
+    if (p.parts > 1) window_join_kernel<D, F16, true><<<static_cast<unsigned>((rows * (D / 4) + 255) / 256), 256, 0, st>>>(p);
+    return;
+  }
+  window_tile_kernel<D, F16, ROLL><<<8u * (p.whole + p.split * p.parts), 256, 0, st>>>(p);
+  if (p.parts > 1)
+    window_join_kernel<D, F16, false><<<static_cast<unsigned>(p.split * 8 * 128 / (1024 / D)), 256, 0, st>>>(p);
 }
 
 }  // namespace
 }  // namespace dfs
 
-extern "C" int64_t dfs_window_attention_workspace_size(const dfs_window_args* a) { return a ? 0 : -1; }
+extern "C" int64_t dfs_window_attention_workspace_size(const dfs_window_args* a) {
+  using namespace dfs;
+  if (!a || a->batch <= 0 || a->kv_heads <= 0 || a->q_heads < a->kv_heads || a->q_rows <= 0 || a->slots <= 0) {
+    set_error("window_attention: batch, heads, q_rows and slots must be positive");
+    return -1;
+  }
+  WindowParams p{};
+  plan(a, p);
+  return part_rows(a, p) * (a->head_dim + 2) * 4;
+}
 
 extern "C" int dfs_window_attention(const dfs_window_args* a, dfs_stream_t stream) {
   using namespace dfs;
@@ -120,6 +695,12 @@ extern "C" int dfs_window_attention(const dfs_window_args* a, dfs_stream_t strea
                 "%s: a rolling cache needs sinks + left + q_rows = %lld slots, got %lld", name,
                 (long long)(a->sinks + a->left + a->q_rows), (long long)a->slots);
   }
+  constexpr int64_t kTileBytes = int64_t(1) << 31;
+  DFS_REQUIRE(a->k_row_stride * 256 < kTileBytes && a->v_row_stride * 256 < kTileBytes,
+              "%s: row strides of k and v are too large", name);
+  DFS_REQUIRE(!a->rolling || (a->k_row_stride * a->slots * 2 < 2 * kTileBytes - 65536 &&
+                              a->v_row_stride * a->slots * 2 < 2 * kTileBytes - 65536),
+              "%s: a rolling cache's rows of one head must lie within 4 GB", name);
   auto limit = [](int64_t n) { return static_cast<int>(n < 0 || n > kNoLimit ? kNoLimit : n); };
   WindowParams p{};
   p.q = static_cast<const uint16_t*>(a->q);
@@ -143,14 +724,28 @@ extern "C" int dfs_window_attention(const dfs_window_args* a, dfs_stream_t strea
   p.sinks = limit(a->sinks);
   p.rolling = a->rolling != 0;
   p.scale_log2 = static_cast<float>(a->scale * 1.4426950408889634);
-  const int64_t blocks = (a->batch * a->q_heads * a->q_rows + 3) / 4;
-  DFS_REQUIRE(blocks < (int64_t(1) << 31), "%s: too many rows", name);
+  plan(a, p);
+  const int64_t spare = part_rows(a, p), need = spare * (a->head_dim + 2) * 4;
+  DFS_REQUIRE(need == 0 || (a->workspace != nullptr && a->workspace_bytes >= need &&
+                            reinterpret_cast<uintptr_t>(a->workspace) % 16 == 0),
+              "%s: a 16-byte aligned workspace of %lld bytes is needed", name, (long long)need);
+  p.part_o = static_cast<float*>(a->workspace);
+  p.part_ml = p.part_o + spare * a->head_dim;
+  DFS_REQUIRE((p.whole + static_cast<int64_t>(p.split) * p.parts) * 8 < (int64_t(1) << 31) &&
+                  a->batch * a->kv_heads * p.parts < (int64_t(1) << 31) && a->q_rows * p.group < kNoLimit,
+              "%s: too many rows", name);
   hipStream_t st = reinterpret_cast<hipStream_t>(stream);
-  const dim3 grid(static_cast<unsigned>(blocks));
-  const bool f16 = a->dtype == DFS_DTYPE_F16;
-  if (a->head_dim == 128)
-    f16 ? window_simple_kernel<128, true><<<grid, 256, 0, st>>>(p) : window_simple_kernel<128, false><<<grid, 256, 0, st>>>(p);
-  else
-    f16 ? window_simple_kernel<64, true><<<grid, 256, 0, st>>>(p) : window_simple_kernel<64, false><<<grid, 256, 0, st>>>(p);
+  const bool f16 = a->dtype == DFS_DTYPE_F16, roll = p.rolling;
+  if (a->head_dim == 128) {
+    if (f16)
+      roll ? launch<128, true, true>(p, st) : launch<128, true, false>(p, st);
+    else
+      roll ? launch<128, false, true>(p, st) : launch<128, false, false>(p, st);
+  } else {
+    if (f16)
+      roll ? launch<64, true, true>(p, st) : launch<64, true, false>(p, st);
+    else
+      roll ? launch<64, false, true>(p, st) : launch<64, false, false>(p, st);
+  }
   return check_launch(name);
 }
