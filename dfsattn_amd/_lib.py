@@ -51,7 +51,7 @@ SIGNATURES = {
                       _p, _i32, _f32, _p, _i32, _f32, _i32, _i32, _p, _p, _i64, _p],
     "dfs_adaln_modulate": [_p, _i64, _i64, _i32, _p, _p, _p, _p, _f32, _p, _p],
     "dfs_gated_residual": [_p, _p, _p, _i64, _i64, _i32, _p, _p],
-    "dfs_linear_workspace_size": [_i64, _i64, _i64],
+    "dfs_linear_workspace_size": [_i64, _i64, _i64, _i32],
     "dfs_linear": [_p, _i64, _p, _i64, _i64, _i64, _i64, _i32, _p, _i32, _i32, _p, _p, _i64, _p, _i64, _p, _i64, _p],
     "dfs_window_attention_workspace_size": [_p],
     "dfs_window_attention": [_p, _p],

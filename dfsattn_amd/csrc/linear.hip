@@ -10,6 +10,7 @@
 // groups cover 4 consecutive n; the A operand's rows are dealt to the tiles so
 // that the groups of a wave's tiles join into 8 or 16 consecutive n and leave
 // as 16-byte stores (TileRows).
+#include <algorithm>
 #include <type_traits>
 
 #include "common.h"
@@ -17,6 +18,8 @@
 
 namespace dfs {
 namespace {
+
+constexpr uint32_t kOutside = 0x80000000u;  // byte offset past every buffer's records
 
 enum Activation { kActNone = 0, kActGeluTanh = 1, kActGelu = 2, kActSilu = 3 };
 
@@ -32,6 +35,10 @@ struct LinearParams {
   const uint16_t* residual;  // [M][N], row stride ldr, or NULL; may be out
   uint16_t* out;
   int wide;  // rows of out and residual allow 16-byte accesses at multiples of 8
+  // The channels of a tile are cut into `splits` parts of `depth` (a multiple
+  // of 128); a part's sums go to part [split][M][ceil(N / 8) * 8] in fp32.
+  int splits, depth;
+  float* part;
 };
 
 typedef float f32x2_t __attribute__((ext_vector_type(2)));
@@ -43,6 +50,9 @@ struct Half<false> {
   typedef bf16x8 vec;
   static __device__ __forceinline__ f32x16 mfma(vec a, vec b, f32x16 c) {
     return __builtin_amdgcn_mfma_f32_32x32x16_bf16(a, b, c, 0, 0, 0);
+  }
+  static __device__ __forceinline__ f32x4 mfma16(vec a, vec b, f32x4 c) {
+    return __builtin_amdgcn_mfma_f32_16x16x32_bf16(a, b, c, 0, 0, 0);
   }
   static __device__ __forceinline__ float to_f32(uint32_t bits) { return bf16_bits_to_f32(bits); }
   static __device__ __forceinline__ uint32_t from_f32(float v) { return f32_to_bf16_bits(v); }
@@ -56,6 +66,9 @@ struct Half<true> {
   typedef f16x8 vec;
   static __device__ __forceinline__ f32x16 mfma(vec a, vec b, f32x16 c) {
     return __builtin_amdgcn_mfma_f32_32x32x16_f16(a, b, c, 0, 0, 0);
+  }
+  static __device__ __forceinline__ f32x4 mfma16(vec a, vec b, f32x4 c) {
+    return __builtin_amdgcn_mfma_f32_16x16x32_f16(a, b, c, 0, 0, 0);
   }
   static __device__ __forceinline__ float to_f32(uint32_t bits) { return f16_bits_to_f32(bits); }
   static __device__ __forceinline__ uint32_t from_f32(float v) { return f32_to_f16_bits(v); }
@@ -225,6 +238,133 @@ __global__ void __launch_bounds__(256) linear_any_kernel(LinearParams p) {
   }
 }
 
+// Sums of a workgroup's 16 outputs n0.. for up to 16 rows, one set a wave in LDS
+// ([wave][lane][4]: output 4 g + r of row m lies in register r of lane
+// 16 g + m), joined in the waves' order and finished.
+template <bool F16>
+__device__ __forceinline__ void finish16(const LinearParams& p, int n0, const float* sums, int waves) {
+  const int e = threadIdx.x, n16 = e & 15, m = e >> 4, n = n0 + n16;
+  if (e >= 256 || m >= p.M || n >= p.N) return;
+  float z = 0.f;
+  for (int v = 0; v < waves; ++v) z += sums[v * 256 + ((n16 >> 2) * 16 + m) * 4 + (n16 & 3)];
+  z += bias_at(p, n);
+  with_activation(p.act, [&](auto act) { z = activate<decltype(act)::value>(z); });
+  if (p.gate) z *= p.gate[n];
+  if (p.residual) z += Half<F16>::to_f32(p.residual[m * p.ldr + n]);
+  p.out[m * p.ldo + n] = static_cast<uint16_t>(Half<F16>::from_f32(z));
+}
+
+// At most 16 rows of x: what counts is reading w once. A workgroup owns 16
+// outputs, and its waves deal the channels among themselves in blocks of 128. A
+// wave's blocks of w pass through three LDS buffers of its own that the loads
+// fill directly, 256 bytes of a row at a time; x comes from L2 as it is needed.
+// No barrier before the waves' sums meet. One row by 30,720 x 5,120: 56.8 us
+// (5.5 TB/s); with w read into registers in the products' layout, 64 bytes of a
+// row at a time, 61 to 69; four rows by 5,120 x 13,824: 23.7 and 37.1.
+template <int WAVES, bool F16>
+__global__ void __launch_bounds__(64 * WAVES) linear_few_kernel(LinearParams p) {
+  typedef typename Half<F16>::vec vec;
+  constexpr int kBlock = 16 * 128;  // elements of w in a wave's buffer
+  __shared__ __attribute__((aligned(16))) uint16_t s0[WAVES * kBlock], s1[WAVES * kBlock], s2[WAVES * kBlock];
+  __shared__ __attribute__((aligned(16))) float sums[WAVES * 256];
+  const int lane = threadIdx.x & 63, w = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  const int r16 = lane & 15, c4 = lane >> 4;
+  const int n0 = blockIdx.x * 16;
+  const auto rs = make_rsrc(p.w + n0 * p.ldw, kOutside);
+  // Load j: rows 4 j .. 4 j + 3, chunk c of row r at c ^ r (16 chunks a row).
+  uint32_t wv[4];
+#pragma unroll
+  for (int j = 0; j < 4; ++j) {
+    const int r = 4 * j + c4;
+    wv[j] = static_cast<uint32_t>(min(n0 + r, p.N - 1) - n0) * static_cast<uint32_t>(p.ldw * 2) + (r16 ^ r) * 16;
+  }
+  const uint16_t* const xr = p.x + min(r16, p.M - 1) * p.ldx;
+  const int blocks = (p.K + 127) >> 7;
+  auto load = [&](int b, uint16_t* buf) {  // past the last block: zeros, without a memory access
+    const int left = p.K - b * 128;
+#pragma unroll
+    for (int j = 0; j < 4; ++j) {
+      const bool in = (r16 ^ (4 * j + c4)) * 8 < left;
+      load_lds16(rs, buf + w * kBlock + j * 512, in ? wv[j] + b * 256 : kOutside, 0);
+    }
+  };
+  f32x4 acc = f32x4{};
+  auto step = [&](int b, const uint16_t* buf, uint16_t* next) {
+    uint4 x[4];
+#pragma unroll
+    for (int s = 0; s < 4; ++s) {
+      const int k = b * 128 + s * 32 + c4 * 8;
+      x[s] = make_uint4(0, 0, 0, 0);
+      if (r16 < p.M && k < p.K) x[s] = *reinterpret_cast<const uint4*>(xr + k);
+    }
+    wait_lgkm_0();  // the reads of `next`, a step ago, are done (zeros come at once)
+    load(b + 2 * WAVES, next);
+    const uint16_t* const row = buf + w * kBlock + r16 * 128;
+#pragma unroll
+    for (int s = 0; s < 4; ++s) {
+      const uint4 a = *reinterpret_cast<const uint4*>(row + ((s * 4 + c4) ^ r16) * 8);
+      acc = Half<F16>::mfma16(__builtin_bit_cast(vec, a), __builtin_bit_cast(vec, x[s]), acc);
+    }
+  };
+  load(w, s0);
+  load(w + WAVES, s1);
+  for (int b = w; b < blocks; b += 3 * WAVES) {
+    step(b, s0, s2);
+    step(b + WAVES, s1, s0);
+    step(b + 2 * WAVES, s2, s1);
+  }
+  wait_vmcnt_0();
+  *reinterpret_cast<f32x4*>(sums + (w * 64 + lane) * 4) = acc;
+  __syncthreads();
+  finish16<F16>(p, n0, sums, WAVES);
+}
+
+// The same for rows on no 16-byte boundary, which only loads into registers
+// take, there in the products' layout.
+template <bool F16>
+__global__ void __launch_bounds__(512) linear_few_any_kernel(LinearParams p) {
+  typedef typename Half<F16>::vec vec;
+  constexpr int WAVES = 8;
+  __shared__ __attribute__((aligned(16))) float sums[WAVES * 256];
+  const int lane = threadIdx.x & 63, w = threadIdx.x >> 6;
+  const int r16 = lane & 15, kc = (lane >> 4) * 8;
+  const int n0 = blockIdx.x * 16;
+  const uint16_t* const wr = p.w + min(n0 + r16, p.N - 1) * p.ldw;
+  const uint16_t* const xr = p.x + min(r16, p.M - 1) * p.ldx;
+  f32x4 acc = f32x4{};
+  struct Block {
+    uint4 a[4], b[4];
+  };
+  auto load = [&](int k0, Block& f) {
+#pragma unroll
+    for (int s = 0; s < 4; ++s) {
+      const int k = k0 + s * 32 + kc;
+      f.a[s] = load_row8(wr, k, p.K);
+      f.b[s] = r16 < p.M ? load_row8(xr, k, p.K) : make_uint4(0, 0, 0, 0);
+    }
+  };
+  auto multiply = [&](const Block& f) {
+#pragma unroll
+    for (int s = 0; s < 4; ++s)
+      acc = Half<F16>::mfma16(__builtin_bit_cast(vec, f.a[s]), __builtin_bit_cast(vec, f.b[s]), acc);
+  };
+  constexpr int kHop = WAVES * 128;
+  if (w * 128 < p.K) {
+    Block f, g;
+    load(w * 128, f);
+    for (int k0 = w * 128; k0 < p.K; k0 += 2 * kHop) {  // the block after is on its way
+      if (k0 + kHop < p.K) load(k0 + kHop, g);
+      multiply(f);
+      if (k0 + kHop >= p.K) break;
+      if (k0 + 2 * kHop < p.K) load(k0 + 2 * kHop, f);
+      multiply(g);
+    }
+  }
+  *reinterpret_cast<f32x4*>(sums + (w * 64 + lane) * 4) = acc;
+  __syncthreads();
+  finish16<F16>(p, n0, sums, WAVES);
+}
+
 // Tiles of BN = 32 NI WN outputs by BM = 32 MI WM rows, a workgroup of WN x WM
 // = 4 waves with NI x MI products of 32 x 32 each, 64 channels a step through
 // two LDS buffers that the loads fill directly. For operands on 16-byte rows.
@@ -240,8 +380,6 @@ __global__ void __launch_bounds__(256) linear_any_kernel(LinearParams p) {
 // step's data is waited for and, behind the barrier, its successor's loads go
 // into the buffer just read. So there is one barrier a step, the products of a
 // quarter are there on both sides of it, and a load has a whole step to land.
-constexpr uint32_t kOutside = 0x80000000u;  // byte offset past every buffer's records
-
 template <int NI, int MI, int WN, int WM, bool F16>
 struct Tile {
   static constexpr int BN = 32 * NI * WN, BM = 32 * MI * WM;
@@ -263,7 +401,7 @@ __device__ __forceinline__ void tile_of(int id, int mt, int nt, int& tm, int& tn
 }
 
 template <int NI, int MI, int WN, int WM, bool F16>
-__global__ void __launch_bounds__(256, NI * MI == 16 ? 1 : 2) linear_tile_kernel(LinearParams p) {
+__global__ void __launch_bounds__(256, 2) linear_tile_kernel(LinearParams p) {
   typedef Tile<NI, MI, WN, WM, F16> T;
   typedef typename T::vec vec;
   constexpr int JW = T::BN / 32, JX = T::BM / 32;  // loads of 1 KB a wave and step
@@ -273,11 +411,14 @@ __global__ void __launch_bounds__(256, NI * MI == 16 ? 1 : 2) linear_tile_kernel
   __shared__ __attribute__((aligned(16))) uint16_t x1[T::BM * 64];
   const int lane = threadIdx.x & 63, w = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const int l32 = lane & 31, hl = lane >> 5;
+  const int mt = (p.M + T::BM - 1) / T::BM, nt = (p.N + T::BN - 1) / T::BN;
+  const int split = p.splits > 1 ? blockIdx.x / (mt * nt) : 0, from = split * p.depth;
   int tm, tn;
-  tile_of(blockIdx.x, (p.M + T::BM - 1) / T::BM, (p.N + T::BN - 1) / T::BN, tm, tn);
+  tile_of(blockIdx.x - split * mt * nt, mt, nt, tm, tn);
   const int n0 = tn * T::BN, m0 = tm * T::BM;
-  const auto wrs = make_rsrc(p.w + static_cast<int64_t>(n0) * p.ldw, kOutside);
-  const auto xrs = make_rsrc(p.x + static_cast<int64_t>(m0) * p.ldx, kOutside);
+  const int K = p.splits > 1 ? min(p.K - from, p.depth) : p.K;
+  const auto wrs = make_rsrc(p.w + static_cast<int64_t>(n0) * p.ldw + from, kOutside);
+  const auto xrs = make_rsrc(p.x + static_cast<int64_t>(m0) * p.ldx + from, kOutside);
   // Byte offsets of this lane's chunks in step 0; rows past the matrix repeat
   // its last one.
   uint32_t wv[JW], xv[JX];
@@ -294,9 +435,9 @@ __global__ void __launch_bounds__(256, NI * MI == 16 ? 1 : 2) linear_tile_kernel
     xv[j] = static_cast<uint32_t>(min(m0 + r, p.M - 1) - m0) * static_cast<uint32_t>(p.ldx * 2) +
             (c8 ^ T::swz_x(r)) * 16;
   }
-  const int steps = (p.K + 127) >> 7 << 1;  // an even number: the last may be all zeros
+  const int steps = (K + 127) >> 7 << 1;  // an even number: the last may be all zeros
   auto issue = [&](int t, uint16_t* wb, uint16_t* xb) {
-    const int left = p.K - t * 64;
+    const int left = K - t * 64;
     if (left < 64) {  // the last steps: chunks past K come as zeros
 #pragma unroll
       for (int j = 0; j < JX; ++j)
@@ -380,6 +521,22 @@ __global__ void __launch_bounds__(256, NI * MI == 16 ? 1 : 2) linear_tile_kernel
   }
   wait_vmcnt_0();  // the trailing loads have landed before the workgroup's LDS is released
   const int nb = n0 + wn * 32 * NI + hl * 4 * NI, mb = m0 + wm * 32 * MI + l32;
+  if (p.splits > 1) {  // four outputs a register group, n = nb + ...; 16-byte stores
+    const int64_t ld = (p.N + 7) & ~7;
+    float* const part = p.part + static_cast<int64_t>(split) * p.M * ld;
+#pragma unroll
+    for (int j = 0; j < MI; ++j)
+#pragma unroll
+      for (int i = 0; i < NI; ++i)
+#pragma unroll
+        for (int g = 0; g < 4; ++g) {
+          const int n = nb + g * 8 * NI + i * 4, m = mb + j * 32;
+          const f32x16& z = acc[i][j];
+          if (m < p.M && n < ld)
+            *reinterpret_cast<float4*>(part + m * ld + n) = make_float4(z[g * 4], z[g * 4 + 1], z[g * 4 + 2], z[g * 4 + 3]);
+        }
+    return;
+  }
   with_activation(p.act, [&](auto act) {
     if constexpr (NI == 1) {
 #pragma unroll
@@ -628,26 +785,128 @@ __global__ void __launch_bounds__(256, 1) linear_big_kernel(LinearParams p) {
   }
 }
 
+// Joins the parts of a cut product, in their order, and finishes: a thread has
+// eight outputs.
+template <bool F16>
+__global__ void __launch_bounds__(256) linear_join_kernel(LinearParams p) {
+  const int chunks = (p.N + 7) / 8;
+  const int64_t id = static_cast<int64_t>(blockIdx.x) * 256 + threadIdx.x;
+  const int m = static_cast<int>(id / chunks), n = static_cast<int>(id - static_cast<int64_t>(m) * chunks) * 8;
+  if (m >= p.M) return;
+  const int64_t ld = chunks * 8;
+  const float* src = p.part + m * ld + n;
+  float z[8] = {};
+  for (int i = 0; i < p.splits; ++i, src += p.M * ld) {
+    const float4 a = *reinterpret_cast<const float4*>(src), b = *reinterpret_cast<const float4*>(src + 4);
+    z[0] += a.x; z[1] += a.y; z[2] += a.z; z[3] += a.w;
+    z[4] += b.x; z[5] += b.y; z[6] += b.z; z[7] += b.w;
+  }
+  float bias[8], gate[8];
+  load_columns8(p, n, bias, gate);
+  with_activation(p.act, [&](auto act) { finish8<F16, decltype(act)::value>(p, m, n, z, bias, gate); });
+}
+
 template <int NI, int MI, int WN, int WM>
 void launch_tile(const LinearParams& p, bool f16, hipStream_t st) {
   const int64_t mt = (p.M + 32 * MI * WM - 1) / (32 * MI * WM), nt = (p.N + 32 * NI * WN - 1) / (32 * NI * WN);
-  const dim3 grid(static_cast<unsigned>(mt * nt));
+  const dim3 grid(static_cast<unsigned>(mt * nt * p.splits));
   if (f16)
     linear_tile_kernel<NI, MI, WN, WM, true><<<grid, 256, 0, st>>>(p);
   else
     linear_tile_kernel<NI, MI, WN, WM, false><<<grid, 256, 0, st>>>(p);
+  if (p.splits > 1) {
+    const int64_t threads = static_cast<int64_t>(p.M) * ((p.N + 7) / 8);
+    const dim3 join(static_cast<unsigned>((threads + 255) / 256));
+    if (f16)
+      linear_join_kernel<true><<<join, 256, 0, st>>>(p);
+    else
+      linear_join_kernel<false><<<join, 256, 0, st>>>(p);
+  }
+}
+
+void launch_few(const LinearParams& p, bool f16, hipStream_t st) {
+  const int groups = (p.N + 15) / 16;
+  if (groups >= 256)
+    f16 ? linear_few_kernel<4, true><<<groups, 256, 0, st>>>(p) : linear_few_kernel<4, false><<<groups, 256, 0, st>>>(p);
+  else  // more waves a workgroup where there are few
+    f16 ? linear_few_kernel<8, true><<<groups, 512, 0, st>>>(p) : linear_few_kernel<8, false><<<groups, 512, 0, st>>>(p);
+}
+
+// Rows of K elements, any stride, into rows of `wide` >= K elements on 16-byte
+// boundaries, zeros behind the K: eight elements a thread.
+__global__ void __launch_bounds__(256) pad_rows_kernel(const uint16_t* src, int64_t ld, int64_t rows, int K, int wide,
+                                                       uint16_t* dst) {
+  const int64_t id = static_cast<int64_t>(blockIdx.x) * 256 + threadIdx.x;
+  const int chunks = wide / 8;
+  const int64_t r = id / chunks;
+  const int c = static_cast<int>(id - r * chunks);
+  if (r < rows) *reinterpret_cast<uint4*>(dst + id * 8) = load_row8(src + r * ld, c * 8, K);
+}
+
+// How a product is cut: its form and, for the tiles, the parts of the channels.
+enum Form { kFew, kFewAny, kTileAny, kTile64, kTile128, kTile256 };
+struct Cut {
+  Form form;
+  int splits, depth;
+  bool pad;  // operands are laid out on 16-byte rows first
+};
+Cut cut_of(int64_t rows, int64_t n, int64_t k, bool chunks) {
+  // Rows on no 16-byte boundary: as they are where little is computed with
+  // what is read (padding took a row's time again and more), laid out anew
+  // otherwise.
+  if (!chunks && rows <= 16) return Cut{kFewAny, 1, 0, false};
+  if (!chunks && rows * n * k < (int64_t(1) << 30)) return Cut{kTileAny, 1, 0, false};
+  if (rows <= 8) return Cut{kFew, 1, 0, !chunks};
+  // The tiles and parts with the least time by what each took alone and in
+  // company, a step of 64 channels of a workgroup in us on one CU (CUs that get
+  // one workgroup more than others run it half hidden), and by writing and
+  // joining the parts' sums at 3 TB/s behind 5 us. Measured, us: 64 rows by
+  // 5,120 x 5,120 39.8 in one part, 18.8 in eight; 128 rows 41.0 and 22.6 in
+  // four; 512 by 5,120 x 4,096 37.8 with 64 x 64, 44.6 with 128 x 128, 70 with
+  // 256 x 256; 1,000 by 5,120 x 5,120 101, 73.6, 98.7; 1,560 140, 134, 102.7.
+  struct {
+    Form form;
+    int tile, most;  // most: parts
+    double alone, shared;
+  } const kinds[3] = {{kTile64, 64, 8, 0.49, 0.235}, {kTile128, 128, 4, 0.72, 0.59}, {kTile256, 256, 1, 1.40, 1.40}};
+  Cut best{kTile64, 1, 0, !chunks};
+  double least = 1e30;
+  for (const auto& f : kinds)
+    for (int s = 1; s <= f.most; s *= 2) {
+      const int64_t depth = ((k + s - 1) / s + 127) / 128 * 128, parts = (k + depth - 1) / depth;
+      if (s > 1 && (depth < 256 || parts < 2)) break;
+      const int64_t groups = ((rows + f.tile - 1) / f.tile) * ((n + f.tile - 1) / f.tile) * parts;
+      const double each = 0.5 * (static_cast<double>((groups + 255) / 256) + static_cast<double>(groups) / 256.0);
+      double us = static_cast<double>(depth / 64) * std::max(f.alone, f.shared * each);
+      if (parts > 1) us += 5.0 + 8e-6 / 3.0 * static_cast<double>(parts * rows * n);
+      if (us < least) {
+        least = us;
+        best.form = f.form;
+        best.splits = static_cast<int>(parts);
+        best.depth = static_cast<int>(depth);
+      }
+    }
+  return best;
+}
+
+int64_t padded(int64_t k) { return (k + 7) / 8 * 8; }
+int64_t part_bytes(const Cut& c, int64_t rows, int64_t n) {
+  return c.splits > 1 ? c.splits * rows * padded(n) * 4 : 0;  // a multiple of 32
+}
+int64_t workspace_bytes_of(const Cut& c, int64_t rows, int64_t n, int64_t k) {
+  return part_bytes(c, rows, n) + (c.pad ? (rows + n) * padded(k) * 2 : 0);
 }
 
 }  // namespace
 }  // namespace dfs
 
-extern "C" int64_t dfs_linear_workspace_size(int64_t rows, int64_t n, int64_t k) {
+extern "C" int64_t dfs_linear_workspace_size(int64_t rows, int64_t n, int64_t k, int aligned) {
   using namespace dfs;
   if (rows <= 0 || n <= 0 || k <= 0) {
     set_error("linear: rows=%lld n=%lld k=%lld must be positive", (long long)rows, (long long)n, (long long)k);
     return -1;
   }
-  return 0;
+  return workspace_bytes_of(cut_of(rows, n, k, aligned != 0), rows, n, k);
 }
 
 extern "C" int dfs_linear(const void* x, int64_t x_stride, const void* w, int64_t w_stride, int64_t rows, int64_t n,
@@ -673,9 +932,13 @@ extern "C" int dfs_linear(const void* x, int64_t x_stride, const void* w, int64_
   DFS_REQUIRE(addr(x) % 2 == 0 && addr(w) % 2 == 0 && addr(out) % 2 == 0 && addr(residual) % 2 == 0 &&
                   addr(gate) % 4 == 0 && addr(bias) % (bias_dtype == DFS_DTYPE_F32 ? 4 : 2) == 0,
               "%s: operands must be aligned to their elements", name);
-  const int64_t need = dfs_linear_workspace_size(rows, n, k);
-  DFS_REQUIRE(need == 0 || (workspace != nullptr && workspace_bytes >= need), "%s: workspace of %lld bytes needed",
-              name, (long long)need);
+  const bool chunks = k % 8 == 0 && x_stride % 8 == 0 && w_stride % 8 == 0 && addr(x) % 16 == 0 && addr(w) % 16 == 0 &&
+                      x_stride < (1 << 21) && w_stride < (1 << 21);
+  const Cut cut = cut_of(rows, n, k, chunks);
+  const int64_t need = workspace_bytes_of(cut, rows, n, k);
+  DFS_REQUIRE(need == 0 || (workspace != nullptr && workspace_bytes >= need && addr(workspace) % 16 == 0),
+              "%s: a 16-byte aligned workspace of %lld bytes is needed", name, (long long)need);
+  DFS_REQUIRE(!cut.pad || k < (1 << 21), "%s: k=%lld must be below 2^21 for operands off 16-byte rows", name, (long long)k);
   LinearParams p{};
   p.x = static_cast<const uint16_t*>(x);
   p.w = static_cast<const uint16_t*>(w);
@@ -694,32 +957,54 @@ extern "C" int dfs_linear(const void* x, int64_t x_stride, const void* w, int64_
   p.out = static_cast<uint16_t*>(out);
   p.wide = o_stride % 8 == 0 && addr(out) % 16 == 0 && (!residual || (r_stride % 8 == 0 && addr(residual) % 16 == 0));
   hipStream_t st = reinterpret_cast<hipStream_t>(stream);
-  const bool chunks = k % 8 == 0 && x_stride % 8 == 0 && w_stride % 8 == 0 && addr(x) % 16 == 0 && addr(w) % 16 == 0 &&
-                      x_stride < (1 << 21) && w_stride < (1 << 21);
-  if (chunks) {
-    const int64_t big = ((rows + 255) / 256) * ((n + 255) / 256);
-    const int64_t mid = ((rows + 127) / 128) * ((n + 127) / 128);
-    const bool f16 = dtype == DFS_DTYPE_F16;
-    if (big >= 256) {
-      const dim3 grid(static_cast<unsigned>(big));
+  p.splits = cut.splits;
+  p.depth = cut.depth;
+  p.part = static_cast<float*>(workspace);
+  const bool f16 = dtype == DFS_DTYPE_F16;
+  if (cut.pad) {
+    uint16_t* const wide = reinterpret_cast<uint16_t*>(static_cast<char*>(workspace) + part_bytes(cut, rows, n));
+    const int64_t kp = padded(k);
+    auto lay = [&](const uint16_t* src, int64_t ld, int64_t count, uint16_t* dst) {
+      const unsigned grid = static_cast<unsigned>((count * kp / 8 + 255) / 256);
+      pad_rows_kernel<<<grid, 256, 0, st>>>(src, ld, count, static_cast<int>(k), static_cast<int>(kp), dst);
+    };
+    lay(p.x, p.ldx, rows, wide);
+    lay(p.w, p.ldw, n, wide + rows * kp);
+    p.x = wide;
+    p.w = wide + rows * kp;
+    p.ldx = p.ldw = kp;
+    p.K = static_cast<int>(kp);
+  }
+  switch (cut.form) {
+    case kFew:
+      launch_few(p, f16, st);
+      break;
+    case kFewAny: {
+      const unsigned grid = static_cast<unsigned>((n + 15) / 16);
+      f16 ? linear_few_any_kernel<true><<<grid, 512, 0, st>>>(p) : linear_few_any_kernel<false><<<grid, 512, 0, st>>>(p);
+      break;
+    }
+    case kTileAny: {
+      const dim3 grid(static_cast<unsigned>((n + 63) / 64), static_cast<unsigned>((rows + 63) / 64));
+      f16 ? linear_any_kernel<true><<<grid, 256, 0, st>>>(p) : linear_any_kernel<false><<<grid, 256, 0, st>>>(p);
+      break;
+    }
+    case kTile64:
+      launch_tile<1, 1, 2, 2>(p, f16, st);
+      break;
+    case kTile128:
+      launch_tile<2, 2, 2, 2>(p, f16, st);
+      break;
+    case kTile256: {
+      const dim3 grid(static_cast<unsigned>(((rows + 255) / 256) * ((n + 255) / 256)));
       with_activation(p.act, [&](auto act) {
         if (f16)
           linear_big_kernel<true, decltype(act)::value><<<grid, 256, 0, st>>>(p);
         else
           linear_big_kernel<false, decltype(act)::value><<<grid, 256, 0, st>>>(p);
       });
-    } else if (mid >= 256)
-      launch_tile<2, 2, 2, 2>(p, f16, st);
-    else
-      launch_tile<1, 1, 2, 2>(p, f16, st);
-    return check_launch(name);
+      break;
+    }
   }
-  const int64_t mt = (rows + 63) / 64, nt = (n + 63) / 64;
-  DFS_REQUIRE(mt < 65536, "%s: too many rows", name);
-  const dim3 grid(static_cast<unsigned>(nt), static_cast<unsigned>(mt));
-  if (dtype == DFS_DTYPE_F16)
-    linear_any_kernel<true><<<grid, 256, 0, st>>>(p);
-  else
-    linear_any_kernel<false><<<grid, 256, 0, st>>>(p);
   return check_launch(name);
 }

@@ -767,8 +767,8 @@ def _matrix(t: torch.Tensor) -> Tuple[torch.Tensor, int]:
 
 
 @functools.lru_cache(maxsize=1024)
-def _linear_workspace(rows: int, n: int, k: int) -> int:
-    return int(_lib.lib().dfs_linear_workspace_size(rows, n, k))
+def _linear_workspace(rows: int, n: int, k: int, aligned: bool) -> int:
+    return int(_lib.lib().dfs_linear_workspace_size(rows, n, k, int(aligned)))
 
 
 def linear(x: torch.Tensor, weight: torch.Tensor, bias: Optional[torch.Tensor] = None,
@@ -815,7 +815,8 @@ def linear(x: torch.Tensor, weight: torch.Tensor, bias: Optional[torch.Tensor] =
     w2, ldw = _matrix(weight)
     r2, ldr = _matrix(residual) if residual is not None else (None, 0)
     rows = x2.shape[0]
-    ws_bytes = _linear_workspace(rows, n, k)
+    aligned = (k | ldx | ldw) % 8 == 0 and (x2.data_ptr() | w2.data_ptr()) % 16 == 0 and max(ldx, ldw) < 1 << 21
+    ws_bytes = _linear_workspace(rows, n, k, aligned)
     ws = torch.empty(ws_bytes, dtype=torch.uint8, device=x.device) if ws_bytes else None
     _call_on(x, "dfs_linear", _ptr(x2), ldx, _ptr(w2), ldw, rows, n, k, DTYPE_CODE[x.dtype], _ptr(bias), b_code,
              ACTIVATION_CODE[activation], _ptr(gate), _ptr(r2), ldr, _ptr(out), n, _ptr(ws), ws_bytes)
