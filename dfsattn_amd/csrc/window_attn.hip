@@ -206,6 +206,20 @@ __device__ __forceinline__ typename Half<F16>::vec values16(const uint16_t* vals
   return __builtin_bit_cast(typename Half<F16>::vec, v);
 }
 
+// Order of an MFMA phase of N products with R LDS reads each: the reads run
+// four products ahead.
+template <int N, int R>
+__device__ __forceinline__ void pin_read_ahead() {
+  constexpr int kMfma = 0x008, kDsRead = 0x100, kAhead = 4;
+  __builtin_amdgcn_sched_group_barrier(kDsRead, kAhead * R, 0);
+#pragma unroll
+  for (int i = 0; i < N - kAhead; ++i) {
+    __builtin_amdgcn_sched_group_barrier(kMfma, 1, 0);
+    __builtin_amdgcn_sched_group_barrier(kDsRead, R, 0);
+  }
+  __builtin_amdgcn_sched_group_barrier(kMfma, kAhead, 0);
+}
+
 // Running maximum, in log2 units, of the scores s[0..N) times c; O and l follow
 // it when some row's maximum has grown by more than 2^kSlack (P then stays
 // below 2^kSlack, which costs neither its relative precision nor fp32's range,
@@ -404,6 +418,7 @@ __global__ void __launch_bounds__(256, 2) window_tile_kernel(WindowParams p) {
         __builtin_amdgcn_s_setprio(1);
 #pragma unroll
         for (int kb = 0; kb < 4; ++kb) s[kb] = scores32<D, F16, T>(k_lds, kb * 32, qf, l32, hl);
+        pin_read_ahead<4 * (D / 16), 1>();
         __builtin_amdgcn_s_setprio(0);
       }
       block_barrier();  // K has been read by all
@@ -425,6 +440,7 @@ __global__ void __launch_bounds__(256, 2) window_tile_kernel(WindowParams p) {
 #pragma unroll
           for (int dc = 0; dc < DCH; ++dc)
             o[dc] = Half<F16>::mfma(values16<D, F16, T>(v_lds, kg * 16, dc, lane), pf[kg], o[dc]);
+        pin_read_ahead<8 * DCH, 2>();
       }
       block_barrier();  // V has been read by all
       vc.template issue<ROLL>(p, vs, p.v_sl, seq.nk, next, v_lds, w);
