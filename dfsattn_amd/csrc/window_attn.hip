@@ -174,19 +174,22 @@ struct KeyTile {
   }
 };
 
-// S^T of 32 keys (LDS rows k0..) and the wave's 32 queries.
+// S^T of T keys (LDS rows) and the wave's 32 queries, 32 keys a product; the
+// products of different keys alternate, so that none waits for the one before.
 template <int D, bool F16, int T>
-__device__ __forceinline__ f32x16 scores32(const uint16_t* keys, int k0, const typename Half<F16>::vec* q, int l32,
-                                           int hl) {
+__device__ __forceinline__ void scores(const uint16_t* keys, const typename Half<F16>::vec* q, int l32, int hl,
+                                       f32x16* s) {
   typedef KeyTile<D, T, 1> KT;
-  f32x16 s = f32x16{};
 #pragma unroll
-  for (int i = 0; i < D / 16; ++i) {
-    const uint4 a =
-        *reinterpret_cast<const uint4*>(keys + (k0 + l32) * D + ((2 * i + hl) ^ KT::swz_k(l32)) * 8);
-    s = Half<F16>::mfma(__builtin_bit_cast(typename Half<F16>::vec, a), q[i], s);
-  }
-  return s;
+  for (int k = 0; k < T / 32; ++k) s[k] = f32x16{};
+#pragma unroll
+  for (int i = 0; i < D / 16; ++i)
+#pragma unroll
+    for (int k = 0; k < T / 32; ++k) {
+      const uint4 a =
+          *reinterpret_cast<const uint4*>(keys + (k * 32 + l32) * D + ((2 * i + hl) ^ KT::swz_k(l32)) * 8);
+      s[k] = Half<F16>::mfma(__builtin_bit_cast(typename Half<F16>::vec, a), q[i], s[k]);
+    }
 }
 
 // V^T operand of 16 keys (LDS rows k0..) and channels dc * 32..: two
@@ -267,7 +270,8 @@ __device__ __forceinline__ void mask32(f32x16& s, int first, int hl, int klo, in
 #pragma unroll
   for (int r = 0; r < 16; ++r) {
     const int key = first + (r >> 2) * 8 + hl * 4 + (r & 3);
-    if (key > khi || (key < klo && key >= sinks)) s[r] = -INFINITY;
+    const bool hidden = (key > khi) | ((key < klo) & (key >= sinks));  // no branches
+    s[r] = hidden ? -INFINITY : s[r];
   }
 }
 
@@ -416,8 +420,7 @@ __global__ void __launch_bounds__(256, 2) window_tile_kernel(WindowParams p) {
       block_barrier();          // ... and everybody else's
       if (seen) {
         __builtin_amdgcn_s_setprio(1);
-#pragma unroll
-        for (int kb = 0; kb < 4; ++kb) s[kb] = scores32<D, F16, T>(k_lds, kb * 32, qf, l32, hl);
+        scores<D, F16, T>(k_lds, qf, l32, hl, s);
         pin_read_ahead<4 * (D / 16), 1>();
         __builtin_amdgcn_s_setprio(0);
       }
@@ -512,7 +515,8 @@ __global__ void __launch_bounds__(64, 2) window_few_kernel(WindowParams p) {
     auto step = [&](int t, uint16_t* kb, uint16_t* vb) {
       wait_vmcnt<2 * KT::LOADS>();  // this tile has landed, the next may be in flight
       const int first = tiles.at(t) * T;
-      f32x16 s = scores32<D, F16, T>(kb, 0, qf, l32, hl);
+      f32x16 s;
+      scores<D, F16, T>(kb, qf, l32, hl, &s);
       mask32(s, first, hl, klo, khi, p.sinks);
       const float ref = follow_max<1, DCH>(&s, p.scale_log2, m, l, o);
       vec pf[2];
