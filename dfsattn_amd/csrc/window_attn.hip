@@ -209,6 +209,47 @@ __device__ __forceinline__ typename Half<F16>::vec values16(const uint16_t* vals
   return __builtin_bit_cast(typename Half<F16>::vec, v);
 }
 
+// The V^T operands of 32 keys at once: the reads of values16 and their wait in
+// one block. The builtin's reads would have the compiler wait for every load
+// into LDS, the next tile's among them.
+template <int D, bool F16>
+__device__ __forceinline__ void values32(const uint16_t* vals, int lane, typename Half<F16>::vec (&v)[2][D / 32]) {
+  typedef __attribute__((address_space(3))) const uint16_t lds_u16;
+  const int i = lane & 15, key = (lane >> 5) * 4 + (i >> 2), low = ((lane >> 4) & 1) * 2 + ((i >> 1) & 1);
+  const int sw = KeyTile<D, 32, 1>::swz_v(key);
+  uint64_t r[D / 32][4];  // keys 0, 8, 16, 24 on
+#pragma unroll
+  for (int dc = 0; dc < D / 32; dc += 2) {
+    const uint32_t a = static_cast<uint32_t>(
+        reinterpret_cast<uintptr_t>((lds_u16*)(vals + key * D + ((dc * 4 + low) ^ sw) * 8 + (i & 1) * 4)));
+    const uint32_t b = static_cast<uint32_t>(
+        reinterpret_cast<uintptr_t>((lds_u16*)(vals + key * D + (((dc + 1) * 4 + low) ^ sw) * 8 + (i & 1) * 4)));
+    asm volatile(
+        "ds_read_b64_tr_b16 %0, %8\n\t"
+        "ds_read_b64_tr_b16 %1, %8 offset:%10\n\t"
+        "ds_read_b64_tr_b16 %2, %8 offset:%11\n\t"
+        "ds_read_b64_tr_b16 %3, %8 offset:%12\n\t"
+        "ds_read_b64_tr_b16 %4, %9\n\t"
+        "ds_read_b64_tr_b16 %5, %9 offset:%10\n\t"
+        "ds_read_b64_tr_b16 %6, %9 offset:%11\n\t"
+        "ds_read_b64_tr_b16 %7, %9 offset:%12\n\t"
+        "s_waitcnt lgkmcnt(0)"
+        : "=&v"(r[dc][0]), "=&v"(r[dc][1]), "=&v"(r[dc][2]), "=&v"(r[dc][3]), "=&v"(r[dc + 1][0]),
+          "=&v"(r[dc + 1][1]), "=&v"(r[dc + 1][2]), "=&v"(r[dc + 1][3])
+        : "v"(a), "v"(b), "n"(16 * D), "n"(32 * D), "n"(48 * D)
+        : "memory");
+  }
+#pragma unroll
+  for (int kg = 0; kg < 2; ++kg)
+#pragma unroll
+    for (int dc = 0; dc < D / 32; ++dc) {
+      const uint64_t lo = r[dc][2 * kg], hi = r[dc][2 * kg + 1];
+      v[kg][dc] = __builtin_bit_cast(typename Half<F16>::vec,
+                                     make_uint4(static_cast<uint32_t>(lo), static_cast<uint32_t>(lo >> 32),
+                                                static_cast<uint32_t>(hi), static_cast<uint32_t>(hi >> 32)));
+    }
+}
+
 // Order of an MFMA phase of N products with R LDS reads each: the reads run
 // four products ahead.
 template <int N, int R>
@@ -521,11 +562,12 @@ __global__ void __launch_bounds__(64, 2) window_few_kernel(WindowParams p) {
       const float ref = follow_max<1, DCH>(&s, p.scale_log2, m, l, o);
       vec pf[2];
       weights32<F16>(s, p.scale_log2, ref, pf, l);
+      vec vf[2][DCH];
+      values32<D, F16>(vb, lane, vf);
 #pragma unroll
       for (int kg = 0; kg < 2; ++kg)
 #pragma unroll
-        for (int dc = 0; dc < DCH; ++dc)
-          o[dc] = Half<F16>::mfma(values16<D, F16, T>(vb, kg * 16, dc, lane), pf[kg], o[dc]);
+        for (int dc = 0; dc < DCH; ++dc) o[dc] = Half<F16>::mfma(vf[kg][dc], pf[kg], o[dc]);
       wait_lgkm_0();  // the buffers have been read
       load(t + 2, kb, vb);
     };
