@@ -27,7 +27,7 @@ struct CacheParams {
   const float *cos_t, *sin_t;  // [table_rows][D / 2] or NULL
   int64_t table_rows;
   const int32_t *lens, *new_lens;
-  int B, T, D, S, sinks, rolling;
+  int B, T, log2d, S, sinks, rolling;  // heads of 2^log2d channels
 };
 
 template <bool F16>
@@ -53,64 +53,80 @@ __device__ __forceinline__ void load_weight8(const void* w, int dtype, int e, fl
     out[i] = dtype == DFS_DTYPE_BF16 ? bf16_bits_to_f32(u16_at(v, i)) : f16_bits_to_f32(u16_at(v, i));
 }
 
-// One wave per token and tensor: the row of H * D channels in registers (16
-// bytes a lane and step of 512 channels; D divides 512, so a lane's channels
-// lie at the same place of every head and one slice of the table row serves
-// them all).
+template <int CTRL>
+__device__ __forceinline__ float dpp_plus(float v) {
+  return v + __int_as_float(__builtin_amdgcn_update_dpp(0, __float_as_int(v), CTRL, 0xF, 0xF, true));
+}
+// Sum over aligned groups of `lanes` lanes (2 to 64), the same bits in each of
+// them: register moves, every step adds a value and its mirror.
+__device__ __forceinline__ float group_sum(float v, int lanes) {
+  v = dpp_plus<0xB1>(v);                   // quad_perm [1, 0, 3, 2]
+  if (lanes >= 4) v = dpp_plus<0x4E>(v);   // quad_perm [2, 3, 0, 1]
+  if (lanes >= 8) v = dpp_plus<0x141>(v);  // row_half_mirror
+  if (lanes >= 16) v = dpp_plus<0x140>(v);  // row_mirror
+  if (lanes >= 32) {
+    const auto a = __builtin_amdgcn_permlane16_swap(__float_as_uint(v), __float_as_uint(v), false, false);
+    v = __uint_as_float(a[0]) + __uint_as_float(a[1]);
+  }
+  if (lanes >= 64) {
+    const auto b = __builtin_amdgcn_permlane32_swap(__float_as_uint(v), __float_as_uint(v), false, false);
+    v = __uint_as_float(b[0]) + __uint_as_float(b[1]);
+  }
+  return v;
+}
+
+// One wave per token and tensor (grid y): the row of H * D channels in
+// registers (16 bytes a lane and step of 512 channels; D divides 512, so a
+// lane's channels lie at the same place of every head and one slice of the
+// table row serves them all). Everything that does not hang on the sequence's
+// length is loaded while that is on its way.
 template <int NCH, bool F16>
 __global__ void __launch_bounds__(256) qkv_cache_kernel(CacheParams p) {
-  const int lane = threadIdx.x & 63;
-  const int64_t item = static_cast<int64_t>(blockIdx.x) * 4 + (threadIdx.x >> 6);
-  const int n = static_cast<int>(item % 3);
-  const int64_t row = item / 3;
-  if (row >= static_cast<int64_t>(p.B) * p.T) return;
-  const int b = static_cast<int>(row / p.T), t = static_cast<int>(row - static_cast<int64_t>(b) * p.T);
-  const bool live = !p.new_lens || t < p.new_lens[b];
-  const int64_t pos = static_cast<int64_t>(p.lens[b]) + t;
-  const int C = p.heads[n] * p.D;
-  const int d = lane * 8 & (p.D - 1);
-  int64_t dst_row = t;
-  if (n > 0) {
-    dst_row = pos;
-    if (p.rolling && pos >= p.sinks) dst_row = p.sinks + (pos - p.sinks) % (p.S - p.sinks);
-    if (!live || pos < 0 || dst_row >= p.S) return;  // a token without a slot is not kept
-  }
-  uint16_t* const dst = p.out[n] + b * p.o_sb[n] + dst_row * p.o_st[n];
-  const uint16_t* const src = p.x[n] + b * p.x_sb[n] + t * p.x_st[n];
-  if (!live) {  // q rows behind the sequence are zero
-#pragma unroll
-    for (int j = 0; j < NCH; ++j) {
-      const int e = j * 512 + lane * 8;
-      if (e < C) *reinterpret_cast<uint4*>(dst + e / p.D * p.o_sh[n] + d) = make_uint4(0, 0, 0, 0);
-    }
-    return;
-  }
+  const int lane = threadIdx.x & 63, n = blockIdx.y;
+  const unsigned row = __builtin_amdgcn_readfirstlane(blockIdx.x * 4 + (threadIdx.x >> 6));
+  if (row >= static_cast<unsigned>(p.B) * static_cast<unsigned>(p.T)) return;
+  const int b = static_cast<int>(row / static_cast<unsigned>(p.T)), t = static_cast<int>(row) - b * p.T;
+  const int len = p.lens[b], live = p.new_lens ? p.new_lens[b] : p.T;
+  const int C = p.heads[n] << p.log2d;
+  const int d = lane * 8 & ((1 << p.log2d) - 1);
+  const uint16_t* const src = p.x[n] + b * p.x_sb[n] + t * p.x_st[n] + d;
+  const int64_t x_sh = p.x_sh[n], o_sh = p.o_sh[n];
   uint4 v[NCH];
 #pragma unroll
   for (int j = 0; j < NCH; ++j) {
     const int e = j * 512 + lane * 8;
     v[j] = make_uint4(0, 0, 0, 0);
-    if (e < C) v[j] = *reinterpret_cast<const uint4*>(src + e / p.D * p.x_sh[n] + d);
+    if (e < C) v[j] = *reinterpret_cast<const uint4*>(src + (e >> p.log2d) * x_sh);
   }
-  if (n == 2) {
+  const int64_t pos = static_cast<int64_t>(len) + t;
+  int64_t dst_row = t;
+  if (n > 0) {
+    dst_row = pos;
+    if (p.rolling && pos >= p.sinks)
+      dst_row = p.sinks + static_cast<uint32_t>(pos - p.sinks) % static_cast<uint32_t>(p.S - p.sinks);
+    if (t >= live || pos < 0 || dst_row >= p.S) return;  // a token without a slot is not kept
+  }
+  uint16_t* const dst = p.out[n] + b * p.o_sb[n] + dst_row * p.o_st[n] + d;
+  if (n == 2 || t >= live) {  // v as it is; q rows behind the sequence are zero
 #pragma unroll
     for (int j = 0; j < NCH; ++j) {
       const int e = j * 512 + lane * 8;
-      if (e < C) *reinterpret_cast<uint4*>(dst + e / p.D * p.o_sh[n] + d) = v[j];
+      if (e < C) *reinterpret_cast<uint4*>(dst + (e >> p.log2d) * o_sh) = n == 2 ? v[j] : make_uint4(0, 0, 0, 0);
     }
     return;
   }
   float cs[4] = {1.f, 1.f, 1.f, 1.f}, sn[4] = {0.f, 0.f, 0.f, 0.f};
   if (p.cos_t) {
     const bool inside = pos >= 0 && pos < p.table_rows;
-    const int64_t at = pos * (p.D >> 1) + (d >> 1);
-#pragma unroll
-    for (int i = 0; i < 4; ++i) {
-      cs[i] = inside ? p.cos_t[at + i] : NAN;  // a position without a table row is not passed over silently
-      sn[i] = inside ? p.sin_t[at + i] : NAN;
-    }
+    const int64_t at = inside ? (pos << p.log2d >> 1) + (d >> 1) : 0;
+    const float4 c = *reinterpret_cast<const float4*>(p.cos_t + at), s = *reinterpret_cast<const float4*>(p.sin_t + at);
+    cs[0] = c.x; cs[1] = c.y; cs[2] = c.z; cs[3] = c.w;
+    sn[0] = s.x; sn[1] = s.y; sn[2] = s.z; sn[3] = s.w;
+    if (!inside) cs[0] = cs[1] = cs[2] = cs[3] = NAN;  // a position without a table row is not passed over silently
   }
   const void* const weight = p.weight[n];
+  const bool w_all = p.w_all[n] != 0;
+  const int w_dtype = p.w_dtype[n];
   float rstd[NCH];
   float all = 0.f;
 #pragma unroll
@@ -124,20 +140,17 @@ __global__ void __launch_bounds__(256) qkv_cache_kernel(CacheParams p) {
     rstd[j] = ss;
     all += ss;
   }
+  float w[8];
   if (weight) {
-    if (p.w_all[n]) {
-#pragma unroll
-      for (int off = 32; off >= 1; off >>= 1) all += __shfl_xor(all, off, 64);
-      const float r = 1.f / sqrtf(all / static_cast<float>(C) + p.eps);
+    if (w_all) {
+      const float r = 1.f / sqrtf(group_sum(all, 64) / static_cast<float>(C) + p.eps);
 #pragma unroll
       for (int j = 0; j < NCH; ++j) rstd[j] = r;
     } else {
+      load_weight8(weight, w_dtype, d, w);
+      const float inv = 1.f / static_cast<float>(1 << p.log2d);
 #pragma unroll
-      for (int j = 0; j < NCH; ++j) {
-        float ss = rstd[j];
-        for (int off = p.D >> 4; off >= 1; off >>= 1) ss += __shfl_xor(ss, off, 64);  // the D / 8 lanes of a head
-        rstd[j] = 1.f / sqrtf(ss / static_cast<float>(p.D) + p.eps);
-      }
+      for (int j = 0; j < NCH; ++j) rstd[j] = 1.f / sqrtf(group_sum(rstd[j], 1 << p.log2d >> 3) * inv + p.eps);
     }
   }
 #pragma unroll
@@ -148,8 +161,7 @@ __global__ void __launch_bounds__(256) qkv_cache_kernel(CacheParams p) {
 #pragma unroll
     for (int i = 0; i < 8; ++i) y[i] = to_f32<F16>(u16_at(v[j], i));
     if (weight) {
-      float w[8];
-      load_weight8(weight, p.w_dtype[n], p.w_all[n] ? e : d, w);
+      if (w_all) load_weight8(weight, w_dtype, e, w);
 #pragma unroll
       for (int i = 0; i < 8; ++i) y[i] = y[i] * rstd[j] * w[i];
     }
@@ -159,12 +171,12 @@ __global__ void __launch_bounds__(256) qkv_cache_kernel(CacheParams p) {
       const float re = y[2 * i] * cs[i] - y[2 * i + 1] * sn[i], im = y[2 * i + 1] * cs[i] + y[2 * i] * sn[i];
       packed[i] = from_f32<F16>(re) | from_f32<F16>(im) << 16;
     }
-    *reinterpret_cast<uint4*>(dst + e / p.D * p.o_sh[n] + d) = make_uint4(packed[0], packed[1], packed[2], packed[3]);
+    *reinterpret_cast<uint4*>(dst + (e >> p.log2d) * o_sh) = make_uint4(packed[0], packed[1], packed[2], packed[3]);
   }
 }
 
 template <int NCH>
-void launch_cache(const CacheParams& p, bool f16, unsigned grid, hipStream_t st) {
+void launch_cache(const CacheParams& p, bool f16, dim3 grid, hipStream_t st) {
   if (f16)
     qkv_cache_kernel<NCH, true><<<grid, 256, 0, st>>>(p);
   else
@@ -196,7 +208,10 @@ extern "C" int dfs_qkv_cache(const dfs_cache_args* a, dfs_stream_t stream) {
               (long long)(a->slots - a->sinks));
   DFS_REQUIRE((a->cos_table == nullptr) == (a->sin_table == nullptr), "%s: pass both cos and sin tables or neither",
               name);
-  DFS_REQUIRE(a->cos_table == nullptr || a->table_rows > 0, "%s: table_rows must be positive", name);
+  DFS_REQUIRE(a->cos_table == nullptr ||
+                  (a->table_rows > 0 && (reinterpret_cast<uintptr_t>(a->cos_table) |
+                                         reinterpret_cast<uintptr_t>(a->sin_table)) % 16 == 0),
+              "%s: tables must have rows and be 16-byte aligned", name);
   DFS_REQUIRE(a->eps >= 0., "%s: eps must be non-negative", name);
   const void* xs[3] = {a->q, a->k, a->v};
   void* os[3] = {a->q_out, a->k_cache, a->v_cache};
@@ -237,11 +252,11 @@ extern "C" int dfs_qkv_cache(const dfs_cache_args* a, dfs_stream_t stream) {
   p.new_lens = a->new_lens;
   p.B = static_cast<int>(a->batch);
   p.T = static_cast<int>(a->tokens);
-  p.D = static_cast<int>(a->head_dim);
+  while ((int64_t(1) << p.log2d) < a->head_dim) ++p.log2d;
   p.S = static_cast<int>(a->slots);
   p.sinks = static_cast<int>(a->sinks < kMax ? a->sinks : kMax);
   p.rolling = a->rolling != 0;
-  const unsigned grid = static_cast<unsigned>((a->batch * a->tokens * 3 + 3) / 4);
+  const dim3 grid(static_cast<unsigned>((a->batch * a->tokens + 3) / 4), 3);
   const bool f16 = a->dtype == DFS_DTYPE_F16;
   hipStream_t st = reinterpret_cast<hipStream_t>(stream);
   switch ((widest + 1023) / 1024) {  // chunks of 512 channels, rounded up to an even count

@@ -996,6 +996,7 @@ def qkv_cache(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, k_cache: torch.
                     not t.is_contiguous()) or t.shape[0] == 0:
                 raise ValueError(f"{entry}: tables must be contiguous float32 [P, {dim // 2}], got {t.dtype} "
                                  f"{tuple(t.shape)}")
+        cos, sin = (t if t.data_ptr() % 16 == 0 else t.clone() for t in (cos, sin))
         a.cos_table, a.sin_table, a.table_rows = cos.data_ptr(), sin.data_ptr(), cos.shape[0]
     _require_device(q, k, v, k_cache, v_cache, lens, q_weight, k_weight, cos, sin, new_lens)
     out = torch.empty((batch, tokens, heads, dim), dtype=q.dtype, device=q.device)
