@@ -195,26 +195,31 @@ __global__ void __launch_bounds__(256) linear_any_kernel(LinearParams p) {
   const int tid = threadIdx.x, lane = tid & 63, w = tid >> 6, l32 = lane & 31, hl = lane >> 5;
   const int n0 = blockIdx.x * 64, m0 = blockIdx.y * 64;
   f32x16 acc = f32x16{};
-  for (int k0 = 0; k0 < p.K; k0 += 64) {
-    uint4 a[2], b[2];
+  uint4 a[2], b[2];  // a step's chunks, loaded under the products of the one before
+  auto load = [&](int k0) {
 #pragma unroll
     for (int j = 0; j < 2; ++j) {
       const int r = j * 32 + (tid >> 3), k = k0 + (tid & 7) * 8;
       a[j] = load_row8(p.w + min(n0 + r, p.N - 1) * p.ldw, k, p.K);
       b[j] = load_row8(p.x + min(m0 + r, p.M - 1) * p.ldx, k, p.K);
     }
+  };
+  load(0);
+  for (int k0 = 0; k0 < p.K; k0 += 64) {
     __syncthreads();
 #pragma unroll
     for (int j = 0; j < 2; ++j) {
-      const int r = j * 32 + (tid >> 3), c = (tid & 7) ^ (r & 7);
+      const int r = j * 32 + (tid >> 3), c = (tid & 7) ^ (r >> 1 & 7);
       *reinterpret_cast<uint4*>(ws + (r * 8 + c) * 8) = a[j];
       *reinterpret_cast<uint4*>(xs + (r * 8 + c) * 8) = b[j];
     }
     __syncthreads();
+    if (k0 + 64 < p.K) load(k0 + 64);
 #pragma unroll
     for (int s = 0; s < 4; ++s) {
-      const uint4 fa = lds_chunk<8>(ws, (w & 1) * 32 + l32, 2 * s + hl);
-      const uint4 fb = lds_chunk<8>(xs, (w >> 1) * 32 + l32, 2 * s + hl);
+      const int wr = (w & 1) * 32 + l32, xr = (w >> 1) * 32 + l32, c = 2 * s + hl;
+      const uint4 fa = *reinterpret_cast<const uint4*>(ws + (wr * 8 + (c ^ (wr >> 1 & 7))) * 8);
+      const uint4 fb = *reinterpret_cast<const uint4*>(xs + (xr * 8 + (c ^ (xr >> 1 & 7))) * 8);
       acc = Half<F16>::mfma(__builtin_bit_cast(typename Half<F16>::vec, fa),
                             __builtin_bit_cast(typename Half<F16>::vec, fb), acc);
     }

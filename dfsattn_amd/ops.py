@@ -9,6 +9,7 @@ from __future__ import annotations
 import ctypes
 import functools
 import math
+import struct
 from dataclasses import dataclass
 from typing import Dict, Optional, Sequence, Tuple
 
@@ -702,68 +703,132 @@ def gated_residual(x: torch.Tensor, y: torch.Tensor, gate: torch.Tensor,
 
 # --------------------------------------------------------------------------
 # Products with their epilogue, windowed attention and its cache
+#
+# What follows from shapes, strides and options alone (the checks, the argument
+# block up to the pointers, the workspace's size) is worked out once for each
+# set of them; a call looks at its pointers, devices and lengths.
 # --------------------------------------------------------------------------
 
 ACTIVATION_CODE = {None: 0, "gelu_tanh": 1, "gelu": 2, "silu": 3}
 HALF = (torch.bfloat16, torch.float16)
+Shape = Tuple[int, ...]
 
 
 def _refuse_grad(entry: str, *tensors: Optional[torch.Tensor]) -> None:
     """These operators have no backward pass: a graph would lose it silently."""
-    if torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in tensors):
-        raise RuntimeError(f"{entry} has no backward pass: call it under torch.no_grad() or inference_mode()")
+    if torch.is_grad_enabled():
+        for t in tensors:
+            if t is not None and t.requires_grad:
+                raise RuntimeError(f"{entry} has no backward pass: call it under torch.no_grad() or inference_mode()")
 
 
-def _call_on(t: torch.Tensor, entry: str, *args) -> None:
-    """An entry point on t's device and that device's current stream (the
-    last argument), whichever device the caller has current."""
-    if t.device.index == torch.cuda.current_device():
-        _lib.call(entry, *args, _stream(t))
+def _call_on(device: torch.device, entry: str, *args) -> None:
+    """An entry point on a device and its current stream (the last argument),
+    whichever device the caller has current."""
+    index = device.index
+    if index == torch.cuda.current_device():
+        _lib.call(entry, *args, torch._C._cuda_getCurrentRawStream(index))
     else:
-        with torch.cuda.device(t.device):
-            _lib.call(entry, *args, _stream(t))
+        with torch.cuda.device(device):
+            _lib.call(entry, *args, torch._C._cuda_getCurrentRawStream(index))
 
 
-def _span(t: torch.Tensor) -> Tuple[int, int]:
-    """First byte and the byte behind the last one that t's elements touch."""
-    last = sum((n - 1) * s for n, s in zip(t.shape, t.stride()))
-    return t.data_ptr(), t.data_ptr() + (last + 1) * t.element_size()
+def _one_device(first: torch.Tensor, *tensors: Optional[torch.Tensor]) -> None:
+    """_require_device, told apart by device numbers (-1: the CPU)."""
+    index = first.get_device()
+    if index < 0 or any([t is not None and t.get_device() != index for t in tensors]):
+        _require_device(first, *tensors)
+
+
+def _reach(shape: Shape, stride: Shape) -> int:
+    """Elements from a tensor's first to behind its last one."""
+    return 1 + sum((n - 1) * s for n, s in zip(shape, stride)) if 0 not in shape else 0
 
 
 def _refuse_overlap(entry: str, name: str, out: torch.Tensor, *tensors: Optional[torch.Tensor]) -> None:
-    if out.numel() == 0:
-        return
-    lo, hi = _span(out)
+    lo = out.data_ptr()
+    hi = lo + _reach(out.shape, out.stride()) * out.element_size()
     for t in tensors:
-        if t is not None and t.numel():
-            a, b = _span(t)
-            if a < hi and lo < b:
+        if t is not None:
+            at = t.data_ptr()
+            if at < hi and lo < at + _reach(t.shape, t.stride()) * t.element_size():
                 raise ValueError(f"{entry}: {name} overlaps an input")
 
 
-def _axis_strides(t: torch.Tensor) -> Tuple[int, ...]:
+def _axis_strides(shape: Shape, stride: Shape) -> Shape:
     """Strides with 0 for axes of one, which have none."""
-    return tuple(s if n > 1 else 0 for n, s in zip(t.shape, t.stride()))
+    return tuple(s if n > 1 else 0 for n, s in zip(shape, stride))
 
 
-def _chunk_rows(t: torch.Tensor) -> bool:
-    """Whether rows of the last axis lie on 16-byte boundaries (16-bit elements)."""
-    strides = _axis_strides(t)
-    return strides[-1] in (0, 1) and t.data_ptr() % 16 == 0 and all(s % 8 == 0 for s in strides[:-1])
+def _contiguous_stride(shape: Shape) -> Shape:
+    return tuple(math.prod(shape[i + 1:]) for i in range(len(shape)))
 
 
-def _own_rows(t: torch.Tensor) -> bool:
-    """Rows to write to: on 16-byte boundaries, none of them shared."""
-    return _chunk_rows(t) and not any(n > 1 and s == 0 for n, s in zip(t.shape, t.stride()))
+def _dense(shape: Shape, stride: Shape) -> bool:
+    """Whether the elements fill their memory without gaps, in any order of axes."""
+    size = 1
+    for s, n in sorted((s, n) for n, s in zip(shape, stride) if n > 1):
+        if s != size:
+            return False
+        size *= n
+    return True
 
 
-def _matrix(t: torch.Tensor) -> Tuple[torch.Tensor, int]:
-    """(t as [rows, channels] with channel stride 1, row stride); a copy where
-    t's axes do not join."""
-    m = t.reshape(-1, t.shape[-1])
-    if m.stride(1) != 1 and m.shape[1] > 1:
-        m = m.contiguous()
-    return m, (m.stride(0) if m.shape[0] > 1 else m.shape[1])
+def _chunk_rows(shape: Shape, stride: Shape) -> bool:
+    """Whether rows of the last axis are whole and follow each other in
+    16-byte steps (16-bit elements)."""
+    strides = _axis_strides(shape, stride)
+    return strides[-1] in (0, 1) and all(s % 8 == 0 for s in strides[:-1])
+
+
+def _in_chunks(t: torch.Tensor) -> torch.Tensor:
+    """t, or a contiguous copy where its rows lie off 16-byte boundaries."""
+    whole = _chunk_rows(t.shape, t.stride()) and t.data_ptr() % 16 == 0
+    return t if whole else t.clone(memory_format=torch.contiguous_format)
+
+
+def _own_rows(shape: Shape, stride: Shape) -> bool:
+    """Rows to write to: whole, in 16-byte steps, none of them shared."""
+    return _chunk_rows(shape, stride) and not any(n > 1 and s == 0 for n, s in zip(shape, stride))
+
+
+def _row_stride(shape: Shape, stride: Shape) -> Optional[int]:
+    """Stride of a tensor's rows when its leading axes join into one and its
+    channels are contiguous; None where they do not."""
+    if shape[-1] > 1 and stride[-1] != 1:
+        return None
+    ld, joined = None, 0
+    for n, s in zip(reversed(shape[:-1]), reversed(stride[:-1])):
+        if n == 1:
+            continue
+        if ld is None:
+            ld, joined = s, s * n
+        elif s != joined:
+            return None
+        else:
+            joined = s * n
+    return shape[-1] if ld is None else ld
+
+
+@functools.lru_cache(maxsize=1024)
+def _linear_plan(x_shape: Shape, x_stride: Shape, w_shape: Shape, w_stride: Shape, x_dtype: torch.dtype,
+                 w_dtype: torch.dtype, activation: Optional[str], r_shape: Optional[Shape],
+                 r_stride: Optional[Shape]):
+    """(rows, shape of out, row strides of x, weight and residual or None
+    where they are copied first) of a ``linear`` call."""
+    if x_dtype not in HALF or w_dtype != x_dtype:
+        raise ValueError(f"linear: x and weight must both be bf16 or f16, got {x_dtype} and {w_dtype}")
+    if len(x_shape) < 1 or len(w_shape) != 2 or w_shape[1] != x_shape[-1]:
+        raise ValueError(f"linear: weight must be [N, K] for x [..., K], got {tuple(w_shape)} and {tuple(x_shape)}")
+    if 0 in w_shape:
+        raise ValueError(f"linear: weight {tuple(w_shape)} has no elements")
+    if activation not in ACTIVATION_CODE:
+        raise ValueError(f"linear: activation must be one of {list(ACTIVATION_CODE)}, got {activation!r}")
+    shape = (*x_shape[:-1], w_shape[0])
+    if r_shape is not None and tuple(r_shape) != shape:
+        raise ValueError(f"linear: residual must be {shape}, got {tuple(r_shape)}")
+    return (math.prod(x_shape[:-1]), shape, _row_stride(x_shape, x_stride), _row_stride(w_shape, w_stride),
+            None if r_shape is None else _row_stride(r_shape, r_stride))
 
 
 @functools.lru_cache(maxsize=1024)
@@ -781,50 +846,49 @@ def linear(x: torch.Tensor, weight: torch.Tensor, bias: Optional[torch.Tensor] =
     to x's dtype (bf16 or f16). ``out`` may be the residual itself. No
     backward pass."""
     _refuse_grad("linear", x, weight, bias, gate, residual)
-    if x.dtype not in HALF or weight.dtype != x.dtype:
-        raise ValueError(f"linear: x and weight must both be bf16 or f16, got {x.dtype} and {weight.dtype}")
-    if x.dim() < 1 or weight.dim() != 2 or weight.shape[1] != x.shape[-1]:
-        raise ValueError(f"linear: weight must be [N, K] for x [..., K], got {tuple(weight.shape)} and {tuple(x.shape)}")
+    rows, shape, ldx, ldw, ldr = _linear_plan(
+        x.shape, x.stride(), weight.shape, weight.stride(), x.dtype, weight.dtype, activation,
+        None if residual is None else residual.shape, None if residual is None else residual.stride())
     n, k = weight.shape
-    if n == 0 or k == 0:
-        raise ValueError(f"linear: weight {tuple(weight.shape)} has no elements")
-    if activation not in ACTIVATION_CODE:
-        raise ValueError(f"linear: activation must be one of {list(ACTIVATION_CODE)}, got {activation!r}")
+    dtype = x.dtype
     b_code = 0
     if bias is not None:
-        if bias.dim() != 1 or bias.numel() != n or bias.dtype not in (x.dtype, torch.float32):
+        if bias.dim() != 1 or bias.shape[0] != n or bias.dtype not in (dtype, torch.float32):
             raise ValueError(f"linear: bias must hold {n} values of x's dtype or float32, got {bias.dtype} "
                              f"{tuple(bias.shape)}")
         bias, b_code = bias.contiguous(), DTYPE_CODE[bias.dtype]
-    gate = _vec(gate, n, "linear: gate")
-    shape = (*x.shape[:-1], n)
-    for name, t in (("residual", residual), ("out", out)):
-        if t is not None and (tuple(t.shape) != shape or t.dtype != x.dtype):
-            raise ValueError(f"linear: {name} must be {x.dtype} {shape}, got {t.dtype} {tuple(t.shape)}")
-    _require_device(x, weight, bias, gate, residual, out)
+    if gate is not None and not (gate.dim() == 1 and gate.shape[0] == n and gate.dtype == torch.float32
+                                 and gate.is_contiguous()):
+        gate = _vec(gate, n, "linear: gate")
+    if residual is not None and residual.dtype != dtype:
+        raise ValueError(f"linear: residual must be {dtype}, got {residual.dtype}")
+    if out is not None and (tuple(out.shape) != shape or out.dtype != dtype or not out.is_contiguous()):
+        raise ValueError(f"linear: out must be contiguous {dtype} {shape}, got {out.dtype} {tuple(out.shape)}")
+    _one_device(x, weight, bias, gate, residual, out)
     if out is None:
-        out = torch.empty(shape, dtype=x.dtype, device=x.device)
-    elif not out.is_contiguous():
-        raise ValueError("linear: out must be contiguous")
+        out = torch.empty(shape, dtype=dtype, device=x.device)
     else:
         same = residual is not None and residual.data_ptr() == out.data_ptr() and residual.is_contiguous()
         _refuse_overlap("linear", "out", out, x, weight, bias, gate, None if same else residual)
-    if out.numel() == 0:
+    if rows == 0:
         return out
-    x2, ldx = _matrix(x)
-    w2, ldw = _matrix(weight)
-    r2, ldr = _matrix(residual) if residual is not None else (None, 0)
-    rows = x2.shape[0]
-    aligned = (k | ldx | ldw) % 8 == 0 and (x2.data_ptr() | w2.data_ptr()) % 16 == 0 and max(ldx, ldw) < 1 << 21
-    ws_bytes = _linear_workspace(rows, n, k, aligned)
+    if ldx is None:
+        x, ldx = x.contiguous(), k
+    if ldw is None:
+        weight, ldw = weight.contiguous(), k
+    if residual is not None and ldr is None:
+        residual, ldr = residual.contiguous(), n
+    px, pw = x.data_ptr(), weight.data_ptr()
+    ws_bytes = _linear_workspace(rows, n, k, (k | ldx | ldw) % 8 == 0 and (px | pw) % 16 == 0
+                                 and ldx < 1 << 21 and ldw < 1 << 21)
     ws = torch.empty(ws_bytes, dtype=torch.uint8, device=x.device) if ws_bytes else None
-    _call_on(x, "dfs_linear", _ptr(x2), ldx, _ptr(w2), ldw, rows, n, k, DTYPE_CODE[x.dtype], _ptr(bias), b_code,
-             ACTIVATION_CODE[activation], _ptr(gate), _ptr(r2), ldr, _ptr(out), n, _ptr(ws), ws_bytes)
+    _call_on(x.device, "dfs_linear", px, ldx, pw, ldw, rows, n, k, DTYPE_CODE[dtype], _ptr(bias), b_code,
+             ACTIVATION_CODE[activation], _ptr(gate), _ptr(residual), ldr or 0, out.data_ptr(), n, _ptr(ws), ws_bytes)
     return out
 
 
 def _check_lens(entry: str, name: str, t: Optional[torch.Tensor], batch: int) -> None:
-    if t is not None and (t.dtype != torch.int32 or tuple(t.shape) != (batch,) or not t.is_contiguous()):
+    if t is not None and (t.dtype != torch.int32 or t.dim() != 1 or t.shape[0] != batch or not t.is_contiguous()):
         raise ValueError(f"{entry}: {name} must be a contiguous int32 [{batch}] vector, got {t.dtype} "
                          f"{tuple(t.shape)}")
 
@@ -835,6 +899,63 @@ def _limit(entry: str, name: str, n: Optional[int]) -> int:
     if int(n) < 0:
         raise ValueError(f"{entry}: {name} must be None (no limit) or not negative, got {n}")
     return int(n)
+
+
+def _pointers(block: ctypes.Structure, first: str) -> int:
+    """Where an argument block's pointers begin."""
+    return getattr(type(block), first).offset
+
+
+_WINDOW_POINTERS = struct.Struct("@8P")
+_CACHE_POINTERS = struct.Struct("@12P")
+
+
+@functools.lru_cache(maxsize=1024)
+def _window_plan(q_shape: Shape, q_stride: Shape, k_shape: Shape, k_stride: Shape, v_shape: Shape, v_stride: Shape,
+                 dtypes: Tuple[torch.dtype, ...], out_stride: Optional[Shape], left: Optional[int],
+                 right: Optional[int], sinks: int, lens: bool, rolling: bool, scale: Optional[float]):
+    """(argument block up to the pointers, workspace bytes, strides of out,
+    whether q, k and v are read in place) of a ``window_attention`` call."""
+    entry = "window_attention"
+    if dtypes[0] not in HALF or dtypes[1] != dtypes[0] or dtypes[2] != dtypes[0]:
+        raise ValueError(f"{entry}: q, k and v must all be bf16 or f16, got {dtypes}")
+    if (len(q_shape) != 4 or len(k_shape) != 4 or v_shape != k_shape or k_shape[0] != q_shape[0]
+            or k_shape[3] != q_shape[3]):
+        raise ValueError(f"{entry}: q must be [B, H, L, D] and k and v [B, G, S, D], got {tuple(q_shape)}, "
+                         f"{tuple(k_shape)}, {tuple(v_shape)}")
+    batch, heads, rows, dim = q_shape
+    groups, slots = k_shape[1], k_shape[2]
+    if dim not in (64, 128):
+        raise ValueError(f"{entry}: head dim {dim} (supported: 64, 128)")
+    if groups == 0 or heads % groups:
+        raise ValueError(f"{entry}: {heads} query heads over {groups} key heads")
+    lo, hi = _limit(entry, "left", left), _limit(entry, "right", right)
+    if sinks < 0:
+        raise ValueError(f"{entry}: sinks must not be negative, got {sinks}")
+    if rolling and (not lens or lo < 0 or slots < sinks + lo + rows):
+        raise ValueError(f"{entry}: a rolling cache needs kv_lens, left and at least sinks + left + L slots, got "
+                         f"{slots} for sinks={sinks}, left={left}, L={rows}")
+    scale = 1.0 / math.sqrt(dim) if scale is None else float(scale)
+    if not 0.0 < scale < 1e30:
+        raise ValueError(f"{entry}: scale must be positive and finite, got {scale}")
+    if out_stride is None:  # q's storage order, where it leaves no gaps
+        dense = _chunk_rows(q_shape, q_stride) and _dense(q_shape, q_stride)
+        out_stride = q_stride if dense else _contiguous_stride(q_shape)
+    qkv = ((q_shape, q_stride), (k_shape, k_stride), (v_shape, v_stride))
+    in_place = all(_chunk_rows(shape, stride) for shape, stride in qkv)
+    strides = [_axis_strides(shape, stride) for shape, stride in qkv]
+    a = _lib.WindowArgs()
+    a.batch, a.q_heads, a.kv_heads, a.q_rows, a.slots, a.head_dim = batch, heads, groups, rows, slots, dim
+    a.dtype, a.left, a.right, a.sinks, a.rolling = DTYPE_CODE[dtypes[0]], lo, hi, sinks, int(rolling)
+    (a.q_batch_stride, a.q_head_stride, a.q_row_stride, _), (a.k_batch_stride, a.k_head_stride, a.k_row_stride, _), \
+        (a.v_batch_stride, a.v_head_stride, a.v_row_stride, _) = strides
+    a.out_batch_stride, a.out_head_stride, a.out_row_stride, _ = _axis_strides(q_shape, out_stride)
+    a.scale = scale
+    size = 0
+    if math.prod(q_shape) and slots:
+        size = max(int(_lib.lib().dfs_window_attention_workspace_size(ctypes.byref(a))), 0)
+    a.workspace_bytes = size
+    return bytes(a)[:_pointers(a, "q")], size, out_stride, in_place
 
 
 def window_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, left: Optional[int] = None,
@@ -861,60 +982,97 @@ def window_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, left: Op
     the sequence must be finite. No backward pass."""
     entry = "window_attention"
     _refuse_grad(entry, q, k, v)
-    if q.dtype not in HALF or k.dtype != q.dtype or v.dtype != q.dtype:
-        raise ValueError(f"{entry}: q, k and v must all be bf16 or f16, got {q.dtype}, {k.dtype}, {v.dtype}")
-    if q.dim() != 4 or k.dim() != 4 or v.shape != k.shape or k.shape[0] != q.shape[0] or k.shape[3] != q.shape[3]:
-        raise ValueError(f"{entry}: q must be [B, H, L, D] and k and v [B, G, S, D], got {tuple(q.shape)}, "
-                         f"{tuple(k.shape)}, {tuple(v.shape)}")
-    batch, heads, rows, dim = q.shape
-    groups, slots = k.shape[1], k.shape[2]
-    if dim not in (64, 128):
-        raise ValueError(f"{entry}: head dim {dim} (supported: 64, 128)")
-    if groups == 0 or heads % groups:
-        raise ValueError(f"{entry}: {heads} query heads over {groups} key heads")
-    lo, hi, sinks = _limit(entry, "left", left), _limit(entry, "right", right), int(sinks)
-    if sinks < 0:
-        raise ValueError(f"{entry}: sinks must not be negative, got {sinks}")
+    if out is not None and (out.shape != q.shape or out.dtype != q.dtype or out.data_ptr() % 16
+                            or not _own_rows(out.shape, out.stride())):
+        raise ValueError(f"{entry}: out must be {q.dtype} {tuple(q.shape)} with rows of its own on 16-byte boundaries")
+    head, size, out_stride, in_place = _window_plan(
+        q.shape, q.stride(), k.shape, k.stride(), v.shape, v.stride(), (q.dtype, k.dtype, v.dtype),
+        None if out is None else out.stride(), left, right, int(sinks), kv_lens is not None, bool(rolling), scale)
+    batch = q.shape[0]
     _check_lens(entry, "q_lens", q_lens, batch)
     _check_lens(entry, "kv_lens", kv_lens, batch)
-    if rolling and (kv_lens is None or lo < 0 or slots < sinks + lo + rows):
-        raise ValueError(f"{entry}: a rolling cache needs kv_lens, left and at least sinks + left + L slots, got "
-                         f"{slots} for sinks={sinks}, left={left}, L={rows}")
-    scale = 1.0 / math.sqrt(dim) if scale is None else float(scale)
-    if not 0.0 < scale < 1e30:
-        raise ValueError(f"{entry}: scale must be positive and finite, got {scale}")
-    _require_device(q, k, v, q_lens, kv_lens, out)
+    _one_device(q, k, v, q_lens, kv_lens, out)
+    device = q.device
     if out is None:
-        out = torch.empty_like(q)  # q's storage order
-        if not _chunk_rows(out):
-            out = torch.empty(q.shape, dtype=q.dtype, device=q.device)
+        out = torch.empty_strided(q.shape, out_stride, dtype=q.dtype, device=device)
     else:
-        if out.shape != q.shape or out.dtype != q.dtype or not _own_rows(out):
-            raise ValueError(f"{entry}: out must be {q.dtype} {tuple(q.shape)} with rows of its own on 16-byte "
-                             "boundaries")
         _refuse_overlap(entry, "out", out, q, k, v)
-    lse = torch.empty((batch, heads, rows), dtype=torch.float32, device=q.device) if want_lse else None
-    if out.numel() == 0 or slots == 0:
+    lse = torch.empty(q.shape[:3], dtype=torch.float32, device=device) if want_lse else None
+    if out.numel() == 0 or k.shape[2] == 0:
         out.zero_()
         if want_lse:
             lse.fill_(-math.inf)
         return (out, lse) if want_lse else out
-    q, k, v = (t if _chunk_rows(t) else t.clone(memory_format=torch.contiguous_format) for t in (q, k, v))
-    a = _lib.WindowArgs()
-    a.batch, a.q_heads, a.kv_heads, a.q_rows, a.slots, a.head_dim = batch, heads, groups, rows, slots, dim
-    a.dtype, a.left, a.right, a.sinks, a.rolling = DTYPE_CODE[q.dtype], lo, hi, sinks, int(rolling)
-    a.q_batch_stride, a.q_head_stride, a.q_row_stride, _ = _axis_strides(q)
-    a.k_batch_stride, a.k_head_stride, a.k_row_stride, _ = _axis_strides(k)
-    a.v_batch_stride, a.v_head_stride, a.v_row_stride, _ = _axis_strides(v)
-    a.out_batch_stride, a.out_head_stride, a.out_row_stride, _ = _axis_strides(out)
-    a.scale = scale
-    a.q, a.k, a.v, a.out = q.data_ptr(), k.data_ptr(), v.data_ptr(), out.data_ptr()
-    a.lse, a.q_lens, a.kv_lens = _ptr(lse), _ptr(q_lens), _ptr(kv_lens)
-    size = int(_lib.lib().dfs_window_attention_workspace_size(ctypes.byref(a)))
-    ws = torch.empty(size, dtype=torch.uint8, device=q.device) if size > 0 else None
-    a.workspace, a.workspace_bytes = _ptr(ws), max(size, 0)
-    _call_on(q, "dfs_window_attention", ctypes.byref(a))
+    pq, pk, pv = q.data_ptr(), k.data_ptr(), v.data_ptr()
+    if not (in_place and (pq | pk | pv) % 16 == 0):
+        return window_attention(_in_chunks(q), _in_chunks(k), _in_chunks(v), left, right, sinks, q_lens, kv_lens,
+                                rolling, scale, out, want_lse)
+    ws = torch.empty(size, dtype=torch.uint8, device=device) if size else None
+    block = head + _WINDOW_POINTERS.pack(pq, pk, pv, out.data_ptr(), _ptr(lse) or 0,
+                                         _ptr(q_lens) or 0, _ptr(kv_lens) or 0, _ptr(ws) or 0)
+    _call_on(device, "dfs_window_attention", block)
     return (out, lse) if want_lse else out
+
+
+@functools.lru_cache(maxsize=1024)
+def _cache_plan(shapes: Tuple[Shape, ...], strides: Tuple[Shape, ...], dtypes: Tuple[torch.dtype, ...],
+                weights: Tuple[Optional[Tuple[Shape, torch.dtype]], ...], tables: Optional[Tuple[Shape, Shape]],
+                eps: float, sinks: int, rolling: bool):
+    """(argument block up to the pointers, whether q, k and v are read in
+    place, bytes that each tensor reaches over) of a ``qkv_cache`` call on q,
+    k, v, k_cache and v_cache."""
+    entry = "qkv_cache"
+    q_shape, k_shape, v_shape, kc_shape, vc_shape = shapes
+    if dtypes[0] not in HALF or any(d != dtypes[0] for d in dtypes):
+        raise ValueError(f"{entry}: q, k, v and the caches must share bf16 or f16, got {dtypes}")
+    if (len(q_shape) != 4 or len(k_shape) != 4 or v_shape != k_shape or k_shape[:2] != q_shape[:2]
+            or k_shape[3] != q_shape[3]):
+        raise ValueError(f"{entry}: q must be [B, T, H, D] and k and v [B, T, G, D], got {tuple(q_shape)}, "
+                         f"{tuple(k_shape)}, {tuple(v_shape)}")
+    batch, tokens, heads, dim = q_shape
+    groups = k_shape[2]
+    if dim < 16 or dim > 512 or dim & (dim - 1):
+        raise ValueError(f"{entry}: head dim {dim} must be a power of two from 16 to 512")
+    if heads == 0 or groups == 0 or max(heads, groups) * dim > 8192:
+        raise ValueError(f"{entry}: {max(heads, groups)} heads of {dim} channels (supported: up to 8192 channels)")
+    if len(kc_shape) != 4 or vc_shape != kc_shape or (kc_shape[0], kc_shape[1], kc_shape[3]) != (batch, groups, dim):
+        raise ValueError(f"{entry}: caches must be [{batch}, {groups}, S, {dim}], got {tuple(kc_shape)} and "
+                         f"{tuple(vc_shape)}")
+    if not _own_rows(kc_shape, strides[3]) or not _own_rows(vc_shape, strides[4]):
+        raise ValueError(f"{entry}: the caches must have rows of their own on 16-byte boundaries")
+    slots = kc_shape[2]
+    if sinks < 0:
+        raise ValueError(f"{entry}: sinks must not be negative, got {sinks}")
+    if tokens > slots - (sinks if rolling else 0):
+        raise ValueError(f"{entry}: {tokens} new tokens do not fit a cache of {slots} slots"
+                         + (f" with {sinks} sinks" if rolling else ""))
+    if not eps >= 0.0:
+        raise ValueError(f"{entry}: eps must not be negative, got {eps}")
+    a = _lib.CacheArgs()
+    for side, w, count in (("q", weights[0], heads), ("k", weights[1], groups)):
+        if w is None:
+            continue
+        w_shape, w_dtype = w
+        if len(w_shape) != 1 or w_shape[0] not in (dim, count * dim) or w_dtype not in DTYPE_CODE:
+            raise ValueError(f"{entry}: {side}_weight must be a [{dim}] or [{count * dim}] vector, got {w_dtype} "
+                             f"{tuple(w_shape)}")
+        setattr(a, f"{side}_weight_dtype", DTYPE_CODE[w_dtype])
+        setattr(a, f"{side}_norm_all", int(w_shape[0] != dim))
+    if tables is not None:
+        if tables[0] != tables[1] or len(tables[0]) != 2 or tables[0][1] != dim // 2 or tables[0][0] == 0:
+            raise ValueError(f"{entry}: tables must be [P, {dim // 2}], got {tuple(tables[0])} and {tuple(tables[1])}")
+        a.table_rows = tables[0][0]
+    a.batch, a.tokens, a.q_heads, a.kv_heads, a.head_dim, a.slots = batch, tokens, heads, groups, dim, slots
+    a.dtype, a.sinks, a.rolling, a.eps = DTYPE_CODE[dtypes[0]], sinks, int(rolling), eps
+    in_place = all(_chunk_rows(shape, stride) for shape, stride in zip(shapes[:3], strides[:3]))
+    (a.q_batch_stride, a.q_token_stride, a.q_head_stride, _), \
+        (a.k_batch_stride, a.k_token_stride, a.k_head_stride, _), \
+        (a.v_batch_stride, a.v_token_stride, a.v_head_stride, _) = (
+            _axis_strides(shape, stride) for shape, stride in zip(shapes[:3], strides[:3]))
+    a.q_out_batch_stride, a.q_out_token_stride, a.q_out_head_stride = tokens * heads * dim, heads * dim, dim
+    a.k_cache_batch_stride, a.k_cache_head_stride, a.k_cache_slot_stride, _ = _axis_strides(kc_shape, strides[3])
+    a.v_cache_batch_stride, a.v_cache_head_stride, a.v_cache_slot_stride, _ = _axis_strides(vc_shape, strides[4])
+    return bytes(a)[:_pointers(a, "q")], in_place, tuple(2 * _reach(x, y) for x, y in zip(shapes, strides))
 
 
 def qkv_cache(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tensor,
@@ -938,80 +1096,49 @@ def qkv_cache(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, k_cache: torch.
     dropped, and a position past the table makes its rows NaN. No backward
     pass."""
     entry = "qkv_cache"
-    cos, sin = table if table is not None else (None, None)
     _refuse_grad(entry, q, k, v, q_weight, k_weight)
-    if q.dtype not in HALF or any(t.dtype != q.dtype for t in (k, v, k_cache, v_cache)):
-        raise ValueError(f"{entry}: q, k, v and the caches must share bf16 or f16")
-    if q.dim() != 4 or k.dim() != 4 or v.shape != k.shape or k.shape[:2] != q.shape[:2] or k.shape[3] != q.shape[3]:
-        raise ValueError(f"{entry}: q must be [B, T, H, D] and k and v [B, T, G, D], got {tuple(q.shape)}, "
-                         f"{tuple(k.shape)}, {tuple(v.shape)}")
-    batch, tokens, heads, dim = q.shape
-    groups = k.shape[2]
-    if dim < 16 or dim > 512 or dim & (dim - 1):
-        raise ValueError(f"{entry}: head dim {dim} must be a power of two from 16 to 512")
-    if heads == 0 or groups == 0 or max(heads, groups) * dim > 8192:
-        raise ValueError(f"{entry}: {max(heads, groups)} heads of {dim} channels (supported: up to 8192 channels)")
-    if k_cache.dim() != 4 or v_cache.shape != k_cache.shape or (
-            k_cache.shape[0], k_cache.shape[1], k_cache.shape[3]) != (batch, groups, dim):
-        raise ValueError(f"{entry}: caches must be [{batch}, {groups}, S, {dim}], got {tuple(k_cache.shape)} and "
-                         f"{tuple(v_cache.shape)}")
-    slots, sinks = k_cache.shape[2], int(sinks)
-    if sinks < 0:
-        raise ValueError(f"{entry}: sinks must not be negative, got {sinks}")
-    if tokens > slots - (sinks if rolling else 0):
-        raise ValueError(f"{entry}: {tokens} new tokens do not fit a cache of {slots} slots"
-                         + (f" with {sinks} sinks" if rolling else ""))
-    for name, t in (("k_cache", k_cache), ("v_cache", v_cache)):
-        if not _own_rows(t):
-            raise ValueError(f"{entry}: {name} must have rows of its own on 16-byte boundaries")
-    for name, t in (("k_cache", k_cache), ("v_cache", v_cache)):
-        _refuse_overlap(entry, name, t, q, k, v)
-    if k_cache.data_ptr() == v_cache.data_ptr() and k_cache.numel():  # their rows may alternate in one tensor
-        raise ValueError(f"{entry}: k_cache and v_cache are the same memory")
     if lens is None:
         raise ValueError(f"{entry}: lens is needed")
-    _check_lens(entry, "lens", lens, batch)
-    _check_lens(entry, "new_lens", new_lens, batch)
-    if not eps >= 0.0:
-        raise ValueError(f"{entry}: eps must not be negative, got {eps}")
-    a = _lib.CacheArgs()
-    refs = []
-    for side, w, count in (("q", q_weight, heads), ("k", k_weight, groups)):
-        if w is None:
-            continue
-        if w.dim() != 1 or w.numel() not in (dim, count * dim) or w.dtype not in DTYPE_CODE:
-            raise ValueError(f"{entry}: {side}_weight must be a [{dim}] or [{count * dim}] vector, got {w.dtype} "
-                             f"{tuple(w.shape)}")
-        if not w.is_contiguous() or w.data_ptr() % 16:
-            w = w.clone(memory_format=torch.contiguous_format)
-        refs.append(w)
-        setattr(a, f"{side}_weight", w.data_ptr())
-        setattr(a, f"{side}_weight_dtype", DTYPE_CODE[w.dtype])
-        setattr(a, f"{side}_norm_all", int(w.numel() != dim))
+    cos, sin = table if table is not None else (None, None)
     if (cos is None) != (sin is None):
         raise ValueError(f"{entry}: pass both cos and sin or neither")
+    head, in_place, reach = _cache_plan(
+        (q.shape, k.shape, v.shape, k_cache.shape, v_cache.shape),
+        (q.stride(), k.stride(), v.stride(), k_cache.stride(), v_cache.stride()),
+        (q.dtype, k.dtype, v.dtype, k_cache.dtype, v_cache.dtype),
+        (None if q_weight is None else (q_weight.shape, q_weight.dtype),
+         None if k_weight is None else (k_weight.shape, k_weight.dtype)),
+        None if cos is None else (cos.shape, sin.shape), float(eps), int(sinks), bool(rolling))
+    batch, tokens, heads, dim = q.shape
+    at = (q.data_ptr(), k.data_ptr(), v.data_ptr())
+    pk, pv = k_cache.data_ptr(), v_cache.data_ptr()
+    if (pk | pv) % 16:
+        raise ValueError(f"{entry}: the caches must have rows of their own on 16-byte boundaries")
+    for x, n in zip(at, reach):
+        if (x < pk + reach[3] and pk < x + n) or (x < pv + reach[4] and pv < x + n):
+            raise ValueError(f"{entry}: a cache overlaps an input")
+    if pk == pv and reach[3]:  # their rows may alternate in one tensor
+        raise ValueError(f"{entry}: k_cache and v_cache are the same memory")
+    _check_lens(entry, "lens", lens, batch)
+    _check_lens(entry, "new_lens", new_lens, batch)
     if cos is not None:
         for t in (cos, sin):
-            if t.dtype != torch.float32 or t.dim() != 2 or t.shape != cos.shape or t.shape[1] != dim // 2 or (
-                    not t.is_contiguous()) or t.shape[0] == 0:
-                raise ValueError(f"{entry}: tables must be contiguous float32 [P, {dim // 2}], got {t.dtype} "
-                                 f"{tuple(t.shape)}")
-        cos, sin = (t if t.data_ptr() % 16 == 0 else t.clone() for t in (cos, sin))
-        a.cos_table, a.sin_table, a.table_rows = cos.data_ptr(), sin.data_ptr(), cos.shape[0]
-    _require_device(q, k, v, k_cache, v_cache, lens, q_weight, k_weight, cos, sin, new_lens)
-    out = torch.empty((batch, tokens, heads, dim), dtype=q.dtype, device=q.device)
+            if t.dtype != torch.float32 or not t.is_contiguous():
+                raise ValueError(f"{entry}: tables must be contiguous float32, got {t.dtype}")
+    _one_device(q, k, v, k_cache, v_cache, lens, q_weight, k_weight, cos, sin, new_lens)
+    device = q.device
+    out = torch.empty(q.shape, dtype=q.dtype, device=device)
     if out.numel() == 0:
         return out.transpose(1, 2)
-    q, k, v = (t if _chunk_rows(t) else t.clone(memory_format=torch.contiguous_format) for t in (q, k, v))
-    a.batch, a.tokens, a.q_heads, a.kv_heads, a.head_dim, a.slots = batch, tokens, heads, groups, dim, slots
-    a.dtype, a.sinks, a.rolling, a.eps = DTYPE_CODE[q.dtype], sinks, int(rolling), float(eps)
-    a.q_batch_stride, a.q_token_stride, a.q_head_stride, _ = _axis_strides(q)
-    a.k_batch_stride, a.k_token_stride, a.k_head_stride, _ = _axis_strides(k)
-    a.v_batch_stride, a.v_token_stride, a.v_head_stride, _ = _axis_strides(v)
-    a.q_out_batch_stride, a.q_out_token_stride, a.q_out_head_stride, _ = _axis_strides(out)
-    a.k_cache_batch_stride, a.k_cache_head_stride, a.k_cache_slot_stride, _ = _axis_strides(k_cache)
-    a.v_cache_batch_stride, a.v_cache_head_stride, a.v_cache_slot_stride, _ = _axis_strides(v_cache)
-    a.q, a.k, a.v, a.q_out = q.data_ptr(), k.data_ptr(), v.data_ptr(), out.data_ptr()
-    a.k_cache, a.v_cache, a.lens, a.new_lens = k_cache.data_ptr(), v_cache.data_ptr(), lens.data_ptr(), _ptr(new_lens)
-    _call_on(q, "dfs_qkv_cache", ctypes.byref(a))
+    if not (in_place and (at[0] | at[1] | at[2]) % 16 == 0):
+        return qkv_cache(_in_chunks(q), _in_chunks(k), _in_chunks(v), k_cache, v_cache, lens, q_weight, k_weight, eps,
+                         table, new_lens, sinks, rolling)
+    vectors = [0 if t is None else t.data_ptr() for t in (q_weight, k_weight, cos, sin)]
+    if (vectors[0] | vectors[1] | vectors[2] | vectors[3]) % 16 or any(
+            [t is not None and not t.is_contiguous() for t in (q_weight, k_weight)]):
+        q_weight, k_weight, cos, sin = (None if t is None else t.clone(memory_format=torch.contiguous_format)
+                                        for t in (q_weight, k_weight, cos, sin))
+        vectors = [_ptr(t) or 0 for t in (q_weight, k_weight, cos, sin)]
+    block = head + _CACHE_POINTERS.pack(*at, out.data_ptr(), pk, pv, *vectors, lens.data_ptr(), _ptr(new_lens) or 0)
+    _call_on(device, "dfs_qkv_cache", block)
     return out.transpose(1, 2)
