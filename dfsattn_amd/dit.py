@@ -171,6 +171,17 @@ class DiTBlock(nn.Module):
     # _addmm_activation: 8.2 -> 7.5 ms per call at 75,600 x 5,120 x 13,824; the
     # activation is applied before the bf16 rounding instead of after it).
     fused_elementwise: bool = True
+    # The FFN's products with their GELU and their gated residual in this
+    # library's kernel (ops.linear, fused path only): one pass less over the
+    # hidden states, results rounded once instead of twice.
+    native_ffn: bool = False
+
+    def _ffn_native(self, h: torch.Tensor, x: torch.Tensor, gate: torch.Tensor) -> torch.Tensor:
+        from . import ops
+
+        lin1, _, lin2 = self.ffn
+        a = ops.linear(h, lin1.weight, lin1.bias, activation="gelu_tanh")
+        return ops.linear(a, lin2.weight, lin2.bias, gate=gate, residual=x)
 
     def _ffn_fused(self, h: torch.Tensor) -> torch.Tensor:
         lin1, act, lin2 = self.ffn
@@ -190,6 +201,8 @@ class DiTBlock(nn.Module):
             h = ops.adaln_modulate(x, self.norm2.eps, weight=self.norm2.weight.float(), bias=self.norm2.bias.float())
             x = x + self.attn2(h, context)
             h = ops.adaln_modulate(x, self.norm3.eps, scale=c_scale, shift=c_shift)
+            if self.native_ffn:
+                return self._ffn_native(h, x, c_gate)
             return ops.gated_residual(x, self._ffn_fused(h), c_gate)
         h = (self.norm1(x.float()) * (1 + scale_msa) + shift_msa).type_as(x)
         x = (x.float() + self.attn1(h, None, None, rotary_emb) * gate_msa).type_as(x)
@@ -233,7 +246,8 @@ class WanLikeDiT(nn.Module):
 
     def unpatchify(self, tokens: torch.Tensor) -> torch.Tensor:
         b = tokens.shape[0]
-        f, h, w = self.cfg.grid
+        _, h, w = self.cfg.grid
+        f = tokens.shape[1] // (h * w)  # the grid's frames, or those of a stream's chunk
         pf, ph, pw = self.cfg.patch
         c = self.cfg.in_channels
         x = tokens.reshape(b, f, h, w, c, pf, ph, pw).permute(0, 4, 1, 5, 2, 6, 3, 7)
@@ -285,16 +299,19 @@ def synth_inputs(cfg: DiTConfig, device, seed: Optional[int] = None):
 def install_dfs_processors(model: WanLikeDiT, mode: str = "dfs", sparsity: float = 0.3, tile_size: int = 16,
                            block_size: int = 128, video_perm: Optional[torch.Tensor] = None,
                            skip_layers: Sequence[int] = (), skip_steps: int = 12, cache_interval: int = 12,
-                           sparsity_dcrt: float = 0.0, cache_flag: bool = True) -> list:
+                           sparsity_dcrt: float = 0.0, cache_flag: bool = True,
+                           window: Tuple[Optional[int], Optional[int]] = (None, None), sinks: int = 0) -> list:
     """One Wan_DFSAttn_Processor2_0 per attention module, built as the Wan
     driver builds them (wan21_t2v_inference.py:150-173): processor_id is the
-    module's index, cross_flag marks the attn2 (text) modules."""
+    module's index, cross_flag marks the attn2 (text) modules. ``window`` and
+    ``sinks`` are mode "window"'s."""
     from .replace_wan import Wan_DFSAttn_Processor2_0
 
     procs = []
     for i, (name, module) in enumerate(model.attention_modules()):
         proc = Wan_DFSAttn_Processor2_0(mode, sparsity, tile_size, block_size, video_perm, i, list(skip_layers),
-                                        skip_steps, cache_interval, sparsity_dcrt, cache_flag, "attn2" in name)
+                                        skip_steps, cache_interval, sparsity_dcrt, cache_flag, "attn2" in name,
+                                        window=window, sinks=sinks)
         module.set_processor(proc)
         procs.append(proc)
     return procs

@@ -15,6 +15,10 @@
   host; nothing here reads a device tensor back.
 * ``"torch"``: ``scaled_dot_product_attention`` on the tensors as given.
 * ``"vanilla"``: explicit softmax(Q K^T / sqrt(D) + bias) V.
+* ``"window"``: this library's ``window_attention`` of one whole sequence a
+  row: a sliding window of ``window`` = (left, right) tokens (None: no limit,
+  right 0: causal) and the first ``sinks`` tokens. Not among the reference's
+  modes.
 """
 from __future__ import annotations
 
@@ -174,7 +178,8 @@ def full_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, mode: str 
                    attn_mask: Optional[torch.Tensor] = None, causal: bool = False,
                    cu_seqlens_q: Optional[torch.Tensor] = None, cu_seqlens_kv: Optional[torch.Tensor] = None,
                    max_seqlen_q: Optional[int] = None, max_seqlen_kv: Optional[int] = None,
-                   batch_size: int = 1, operand_dtype: Optional[torch.dtype] = None) -> torch.Tensor:
+                   batch_size: int = 1, operand_dtype: Optional[torch.dtype] = None,
+                   window: Tuple[Optional[int], Optional[int]] = (None, None), sinks: int = 0) -> torch.Tensor:
     """Dense attention, [B, H, S, D] in and out (fullattention.py:60-153).
     ``operand_dtype`` picks the native kernel's operand precision (f16 by
     default, with every finite bf16 input kept; bf16 for the reference
@@ -186,6 +191,14 @@ def full_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, mode: str 
         if drop_rate:
             raise NotImplementedError("dropout is not used by the DFS processors (inference)")
         return _flash(q, k, v, cu_seqlens_q, cu_seqlens_kv, batch_size, operand_dtype)
+    if mode == "window":
+        if drop_rate or attn_mask is not None or causal:
+            raise NotImplementedError("window attention takes its mask from window and sinks alone, without dropout")
+        for cu, total in ((cu_seqlens_q, q.shape[2]), (cu_seqlens_kv, k.shape[2])):
+            if cu is not None and (cu.device.type != "cpu" or [int(x) for x in cu.tolist()][:2] != [0, total]):
+                raise NotImplementedError("window attention runs one whole sequence a row; pass host cu_seqlens of it "
+                                          "or none")
+        return ops.window_attention(q, k, v, window[0], window[1], sinks)
     if mode == "torch":
         if attn_mask is not None and attn_mask.dtype != torch.bool:
             attn_mask = attn_mask.to(q.dtype)

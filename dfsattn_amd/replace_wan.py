@@ -15,7 +15,9 @@ model's norm modules and the float64 complex product of the reference's
 fallback (replace_wan.py:166-218) run in torch. The attention runs on this
 library: ``dfs_attention`` for sparse steps and ``full_attention`` (the
 block-sparse kernel with every block kept) for dense ones, chosen as at
-replace_wan.py:252-308.
+replace_wan.py:252-308. With mode "window", which the reference does not have,
+every self-attention step runs ``window_attention`` in token order with the
+processor's ``window`` and ``sinks``.
 """
 from __future__ import annotations
 
@@ -114,7 +116,7 @@ class Wan_DFSAttn_Processor2_0:
                  cache_interval, sparsity_dcrt, cache_flag, cross_flag, dense_step_idx=-1, dense_interval=0,
                  rest_steps=0, skip_steps2=0, record_density=False, sparse_execution="native",
                  hybrid_threshold=8, flashinfer64_top_p=0.25, flashinfer64_token_top_k=None,
-                 flashinfer64_token_top_ratio=0.10):
+                 flashinfer64_token_top_ratio=0.10, window=(None, None), sinks=0):
         self.mode = mode
         self.sparsity = sparsity
         self.tile_size = tile_size
@@ -138,12 +140,16 @@ class Wan_DFSAttn_Processor2_0:
         self.flashinfer64_top_p = flashinfer64_top_p
         self.flashinfer64_token_top_k = flashinfer64_token_top_k
         self.flashinfer64_token_top_ratio = flashinfer64_token_top_ratio
+        self.window = window
+        self.sinks = sinks
         if not hasattr(F, "scaled_dot_product_attention"):
             raise ImportError("WanAttnProcessor requires PyTorch 2.0 or higher.")
 
     # --- branch selection (replace_wan.py:252-271) ---------------------------
     def branch(self) -> str:
-        """'dfs' or 'dense' for the current call."""
+        """'dfs', 'dense' or, in that mode, 'window' for the current call."""
+        if self.mode == "window" and self.cross_flag is False:
+            return "window"
         if self.mode != "dfs" or self.cross_flag is not False:
             return "dense"
         real_step = self.step_idx // 2  # the step counter counts CFG passes
@@ -215,7 +221,12 @@ class Wan_DFSAttn_Processor2_0:
         cu_seqlens_q = torch.tensor([0, s_q, s_q], dtype=torch.int32)
         cu_seqlens_kv = torch.tensor([0, s_k, s_k_total], dtype=torch.int32)
 
-        if self.branch() == "dfs":
+        branch = self.branch()
+        if branch == "window":
+            hidden_states = full_attention(
+                query, key, value, mode="window", attn_mask=attention_mask, cu_seqlens_q=cu_seqlens_q,
+                cu_seqlens_kv=cu_seqlens_kv, window=self.window, sinks=self.sinks)
+        elif branch == "dfs":
             hidden_states = dfs_attention(
                 query, key, value, step_idx=self.step_idx, skip_steps=self.skip_steps,
                 cache_interval=self.cache_interval, layer_idx=self.layer_idx, sparsity=self.sparsity,

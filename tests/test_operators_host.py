@@ -135,3 +135,23 @@ def test_rolling_slots_hold_the_sinks_and_the_newest_tokens():
             ring = slots - sinks
             want = [p for p in range(pos + 1) if p < sinks or p > pos - ring]
             assert kept == want
+
+
+def test_window_mode_of_full_attention_refuses_what_it_does_not_do():
+    from dfsattn_amd.fullattention import full_attention
+
+    q = _t(1, 2, 8, 64)
+    for kw in ({"attn_mask": torch.ones(8, 8, dtype=torch.bool)}, {"causal": True}, {"drop_rate": 0.1},
+               {"cu_seqlens_q": torch.tensor([0, 5, 8], dtype=torch.int32)}):
+        with pytest.raises(NotImplementedError):
+            full_attention(q, q, q, mode="window", window=(4, 0), **kw)
+    with pytest.raises(ValueError):
+        full_attention(q, q, q, mode="window", window=(-4, 0))
+
+
+def test_window_mode_of_the_processor_leaves_text_modules_dense():
+    from dfsattn_amd.replace_wan import Wan_DFSAttn_Processor2_0
+
+    args = ("window", 0.3, 16, 128, None, 0, [], 12, 12, 0.0, True)
+    assert Wan_DFSAttn_Processor2_0(*args, False, window=(4, 4), sinks=2).branch() == "window"
+    assert Wan_DFSAttn_Processor2_0(*args, True).branch() == "dense"
