@@ -27,8 +27,9 @@ typedef __attribute__((address_space(3))) void lds_void;
 
 // One 16-byte load per lane straight into LDS: the wave fills 1 KB from `lds`
 // on in lane order, each lane from its own byte offset voff + soff.
+template <bool STREAM = false>
 __device__ __forceinline__ void load_lds16(__amdgpu_buffer_rsrc_t rs, void* lds, uint32_t voff, int soff) {
-  __builtin_amdgcn_raw_ptr_buffer_load_lds(rs, (lds_void*)lds, 16, voff, soff, 0, 0);
+  __builtin_amdgcn_raw_ptr_buffer_load_lds(rs, (lds_void*)lds, 16, voff, soff, 0, STREAM ? 2 : 0);
 }
 
 // Copy of one tile into LDS with the chunk swizzle by NW waves, as 16-byte

@@ -263,10 +263,12 @@ __device__ __forceinline__ void finish16(const LinearParams& p, int n0, const fl
 // outputs, and its waves deal the channels among themselves in blocks of 128. A
 // wave's blocks of w pass through three LDS buffers of its own that the loads
 // fill directly, 256 bytes of a row at a time; x comes from L2 as it is needed.
-// No barrier before the waves' sums meet. One row by 30,720 x 5,120: 56.8 us
-// (5.5 TB/s); with w read into registers in the products' layout, 64 bytes of a
-// row at a time, 61 to 69; four rows by 5,120 x 13,824: 23.7 and 37.1.
-template <int WAVES, bool F16>
+// No barrier before the waves' sums meet. One row by 30,720 x 5,120: 54.4 us
+// (5.8 TB/s) with streaming loads, taken where w is beyond the last-level cache,
+// 58.2 with ordinary ones; with w read into registers in the products' layout,
+// 64 bytes of a row at a time, 61 to 69. Four rows by 5,120 x 13,824: 23.7 and
+// 37.1 (streaming 46).
+template <int WAVES, bool F16, bool STREAM>
 __global__ void __launch_bounds__(64 * WAVES) linear_few_kernel(LinearParams p) {
   typedef typename Half<F16>::vec vec;
   constexpr int kBlock = 16 * 128;  // elements of w in a wave's buffer
@@ -290,7 +292,7 @@ __global__ void __launch_bounds__(64 * WAVES) linear_few_kernel(LinearParams p) 
 #pragma unroll
     for (int j = 0; j < 4; ++j) {
       const bool in = (r16 ^ (4 * j + c4)) * 8 < left;
-      load_lds16(rs, buf + w * kBlock + j * 512, in ? wv[j] + b * 256 : kOutside, 0);
+      load_lds16<STREAM>(rs, buf + w * kBlock + j * 512, in ? wv[j] + b * 256 : kOutside, 0);
     }
   };
   f32x4 acc = f32x4{};
@@ -830,12 +832,15 @@ void launch_tile(const LinearParams& p, bool f16, hipStream_t st) {
   }
 }
 
-void launch_few(const LinearParams& p, bool f16, hipStream_t st) {
+template <bool F16>
+void launch_few(const LinearParams& p, hipStream_t st) {
   const int groups = (p.N + 15) / 16;
-  if (groups >= 256)
-    f16 ? linear_few_kernel<4, true><<<groups, 256, 0, st>>>(p) : linear_few_kernel<4, false><<<groups, 256, 0, st>>>(p);
+  if (static_cast<int64_t>(p.N) * p.K * 2 > kLastLevelCache)
+    linear_few_kernel<4, F16, true><<<groups, 256, 0, st>>>(p);
+  else if (groups >= 256)
+    linear_few_kernel<4, F16, false><<<groups, 256, 0, st>>>(p);
   else  // more waves a workgroup where there are few
-    f16 ? linear_few_kernel<8, true><<<groups, 512, 0, st>>>(p) : linear_few_kernel<8, false><<<groups, 512, 0, st>>>(p);
+    linear_few_kernel<8, F16, false><<<groups, 512, 0, st>>>(p);
 }
 
 // Rows of K elements, any stride, into rows of `wide` >= K elements on 16-byte
@@ -983,7 +988,7 @@ extern "C" int dfs_linear(const void* x, int64_t x_stride, const void* w, int64_
   }
   switch (cut.form) {
     case kFew:
-      launch_few(p, f16, st);
+      f16 ? launch_few<true>(p, st) : launch_few<false>(p, st);
       break;
     case kFewAny: {
       const unsigned grid = static_cast<unsigned>((n + 15) / 16);
