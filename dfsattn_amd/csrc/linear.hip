@@ -374,7 +374,10 @@ __global__ void __launch_bounds__(512) linear_few_any_kernel(LinearParams p) {
 
 // Tiles of BN = 32 NI WN outputs by BM = 32 MI WM rows, a workgroup of WN x WM
 // = 4 waves with NI x MI products of 32 x 32 each, 64 channels a step through
-// two LDS buffers that the loads fill directly. For operands on 16-byte rows.
+// NS LDS buffers that the loads fill directly. For operands on 16-byte rows.
+// Few workgroups wait for memory unless several steps are on their way (64 x 64
+// alone on a CU: 0.5 us a step with two buffers, 0.26 with four); many hide it
+// from each other and want the room.
 //
 // A step's 128-byte rows hold eight 16-byte chunks; chunk c of row r lies at
 // c ^ f(r) with f such that any 16 rows that one quarter of a wave reads
@@ -384,9 +387,9 @@ __global__ void __launch_bounds__(512) linear_few_any_kernel(LinearParams p) {
 //
 // Order of a step: the fragments of a quarter (16 channels) are read while the
 // quarter before is multiplied; before the last quarter's products, the next
-// step's data is waited for and, behind the barrier, its successor's loads go
-// into the buffer just read. So there is one barrier a step, the products of a
-// quarter are there on both sides of it, and a load has a whole step to land.
+// step's data is waited for and, behind the barrier, the loads of the step NS on
+// go into the buffer just read. So there is one barrier a step, the products of
+// a quarter are there on both sides of it, and a load has NS - 1 steps to land.
 template <int NI, int MI, int WN, int WM, bool F16>
 struct Tile {
   static constexpr int BN = 32 * NI * WN, BM = 32 * MI * WM;
@@ -408,15 +411,15 @@ __device__ __forceinline__ void tile_of(int id, int mt, int nt, int& tm, int& tn
   tm = band * 4 + at - tn * rows;
 }
 
-template <int NI, int MI, int WN, int WM, bool F16>
+template <int NI, int MI, int WN, int WM, int NS, bool F16>
 __global__ void __launch_bounds__(256, 2) linear_tile_kernel(LinearParams p) {
   typedef Tile<NI, MI, WN, WM, F16> T;
   typedef typename T::vec vec;
   constexpr int JW = T::BN / 32, JX = T::BM / 32;  // loads of 1 KB a wave and step
-  __shared__ __attribute__((aligned(16))) uint16_t w0[T::BN * 64];
-  __shared__ __attribute__((aligned(16))) uint16_t x0[T::BM * 64];
-  __shared__ __attribute__((aligned(16))) uint16_t w1[T::BN * 64];
-  __shared__ __attribute__((aligned(16))) uint16_t x1[T::BM * 64];
+  // Of buffers 2 and 3, those past NS are empty.
+  constexpr int N2 = NS > 2 ? 64 : 1, N3 = NS > 3 ? 64 : 1;
+  __shared__ __attribute__((aligned(16))) uint16_t w0[T::BN * 64], w1[T::BN * 64], w2[T::BN * N2], w3[T::BN * N3];
+  __shared__ __attribute__((aligned(16))) uint16_t x0[T::BM * 64], x1[T::BM * 64], x2[T::BM * N2], x3[T::BM * N3];
   const int lane = threadIdx.x & 63, w = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const int l32 = lane & 31, hl = lane >> 5;
   const int mt = (p.M + T::BM - 1) / T::BM, nt = (p.N + T::BN - 1) / T::BN;
@@ -443,7 +446,7 @@ __global__ void __launch_bounds__(256, 2) linear_tile_kernel(LinearParams p) {
     xv[j] = static_cast<uint32_t>(min(m0 + r, p.M - 1) - m0) * static_cast<uint32_t>(p.ldx * 2) +
             (c8 ^ T::swz_x(r)) * 16;
   }
-  const int steps = (K + 127) >> 7 << 1;  // an even number: the last may be all zeros
+  const int steps = (K + 64 * NS - 1) / (64 * NS) * NS;  // the last may be all zeros
   auto issue = [&](int t, uint16_t* wb, uint16_t* xb) {
     const int left = K - t * 64;
     if (left < 64) {  // the last steps: chunks past K come as zeros
@@ -510,9 +513,9 @@ __global__ void __launch_bounds__(256, 2) linear_tile_kernel(LinearParams p) {
     multiply(a0, b0);
     pin(false);
     __builtin_amdgcn_sched_barrier(0);
-    wait_vmcnt_0();
+    wait_vmcnt<(NS - 2) * (JW + JX)>();
     block_barrier();
-    issue(t + 2, wc, xc);  // past the last step: zeros, without a memory access
+    issue(t + NS, wc, xc);  // past the last step: zeros, without a memory access
     fetch(wnext, xnext, 0, a0, b0);  // past the last step: read and not used
     multiply(a1, b1);
     pin(true);
@@ -520,12 +523,23 @@ __global__ void __launch_bounds__(256, 2) linear_tile_kernel(LinearParams p) {
   };
   issue(0, w0, x0);
   issue(1, w1, x1);
-  wait_vmcnt<JW + JX>();
+  if constexpr (NS > 2) issue(2, w2, x2);
+  if constexpr (NS > 3) issue(3, w3, x3);
+  wait_vmcnt<(NS - 1) * (JW + JX)>();
   block_barrier();
   fetch(w0, x0, 0, a0, b0);
-  for (int t = 0; t < steps; t += 2) {
+  for (int t = 0; t < steps; t += NS) {
     step(t, w0, x0, w1, x1);
-    step(t + 1, w1, x1, w0, x0);
+    if constexpr (NS == 2) step(t + 1, w1, x1, w0, x0);
+    if constexpr (NS == 3) {
+      step(t + 1, w1, x1, w2, x2);
+      step(t + 2, w2, x2, w0, x0);
+    }
+    if constexpr (NS == 4) {
+      step(t + 1, w1, x1, w2, x2);
+      step(t + 2, w2, x2, w3, x3);
+      step(t + 3, w3, x3, w0, x0);
+    }
   }
   wait_vmcnt_0();  // the trailing loads have landed before the workgroup's LDS is released
   const int nb = n0 + wn * 32 * NI + hl * 4 * NI, mb = m0 + wm * 32 * MI + l32;
@@ -814,14 +828,14 @@ __global__ void __launch_bounds__(256) linear_join_kernel(LinearParams p) {
   with_activation(p.act, [&](auto act) { finish8<F16, decltype(act)::value>(p, m, n, z, bias, gate); });
 }
 
-template <int NI, int MI, int WN, int WM>
+template <int NI, int MI, int WN, int WM, int NS>
 void launch_tile(const LinearParams& p, bool f16, hipStream_t st) {
   const int64_t mt = (p.M + 32 * MI * WM - 1) / (32 * MI * WM), nt = (p.N + 32 * NI * WN - 1) / (32 * NI * WN);
   const dim3 grid(static_cast<unsigned>(mt * nt * p.splits));
   if (f16)
-    linear_tile_kernel<NI, MI, WN, WM, true><<<grid, 256, 0, st>>>(p);
+    linear_tile_kernel<NI, MI, WN, WM, NS, true><<<grid, 256, 0, st>>>(p);
   else
-    linear_tile_kernel<NI, MI, WN, WM, false><<<grid, 256, 0, st>>>(p);
+    linear_tile_kernel<NI, MI, WN, WM, NS, false><<<grid, 256, 0, st>>>(p);
   if (p.splits > 1) {
     const int64_t threads = static_cast<int64_t>(p.M) * ((p.N + 7) / 8);
     const dim3 join(static_cast<unsigned>((threads + 255) / 256));
@@ -855,7 +869,7 @@ __global__ void __launch_bounds__(256) pad_rows_kernel(const uint16_t* src, int6
 }
 
 // How a product is cut: its form and, for the tiles, the parts of the channels.
-enum Form { kFew, kFewAny, kTileAny, kTile64, kTile128, kTile256 };
+enum Form { kFew, kFewAny, kTileAny, kTile64, kTile64x128, kTile128Deep, kTile128, kTile256 };
 struct Cut {
   Form form;
   int splits, depth;
@@ -868,27 +882,34 @@ Cut cut_of(int64_t rows, int64_t n, int64_t k, bool chunks) {
   if (!chunks && rows <= 16) return Cut{kFewAny, 1, 0, false};
   if (!chunks && rows * n * k < (int64_t(1) << 30)) return Cut{kTileAny, 1, 0, false};
   if (rows <= 8) return Cut{kFew, 1, 0, !chunks};
-  // The tiles and parts with the least time by what each took alone and in
-  // company, a step of 64 channels of a workgroup in us on one CU (CUs that get
-  // one workgroup more than others run it half hidden), and by writing and
-  // joining the parts' sums at 3 TB/s behind 5 us. Measured, us: 64 rows by
-  // 5,120 x 5,120 39.8 in one part, 18.8 in eight; 128 rows 41.0 and 22.6 in
-  // four; 512 by 5,120 x 4,096 37.8 with 64 x 64, 44.6 with 128 x 128, 70 with
-  // 256 x 256; 1,000 by 5,120 x 5,120 101, 73.6, 98.7; 1,560 140, 134, 102.7.
-  struct {
+  // The tiles and parts with the least time by what each took on an idle CU and
+  // beside others, a step of 64 channels of a workgroup in us, and by writing
+  // and joining the parts' sums at 3 TB/s behind 5 us. Where several fit on a
+  // CU, those that get one more than others run it half hidden. Measured, us,
+  // in the order below: 128 rows by 5,120 x 5,120 20.8, 28.5, 38.7, 58, 93; 256
+  // rows 34.9, 29.4, 39.8, 57, 84; 512 by 5,120 x 4,096 44.9, 38.8, 35.4, 44.6,
+  // 70; 1,000 by 5,120 x 5,120 96, 87, 83, 70, 98; 1,560 144, 129, 130, 132, 89;
+  // 64 rows in four parts of 64 x 64 17.3, in one 20.8.
+  const struct {
     Form form;
-    int tile, most;  // most: parts
-    double alone, shared;
-  } const kinds[3] = {{kTile64, 64, 8, 0.49, 0.235}, {kTile128, 128, 4, 0.72, 0.59}, {kTile256, 256, 1, 1.40, 1.40}};
+    int m, n, most;  // most: parts
+    bool single;     // one workgroup a CU
+    double alone, beside;
+  } kinds[5] = {{kTile64, 64, 64, 8, false, 0.26, 0.25},
+                {kTile64x128, 128, 64, 4, false, 0.36, 0.375},
+                {kTile128Deep, 128, 128, 2, true, 0.55, 0.55},
+                {kTile128, 128, 128, 4, false, 0.72, 0.57},
+                {kTile256, 256, 256, 1, true, 1.15, 1.4}};
   Cut best{kTile64, 1, 0, !chunks};
   double least = 1e30;
   for (const auto& f : kinds)
     for (int s = 1; s <= f.most; s *= 2) {
       const int64_t depth = ((k + s - 1) / s + 127) / 128 * 128, parts = (k + depth - 1) / depth;
       if (s > 1 && (depth < 256 || parts < 2)) break;
-      const int64_t groups = ((rows + f.tile - 1) / f.tile) * ((n + f.tile - 1) / f.tile) * parts;
-      const double each = 0.5 * (static_cast<double>((groups + 255) / 256) + static_cast<double>(groups) / 256.0);
-      double us = static_cast<double>(depth / 64) * std::max(f.alone, f.shared * each);
+      const int64_t groups = ((rows + f.m - 1) / f.m) * ((n + f.n - 1) / f.n) * parts;
+      const double full = static_cast<double>((groups + 255) / 256), part = static_cast<double>(groups) / 256.0;
+      const double each = f.single ? full : 0.5 * (full + part);
+      double us = static_cast<double>((depth + 63) / 64) * std::max(f.alone, f.beside * (f.single && full < 2 ? 0 : each));
       if (parts > 1) us += 5.0 + 8e-6 / 3.0 * static_cast<double>(parts * rows * n);
       if (us < least) {
         least = us;
@@ -1001,10 +1022,16 @@ extern "C" int dfs_linear(const void* x, int64_t x_stride, const void* w, int64_
       break;
     }
     case kTile64:
-      launch_tile<1, 1, 2, 2>(p, f16, st);
+      launch_tile<1, 1, 2, 2, 4>(p, f16, st);
+      break;
+    case kTile64x128:
+      launch_tile<1, 2, 2, 2, 3>(p, f16, st);
+      break;
+    case kTile128Deep:
+      launch_tile<2, 2, 2, 2, 3>(p, f16, st);
       break;
     case kTile128:
-      launch_tile<2, 2, 2, 2>(p, f16, st);
+      launch_tile<2, 2, 2, 2, 2>(p, f16, st);
       break;
     case kTile256: {
       const dim3 grid(static_cast<unsigned>(((rows + 255) / 256) * ((n + 255) / 256)));
