@@ -193,7 +193,8 @@ __global__ void __launch_bounds__(256) linear_any_kernel(LinearParams p) {
   __shared__ __attribute__((aligned(16))) uint16_t ws[64 * 64];
   __shared__ __attribute__((aligned(16))) uint16_t xs[64 * 64];
   const int tid = threadIdx.x, lane = tid & 63, w = tid >> 6, l32 = lane & 31, hl = lane >> 5;
-  const int n0 = blockIdx.x * 64, m0 = blockIdx.y * 64;
+  const unsigned nt = (p.N + 63) / 64;
+  const int m0 = static_cast<int>(blockIdx.x / nt) * 64, n0 = static_cast<int>(blockIdx.x % nt) * 64;
   f32x16 acc = f32x16{};
   uint4 a[2], b[2];  // a step's chunks, loaded under the products of the one before
   auto load = [&](int k0) {
@@ -971,6 +972,7 @@ extern "C" int dfs_linear(const void* x, int64_t x_stride, const void* w, int64_
   DFS_REQUIRE(need == 0 || (workspace != nullptr && workspace_bytes >= need && addr(workspace) % 16 == 0),
               "%s: a 16-byte aligned workspace of %lld bytes is needed", name, (long long)need);
   DFS_REQUIRE(!cut.pad || k < (1 << 21), "%s: k=%lld must be below 2^21 for operands off 16-byte rows", name, (long long)k);
+  DFS_REQUIRE(((rows + 63) / 64) * ((n + 63) / 64) * cut.splits < (int64_t(1) << 31), "%s: too many outputs", name);
   LinearParams p{};
   p.x = static_cast<const uint16_t*>(x);
   p.w = static_cast<const uint16_t*>(w);
@@ -1017,7 +1019,7 @@ extern "C" int dfs_linear(const void* x, int64_t x_stride, const void* w, int64_
       break;
     }
     case kTileAny: {
-      const dim3 grid(static_cast<unsigned>((n + 63) / 64), static_cast<unsigned>((rows + 63) / 64));
+      const unsigned grid = static_cast<unsigned>(((n + 63) / 64) * ((rows + 63) / 64));
       f16 ? linear_any_kernel<true><<<grid, 256, 0, st>>>(p) : linear_any_kernel<false><<<grid, 256, 0, st>>>(p);
       break;
     }

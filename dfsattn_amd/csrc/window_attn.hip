@@ -599,26 +599,29 @@ __global__ void __launch_bounds__(64, 2) window_few_kernel(WindowParams p) {
 }
 
 // Joins the parts of a row: O = sum 2^(m_i - M) O_i over the same sum of l_i.
-// A part without keys (l = 0) has no weight; NaN reaches its row. D / 4 lanes a
-// row.
+// A part without keys (l = 0) has no weight; NaN reaches its row. FEW: a
+// workgroup a row, whose parts may be hundreds (a row by 32,768 keys in 256
+// parts: 4 us, 32 with a wave a row); otherwise a wave. Groups of D / 4 lanes
+// share the parts and are added up in a fixed order.
 template <int D, bool F16, bool FEW>
 __global__ void __launch_bounds__(256) window_join_kernel(WindowParams p) {
-  constexpr int LANES = D / 4;
-  const int lane = threadIdx.x % LANES;
-  const int64_t id = static_cast<int64_t>(blockIdx.x) * (256 / LANES) + threadIdx.x / LANES;
+  constexpr int LANES = D / 4, WAVES = FEW ? 4 : 1, GROUPS = 64 * WAVES / LANES;
+  __shared__ float4 so[4][LANES];
+  __shared__ float sl[4], sm[4];
+  const int lane = threadIdx.x & 63, w = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), sub = lane % LANES;
+  const int grp = (FEW ? static_cast<int>(threadIdx.x) : lane) / LANES;
+  const int64_t id = FEW ? blockIdx.x : static_cast<int64_t>(blockIdx.x) * 4 + w;
   const int rows = p.Lq * p.group;
   int bh, r;
   int64_t first, step;  // row of the first part, rows between parts
   if (FEW) {
     bh = static_cast<int>(id / rows);
     r = static_cast<int>(id - static_cast<int64_t>(bh) * rows);
-    if (bh >= p.B * p.Hkv) return;
     first = static_cast<int64_t>(bh) * p.parts * rows + r;
     step = rows;
   } else {
     const int block = static_cast<int>(id >> 7), x = block & 7, i = p.whole + (block >> 3);
     const int per = (p.blocks + p.chunks - 1) / p.chunks;
-    if (block >= p.split * 8) return;
     const int u = i / per * 8 + x;
     bh = u / p.chunks;
     const int blk = p.blocks - 1 - (u % p.chunks * per + i % per);
@@ -628,24 +631,53 @@ __global__ void __launch_bounds__(256) window_join_kernel(WindowParams p) {
     step = 128;
   }
   float M = -INFINITY;
-  for (int i = 0; i < p.parts; ++i) M = fmaxf(M, p.part_ml[(first + i * step) * 2]);
+  for (int i = FEW ? threadIdx.x : lane; i < p.parts; i += 64 * WAVES) M = fmaxf(M, p.part_ml[(first + i * step) * 2]);
+#pragma unroll
+  for (int off = 32; off >= 1; off >>= 1) M = fmaxf(M, __shfl_xor(M, off, 64));
+  if (FEW) {
+    if (lane == 0) sm[w] = M;
+    __syncthreads();
+    M = fmaxf(fmaxf(sm[0], sm[1]), fmaxf(sm[2], sm[3]));
+  }
   const float ref = M == -INFINITY ? 0.f : M;
   float l = 0.f, o[4] = {};
-  for (int i = 0; i < p.parts; ++i) {
+#pragma unroll 8
+  for (int i = grp; i < p.parts; i += GROUPS) {
     const float2 ml = *reinterpret_cast<const float2*>(p.part_ml + (first + i * step) * 2);
-    const float4 v = *reinterpret_cast<const float4*>(p.part_o + (first + i * step) * D + lane * 4);
-    const float a = exp2_fast(ml.x - ref);
-    if (ml.y == 0.f) continue;  // rows of a dead or keyless part hold no O
+    float4 v = *reinterpret_cast<const float4*>(p.part_o + (first + i * step) * D + sub * 4);
+    const bool none = ml.y == 0.f;  // rows behind a sequence may hold anything
+    const float a = none ? 0.f : exp2_fast(ml.x - ref);
+    if (none) v = make_float4(0.f, 0.f, 0.f, 0.f);
     l += a * ml.y;
     o[0] += a * v.x; o[1] += a * v.y; o[2] += a * v.z; o[3] += a * v.w;
+  }
+#pragma unroll
+  for (int off = LANES; off < 64; off *= 2) {
+    l += __shfl_xor(l, off, 64);
+#pragma unroll
+    for (int i = 0; i < 4; ++i) o[i] += __shfl_xor(o[i], off, 64);
+  }
+  if (FEW) {
+    if (lane < LANES) so[w][sub] = make_float4(o[0], o[1], o[2], o[3]);
+    if (lane == 0) sl[w] = l;
+    __syncthreads();
+    if (threadIdx.x >= LANES) return;
+    l = (sl[0] + sl[1]) + (sl[2] + sl[3]);
+    const float4 a = so[0][sub], b = so[1][sub], c = so[2][sub], d = so[3][sub];
+    o[0] = (a.x + b.x) + (c.x + d.x);
+    o[1] = (a.y + b.y) + (c.y + d.y);
+    o[2] = (a.z + b.z) + (c.z + d.z);
+    o[3] = (a.w + b.w) + (c.w + d.w);
+  } else if (lane >= LANES) {
+    return;
   }
   const float inv = l == 0.f ? 0.f : 1.f / l;
   const int b = bh / p.Hkv, g = bh - b * p.Hkv;
   const Row row = row_of(p, r);
   const int head = g * p.group + row.g;
-  *reinterpret_cast<uint2*>(p.out + b * p.o_sb + head * p.o_sh + row.i * p.o_sl + lane * 4) =
+  *reinterpret_cast<uint2*>(p.out + b * p.o_sb + head * p.o_sh + row.i * p.o_sl + sub * 4) =
       make_uint2(pack2<F16>(o[0] * inv, o[1] * inv), pack2<F16>(o[2] * inv, o[3] * inv));
-  if (p.lse && lane == 0) p.lse[(static_cast<int64_t>(b) * p.Hq + head) * p.Lq + row.i] = lse_of(M, l);
+  if (p.lse && sub == 0) p.lse[(static_cast<int64_t>(b) * p.Hq + head) * p.Lq + row.i] = lse_of(M, l);
 }
 
 // How a call is cut. Slots for two workgroups on each of 256 CUs; the blocks
@@ -711,12 +743,12 @@ void launch(const WindowParams& p, hipStream_t st) {
     else
       window_few_kernel<D, F16, ROLL, false><<<heads * p.parts, 64, 0, st>>>(p);
     const int64_t rows = static_cast<int64_t>(heads) * p.Lq * p.group;
-    if (p.parts > 1) window_join_kernel<D, F16, true><<<static_cast<unsigned>((rows * (D / 4) + 255) / 256), 256, 0, st>>>(p);
+    if (p.parts > 1) window_join_kernel<D, F16, true><<<static_cast<unsigned>(rows), 256, 0, st>>>(p);
     return;
   }
   window_tile_kernel<D, F16, ROLL><<<8u * (p.whole + p.split * p.parts), 256, 0, st>>>(p);
   if (p.parts > 1)
-    window_join_kernel<D, F16, false><<<static_cast<unsigned>(p.split * 8 * 128 / (1024 / D)), 256, 0, st>>>(p);
+    window_join_kernel<D, F16, false><<<static_cast<unsigned>(p.split * 8 * 32), 256, 0, st>>>(p);
 }
 
 }  // namespace

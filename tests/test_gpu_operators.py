@@ -157,6 +157,11 @@ ATTENTION = [
     (1, 1, 1, 140, 300, 128, BF, 0, 0, 200, None, None, False),
     (2, 2, 1, 33, 90, 128, BF, 40, 3, 7, [0, 33], [90, 0], False),
     (1, 5, 5, 260, 260, 64, BF, 128, 128, 128, None, None, False),
+    # keys cut into parts: many for one sequence, with rows that see few or none of them
+    (1, 4, 1, 2, 5003, 128, BF, None, 0, 0, None, None, False),
+    (2, 3, 1, 1, 4100, 64, HF, None, 0, 0, None, [4100, 130], False),
+    (2, 8, 1, 40, 3000, 128, BF, None, 0, 0, [40, 3], [3000, 5], False),
+    (1, 2, 2, 70, 2600, 64, HF, 2400, None, 100, None, [9000], True),
 ]
 
 
