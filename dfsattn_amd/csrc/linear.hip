@@ -34,7 +34,6 @@ struct LinearParams {
   const float* gate;         // [N] or NULL
   const uint16_t* residual;  // [M][N], row stride ldr, or NULL; may be out
   uint16_t* out;
-  int wide;  // rows of out and residual allow 16-byte accesses at multiples of 8
   // The channels of a tile are cut into `splits` parts of `depth` (a multiple
   // of 128); a part's sums go to part [split][M][ceil(N / 8) * 8] in fp32.
   int splits, depth;
@@ -123,7 +122,7 @@ __device__ __forceinline__ void load_columns8(const LinearParams& p, int n, floa
 }
 
 // Eight consecutive outputs n.. of row m from their sums, all of them inside
-// the matrix and on a 16-byte boundary.
+// the matrix; 16-byte accesses at any 2-byte address.
 template <bool F16, int ACT>
 __device__ __forceinline__ void finish8_wide(const LinearParams& p, int m, int n, const float* z, const float* bias,
                                              const float* gate) {
@@ -135,16 +134,17 @@ __device__ __forceinline__ void finish8_wide(const LinearParams& p, int m, int n
     for (int i = 0; i < 8; ++i) y[i] *= gate[i];
   }
   if (p.residual) {
-    const uint4 rv = *reinterpret_cast<const uint4*>(p.residual + m * p.ldr + n);
+    uint4 rv;
+    __builtin_memcpy(&rv, p.residual + m * p.ldr + n, 16);
 #pragma unroll
     for (int i = 0; i < 8; ++i) y[i] += Half<F16>::to_f32(u16_at(rv, i));
   }
-  *reinterpret_cast<uint4*>(p.out + m * p.ldo + n) =
-      make_uint4(Half<F16>::pack(y[0], y[1]), Half<F16>::pack(y[2], y[3]), Half<F16>::pack(y[4], y[5]),
-                 Half<F16>::pack(y[6], y[7]));
+  const uint4 packed = make_uint4(Half<F16>::pack(y[0], y[1]), Half<F16>::pack(y[2], y[3]),
+                                  Half<F16>::pack(y[4], y[5]), Half<F16>::pack(y[6], y[7]));
+  __builtin_memcpy(p.out + m * p.ldo + n, &packed, 16);
 }
 
-// The same at the matrix's edge, or for rows on no 16-byte boundary.
+// The same at the matrix's edge.
 template <bool F16, int ACT>
 __device__ __forceinline__ void finish8_edge(const LinearParams& p, int m, int n, const float* z, const float* bias,
                                              const float* gate) {
@@ -163,7 +163,7 @@ template <bool F16, int ACT>
 __device__ __forceinline__ void finish8(const LinearParams& p, int m, int n, const float* z, const float* bias,
                                         const float* gate) {
   if (m >= p.M || n >= p.N) return;
-  if (p.wide && n + 8 <= p.N)
+  if (n + 8 <= p.N)
     finish8_wide<F16, ACT>(p, m, n, z, bias, gate);
   else
     finish8_edge<F16, ACT>(p, m, n, z, bias, gate);
@@ -765,7 +765,7 @@ __global__ void __launch_bounds__(256, 1) linear_big_kernel(LinearParams p) {
   // sums go through LDS, 32 rows x 64 outputs at a time, in the wave's own part
   // of it: whole rows of 128 bytes leave (and come, for the residual).
   float* const st = stage + w * 2048;
-  const bool inside = p.wide && m0 + 256 <= p.M && n0 + 256 <= p.N;
+  const bool inside = m0 + 256 <= p.M && n0 + 256 <= p.N;
 #pragma unroll
   for (int gp = 0; gp < 2; ++gp) {
     const int n = n0 + wn * 128 + gp * 64 + (lane & 7) * 8, c = (lane & 7) * 2;
@@ -989,7 +989,6 @@ extern "C" int dfs_linear(const void* x, int64_t x_stride, const void* w, int64_
   p.gate = gate;
   p.residual = static_cast<const uint16_t*>(residual);
   p.out = static_cast<uint16_t*>(out);
-  p.wide = o_stride % 8 == 0 && addr(out) % 16 == 0 && (!residual || (r_stride % 8 == 0 && addr(residual) % 16 == 0));
   hipStream_t st = reinterpret_cast<hipStream_t>(stream);
   p.splits = cut.splits;
   p.depth = cut.depth;

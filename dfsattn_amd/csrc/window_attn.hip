@@ -599,18 +599,18 @@ __global__ void __launch_bounds__(64, 2) window_few_kernel(WindowParams p) {
 }
 
 // Joins the parts of a row: O = sum 2^(m_i - M) O_i over the same sum of l_i.
-// A part without keys (l = 0) has no weight; NaN reaches its row. FEW: a
-// workgroup a row, whose parts may be hundreds (a row by 32,768 keys in 256
-// parts: 4 us, 32 with a wave a row); otherwise a wave. Groups of D / 4 lanes
-// share the parts and are added up in a fixed order.
-template <int D, bool F16, bool FEW>
+// A part without keys (l = 0) has no weight; NaN reaches its row. WAVES: one
+// wave a row, or four where the parts are many (a row by 32,768 keys in 256
+// parts: 4 us, 32 with one). Groups of D / 4 lanes share the parts and are added
+// up in a fixed order.
+template <int D, bool F16, bool FEW, int WAVES>
 __global__ void __launch_bounds__(256) window_join_kernel(WindowParams p) {
-  constexpr int LANES = D / 4, WAVES = FEW ? 4 : 1, GROUPS = 64 * WAVES / LANES;
+  constexpr int LANES = D / 4, GROUPS = 64 * WAVES / LANES;
   __shared__ float4 so[4][LANES];
   __shared__ float sl[4], sm[4];
   const int lane = threadIdx.x & 63, w = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), sub = lane % LANES;
-  const int grp = (FEW ? static_cast<int>(threadIdx.x) : lane) / LANES;
-  const int64_t id = FEW ? blockIdx.x : static_cast<int64_t>(blockIdx.x) * 4 + w;
+  const int grp = (WAVES == 4 ? static_cast<int>(threadIdx.x) : lane) / LANES;
+  const int64_t id = WAVES == 4 ? blockIdx.x : static_cast<int64_t>(blockIdx.x) * 4 + w;
   const int rows = p.Lq * p.group;
   int bh, r;
   int64_t first, step;  // row of the first part, rows between parts
@@ -631,10 +631,10 @@ __global__ void __launch_bounds__(256) window_join_kernel(WindowParams p) {
     step = 128;
   }
   float M = -INFINITY;
-  for (int i = FEW ? threadIdx.x : lane; i < p.parts; i += 64 * WAVES) M = fmaxf(M, p.part_ml[(first + i * step) * 2]);
+  for (int i = WAVES == 4 ? threadIdx.x : lane; i < p.parts; i += 64 * WAVES) M = fmaxf(M, p.part_ml[(first + i * step) * 2]);
 #pragma unroll
   for (int off = 32; off >= 1; off >>= 1) M = fmaxf(M, __shfl_xor(M, off, 64));
-  if (FEW) {
+  if (WAVES == 4) {
     if (lane == 0) sm[w] = M;
     __syncthreads();
     M = fmaxf(fmaxf(sm[0], sm[1]), fmaxf(sm[2], sm[3]));
@@ -657,7 +657,7 @@ __global__ void __launch_bounds__(256) window_join_kernel(WindowParams p) {
 #pragma unroll
     for (int i = 0; i < 4; ++i) o[i] += __shfl_xor(o[i], off, 64);
   }
-  if (FEW) {
+  if (WAVES == 4) {
     if (lane < LANES) so[w][sub] = make_float4(o[0], o[1], o[2], o[3]);
     if (lane == 0) sl[w] = l;
     __syncthreads();
@@ -743,12 +743,15 @@ void launch(const WindowParams& p, hipStream_t st) {
     else
       window_few_kernel<D, F16, ROLL, false><<<heads * p.parts, 64, 0, st>>>(p);
     const int64_t rows = static_cast<int64_t>(heads) * p.Lq * p.group;
-    if (p.parts > 1) window_join_kernel<D, F16, true><<<static_cast<unsigned>(rows), 256, 0, st>>>(p);
+    if (p.parts > 1) window_join_kernel<D, F16, true, 4><<<static_cast<unsigned>(rows), 256, 0, st>>>(p);
     return;
   }
   window_tile_kernel<D, F16, ROLL><<<8u * (p.whole + p.split * p.parts), 256, 0, st>>>(p);
-  if (p.parts > 1)
-    window_join_kernel<D, F16, false><<<static_cast<unsigned>(p.split * 8 * 32), 256, 0, st>>>(p);
+  const unsigned cut = static_cast<unsigned>(p.split) * 8 * 128;  // rows of the blocks that were
+  if (p.parts > 8)
+    window_join_kernel<D, F16, false, 4><<<cut, 256, 0, st>>>(p);
+  else if (p.parts > 1)
+    window_join_kernel<D, F16, false, 1><<<cut / 4, 256, 0, st>>>(p);
 }
 
 }  // namespace
