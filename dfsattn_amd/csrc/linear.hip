@@ -9,7 +9,7 @@
 // and its columns rows m of x, so a lane holds one row of out. Its register
 // groups cover 4 consecutive n; the A operand's rows are dealt to the tiles so
 // that the groups of a wave's tiles join into 8 or 16 consecutive n and leave
-// as 16-byte stores (TileRows).
+// as 16-byte stores.
 #include <algorithm>
 #include <type_traits>
 
@@ -322,52 +322,6 @@ __global__ void __launch_bounds__(64 * WAVES) linear_few_kernel(LinearParams p) 
     step(b + 2 * WAVES, s2, s1);
   }
   wait_vmcnt_0();
-  *reinterpret_cast<f32x4*>(sums + (w * 64 + lane) * 4) = acc;
-  __syncthreads();
-  finish16<F16>(p, n0, sums, WAVES);
-}
-
-// The same for rows on no 16-byte boundary, which only loads into registers
-// take, there in the products' layout.
-template <bool F16>
-__global__ void __launch_bounds__(512) linear_few_any_kernel(LinearParams p) {
-  typedef typename Half<F16>::vec vec;
-  constexpr int WAVES = 8;
-  __shared__ __attribute__((aligned(16))) float sums[WAVES * 256];
-  const int lane = threadIdx.x & 63, w = threadIdx.x >> 6;
-  const int r16 = lane & 15, kc = (lane >> 4) * 8;
-  const int n0 = blockIdx.x * 16;
-  const uint16_t* const wr = p.w + min(n0 + r16, p.N - 1) * p.ldw;
-  const uint16_t* const xr = p.x + min(r16, p.M - 1) * p.ldx;
-  f32x4 acc = f32x4{};
-  struct Block {
-    uint4 a[4], b[4];
-  };
-  auto load = [&](int k0, Block& f) {
-#pragma unroll
-    for (int s = 0; s < 4; ++s) {
-      const int k = k0 + s * 32 + kc;
-      f.a[s] = load_row8(wr, k, p.K);
-      f.b[s] = r16 < p.M ? load_row8(xr, k, p.K) : make_uint4(0, 0, 0, 0);
-    }
-  };
-  auto multiply = [&](const Block& f) {
-#pragma unroll
-    for (int s = 0; s < 4; ++s)
-      acc = Half<F16>::mfma16(__builtin_bit_cast(vec, f.a[s]), __builtin_bit_cast(vec, f.b[s]), acc);
-  };
-  constexpr int kHop = WAVES * 128;
-  if (w * 128 < p.K) {
-    Block f, g;
-    load(w * 128, f);
-    for (int k0 = w * 128; k0 < p.K; k0 += 2 * kHop) {  // the block after is on its way
-      if (k0 + kHop < p.K) load(k0 + kHop, g);
-      multiply(f);
-      if (k0 + kHop >= p.K) break;
-      if (k0 + 2 * kHop < p.K) load(k0 + 2 * kHop, f);
-      multiply(g);
-    }
-  }
   *reinterpret_cast<f32x4*>(sums + (w * 64 + lane) * 4) = acc;
   __syncthreads();
   finish16<F16>(p, n0, sums, WAVES);
@@ -858,30 +812,31 @@ void launch_few(const LinearParams& p, hipStream_t st) {
     linear_few_kernel<8, F16, false><<<groups, 512, 0, st>>>(p);
 }
 
-// Rows of K elements, any stride, into rows of `wide` >= K elements on 16-byte
-// boundaries, zeros behind the K: eight elements a thread.
-__global__ void __launch_bounds__(256) pad_rows_kernel(const uint16_t* src, int64_t ld, int64_t rows, int K, int wide,
-                                                       uint16_t* dst) {
-  const int64_t id = static_cast<int64_t>(blockIdx.x) * 256 + threadIdx.x;
-  const int chunks = wide / 8;
-  const int64_t r = id / chunks;
-  const int c = static_cast<int>(id - r * chunks);
-  if (r < rows) *reinterpret_cast<uint4*>(dst + id * 8) = load_row8(src + r * ld, c * 8, K);
+// The rows of x, then those of w, K elements each at any stride, into rows of
+// `wide` >= K elements on 16-byte boundaries, zeros behind the K: eight elements
+// a thread, a row a grid row.
+__global__ void __launch_bounds__(256) pad_rows_kernel(LinearParams p, int wide, uint16_t* dst) {
+  const int k = (blockIdx.x * 256 + threadIdx.x) * 8;
+  if (k >= wide) return;
+  for (int r = blockIdx.y; r < p.M + p.N; r += gridDim.y) {
+    const uint16_t* const src = r < p.M ? p.x + r * p.ldx : p.w + (r - p.M) * p.ldw;
+    *reinterpret_cast<uint4*>(dst + static_cast<int64_t>(r) * wide + k) = load_row8(src, k, p.K);
+  }
 }
 
 // How a product is cut: its form and, for the tiles, the parts of the channels.
-enum Form { kFew, kFewAny, kTileAny, kTile64, kTile64x128, kTile128Deep, kTile128, kTile256 };
+enum Form { kFew, kTileAny, kTile64, kTile64x128, kTile128Deep, kTile128, kTile256 };
 struct Cut {
   Form form;
   int splits, depth;
   bool pad;  // operands are laid out on 16-byte rows first
 };
 Cut cut_of(int64_t rows, int64_t n, int64_t k, bool chunks) {
-  // Rows on no 16-byte boundary: as they are where little is computed with
-  // what is read (padding took a row's time again and more), laid out anew
-  // otherwise.
-  if (!chunks && rows <= 16) return Cut{kFewAny, 1, 0, false};
-  if (!chunks && rows * n * k < (int64_t(1) << 30)) return Cut{kTileAny, 1, 0, false};
+  // Rows on no 16-byte boundary: small products of few steps as they are, the
+  // others laid out anew (us, as they are and anew: 333 by 1,017 x 709 10.5 and
+  // 11.3, 100 by 5,119 x 1,001 13.1 and 15.9; 400 by 1,001 x 3,001 29.0 and
+  // 23.1, 1 by 5,119 x 5,119 54.6 and 29.5, 6,694 by 1,422 x 5,465 370 and 148).
+  if (!chunks && k <= 1024 && rows * n * k < (int64_t(1) << 30)) return Cut{kTileAny, 1, 0, false};
   if (rows <= 8) return Cut{kFew, 1, 0, !chunks};
   // The tiles and parts with the least time by what each took on an idle CU and
   // beside others, a step of 64 channels of a workgroup in us, and by writing
@@ -997,12 +952,8 @@ extern "C" int dfs_linear(const void* x, int64_t x_stride, const void* w, int64_
   if (cut.pad) {
     uint16_t* const wide = reinterpret_cast<uint16_t*>(static_cast<char*>(workspace) + part_bytes(cut, rows, n));
     const int64_t kp = padded(k);
-    auto lay = [&](const uint16_t* src, int64_t ld, int64_t count, uint16_t* dst) {
-      const unsigned grid = static_cast<unsigned>((count * kp / 8 + 255) / 256);
-      pad_rows_kernel<<<grid, 256, 0, st>>>(src, ld, count, static_cast<int>(k), static_cast<int>(kp), dst);
-    };
-    lay(p.x, p.ldx, rows, wide);
-    lay(p.w, p.ldw, n, wide + rows * kp);
+    const dim3 grid(static_cast<unsigned>((kp + 2047) / 2048), static_cast<unsigned>(std::min<int64_t>(rows + n, 65535)));
+    pad_rows_kernel<<<grid, 256, 0, st>>>(p, static_cast<int>(kp), wide);
     p.x = wide;
     p.w = wide + rows * kp;
     p.ldx = p.ldw = kp;
@@ -1012,11 +963,6 @@ extern "C" int dfs_linear(const void* x, int64_t x_stride, const void* w, int64_
     case kFew:
       f16 ? launch_few<true>(p, st) : launch_few<false>(p, st);
       break;
-    case kFewAny: {
-      const unsigned grid = static_cast<unsigned>((n + 15) / 16);
-      f16 ? linear_few_any_kernel<true><<<grid, 512, 0, st>>>(p) : linear_few_any_kernel<false><<<grid, 512, 0, st>>>(p);
-      break;
-    }
     case kTileAny: {
       const unsigned grid = static_cast<unsigned>(((n + 63) / 64) * ((rows + 63) / 64));
       f16 ? linear_any_kernel<true><<<grid, 256, 0, st>>>(p) : linear_any_kernel<false><<<grid, 256, 0, st>>>(p);
