@@ -79,7 +79,9 @@ __device__ __forceinline__ float group_sum(float v, int lanes) {
 // registers (16 bytes a lane and step of 512 channels; D divides 512, so a
 // lane's channels lie at the same place of every head and one slice of the
 // table row serves them all). Everything that does not hang on the sequence's
-// length is loaded while that is on its way.
+// length is loaded while that is on its way. Bound by memory: 3,600 tokens x 40
+// heads in 41 us (223 MB, 5.4 TB/s), 65 with sums through LDS, 64-bit divisions
+// and the loads behind the length; 32 single tokens 6.9 us (11.6), latency.
 template <int NCH, bool F16>
 __global__ void __launch_bounds__(256) qkv_cache_kernel(CacheParams p) {
   const int lane = threadIdx.x & 63, n = blockIdx.y;

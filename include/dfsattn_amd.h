@@ -508,8 +508,10 @@ int dfs_linear(const void* x, int64_t x_stride, const void* w, int64_t w_stride,
  * nk = kv_lens[b] keys (slots without kv_lens; device int32, clamped to the
  * tensors): query i stands at position p = nk - nq + i and sees key j where
  * j < nk, j <= p + right and (j >= p - left or j < sinks); left and right -1:
- * no limit. Rows that see no key, rows from nq on among them, are 0 and their
- * lse (fp32 [B][q_heads][q_rows], optional) is -inf.
+ * no limit. Keys and values behind nk may hold anything; keys that a row does
+ * not see too, but values inside the sequence must be finite (their weight of
+ * 0 is multiplied). Rows that see no key, rows from nq on among them, are 0 and
+ * their lse (fp32 [B][q_heads][q_rows], optional) is -inf.
  * rolling: key j lies in slot j < sinks ? j : sinks + (j - sinks) mod
  * (slots - sinks); kv_lens counts all keys ever written and slots - sinks must
  * be at least left + q_rows. The workspace is the caller's,
