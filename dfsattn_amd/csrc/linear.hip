@@ -915,7 +915,7 @@ extern "C" int dfs_linear(const void* x, int64_t x_stride, const void* w, int64_
   DFS_REQUIRE(rows > 0 && n > 0 && k > 0, "%s: rows=%lld n=%lld k=%lld must be positive", name, (long long)rows,
               (long long)n, (long long)k);
   constexpr int64_t kMax = int64_t(1) << 30;
-  DFS_REQUIRE(rows < kMax && n < kMax && k < kMax, "%s: rows, n and k must be below 2^30", name);
+  DFS_REQUIRE(rows < kMax && n < kMax && k < (1 << 21), "%s: rows and n must be below 2^30, k below 2^21", name);
   DFS_REQUIRE(dtype == DFS_DTYPE_BF16 || dtype == DFS_DTYPE_F16, "%s: dtype must be bf16 or f16", name);
   DFS_REQUIRE(x_stride >= 0 && w_stride >= 0 && o_stride >= n && (!residual || r_stride >= 0),
               "%s: strides must be non-negative, and out's rows must not overlap", name);
@@ -934,8 +934,9 @@ extern "C" int dfs_linear(const void* x, int64_t x_stride, const void* w, int64_
   const int64_t need = workspace_bytes_of(cut, rows, n, k);
   DFS_REQUIRE(need == 0 || (workspace != nullptr && workspace_bytes >= need && addr(workspace) % 16 == 0),
               "%s: a 16-byte aligned workspace of %lld bytes is needed", name, (long long)need);
-  DFS_REQUIRE(!cut.pad || k < (1 << 21), "%s: k=%lld must be below 2^21 for operands off 16-byte rows", name, (long long)k);
-  DFS_REQUIRE(((rows + 63) / 64) * ((n + 63) / 64) * cut.splits < (int64_t(1) << 31), "%s: too many outputs", name);
+  // A launch holds fewer than 2^32 threads.
+  DFS_REQUIRE(((rows + 63) / 64) * ((n + 63) / 64) * cut.splits < (1 << 24) && (cut.form != kFew || n < (1 << 27)),
+              "%s: too many outputs", name);
   LinearParams p{};
   p.x = static_cast<const uint16_t*>(x);
   p.w = static_cast<const uint16_t*>(w);

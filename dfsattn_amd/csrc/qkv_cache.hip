@@ -202,7 +202,7 @@ extern "C" int dfs_qkv_cache(const dfs_cache_args* a, dfs_stream_t stream) {
               "%s: heads*head_dim = %lld exceeds %d", name, (long long)widest, 512 * kMaxChunks);
   DFS_REQUIRE(a->dtype == DFS_DTYPE_BF16 || a->dtype == DFS_DTYPE_F16, "%s: dtype must be bf16 or f16", name);
   constexpr int64_t kMax = int64_t(1) << 30;
-  DFS_REQUIRE(a->batch < kMax && a->tokens < kMax && a->slots < kMax && a->batch * a->tokens < kMax,
+  DFS_REQUIRE(a->batch < kMax && a->tokens < kMax && a->slots < kMax && a->batch * a->tokens < (1 << 26) - 4,
               "%s: sizes too large", name);
   DFS_REQUIRE(a->sinks >= 0, "%s: sinks must not be negative", name);
   DFS_REQUIRE(!a->rolling || a->tokens <= a->slots - a->sinks,

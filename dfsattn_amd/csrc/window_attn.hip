@@ -847,8 +847,9 @@ extern "C" int dfs_window_attention(const dfs_window_args* a, dfs_stream_t strea
               "%s: a 16-byte aligned workspace of %lld bytes is needed", name, (long long)need);
   p.part_o = static_cast<float*>(a->workspace);
   p.part_ml = p.part_o + spare * a->head_dim;
-  DFS_REQUIRE((p.whole + static_cast<int64_t>(p.split) * p.parts) * 8 < (int64_t(1) << 31) &&
-                  a->batch * a->kv_heads * p.parts < (int64_t(1) << 31) && a->q_rows * p.group < kNoLimit,
+  // A launch holds fewer than 2^32 threads.
+  DFS_REQUIRE((p.whole + static_cast<int64_t>(p.split) * p.parts) * 8 < (1 << 24) &&
+                  a->batch * a->kv_heads * p.parts < (1 << 26) && a->q_rows * p.group < kNoLimit,
               "%s: too many rows", name);
   hipStream_t st = reinterpret_cast<hipStream_t>(stream);
   const bool f16 = a->dtype == DFS_DTYPE_F16, roll = p.rolling;

@@ -845,7 +845,7 @@ def linear(x: torch.Tensor, weight: torch.Tensor, bias: Optional[torch.Tensor] =
     "gelu" (erf form) or "silu". Sums and the epilogue are fp32, rounded once
     to x's dtype (bf16 or f16). ``out`` may be the residual itself. No
     backward pass."""
-    _refuse_grad("linear", x, weight, bias, gate, residual)
+    _refuse_grad("linear", x, weight, bias, gate, residual, out)
     rows, shape, ldx, ldw, ldr = _linear_plan(
         x.shape, x.stride(), weight.shape, weight.stride(), x.dtype, weight.dtype, activation,
         None if residual is None else residual.shape, None if residual is None else residual.stride())
@@ -898,7 +898,7 @@ def _limit(entry: str, name: str, n: Optional[int]) -> int:
         return -1
     if int(n) < 0:
         raise ValueError(f"{entry}: {name} must be None (no limit) or not negative, got {n}")
-    return int(n)
+    return min(int(n), 1 << 40)  # behind every length
 
 
 def _pointers(block: ctypes.Structure, first: str) -> int:
@@ -935,7 +935,7 @@ def _window_plan(q_shape: Shape, q_stride: Shape, k_shape: Shape, k_stride: Shap
     if rolling and (not lens or lo < 0 or slots < sinks + lo + rows):
         raise ValueError(f"{entry}: a rolling cache needs kv_lens, left and at least sinks + left + L slots, got "
                          f"{slots} for sinks={sinks}, left={left}, L={rows}")
-    scale = 1.0 / math.sqrt(dim) if scale is None else float(scale)
+    scale = 1.0 / math.sqrt(dim) if scale is None else scale
     if not 0.0 < scale < 1e30:
         raise ValueError(f"{entry}: scale must be positive and finite, got {scale}")
     if out_stride is None:  # q's storage order, where it leaves no gaps
@@ -946,7 +946,8 @@ def _window_plan(q_shape: Shape, q_stride: Shape, k_shape: Shape, k_stride: Shap
     strides = [_axis_strides(shape, stride) for shape, stride in qkv]
     a = _lib.WindowArgs()
     a.batch, a.q_heads, a.kv_heads, a.q_rows, a.slots, a.head_dim = batch, heads, groups, rows, slots, dim
-    a.dtype, a.left, a.right, a.sinks, a.rolling = DTYPE_CODE[dtypes[0]], lo, hi, sinks, int(rolling)
+    a.dtype, a.left, a.right, a.rolling = DTYPE_CODE[dtypes[0]], lo, hi, int(rolling)
+    a.sinks = _limit(entry, "sinks", sinks)
     (a.q_batch_stride, a.q_head_stride, a.q_row_stride, _), (a.k_batch_stride, a.k_head_stride, a.k_row_stride, _), \
         (a.v_batch_stride, a.v_head_stride, a.v_row_stride, _) = strides
     a.out_batch_stride, a.out_head_stride, a.out_row_stride, _ = _axis_strides(q_shape, out_stride)
@@ -981,13 +982,15 @@ def window_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, left: Op
     Keys behind kv_lens may hold anything; values a query does not see inside
     the sequence must be finite. No backward pass."""
     entry = "window_attention"
-    _refuse_grad(entry, q, k, v)
+    _refuse_grad(entry, q, k, v, out)
     if out is not None and (out.shape != q.shape or out.dtype != q.dtype or out.data_ptr() % 16
                             or not _own_rows(out.shape, out.stride())):
         raise ValueError(f"{entry}: out must be {q.dtype} {tuple(q.shape)} with rows of its own on 16-byte boundaries")
     head, size, out_stride, in_place = _window_plan(
         q.shape, q.stride(), k.shape, k.stride(), v.shape, v.stride(), (q.dtype, k.dtype, v.dtype),
-        None if out is None else out.stride(), left, right, int(sinks), kv_lens is not None, bool(rolling), scale)
+        None if out is None else out.stride(), None if left is None else int(left),
+        None if right is None else int(right), int(sinks), kv_lens is not None, bool(rolling),
+        None if scale is None else float(scale))
     batch = q.shape[0]
     _check_lens(entry, "q_lens", q_lens, batch)
     _check_lens(entry, "kv_lens", kv_lens, batch)
@@ -1096,10 +1099,10 @@ def qkv_cache(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, k_cache: torch.
     dropped, and a position past the table makes its rows NaN. No backward
     pass."""
     entry = "qkv_cache"
-    _refuse_grad(entry, q, k, v, q_weight, k_weight)
+    cos, sin = table if table is not None else (None, None)
+    _refuse_grad(entry, q, k, v, k_cache, v_cache, q_weight, k_weight, cos, sin)
     if lens is None:
         raise ValueError(f"{entry}: lens is needed")
-    cos, sin = table if table is not None else (None, None)
     if (cos is None) != (sin is None):
         raise ValueError(f"{entry}: pass both cos and sin or neither")
     head, in_place, reach = _cache_plan(

@@ -485,8 +485,8 @@ int dfs_gated_residual(const void* x, const void* y, const float* gate,
  * [rows][n], all bf16 or f16; bias [n] (bf16, f16 or f32), gate fp32 [n],
  * each of bias, gate and residual optional (NULL). Sums and everything behind
  * them are fp32, rounded once. activation: 0 none, 1 GELU (tanh form), 2 GELU
- * (erf form), 3 SiLU. Any sizes and strides; out may be the residual itself,
- * but overlap nothing else. The workspace is the caller's,
+ * (erf form), 3 SiLU. Any strides, k below 2^21; out may be the residual
+ * itself, but overlap nothing else. The workspace is the caller's,
  * dfs_linear_workspace_size bytes (0: none), with `aligned` saying that x and w
  * lie on 16-byte boundaries, their strides below 2^21 and, like k, multiples
  * of 8 (they are laid out anew otherwise, but for small products).

@@ -364,3 +364,18 @@ def test_operators_in_a_graph(dev):
         want = layer()
         assert torch.equal(got, want) and torch.equal(gk, kc) and torch.equal(gv, vc)
         assert bool(torch.isfinite(got).all())
+
+
+def test_options_given_as_tensors_are_read_at_each_call(dev):
+    gen = torch.Generator().manual_seed(77)
+    q, k, v = (_randn(gen, 1, 2, 40, 64, dtype=BF).to(dev) for _ in range(3))
+    scale, left = torch.tensor(0.125), torch.tensor(3)
+    first = ops.window_attention(q, k, v, left, 0, scale=scale)
+    assert torch.equal(first, ops.window_attention(q, k, v, 3, 0, scale=0.125))
+    scale.fill_(0.5)
+    left.fill_(20)
+    again = ops.window_attention(q, k, v, left, 0, scale=scale)
+    assert torch.equal(again, ops.window_attention(q, k, v, 20, 0, scale=0.5))
+    assert not torch.equal(first, again)
+    wide = ops.window_attention(q, k, v, 1 << 64, 1 << 64, sinks=1 << 64)
+    assert torch.equal(wide, ops.window_attention(q, k, v))

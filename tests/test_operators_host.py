@@ -4,7 +4,7 @@ import pytest
 import torch
 
 import operator_refs as refs
-from dfsattn_amd import ops
+from dfsattn_amd import _lib, ops
 
 BF = torch.bfloat16
 
@@ -155,3 +155,50 @@ def test_window_mode_of_the_processor_leaves_text_modules_dense():
     args = ("window", 0.3, 16, 128, None, 0, [], 12, 12, 0.0, True)
     assert Wan_DFSAttn_Processor2_0(*args, False, window=(4, 4), sinks=2).branch() == "window"
     assert Wan_DFSAttn_Processor2_0(*args, True).branch() == "dense"
+
+
+def test_operators_refuse_gradients_of_what_they_write():
+    with pytest.raises(RuntimeError, match="no backward"):
+        ops.linear(_t(4, 16), _t(8, 16), out=_t(4, 8).requires_grad_())
+    with pytest.raises(RuntimeError, match="no backward"):
+        ops.window_attention(**ATT, out=_t(2, 4, 3, 64).requires_grad_())
+    for name in ("k_cache", "v_cache"):
+        with pytest.raises(RuntimeError, match="no backward"):
+            ops.qkv_cache(**{**CACHE, name: _t(2, 2, 9, 64).requires_grad_()})
+
+
+def test_limits_behind_every_length_are_kept_within_their_type():
+    for n in (1 << 40, 1 << 63, 1 << 64, 10 ** 30):
+        assert ops._limit("window_attention", "left", n) == 1 << 40
+    assert ops._limit("window_attention", "left", None) == -1
+    with pytest.raises(ValueError):  # more sinks than the cache has slots
+        ops.window_attention(**{**ATT, "rolling": True, "left": 0, "sinks": 1 << 64,
+                                "kv_lens": torch.zeros(2, dtype=torch.int32)})
+
+
+def test_sizes_beyond_a_launch_are_refused():
+    """The library's own checks, which end a call before its launch."""
+    def linear(rows, n, k):
+        size = max(_lib.lib().dfs_linear_workspace_size(rows, n, k, 1), 0)
+        _lib.call("dfs_linear", 16, k, 16, k, rows, n, k, 0, None, 0, 0, None, None, 0, 16, n, 16, size, None)
+
+    with pytest.raises(_lib.DfsKernelError, match="2\\^21"):
+        linear(1, 8, 1 << 21)
+    with pytest.raises(_lib.DfsKernelError, match="too many outputs"):
+        linear(1 << 20, 1 << 20, 64)
+    with pytest.raises(_lib.DfsKernelError, match="too many outputs"):
+        linear(1, 1 << 28, 8)
+    a = _lib.CacheArgs()
+    a.batch, a.tokens, a.q_heads, a.kv_heads, a.head_dim, a.slots = 1 << 6, 1 << 20, 1, 1, 16, 1 << 20
+    for name in ("q", "k", "v", "q_out", "k_cache", "v_cache", "lens"):
+        setattr(a, name, 16)
+    with pytest.raises(_lib.DfsKernelError, match="sizes too large"):
+        _lib.call("dfs_qkv_cache", bytes(a), None)
+    a = _lib.WindowArgs()
+    a.batch, a.q_heads, a.kv_heads, a.q_rows, a.slots, a.head_dim = 1 << 13, 1 << 13, 1 << 13, 1, 8, 64
+    a.left = a.right = -1
+    a.scale = 0.125
+    for name in ("q", "k", "v", "out"):
+        setattr(a, name, 16)
+    with pytest.raises(_lib.DfsKernelError, match="too many rows"):
+        _lib.call("dfs_window_attention", bytes(a), None)
