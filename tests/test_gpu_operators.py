@@ -379,3 +379,63 @@ def test_options_given_as_tensors_are_read_at_each_call(dev):
     assert not torch.equal(first, again)
     wide = ops.window_attention(q, k, v, 1 << 64, 1 << 64, sinks=1 << 64)
     assert torch.equal(wide, ops.window_attention(q, k, v))
+
+
+# --------------------------------------------------------------------------
+# long: positions near 2^30, offsets beyond 32 bits
+# --------------------------------------------------------------------------
+
+@pytest.mark.parametrize("L", [1, 48])
+def test_rolling_positions_near_two_to_the_thirty(dev, L):
+    """The same slots in the same tiles, 2^30 tokens later: the same bits."""
+    gen = torch.Generator().manual_seed(78)
+    sinks, ring = 128, 1024
+    q = _randn(gen, 2, 4, L, 128, dtype=BF).to(dev)
+    k, v = (_randn(gen, 2, 2, sinks + ring, 128, dtype=BF).to(dev) for _ in range(2))
+    lens = torch.tensor([5000, 7001], dtype=torch.int32, device=dev)
+    args = dict(left=900, right=0, sinks=sinks, rolling=True)
+    near = ops.window_attention(q, k, v, kv_lens=lens, **args)
+    far = ops.window_attention(q, k, v, kv_lens=lens + (1 << 30), **args)
+    assert torch.equal(near, far)
+    new = _randn(gen, 2, L, 2, 128, dtype=BF).to(dev)
+    k2, v2 = k.clone(), v.clone()
+    a = ops.qkv_cache(q.transpose(1, 2), new, new, k, v, lens, sinks=sinks, rolling=True)
+    b = ops.qkv_cache(q.transpose(1, 2), new, new, k2, v2, lens + (1 << 30), sinks=sinks, rolling=True)
+    assert torch.equal(a, b) and torch.equal(k, k2) and torch.equal(v, v2)
+
+
+def test_linear_offsets_beyond_32_bits(dev):
+    gen = torch.Generator().manual_seed(79)
+    x, w = _randn(gen, 300_000, 64, dtype=BF), _randn(gen, 8192, 64, dtype=BF)
+    out = ops.linear(x.to(dev), w.to(dev))
+    tail, tol = refs.linear(x[-70:], w)
+    _within(out[-70:], tail, tol, "out")
+    del out
+    wide = torch.empty(3000, 1 << 20, dtype=BF, device=dev)
+    for m, n in ((3000, 200), (8, 3000)):  # x, then w far apart
+        a, b = _randn(gen, m, 64, dtype=BF), _randn(gen, n, 64, dtype=BF)
+        wide[-m if m > n else -n:, 64:128] = (a if m > n else b).to(dev)
+        far = wide[-max(m, n):, 64:128]
+        got = ops.linear(far, b.to(dev)) if m > n else ops.linear(a.to(dev), far)
+        ref, tol = refs.linear(a, b)
+        _within(got, ref, tol, f"{m} x {n}")
+
+
+@pytest.mark.parametrize("L", [1, 200])
+def test_caches_beyond_32_bits(dev, L):
+    gen = torch.Generator().manual_seed(80)
+    slots, near = 18_000_128, 1152  # 4.6 GB a cache; both ends on a tile's boundary
+    kc, vc = (torch.empty(1, 1, slots, 128, dtype=BF, device=dev) for _ in range(2))
+    kc[:, :, -near:] = _randn(gen, 1, 1, near, 128, dtype=BF).to(dev)
+    vc[:, :, -near:] = _randn(gen, 1, 1, near, 128, dtype=BF).to(dev)
+    q = _randn(gen, 1, L, 2, 128, dtype=BF).to(dev)
+    new = [_randn(gen, 1, L, 1, 128, dtype=BF).to(dev) for _ in range(2)]
+    lens = torch.tensor([slots - L], dtype=torch.int32, device=dev)
+    ks, vs = kc[:, :, -near:].clone(), vc[:, :, -near:].clone()
+    qn = ops.qkv_cache(q, *new, kc, vc, lens)
+    ops.qkv_cache(q, *new, ks, vs, lens - (slots - near))
+    assert torch.equal(kc[:, :, -near:], ks) and torch.equal(vc[:, :, -near:], vs)
+    assert torch.equal(kc[0, 0, -L:], new[0][0, :, 0])
+    got = ops.window_attention(qn, kc, vc, left=500, right=0)
+    ref, tol = refs.window_attention(qn.cpu(), ks.cpu(), vs.cpu(), left=500, right=0)[::2][:2]
+    _within(got, ref, tol, "attention")
