@@ -169,62 +169,110 @@ __device__ __forceinline__ void finish8(const LinearParams& p, int m, int n, con
     finish8_edge<F16, ACT>(p, m, n, z, bias, gate);
 }
 
-// Eight elements k..k+7 of a row of K that may start at any 2-byte address;
-// zeros past the row's end.
+// Elements k..k+7 of a row of K, zeros past its end: one by one, but all on
+// their way at once.
+__device__ __forceinline__ uint4 load_edge8(const uint16_t* row, int k, int K) {
+  uint16_t t[8];
+#pragma unroll
+  for (int i = 0; i < 8; ++i) t[i] = row[min(k + i, K - 1)];
+#pragma unroll
+  for (int i = 0; i < 8; ++i) t[i] = k + i < K ? t[i] : 0;
+  uint4 v;
+  __builtin_memcpy(&v, t, 16);
+  return v;
+}
+
+// The same from a row that may start at any 2-byte address.
 __device__ __forceinline__ uint4 load_row8(const uint16_t* row, int k, int K) {
   uint4 v = make_uint4(0, 0, 0, 0);
   if (k + 8 <= K) {
     __builtin_memcpy(&v, row + k, 16);
   } else if (k < K) {
-    uint16_t t[8] = {};
-#pragma unroll
-    for (int i = 0; i < 8; ++i)
-      if (k + i < K) t[i] = row[k + i];
-    __builtin_memcpy(&v, t, 16);
+    v = load_edge8(row, k, K);
   }
   return v;
 }
 
 // 64 x 64 outputs a workgroup, four waves of 32 x 32, 64 channels a step, any
-// strides and sizes: rows are loaded into registers and stored to LDS from
-// there.
+// strides and sizes: rows are loaded into registers, four steps ahead, and
+// stored to one of two LDS buffers from there, one barrier a step. The channels
+// behind the last whole step go first, so that the steps' loads have no edge.
 template <bool F16>
 __global__ void __launch_bounds__(256) linear_any_kernel(LinearParams p) {
-  __shared__ __attribute__((aligned(16))) uint16_t ws[64 * 64];
-  __shared__ __attribute__((aligned(16))) uint16_t xs[64 * 64];
+  __shared__ __attribute__((aligned(16))) uint16_t ws[2][64 * 64];
+  __shared__ __attribute__((aligned(16))) uint16_t xs[2][64 * 64];
   const int tid = threadIdx.x, lane = tid & 63, w = tid >> 6, l32 = lane & 31, hl = lane >> 5;
   const unsigned nt = (p.N + 63) / 64;
   const int m0 = static_cast<int>(blockIdx.x / nt) * 64, n0 = static_cast<int>(blockIdx.x % nt) * 64;
-  f32x16 acc = f32x16{};
-  uint4 a[2], b[2];  // a step's chunks, loaded under the products of the one before
-  auto load = [&](int k0) {
+  const int steps = p.K >> 6, c8 = (tid & 7) * 8;
+  const uint16_t *wrow[2], *xrow[2];
+#pragma unroll
+  for (int j = 0; j < 2; ++j) {
+    const int r = j * 32 + (tid >> 3);
+    wrow[j] = p.w + min(n0 + r, p.N - 1) * p.ldw + c8;
+    xrow[j] = p.x + min(m0 + r, p.M - 1) * p.ldx + c8;
+  }
+  typedef uint32_t u32x4 __attribute__((ext_vector_type(4)));
+  typedef u32x4 Chunks[4];  // two of w, two of x
+  auto load = [&](int t, Chunks& c) {  // past the last step: that again, unread
+    const int k = min(t, steps - 1) * 64;
 #pragma unroll
     for (int j = 0; j < 2; ++j) {
-      const int r = j * 32 + (tid >> 3), k = k0 + (tid & 7) * 8;
-      a[j] = load_row8(p.w + min(n0 + r, p.N - 1) * p.ldw, k, p.K);
-      b[j] = load_row8(p.x + min(m0 + r, p.M - 1) * p.ldx, k, p.K);
+      u32x4 a, b;
+      __builtin_memcpy(&a, wrow[j] + k, 16);
+      __builtin_memcpy(&b, xrow[j] + k, 16);
+      c[j] = a;
+      c[2 + j] = b;
     }
   };
-  load(0);
-  for (int k0 = 0; k0 < p.K; k0 += 64) {
-    __syncthreads();
+  f32x16 acc = f32x16{};
+  auto step = [&](const Chunks& ch, int buf) {
 #pragma unroll
     for (int j = 0; j < 2; ++j) {
       const int r = j * 32 + (tid >> 3), c = (tid & 7) ^ (r >> 1 & 7);
-      *reinterpret_cast<uint4*>(ws + (r * 8 + c) * 8) = a[j];
-      *reinterpret_cast<uint4*>(xs + (r * 8 + c) * 8) = b[j];
+      *reinterpret_cast<u32x4*>(ws[buf] + (r * 8 + c) * 8) = ch[j];
+      *reinterpret_cast<u32x4*>(xs[buf] + (r * 8 + c) * 8) = ch[2 + j];
     }
-    __syncthreads();
-    if (k0 + 64 < p.K) load(k0 + 64);
+    block_barrier();  // stored by all; the other buffer has been read by all
 #pragma unroll
     for (int s = 0; s < 4; ++s) {
       const int wr = (w & 1) * 32 + l32, xr = (w >> 1) * 32 + l32, c = 2 * s + hl;
-      const uint4 fa = *reinterpret_cast<const uint4*>(ws + (wr * 8 + (c ^ (wr >> 1 & 7))) * 8);
-      const uint4 fb = *reinterpret_cast<const uint4*>(xs + (xr * 8 + (c ^ (xr >> 1 & 7))) * 8);
+      const uint4 fa = *reinterpret_cast<const uint4*>(ws[buf] + (wr * 8 + (c ^ (wr >> 1 & 7))) * 8);
+      const uint4 fb = *reinterpret_cast<const uint4*>(xs[buf] + (xr * 8 + (c ^ (xr >> 1 & 7))) * 8);
       acc = Half<F16>::mfma(__builtin_bit_cast(typename Half<F16>::vec, fa),
                             __builtin_bit_cast(typename Half<F16>::vec, fb), acc);
     }
+  };
+  Chunks c0, c1, c2, c3;
+  if (steps > 0) {
+    load(0, c0);
+    load(1, c1);
+    load(2, c2);
+    load(3, c3);
   }
+  if (p.K & 63) {
+    Chunks tail;
+#pragma unroll
+    for (int j = 0; j < 2; ++j) {
+      tail[j] = __builtin_bit_cast(u32x4, load_edge8(wrow[j] - c8, steps * 64 + c8, p.K));
+      tail[2 + j] = __builtin_bit_cast(u32x4, load_edge8(xrow[j] - c8, steps * 64 + c8, p.K));
+    }
+    step(tail, 1);
+  }
+  int t = 0;
+  for (; t + 4 <= steps; t += 4) {
+    step(c0, 0);
+    load(t + 4, c0);
+    step(c1, 1);
+    load(t + 5, c1);
+    step(c2, 0);
+    load(t + 6, c2);
+    step(c3, 1);
+    load(t + 7, c3);
+  }
+  if (t < steps) step(c0, 0);
+  if (t + 1 < steps) step(c1, 1);
+  if (t + 2 < steps) step(c2, 0);
   // The lane halves hold alternate groups of four n: joined into eight by an
   // exchange, half 0 keeps the even eights.
   const int m = m0 + (w >> 1) * 32 + l32;

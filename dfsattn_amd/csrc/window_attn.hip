@@ -439,7 +439,8 @@ __global__ void __launch_bounds__(256, 2) window_tile_kernel(WindowParams p) {
   const int wr = r0 + w * 32;
   const int wq0 = min(wr, rows - 1) / p.group, wq1 = min(min(wr + 31, rows - 1) / p.group, seq.nq - 1);
   const int wlo0 = first_key(p, seq, wq0), wlo1 = first_key(p, seq, wq1);
-  const int whi0 = last_key(p, seq, wq0), whi1 = wq1 < wq0 ? -1 : last_key(p, seq, wq1);
+  // (a wave behind the last row sees nothing and only copies)
+  const int whi0 = last_key(p, seq, wq0), whi1 = wq1 < wq0 || wr >= rows ? -1 : last_key(p, seq, wq1);
   const bool in = wr + l32 < rows;
   const Row row = row_of(p, min(wr + l32, rows - 1));
   const int klo = first_key(p, seq, row.i), khi = last_key(p, seq, row.i);

@@ -716,17 +716,15 @@ Shape = Tuple[int, ...]
 
 def _refuse_grad(entry: str, *tensors: Optional[torch.Tensor]) -> None:
     """These operators have no backward pass: a graph would lose it silently."""
-    if torch.is_grad_enabled():
-        for t in tensors:
-            if t is not None and t.requires_grad:
-                raise RuntimeError(f"{entry} has no backward pass: call it under torch.no_grad() or inference_mode()")
+    if any([t is not None and t.requires_grad for t in tensors]) and torch.is_grad_enabled():
+        raise RuntimeError(f"{entry} has no backward pass: call it under torch.no_grad() or inference_mode()")
 
 
 def _call_on(device: torch.device, entry: str, *args) -> None:
     """An entry point on a device and its current stream (the last argument),
     whichever device the caller has current."""
     index = device.index
-    if index == torch.cuda.current_device():
+    if index == torch._C._cuda_getDevice():
         _lib.call(entry, *args, torch._C._cuda_getCurrentRawStream(index))
     else:
         with torch.cuda.device(device):
@@ -866,7 +864,7 @@ def linear(x: torch.Tensor, weight: torch.Tensor, bias: Optional[torch.Tensor] =
         raise ValueError(f"linear: out must be contiguous {dtype} {shape}, got {out.dtype} {tuple(out.shape)}")
     _one_device(x, weight, bias, gate, residual, out)
     if out is None:
-        out = torch.empty(shape, dtype=dtype, device=x.device)
+        out = x.new_empty(shape)
     else:
         same = residual is not None and residual.data_ptr() == out.data_ptr() and residual.is_contiguous()
         _refuse_overlap("linear", "out", out, x, weight, bias, gate, None if same else residual)
@@ -881,7 +879,7 @@ def linear(x: torch.Tensor, weight: torch.Tensor, bias: Optional[torch.Tensor] =
     px, pw = x.data_ptr(), weight.data_ptr()
     ws_bytes = _linear_workspace(rows, n, k, (k | ldx | ldw) % 8 == 0 and (px | pw) % 16 == 0
                                  and ldx < 1 << 21 and ldw < 1 << 21)
-    ws = torch.empty(ws_bytes, dtype=torch.uint8, device=x.device) if ws_bytes else None
+    ws = x.new_empty(ws_bytes // 2) if ws_bytes else None  # of two bytes an element
     _call_on(x.device, "dfs_linear", px, ldx, pw, ldw, rows, n, k, DTYPE_CODE[dtype], _ptr(bias), b_code,
              ACTIVATION_CODE[activation], _ptr(gate), _ptr(residual), ldr or 0, out.data_ptr(), n, _ptr(ws), ws_bytes)
     return out
@@ -997,7 +995,7 @@ def window_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, left: Op
     _one_device(q, k, v, q_lens, kv_lens, out)
     device = q.device
     if out is None:
-        out = torch.empty_strided(q.shape, out_stride, dtype=q.dtype, device=device)
+        out = q.new_empty_strided(q.shape, out_stride)
     else:
         _refuse_overlap(entry, "out", out, q, k, v)
     lse = torch.empty(q.shape[:3], dtype=torch.float32, device=device) if want_lse else None
@@ -1010,7 +1008,7 @@ def window_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, left: Op
     if not (in_place and (pq | pk | pv) % 16 == 0):
         return window_attention(_in_chunks(q), _in_chunks(k), _in_chunks(v), left, right, sinks, q_lens, kv_lens,
                                 rolling, scale, out, want_lse)
-    ws = torch.empty(size, dtype=torch.uint8, device=device) if size else None
+    ws = q.new_empty(size // 2) if size else None  # of two bytes an element
     block = head + _WINDOW_POINTERS.pack(pq, pk, pv, out.data_ptr(), _ptr(lse) or 0,
                                          _ptr(q_lens) or 0, _ptr(kv_lens) or 0, _ptr(ws) or 0)
     _call_on(device, "dfs_window_attention", block)
@@ -1117,28 +1115,28 @@ def qkv_cache(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, k_cache: torch.
     pk, pv = k_cache.data_ptr(), v_cache.data_ptr()
     if (pk | pv) % 16:
         raise ValueError(f"{entry}: the caches must have rows of their own on 16-byte boundaries")
+    ek, ev = pk + reach[3], pv + reach[4]
     for x, n in zip(at, reach):
-        if (x < pk + reach[3] and pk < x + n) or (x < pv + reach[4] and pv < x + n):
+        if x < ek and pk < x + n or x < ev and pv < x + n:
             raise ValueError(f"{entry}: a cache overlaps an input")
     if pk == pv and reach[3]:  # their rows may alternate in one tensor
         raise ValueError(f"{entry}: k_cache and v_cache are the same memory")
     _check_lens(entry, "lens", lens, batch)
     _check_lens(entry, "new_lens", new_lens, batch)
-    if cos is not None:
-        for t in (cos, sin):
-            if t.dtype != torch.float32 or not t.is_contiguous():
-                raise ValueError(f"{entry}: tables must be contiguous float32, got {t.dtype}")
+    if cos is not None and not (cos.dtype == sin.dtype == torch.float32 and cos.is_contiguous()
+                                and sin.is_contiguous()):
+        raise ValueError(f"{entry}: tables must be contiguous float32, got {cos.dtype} and {sin.dtype}")
     _one_device(q, k, v, k_cache, v_cache, lens, q_weight, k_weight, cos, sin, new_lens)
     device = q.device
-    out = torch.empty(q.shape, dtype=q.dtype, device=device)
+    out = q.new_empty(q.shape)
     if out.numel() == 0:
         return out.transpose(1, 2)
     if not (in_place and (at[0] | at[1] | at[2]) % 16 == 0):
         return qkv_cache(_in_chunks(q), _in_chunks(k), _in_chunks(v), k_cache, v_cache, lens, q_weight, k_weight, eps,
                          table, new_lens, sinks, rolling)
     vectors = [0 if t is None else t.data_ptr() for t in (q_weight, k_weight, cos, sin)]
-    if (vectors[0] | vectors[1] | vectors[2] | vectors[3]) % 16 or any(
-            [t is not None and not t.is_contiguous() for t in (q_weight, k_weight)]):
+    if ((vectors[0] | vectors[1] | vectors[2] | vectors[3]) % 16 or q_weight is not None
+            and not q_weight.is_contiguous() or k_weight is not None and not k_weight.is_contiguous()):
         q_weight, k_weight, cos, sin = (None if t is None else t.clone(memory_format=torch.contiguous_format)
                                         for t in (q_weight, k_weight, cos, sin))
         vectors = [_ptr(t) or 0 for t in (q_weight, k_weight, cos, sin)]
