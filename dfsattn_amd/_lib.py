@@ -52,7 +52,7 @@ SIGNATURES = {
     "dfs_adaln_modulate": [_p, _i64, _i64, _i32, _p, _p, _p, _p, _f32, _p, _p],
     "dfs_gated_residual": [_p, _p, _p, _i64, _i64, _i32, _p, _p],
     "dfs_linear_workspace_size": [_i64, _i64, _i64, _i32],
-    "dfs_linear": [_p, _i64, _p, _i64, _i64, _i64, _i64, _i32, _p, _i32, _i32, _p, _p, _i64, _p, _i64, _p, _i64, _p],
+    "dfs_linear": [_p, _p],
     "dfs_window_attention_workspace_size": [_p],
     "dfs_window_attention": [_p, _p],
     "dfs_qkv_cache": [_p, _p],
@@ -69,6 +69,14 @@ class CallArgs(ctypes.Structure):
         ("scale", ctypes.c_double)] + [(n, _p) for n in (
             "q", "k", "v", "perm", "row_ptr", "col_idx", "out", "out_perm", "cu_seqlens_q", "cu_seqlens_k",
             "workspace")]
+
+
+class LinearArgs(ctypes.Structure):
+    """dfs_linear_args, field by field."""
+
+    _fields_ = [(n, _i64) for n in ("rows", "n", "k", "dtype", "bias_dtype", "activation", "x_stride", "w_stride",
+                                    "residual_stride", "out_stride", "workspace_bytes")] + [
+        (n, _p) for n in ("x", "w", "bias", "gate", "residual", "out", "workspace")]
 
 
 class WindowArgs(ctypes.Structure):

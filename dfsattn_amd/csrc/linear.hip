@@ -889,8 +889,8 @@ struct Cut {
 };
 Cut cut_of(int64_t rows, int64_t n, int64_t k, bool chunks) {
   // Rows on no 16-byte boundary: small products of few steps as they are, the
-  // others laid out anew (us, as they are and anew: 333 by 1,017 x 709 10.5 and
-  // 11.3, 100 by 5,119 x 1,001 13.1 and 15.9; 400 by 1,001 x 3,001 29.0 and
+  // others laid out anew (us, as they are and anew: 333 by 1,017 x 709 8.9 and
+  // 11.3, 100 by 5,119 x 1,001 11.9 and 15.9; 400 by 1,001 x 3,001 29.0 and
   // 23.1, 1 by 5,119 x 5,119 54.6 and 29.5, 6,694 by 1,422 x 5,465 370 and 148).
   if (!chunks && k <= 1024 && rows * n * k < (int64_t(1) << 30)) return Cut{kTileAny, 1, 0, false};
   if (rows <= 8) return Cut{kFew, 1, 0, !chunks};
@@ -953,34 +953,34 @@ extern "C" int64_t dfs_linear_workspace_size(int64_t rows, int64_t n, int64_t k,
   return workspace_bytes_of(cut_of(rows, n, k, aligned != 0), rows, n, k);
 }
 
-extern "C" int dfs_linear(const void* x, int64_t x_stride, const void* w, int64_t w_stride, int64_t rows, int64_t n,
-                          int64_t k, int dtype, const void* bias, int bias_dtype, int activation, const float* gate,
-                          const void* residual, int64_t r_stride, void* out, int64_t o_stride, void* workspace,
-                          int64_t workspace_bytes, dfs_stream_t stream) {
+extern "C" int dfs_linear(const dfs_linear_args* a, dfs_stream_t stream) {
   using namespace dfs;
   const char* name = "linear";
-  DFS_REQUIRE(x && w && out, "%s: x, w and out must be non-NULL", name);
+  DFS_REQUIRE(a != nullptr, "%s: args is NULL", name);
+  const void *x = a->x, *w = a->w, *bias = a->bias, *residual = a->residual;
+  const int64_t rows = a->rows, n = a->n, k = a->k, x_stride = a->x_stride, w_stride = a->w_stride;
+  DFS_REQUIRE(x && w && a->out, "%s: x, w and out must be non-NULL", name);
   DFS_REQUIRE(rows > 0 && n > 0 && k > 0, "%s: rows=%lld n=%lld k=%lld must be positive", name, (long long)rows,
               (long long)n, (long long)k);
   constexpr int64_t kMax = int64_t(1) << 30;
   DFS_REQUIRE(rows < kMax && n < kMax && k < (1 << 21), "%s: rows and n must be below 2^30, k below 2^21", name);
-  DFS_REQUIRE(dtype == DFS_DTYPE_BF16 || dtype == DFS_DTYPE_F16, "%s: dtype must be bf16 or f16", name);
-  DFS_REQUIRE(x_stride >= 0 && w_stride >= 0 && o_stride >= n && (!residual || r_stride >= 0),
+  DFS_REQUIRE(a->dtype == DFS_DTYPE_BF16 || a->dtype == DFS_DTYPE_F16, "%s: dtype must be bf16 or f16", name);
+  DFS_REQUIRE(x_stride >= 0 && w_stride >= 0 && a->out_stride >= n && (!residual || a->residual_stride >= 0),
               "%s: strides must be non-negative, and out's rows must not overlap", name);
-  DFS_REQUIRE(bias == nullptr || bias_dtype == DFS_DTYPE_BF16 || bias_dtype == DFS_DTYPE_F16 ||
-                  bias_dtype == DFS_DTYPE_F32,
-              "%s: bias dtype code %d is not supported", name, bias_dtype);
-  DFS_REQUIRE(activation >= kActNone && activation <= kActSilu, "%s: activation code %d is not supported", name,
-              activation);
+  DFS_REQUIRE(bias == nullptr || a->bias_dtype == DFS_DTYPE_BF16 || a->bias_dtype == DFS_DTYPE_F16 ||
+                  a->bias_dtype == DFS_DTYPE_F32,
+              "%s: bias dtype code %lld is not supported", name, (long long)a->bias_dtype);
+  DFS_REQUIRE(a->activation >= kActNone && a->activation <= kActSilu, "%s: activation code %lld is not supported",
+              name, (long long)a->activation);
   auto addr = [](const void* q) { return reinterpret_cast<uintptr_t>(q); };
-  DFS_REQUIRE(addr(x) % 2 == 0 && addr(w) % 2 == 0 && addr(out) % 2 == 0 && addr(residual) % 2 == 0 &&
-                  addr(gate) % 4 == 0 && addr(bias) % (bias_dtype == DFS_DTYPE_F32 ? 4 : 2) == 0,
+  DFS_REQUIRE(addr(x) % 2 == 0 && addr(w) % 2 == 0 && addr(a->out) % 2 == 0 && addr(residual) % 2 == 0 &&
+                  addr(a->gate) % 4 == 0 && addr(bias) % (a->bias_dtype == DFS_DTYPE_F32 ? 4 : 2) == 0,
               "%s: operands must be aligned to their elements", name);
   const bool chunks = k % 8 == 0 && x_stride % 8 == 0 && w_stride % 8 == 0 && addr(x) % 16 == 0 && addr(w) % 16 == 0 &&
                       x_stride < (1 << 21) && w_stride < (1 << 21);
   const Cut cut = cut_of(rows, n, k, chunks);
   const int64_t need = workspace_bytes_of(cut, rows, n, k);
-  DFS_REQUIRE(need == 0 || (workspace != nullptr && workspace_bytes >= need && addr(workspace) % 16 == 0),
+  DFS_REQUIRE(need == 0 || (a->workspace != nullptr && a->workspace_bytes >= need && addr(a->workspace) % 16 == 0),
               "%s: a 16-byte aligned workspace of %lld bytes is needed", name, (long long)need);
   // A launch holds fewer than 2^32 threads.
   DFS_REQUIRE(((rows + 63) / 64) * ((n + 63) / 64) * cut.splits < (1 << 24) && (cut.form != kFew || n < (1 << 27)),
@@ -990,24 +990,24 @@ extern "C" int dfs_linear(const void* x, int64_t x_stride, const void* w, int64_
   p.w = static_cast<const uint16_t*>(w);
   p.ldx = x_stride;
   p.ldw = w_stride;
-  p.ldr = r_stride;
-  p.ldo = o_stride;
+  p.ldr = a->residual_stride;
+  p.ldo = a->out_stride;
   p.M = static_cast<int>(rows);
   p.N = static_cast<int>(n);
   p.K = static_cast<int>(k);
   p.bias = bias;
-  p.bias_dtype = bias_dtype;
-  p.act = activation;
-  p.gate = gate;
+  p.bias_dtype = static_cast<int>(a->bias_dtype);
+  p.act = static_cast<int>(a->activation);
+  p.gate = a->gate;
   p.residual = static_cast<const uint16_t*>(residual);
-  p.out = static_cast<uint16_t*>(out);
+  p.out = static_cast<uint16_t*>(a->out);
   hipStream_t st = reinterpret_cast<hipStream_t>(stream);
   p.splits = cut.splits;
   p.depth = cut.depth;
-  p.part = static_cast<float*>(workspace);
-  const bool f16 = dtype == DFS_DTYPE_F16;
+  p.part = static_cast<float*>(a->workspace);
+  const bool f16 = a->dtype == DFS_DTYPE_F16;
   if (cut.pad) {
-    uint16_t* const wide = reinterpret_cast<uint16_t*>(static_cast<char*>(workspace) + part_bytes(cut, rows, n));
+    uint16_t* const wide = reinterpret_cast<uint16_t*>(static_cast<char*>(a->workspace) + part_bytes(cut, rows, n));
     const int64_t kp = padded(k);
     const dim3 grid(static_cast<unsigned>((kp + 2047) / 2048), static_cast<unsigned>(std::min<int64_t>(rows + n, 65535)));
     pad_rows_kernel<<<grid, 256, 0, st>>>(p, static_cast<int>(kp), wide);

@@ -716,7 +716,7 @@ Shape = Tuple[int, ...]
 
 def _refuse_grad(entry: str, *tensors: Optional[torch.Tensor]) -> None:
     """These operators have no backward pass: a graph would lose it silently."""
-    if any([t is not None and t.requires_grad for t in tensors]) and torch.is_grad_enabled():
+    if torch.is_grad_enabled() and any([t is not None and t.requires_grad for t in tensors]):
         raise RuntimeError(f"{entry} has no backward pass: call it under torch.no_grad() or inference_mode()")
 
 
@@ -808,12 +808,23 @@ def _row_stride(shape: Shape, stride: Shape) -> Optional[int]:
     return shape[-1] if ld is None else ld
 
 
+_LINEAR_POINTERS = struct.Struct("@7P")
+_WINDOW_POINTERS = struct.Struct("@8P")
+_CACHE_POINTERS = struct.Struct("@12P")
+
+
+def _pointers(block: ctypes.Structure, first: str) -> int:
+    """Where an argument block's pointers begin."""
+    return getattr(type(block), first).offset
+
+
 @functools.lru_cache(maxsize=1024)
 def _linear_plan(x_shape: Shape, x_stride: Shape, w_shape: Shape, w_stride: Shape, x_dtype: torch.dtype,
-                 w_dtype: torch.dtype, activation: Optional[str], r_shape: Optional[Shape],
-                 r_stride: Optional[Shape]):
-    """(rows, shape of out, row strides of x, weight and residual or None
-    where they are copied first) of a ``linear`` call."""
+                 w_dtype: torch.dtype, activation: Optional[str], b_shape: Optional[Shape],
+                 b_dtype: Optional[torch.dtype], r_shape: Optional[Shape], r_stride: Optional[Shape]):
+    """(shape of out, whether x, weight and residual are read in place, and the
+    argument block up to the pointers with its workspace bytes: for x and weight
+    off 16-byte boundaries, and on them) of a ``linear`` call."""
     if x_dtype not in HALF or w_dtype != x_dtype:
         raise ValueError(f"linear: x and weight must both be bf16 or f16, got {x_dtype} and {w_dtype}")
     if len(x_shape) < 1 or len(w_shape) != 2 or w_shape[1] != x_shape[-1]:
@@ -822,16 +833,27 @@ def _linear_plan(x_shape: Shape, x_stride: Shape, w_shape: Shape, w_stride: Shap
         raise ValueError(f"linear: weight {tuple(w_shape)} has no elements")
     if activation not in ACTIVATION_CODE:
         raise ValueError(f"linear: activation must be one of {list(ACTIVATION_CODE)}, got {activation!r}")
-    shape = (*x_shape[:-1], w_shape[0])
+    n, k = w_shape
+    if b_shape is not None and (len(b_shape) != 1 or b_shape[0] != n or b_dtype not in (x_dtype, torch.float32)):
+        raise ValueError(f"linear: bias must hold {n} values of x's dtype or float32, got {b_dtype} {tuple(b_shape)}")
+    shape = (*x_shape[:-1], n)
     if r_shape is not None and tuple(r_shape) != shape:
         raise ValueError(f"linear: residual must be {shape}, got {tuple(r_shape)}")
-    return (math.prod(x_shape[:-1]), shape, _row_stride(x_shape, x_stride), _row_stride(w_shape, w_stride),
-            None if r_shape is None else _row_stride(r_shape, r_stride))
-
-
-@functools.lru_cache(maxsize=1024)
-def _linear_workspace(rows: int, n: int, k: int, aligned: bool) -> int:
-    return int(_lib.lib().dfs_linear_workspace_size(rows, n, k, int(aligned)))
+    rows = math.prod(x_shape[:-1])
+    ldx, ldw = _row_stride(x_shape, x_stride), _row_stride(w_shape, w_stride)
+    ldr = 0 if r_shape is None else _row_stride(r_shape, r_stride)
+    if rows == 0 or None in (ldx, ldw, ldr):
+        return shape, (ldx is not None, ldw is not None, ldr is not None), None
+    a = _lib.LinearArgs()
+    a.rows, a.n, a.k, a.dtype, a.activation = rows, n, k, DTYPE_CODE[x_dtype], ACTIVATION_CODE[activation]
+    a.bias_dtype = 0 if b_dtype is None else DTYPE_CODE[b_dtype]
+    a.x_stride, a.w_stride, a.residual_stride, a.out_stride = ldx, ldw, ldr, n
+    chunks = (k | ldx | ldw) % 8 == 0 and ldx < 1 << 21 and ldw < 1 << 21
+    blocks = []
+    for aligned in (False, chunks):
+        a.workspace_bytes = int(_lib.lib().dfs_linear_workspace_size(rows, n, k, int(aligned)))
+        blocks.append((bytes(a)[:_pointers(a, "x")], a.workspace_bytes))
+    return shape, None, blocks
 
 
 def linear(x: torch.Tensor, weight: torch.Tensor, bias: Optional[torch.Tensor] = None,
@@ -844,20 +866,16 @@ def linear(x: torch.Tensor, weight: torch.Tensor, bias: Optional[torch.Tensor] =
     to x's dtype (bf16 or f16). ``out`` may be the residual itself. No
     backward pass."""
     _refuse_grad("linear", x, weight, bias, gate, residual, out)
-    rows, shape, ldx, ldw, ldr = _linear_plan(
-        x.shape, x.stride(), weight.shape, weight.stride(), x.dtype, weight.dtype, activation,
-        None if residual is None else residual.shape, None if residual is None else residual.stride())
-    n, k = weight.shape
     dtype = x.dtype
-    b_code = 0
-    if bias is not None:
-        if bias.dim() != 1 or bias.shape[0] != n or bias.dtype not in (dtype, torch.float32):
-            raise ValueError(f"linear: bias must hold {n} values of x's dtype or float32, got {bias.dtype} "
-                             f"{tuple(bias.shape)}")
-        bias, b_code = bias.contiguous(), DTYPE_CODE[bias.dtype]
-    if gate is not None and not (gate.dim() == 1 and gate.shape[0] == n and gate.dtype == torch.float32
+    shape, in_place, blocks = _linear_plan(
+        x.shape, x.stride(), weight.shape, weight.stride(), dtype, weight.dtype, activation,
+        None if bias is None else bias.shape, None if bias is None else bias.dtype,
+        None if residual is None else residual.shape, None if residual is None else residual.stride())
+    if bias is not None and not bias.is_contiguous():
+        bias = bias.contiguous()
+    if gate is not None and not (gate.dim() == 1 and gate.shape[0] == shape[-1] and gate.dtype == torch.float32
                                  and gate.is_contiguous()):
-        gate = _vec(gate, n, "linear: gate")
+        gate = _vec(gate, shape[-1], "linear: gate")
     if residual is not None and residual.dtype != dtype:
         raise ValueError(f"linear: residual must be {dtype}, got {residual.dtype}")
     if out is not None and (tuple(out.shape) != shape or out.dtype != dtype or not out.is_contiguous()):
@@ -868,25 +886,23 @@ def linear(x: torch.Tensor, weight: torch.Tensor, bias: Optional[torch.Tensor] =
     else:
         same = residual is not None and residual.data_ptr() == out.data_ptr() and residual.is_contiguous()
         _refuse_overlap("linear", "out", out, x, weight, bias, gate, None if same else residual)
-    if rows == 0:
-        return out
-    if ldx is None:
-        x, ldx = x.contiguous(), k
-    if ldw is None:
-        weight, ldw = weight.contiguous(), k
-    if residual is not None and ldr is None:
-        residual, ldr = residual.contiguous(), n
+    if blocks is None:
+        if out.numel() == 0:
+            return out
+        x, weight, residual = (t if t is None or whole else t.contiguous()
+                               for t, whole in zip((x, weight, residual), in_place))
+        return linear(x, weight, bias, activation, gate, residual, out)
     px, pw = x.data_ptr(), weight.data_ptr()
-    ws_bytes = _linear_workspace(rows, n, k, (k | ldx | ldw) % 8 == 0 and (px | pw) % 16 == 0
-                                 and ldx < 1 << 21 and ldw < 1 << 21)
-    ws = x.new_empty(ws_bytes // 2) if ws_bytes else None  # of two bytes an element
-    _call_on(x.device, "dfs_linear", px, ldx, pw, ldw, rows, n, k, DTYPE_CODE[dtype], _ptr(bias), b_code,
-             ACTIVATION_CODE[activation], _ptr(gate), _ptr(residual), ldr or 0, out.data_ptr(), n, _ptr(ws), ws_bytes)
+    head, size = blocks[(px | pw) % 16 == 0]
+    ws = x.new_empty(size // 2) if size else None  # of two bytes an element
+    block = head + _LINEAR_POINTERS.pack(px, pw, _ptr(bias) or 0, _ptr(gate) or 0, _ptr(residual) or 0,
+                                         out.data_ptr(), _ptr(ws) or 0)
+    _call_on(x.device, "dfs_linear", block)
     return out
 
 
-def _check_lens(entry: str, name: str, t: Optional[torch.Tensor], batch: int) -> None:
-    if t is not None and (t.dtype != torch.int32 or t.dim() != 1 or t.shape[0] != batch or not t.is_contiguous()):
+def _check_lens(entry: str, name: str, t: torch.Tensor, batch: int) -> None:
+    if t.dtype != torch.int32 or t.dim() != 1 or t.shape[0] != batch or not t.is_contiguous():
         raise ValueError(f"{entry}: {name} must be a contiguous int32 [{batch}] vector, got {t.dtype} "
                          f"{tuple(t.shape)}")
 
@@ -897,15 +913,6 @@ def _limit(entry: str, name: str, n: Optional[int]) -> int:
     if int(n) < 0:
         raise ValueError(f"{entry}: {name} must be None (no limit) or not negative, got {n}")
     return min(int(n), 1 << 40)  # behind every length
-
-
-def _pointers(block: ctypes.Structure, first: str) -> int:
-    """Where an argument block's pointers begin."""
-    return getattr(type(block), first).offset
-
-
-_WINDOW_POINTERS = struct.Struct("@8P")
-_CACHE_POINTERS = struct.Struct("@12P")
 
 
 @functools.lru_cache(maxsize=1024)
@@ -990,8 +997,9 @@ def window_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, left: Op
         None if right is None else int(right), int(sinks), kv_lens is not None, bool(rolling),
         None if scale is None else float(scale))
     batch = q.shape[0]
-    _check_lens(entry, "q_lens", q_lens, batch)
-    _check_lens(entry, "kv_lens", kv_lens, batch)
+    for name, t in (("q_lens", q_lens), ("kv_lens", kv_lens)):
+        if t is not None:
+            _check_lens(entry, name, t, batch)
     _one_device(q, k, v, q_lens, kv_lens, out)
     device = q.device
     if out is None:
@@ -1122,15 +1130,16 @@ def qkv_cache(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, k_cache: torch.
     if pk == pv and reach[3]:  # their rows may alternate in one tensor
         raise ValueError(f"{entry}: k_cache and v_cache are the same memory")
     _check_lens(entry, "lens", lens, batch)
-    _check_lens(entry, "new_lens", new_lens, batch)
+    if new_lens is not None:
+        _check_lens(entry, "new_lens", new_lens, batch)
     if cos is not None and not (cos.dtype == sin.dtype == torch.float32 and cos.is_contiguous()
                                 and sin.is_contiguous()):
         raise ValueError(f"{entry}: tables must be contiguous float32, got {cos.dtype} and {sin.dtype}")
     _one_device(q, k, v, k_cache, v_cache, lens, q_weight, k_weight, cos, sin, new_lens)
     device = q.device
-    out = q.new_empty(q.shape)
-    if out.numel() == 0:
-        return out.transpose(1, 2)
+    out = q.new_empty_strided((batch, heads, tokens, dim), (tokens * heads * dim, dim, heads * dim, 1))
+    if tokens == 0 or batch == 0:
+        return out
     if not (in_place and (at[0] | at[1] | at[2]) % 16 == 0):
         return qkv_cache(_in_chunks(q), _in_chunks(k), _in_chunks(v), k_cache, v_cache, lens, q_weight, k_weight, eps,
                          table, new_lens, sinks, rolling)
@@ -1142,4 +1151,4 @@ def qkv_cache(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, k_cache: torch.
         vectors = [_ptr(t) or 0 for t in (q_weight, k_weight, cos, sin)]
     block = head + _CACHE_POINTERS.pack(*at, out.data_ptr(), pk, pv, *vectors, lens.data_ptr(), _ptr(new_lens) or 0)
     _call_on(device, "dfs_qkv_cache", block)
-    return out.transpose(1, 2)
+    return out

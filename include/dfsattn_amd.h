@@ -493,12 +493,16 @@ int dfs_gated_residual(const void* x, const void* y, const float* gate,
  */
 enum { DFS_ACT_NONE = 0, DFS_ACT_GELU_TANH = 1, DFS_ACT_GELU = 2, DFS_ACT_SILU = 3 };
 int64_t dfs_linear_workspace_size(int64_t rows, int64_t n, int64_t k, int aligned);
-int dfs_linear(const void* x, int64_t x_stride, const void* w, int64_t w_stride,
-               int64_t rows, int64_t n, int64_t k, int dtype, const void* bias,
-               int bias_dtype, int activation, const float* gate,
-               const void* residual, int64_t r_stride, void* out,
-               int64_t o_stride, void* workspace, int64_t workspace_bytes,
-               dfs_stream_t stream);
+typedef struct dfs_linear_args {
+  int64_t rows, n, k, dtype, bias_dtype, activation;
+  int64_t x_stride, w_stride, residual_stride, out_stride;
+  int64_t workspace_bytes;
+  const void *x, *w, *bias;
+  const float* gate;
+  const void* residual;
+  void *out, *workspace;
+} dfs_linear_args;
+int dfs_linear(const dfs_linear_args* args, dfs_stream_t stream);
 
 /*
  * Attention with a sliding window and sinks. q [B][q_heads][q_rows][D], k and

@@ -179,8 +179,11 @@ def test_limits_behind_every_length_are_kept_within_their_type():
 def test_sizes_beyond_a_launch_are_refused():
     """The library's own checks, which end a call before its launch."""
     def linear(rows, n, k):
-        size = max(_lib.lib().dfs_linear_workspace_size(rows, n, k, 1), 0)
-        _lib.call("dfs_linear", 16, k, 16, k, rows, n, k, 0, None, 0, 0, None, None, 0, 16, n, 16, size, None)
+        a = _lib.LinearArgs()
+        a.rows, a.n, a.k, a.x_stride, a.w_stride, a.out_stride = rows, n, k, k, k, n
+        a.x = a.w = a.out = a.workspace = 16
+        a.workspace_bytes = max(_lib.lib().dfs_linear_workspace_size(rows, n, k, 1), 0)
+        _lib.call("dfs_linear", bytes(a), None)
 
     with pytest.raises(_lib.DfsKernelError, match="2\\^21"):
         linear(1, 8, 1 << 21)
