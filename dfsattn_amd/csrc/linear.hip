@@ -197,6 +197,7 @@ __device__ __forceinline__ uint4 load_row8(const uint16_t* row, int k, int K) {
 // strides and sizes: rows are loaded into registers, four steps ahead, and
 // stored to one of two LDS buffers from there, one barrier a step. The channels
 // behind the last whole step go first, so that the steps' loads have no edge.
+// 333 x 1,017 x 709: 8.9 us; loads a step ahead, with two barriers: 11.9.
 template <bool F16>
 __global__ void __launch_bounds__(256) linear_any_kernel(LinearParams p) {
   __shared__ __attribute__((aligned(16))) uint16_t ws[2][64 * 64];
@@ -607,18 +608,19 @@ __global__ void __launch_bounds__(256, 2) linear_tile_kernel(LinearParams p) {
 // row's 128), and a step is four phases of one quadrant each, 16 products:
 //   (A0, B0) (A1, B0) (A1, B1) (A0, B1)
 // A phase reads one half into registers for the next (A1, B1, then the next
-// step's B0 and A0: the registers just left), and loads the half read in the
-// phase before, two steps on. So all phases are alike: one half read, one
-// loaded seven phases before it is read, one barrier that says both that the
-// half to be read has landed and that the half to be loaded was read by all.
+// step's B0 and A0: the registers just left), and loads a half read in the pair
+// of phases before, two steps on. So all pairs are alike: two halves read, two
+// loaded three pairs before they are read, one barrier that says both that the
+// halves to be read have landed and that those to be loaded were read by all.
 //
-// 75,600 x 13,824 x 5,120: 7.92 ms, 1.35 PFLOP/s (the library's product alone
-// 7.1, 1.50); 16,384 x 16,384 x 5,120: 1.91 ms, 1.44 PFLOP/s (1.77, 1.55). The
-// matrix cores are busy 79% of the cycles and the clock falls to 1.55 GHz: power
-// is the bound. A barrier a step of 64 channels with its loads behind it took
-// 10.6 ms, the phases with a branch for the last step's edge 9.0; outputs stored
-// from the products' layout, 16 bytes of a row at a time, cost 40 us a tile
-// instead of 3.
+// 75,600 x 13,824 x 5,120 with GELU: 7.97 ms, 1.34 PFLOP/s (the library's
+// product alone 7.1, 1.50); 75,600 x 5,120 x 13,824: 7.56 ms, 1.41 PFLOP/s (6.9,
+// 1.55); 16,384 x 16,384 x 5,120: 1.90 ms, 1.45 PFLOP/s (1.77, 1.55). The matrix
+// cores are busy 79% of the cycles and the clock falls to 1.55 GHz: power is the
+// bound, and a barrier a phase costs 0.5%. A barrier a step of 64 channels with
+// its loads behind it took 10.6 ms, the phases with a branch for the last step's
+// edge 9.0; outputs stored from the products' layout, 16 bytes of a row at a
+// time, cost 40 us a tile instead of 3.
 template <bool F16, int ACT>
 __global__ void __launch_bounds__(256, 1) linear_big_kernel(LinearParams p) {
   typedef typename Half<F16>::vec vec;
@@ -718,8 +720,8 @@ __global__ void __launch_bounds__(256, 1) linear_big_kernel(LinearParams p) {
     }
     __builtin_amdgcn_sched_barrier(0);
   };
-  auto landed = [&] {  // the half loaded seven phases ago; six phases' loads are behind it
-    wait_vmcnt<24>();
+  auto landed = [&] {  // the halves loaded three pairs of phases ago; two pairs' loads are behind them
+    wait_vmcnt<16>();
     block_barrier();
   };
   Frag fa0, fa1, fb0, fb1;
@@ -731,19 +733,17 @@ __global__ void __launch_bounds__(256, 1) linear_big_kernel(LinearParams p) {
                   uint16_t* b0n) {
     landed();
     read_w(a1c, c1);
-    load_w(tail, t + 2, 0, a0c);
+    load_x(tail, t + 2, 0, b0c);
     quadrant(c0, fb0, 0, 0);
-    landed();
     read_x(b1c, fb1);
-    load_w(tail, t + 2, 1, a1c);
+    load_w(tail, t + 2, 0, a0c);
     quadrant(c1, fb0, 1, 0);
     landed();
     read_x(b0n, fb0);
-    load_x(tail, t + 2, 1, b1c);
+    load_w(tail, t + 2, 1, a1c);
     quadrant(c1, fb1, 1, 1);
-    landed();
     read_w(a0n, c1);
-    load_x(tail, t + 3, 0, b0n);
+    load_x(tail, t + 2, 1, b1c);
     quadrant(c0, fb1, 0, 1);
   };
   load_x(may_end, 0, 0, b00);
@@ -754,14 +754,12 @@ __global__ void __launch_bounds__(256, 1) linear_big_kernel(LinearParams p) {
   load_w(may_end, 1, 0, a01);
   load_w(may_end, 1, 1, a11);
   load_x(may_end, 1, 1, b11);
-  wait_vmcnt<28>();
+  wait_vmcnt<24>();
   block_barrier();
   read_x(b00, fb0);
-  landed();
   read_w(a00, fa0);
-  load_x(may_end, 2, 0, b00);
   int t = 0;
-  for (; (t + 5) * 64 <= p.K; t += 2) {  // nothing past K is loaded
+  for (; (t + 4) * 64 <= p.K; t += 2) {  // nothing past K is loaded
     step(whole, t, fa0, fa1, a00, a10, b00, b10, a01, b01);
     step(whole, t + 1, fa1, fa0, a01, a11, b01, b11, a00, b00);
   }
@@ -890,8 +888,8 @@ struct Cut {
 Cut cut_of(int64_t rows, int64_t n, int64_t k, bool chunks) {
   // Rows on no 16-byte boundary: small products of few steps as they are, the
   // others laid out anew (us, as they are and anew: 333 by 1,017 x 709 8.9 and
-  // 11.3, 100 by 5,119 x 1,001 11.9 and 15.9; 400 by 1,001 x 3,001 29.0 and
-  // 23.1, 1 by 5,119 x 5,119 54.6 and 29.5, 6,694 by 1,422 x 5,465 370 and 148).
+  // 11.3, 100 by 5,119 x 1,001 11.7 and 15.9; 333 by 1,017 x 1,501 13.6 and 14.9,
+  // 100 by 1,001 x 2,001 16.6 and 13.6, 64 by 640 x 6,001 35.8 and 18.8).
   if (!chunks && k <= 1024 && rows * n * k < (int64_t(1) << 30)) return Cut{kTileAny, 1, 0, false};
   if (rows <= 8) return Cut{kFew, 1, 0, !chunks};
   // The tiles and parts with the least time by what each took on an idle CU and
