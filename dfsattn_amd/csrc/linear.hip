@@ -35,8 +35,10 @@ struct LinearParams {
   const uint16_t* residual;  // [M][N], row stride ldr, or NULL; may be out
   uint16_t* out;
   // The channels of a tile are cut into `splits` parts of `depth` (a multiple
-  // of 128); a part's sums go to part [split][M][ceil(N / 8) * 8] in fp32.
-  int splits, depth;
+  // of 128); a part's sums go to part [split][M][ceil(N / 8) * 8] in fp32. Of the
+  // 256 x 256 tiles the first `whole` are not cut, the others' sums go to part
+  // [split][tile][256][256].
+  int splits, depth, whole;
   float* part;
 };
 
@@ -630,11 +632,15 @@ __global__ void __launch_bounds__(256, 1) linear_big_kernel(LinearParams p) {
   __shared__ __attribute__((aligned(16))) float stage[4 * 2048];
   const int lane = threadIdx.x & 63, w = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const int l32 = lane & 31, hl = lane >> 5;
+  const int mt = (p.M + 255) / 256, nt = (p.N + 255) / 256, cut = mt * nt - p.whole;
+  const bool in_parts = static_cast<int>(blockIdx.x) >= p.whole;
+  const int split = in_parts ? (static_cast<int>(blockIdx.x) - p.whole) / cut : 0, from = split * p.depth;
+  const int K = in_parts ? min(p.K - from, p.depth) : p.K, id = blockIdx.x - split * cut;
   int tm, tn;
-  tile_of(blockIdx.x, (p.M + 255) / 256, (p.N + 255) / 256, tm, tn);
+  tile_of(id, mt, nt, tm, tn);
   const int n0 = tn * 256, m0 = tm * 256;
-  const auto wrs = make_rsrc(p.w + static_cast<int64_t>(n0) * p.ldw, kOutside);
-  const auto xrs = make_rsrc(p.x + static_cast<int64_t>(m0) * p.ldx, kOutside);
+  const auto wrs = make_rsrc(p.w + static_cast<int64_t>(n0) * p.ldw + from, kOutside);
+  const auto xrs = make_rsrc(p.x + static_cast<int64_t>(m0) * p.ldx + from, kOutside);
   // Byte offsets of this lane's chunks in step 0, [half][load]; rows past the
   // matrix repeat its last one. Row q of wave row r's 64 in half h is output
   // r * 128 + (q >> 3) * 16 + h * 8 + (q & 7), so that a lane ends with 16
@@ -651,10 +657,10 @@ __global__ void __launch_bounds__(256, 1) linear_big_kernel(LinearParams p) {
       wv[h][j] = static_cast<uint32_t>(n) * static_cast<uint32_t>(p.ldw * 2) + (c8 ^ T::swz_w(q)) * 16;
       xv[h][j] = static_cast<uint32_t>(m) * static_cast<uint32_t>(p.ldx * 2) + (c8 ^ T::swz_x(q)) * 16;
     }
-  const int steps = (p.K + 127) >> 7 << 1;  // an even number: the last may be all zeros
+  const int steps = (K + 127) >> 7 << 1;  // an even number: the last may be all zeros
   // The last steps' chunks past K (tail) come as zeros, without a memory access.
   auto load_w = [&](auto tail, int t, int h, uint16_t* buf) {
-    const int left = p.K - t * 64;
+    const int left = K - t * 64;
     if (tail.value && left < 64) {
 #pragma unroll
       for (int j = 0; j < 4; ++j)
@@ -664,7 +670,7 @@ __global__ void __launch_bounds__(256, 1) linear_big_kernel(LinearParams p) {
     for (int j = 0; j < 4; ++j) load_lds16(wrs, buf + (j * 4 + w) * 512, wv[h][j], t * 128);
   };
   auto load_x = [&](auto tail, int t, int h, uint16_t* buf) {
-    const int left = p.K - t * 64;
+    const int left = K - t * 64;
     if (tail.value && left < 64) {
 #pragma unroll
       for (int j = 0; j < 4; ++j)
@@ -759,7 +765,7 @@ __global__ void __launch_bounds__(256, 1) linear_big_kernel(LinearParams p) {
   read_x(b00, fb0);
   read_w(a00, fa0);
   int t = 0;
-  for (; (t + 4) * 64 <= p.K; t += 2) {  // nothing past K is loaded
+  for (; (t + 4) * 64 <= K; t += 2) {  // nothing past K is loaded
     step(whole, t, fa0, fa1, a00, a10, b00, b10, a01, b01);
     step(whole, t + 1, fa1, fa0, a01, a11, b01, b11, a00, b00);
   }
@@ -774,6 +780,7 @@ __global__ void __launch_bounds__(256, 1) linear_big_kernel(LinearParams p) {
   // of it: whole rows of 128 bytes leave (and come, for the residual).
   float* const st = stage + w * 2048;
   const bool inside = m0 + 256 <= p.M && n0 + 256 <= p.N;
+  float* const part = p.part + static_cast<int64_t>(split * cut + id - p.whole) * 65536;  // of a tile in parts
 #pragma unroll
   for (int gp = 0; gp < 2; ++gp) {
     const int n = n0 + wn * 128 + gp * 64 + (lane & 7) * 8, c = (lane & 7) * 2;
@@ -797,7 +804,15 @@ __global__ void __launch_bounds__(256, 1) linear_big_kernel(LinearParams p) {
         z[4] = hi.x; z[5] = hi.y; z[6] = hi.z; z[7] = hi.w;
         return m0 + wm * 128 + j * 32 + r;
       };
-      if (inside) {
+      if (in_parts) {
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+          float z[8];
+          float* const at = part + (row(i, z) - m0) * 256 + n - n0;
+          *reinterpret_cast<float4*>(at) = make_float4(z[0], z[1], z[2], z[3]);
+          *reinterpret_cast<float4*>(at + 4) = make_float4(z[4], z[5], z[6], z[7]);
+        }
+      } else if (inside) {
 #pragma unroll
         for (int i = 0; i < 4; ++i) {
           float z[8];
@@ -828,6 +843,27 @@ __global__ void __launch_bounds__(256) linear_join_kernel(LinearParams p) {
   const float* src = p.part + m * ld + n;
   float z[8] = {};
   for (int i = 0; i < p.splits; ++i, src += p.M * ld) {
+    const float4 a = *reinterpret_cast<const float4*>(src), b = *reinterpret_cast<const float4*>(src + 4);
+    z[0] += a.x; z[1] += a.y; z[2] += a.z; z[3] += a.w;
+    z[4] += b.x; z[5] += b.y; z[6] += b.z; z[7] += b.w;
+  }
+  float bias[8], gate[8];
+  load_columns8(p, n, bias, gate);
+  with_activation(p.act, [&](auto act) { finish8<F16, decltype(act)::value>(p, m, n, z, bias, gate); });
+}
+
+// The same for the 256 x 256 tiles in parts, 32 workgroups a tile.
+template <bool F16>
+__global__ void __launch_bounds__(256) linear_join_big_kernel(LinearParams p) {
+  const int mt = (p.M + 255) / 256, nt = (p.N + 255) / 256, cut = mt * nt - p.whole;
+  const int tile = blockIdx.x >> 5, row = (blockIdx.x & 31) * 8 + (threadIdx.x >> 5), col = (threadIdx.x & 31) * 8;
+  int tm, tn;
+  tile_of(p.whole + tile, mt, nt, tm, tn);
+  const int m = tm * 256 + row, n = tn * 256 + col;
+  if (m >= p.M || n >= p.N) return;
+  float z[8] = {};
+  for (int i = 0; i < p.splits; ++i) {
+    const float* const src = p.part + static_cast<int64_t>(i * cut + tile) * 65536 + row * 256 + col;
     const float4 a = *reinterpret_cast<const float4*>(src), b = *reinterpret_cast<const float4*>(src + 4);
     z[0] += a.x; z[1] += a.y; z[2] += a.z; z[3] += a.w;
     z[4] += b.x; z[5] += b.y; z[6] += b.z; z[7] += b.w;
@@ -883,15 +919,17 @@ enum Form { kFew, kTileAny, kTile64, kTile64x128, kTile128Deep, kTile128, kTile2
 struct Cut {
   Form form;
   int splits, depth;
-  bool pad;  // operands are laid out on 16-byte rows first
+  bool pad;       // operands are laid out on 16-byte rows first
+  int64_t whole;  // 256 x 256 tiles that are not cut
 };
+int64_t big_tiles(int64_t rows, int64_t n) { return (rows + 255) / 256 * ((n + 255) / 256); }
 Cut cut_of(int64_t rows, int64_t n, int64_t k, bool chunks) {
   // Rows on no 16-byte boundary: small products of few steps as they are, the
   // others laid out anew (us, as they are and anew: 333 by 1,017 x 709 8.9 and
   // 11.3, 100 by 5,119 x 1,001 11.7 and 15.9; 333 by 1,017 x 1,501 13.6 and 14.9,
   // 100 by 1,001 x 2,001 16.6 and 13.6, 64 by 640 x 6,001 35.8 and 18.8).
-  if (!chunks && k <= 1024 && rows * n * k < (int64_t(1) << 30)) return Cut{kTileAny, 1, 0, false};
-  if (rows <= 8) return Cut{kFew, 1, 0, !chunks};
+  if (!chunks && k <= 1024 && rows * n * k < (int64_t(1) << 30)) return Cut{kTileAny, 1, 0, false, 0};
+  if (rows <= 8) return Cut{kFew, 1, 0, !chunks, 0};
   // The tiles and parts with the least time by what each took on an idle CU and
   // beside others, a step of 64 channels of a workgroup in us, and by writing
   // and joining the parts' sums at 3 TB/s behind 5 us. Where several fit on a
@@ -910,7 +948,7 @@ Cut cut_of(int64_t rows, int64_t n, int64_t k, bool chunks) {
                 {kTile128Deep, 128, 128, 2, true, 0.55, 0.55},
                 {kTile128, 128, 128, 4, false, 0.72, 0.57},
                 {kTile256, 256, 256, 1, true, 1.15, 1.4}};
-  Cut best{kTile64, 1, 0, !chunks};
+  Cut best{kTile64, 1, 0, !chunks, 0};
   double least = 1e30;
   for (const auto& f : kinds)
     for (int s = 1; s <= f.most; s *= 2) {
@@ -928,12 +966,29 @@ Cut cut_of(int64_t rows, int64_t n, int64_t k, bool chunks) {
         best.depth = static_cast<int>(depth);
       }
     }
+  // The 256 x 256 tiles behind the last full round of 256 in parts, which
+  // together fill it (us, whole and in parts: 3,600 by 5,120 x 5,120 204 and 170,
+  // 4,200 by 4,200 x 3,000 164 and 121, 4,680 by 5,120 x 5,120 212 and 206,
+  // 75,600 by 5,120 x 13,824 7,680 and 7,565).
+  const int64_t tiles = big_tiles(rows, n), whole = tiles / 256 * 256, rest = tiles - whole, steps = (k + 63) / 64;
+  best.whole = best.form == kTile256 ? tiles : 0;
+  for (int64_t s = 2; rest > 0 && rest * s <= 256; ++s) {
+    const int64_t depth = ((k + s - 1) / s + 127) / 128 * 128, parts = (k + depth - 1) / depth;
+    if (depth < 512) break;
+    const double us = 1.4 * static_cast<double>(steps * (whole / 256) + depth / 64) + 10.0 +
+                      8e-6 / 3.0 * static_cast<double>(parts * rest * 65536);
+    if (parts == s && us < least) {
+      least = us;
+      best = Cut{kTile256, static_cast<int>(parts), static_cast<int>(depth), best.pad, whole};
+    }
+  }
   return best;
 }
 
 int64_t padded(int64_t k) { return (k + 7) / 8 * 8; }
 int64_t part_bytes(const Cut& c, int64_t rows, int64_t n) {
-  return c.splits > 1 ? c.splits * rows * padded(n) * 4 : 0;  // a multiple of 32
+  if (c.splits <= 1) return 0;
+  return c.form == kTile256 ? c.splits * (big_tiles(rows, n) - c.whole) * 65536 * 4 : c.splits * rows * padded(n) * 4;
 }
 int64_t workspace_bytes_of(const Cut& c, int64_t rows, int64_t n, int64_t k) {
   return part_bytes(c, rows, n) + (c.pad ? (rows + n) * padded(k) * 2 : 0);
@@ -1002,6 +1057,7 @@ extern "C" int dfs_linear(const dfs_linear_args* a, dfs_stream_t stream) {
   hipStream_t st = reinterpret_cast<hipStream_t>(stream);
   p.splits = cut.splits;
   p.depth = cut.depth;
+  p.whole = static_cast<int>(cut.whole);
   p.part = static_cast<float*>(a->workspace);
   const bool f16 = a->dtype == DFS_DTYPE_F16;
   if (cut.pad) {
@@ -1036,13 +1092,18 @@ extern "C" int dfs_linear(const dfs_linear_args* a, dfs_stream_t stream) {
       launch_tile<2, 2, 2, 2, 2>(p, f16, st);
       break;
     case kTile256: {
-      const dim3 grid(static_cast<unsigned>(((rows + 255) / 256) * ((n + 255) / 256)));
+      const int64_t rest = big_tiles(rows, n) - cut.whole;
+      const dim3 grid(static_cast<unsigned>(cut.whole + rest * cut.splits));
       with_activation(p.act, [&](auto act) {
         if (f16)
           linear_big_kernel<true, decltype(act)::value><<<grid, 256, 0, st>>>(p);
         else
           linear_big_kernel<false, decltype(act)::value><<<grid, 256, 0, st>>>(p);
       });
+      if (rest > 0) {
+        const dim3 join(static_cast<unsigned>(rest * 32));
+        f16 ? linear_join_big_kernel<true><<<join, 256, 0, st>>>(p) : linear_join_big_kernel<false><<<join, 256, 0, st>>>(p);
+      }
       break;
     }
   }

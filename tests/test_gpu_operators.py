@@ -7,7 +7,7 @@ import pytest
 import torch
 
 import operator_refs as refs
-from dfsattn_amd import ops
+from dfsattn_amd import _lib, ops
 
 pytestmark = pytest.mark.gpu
 BF, HF = torch.bfloat16, torch.float16
@@ -76,6 +76,24 @@ def test_linear_matches_definition(dev, m, n, k, dtype, bias, act, gate, residua
     if residual:  # in place of the residual
         d[4] = ops.linear(d[0], d[1], d[2], activation=act, gate=d[3], residual=d[4], out=d[4])
         assert torch.equal(got, d[4])
+
+
+@pytest.mark.parametrize("m,n,k,act", [(4200, 4200, 3000, "gelu_tanh"), (2560, 6500, 4104, None)])
+def test_linear_last_tiles_in_parts(dev, m, n, k, act):
+    """More large tiles than compute units: those behind the last full round
+    are cut along k. Rows and outputs picked all over the result."""
+    print(f"linear {m} x {n} x {k} {act}", flush=True)
+    assert _lib.lib().dfs_linear_workspace_size(m, n, k, 1) > 0
+    gen = torch.Generator().manual_seed(m + n + k)
+    x, w = _randn(gen, m, k, dtype=BF), _randn(gen, n, k, dtype=BF, std=2 / math.sqrt(k))
+    b, gate, r = _randn(gen, n, dtype=BF), torch.randn(n, generator=gen), _randn(gen, m, n, dtype=BF)
+    d = [t.to(dev) for t in (x, w, b, gate, r)]
+    got = ops.linear(d[0], d[1], d[2], activation=act, gate=d[3], residual=d[4])
+    assert torch.equal(got, ops.linear(d[0], d[1], d[2], activation=act, gate=d[3], residual=d[4]))
+    rows, cols = torch.arange(0, m, 13), torch.arange(0, n, 11)
+    rows[-1], cols[-1] = m - 1, n - 1
+    ref, tol = refs.linear(x[rows], w[cols], b[cols], act, gate[cols], r[rows][:, cols])
+    _within(got.cpu()[rows][:, cols], ref, tol, "parts")
 
 
 @pytest.mark.parametrize("m", [1, 5, 40, 130, 700])
