@@ -2,6 +2,7 @@
 their 64-bit definitions (operator_refs), within the bounds that their
 roundings allow."""
 import math
+import threading
 
 import pytest
 import torch
@@ -340,6 +341,41 @@ def test_operators_on_another_stream(dev):
         att2 = ops.window_attention(got.view(1, 300, 4, 128).transpose(1, 2), k, k, left=50, right=0)
     side.synchronize()
     assert torch.equal(want, got) and torch.equal(att, att2)
+
+
+def test_operators_from_two_threads(dev):
+    """Two threads on streams of their own, products in parts (a workspace each)
+    and attention over a cut cache: each gets what it gets alone."""
+    gen = torch.Generator().manual_seed(7)
+    jobs = []
+    for _ in range(2):
+        x, w = _randn(gen, 64, 4096, dtype=BF).to(dev), _randn(gen, 640, 4096, dtype=BF, std=0.02).to(dev)
+        q = _randn(gen, 2, 8, 1, 64, dtype=BF).to(dev)
+        k, v = (_randn(gen, 2, 2, 3000, 64, dtype=BF).to(dev) for _ in range(2))
+        jobs.append((x, w, q, k, v))
+    assert _lib.lib().dfs_linear_workspace_size(64, 640, 4096, 1) > 0
+
+    def run(job):
+        return ops.linear(job[0], job[1], activation="silu"), ops.window_attention(*job[2:], right=0)
+
+    want = [run(j) for j in jobs]
+    torch.cuda.synchronize()
+    got = [None, None]
+
+    def work(i):
+        stream = torch.cuda.Stream()
+        with torch.cuda.stream(stream):
+            got[i] = [run(jobs[i]) for _ in range(20)]
+        stream.synchronize()
+
+    threads = [threading.Thread(target=work, args=(i,)) for i in range(2)]
+    for t in threads:
+        t.start()
+    for t in threads:
+        t.join()
+    for i in range(2):
+        for y, o in got[i]:
+            assert torch.equal(y, want[i][0]) and torch.equal(o, want[i][1])
 
 
 def test_operators_in_a_graph(dev):
