@@ -32,6 +32,7 @@ struct WindowParams {
   int stream;  // its keys and values are beyond the last-level cache
   int blocks;  // of 128 rows of a (sequence, key head)
   int chunks, whole, split, parts;
+  int short_last;  // the heads' last blocks, of few rows, come behind all others
   float *part_o, *part_ml;  // O [row][D] and (m, l) [row][2] of the parts
 };
 
@@ -372,13 +373,31 @@ struct Item {
   int bh, blk, piece, pieces, slot;
 };
 
+// Block i of XCD x: its (sequence, key head) and its number there.
+__device__ __forceinline__ void block_of(const WindowParams& p, int x, int i, int& bh, int& blk) {
+  if (p.short_last) {  // chunks == 1: an XCD has whole heads
+    const int full = p.blocks - 1, all = p.B * p.Hkv / 8 * full;
+    const int h = i < all ? i / full : i - all;
+    bh = h * 8 + x;
+    blk = i < all ? full - 1 - (i - h * full) : full;
+    return;
+  }
+  const int per = (p.blocks + p.chunks - 1) / p.chunks;  // blocks of a range
+  const int u = i / per * 8 + x;
+  bh = u / p.chunks;
+  blk = p.blocks - 1 - (u % p.chunks * per + i % per);
+}
+
 // Hardware deals workgroup i to XCD i % 8. The blocks of a (sequence, key
 // head) are cut into p.chunks ranges and range u of them all belongs to XCD
 // u % 8, so neighbouring blocks, which share keys, run on one XCD's L2 and
 // sequences of different lengths spread evenly. Of an XCD's list the first
 // p.whole blocks are one workgroup each, the rest p.parts, joined by
 // window_join_kernel. Late blocks, which see most keys where left has no limit,
-// are started first.
+// are started first; where left has a limit, a head's last block with rows for
+// at most two of its waves comes behind all others and fills places that the
+// last round leaves (40 heads, 1,560 rows by 9,360 keys 358 us, in its place 370;
+// 3,600 by 14,400 963 and 981; without a limit 8 heads x 12,040 458 and 386).
 __device__ __forceinline__ bool item_of(const WindowParams& p, Item& it) {
   const int x = blockIdx.x & 7, j = blockIdx.x >> 3;
   int i = j;
@@ -392,10 +411,7 @@ __device__ __forceinline__ bool item_of(const WindowParams& p, Item& it) {
     it.slot = (t * 8 + x) * p.parts + it.piece;
     i = p.whole + t;
   }
-  const int per = (p.blocks + p.chunks - 1) / p.chunks;  // blocks of a range
-  const int u = i / per * 8 + x;
-  it.bh = u / p.chunks;
-  it.blk = p.blocks - 1 - (u % p.chunks * per + i % per);
+  block_of(p, x, i, it.bh, it.blk);
   return it.bh < p.B * p.Hkv && it.blk >= 0;
 }
 
@@ -634,10 +650,8 @@ __global__ void __launch_bounds__(256) window_join_kernel(WindowParams p) {
     step = rows;
   } else {
     const int block = static_cast<int>(id >> 7), x = block & 7, i = p.whole + (block >> 3);
-    const int per = (p.blocks + p.chunks - 1) / p.chunks;
-    const int u = i / per * 8 + x;
-    bh = u / p.chunks;
-    const int blk = p.blocks - 1 - (u % p.chunks * per + i % per);
+    int blk;
+    block_of(p, x, i, bh, blk);
     r = blk * 128 + static_cast<int>(id & 127);
     if (bh >= p.B * p.Hkv || blk < 0 || r >= rows) return;
     first = static_cast<int64_t>(block) * p.parts * 128 + (id & 127);
@@ -724,6 +738,7 @@ void plan(const dfs_window_args* a, WindowParams& p) {
   p.parts = 1;
   p.split = 0;
   const int64_t rest = list % kSlots;
+  p.short_last = a->left >= 0 && p.chunks == 1 && p.blocks > 1 && rows % 128 > 0 && rows % 128 <= 64 && list < 16 * kSlots;
   if (rest == 0 || list >= 16 * kSlots || tiles < 4) return;
   // Time of the last round in whole blocks: rounds / parts, and a part's own
   // start and store, worth about a tile.

@@ -181,6 +181,9 @@ ATTENTION = [
     (2, 3, 1, 1, 4100, 64, HF, None, 0, 0, None, [4100, 130], False),
     (2, 8, 1, 40, 3000, 128, BF, None, 0, 0, [40, 3], [3000, 5], False),
     (1, 2, 2, 70, 2600, 64, HF, 2400, None, 100, None, [9000], True),
+    # heads for every eighth of the chip, a few rows in their last blocks
+    (1, 8, 8, 150, 900, 128, BF, 500, None, 64, None, [2000], True),
+    (2, 8, 4, 140, 140, 64, HF, 100, 0, 4, [140, 77], [140, 77], False),
 ]
 
 
