@@ -773,10 +773,11 @@ def _dense(shape: Shape, stride: Shape) -> bool:
 
 
 def _chunk_rows(shape: Shape, stride: Shape) -> bool:
-    """Whether rows of the last axis are whole and follow each other in
-    16-byte steps (16-bit elements)."""
+    """Whether rows of the last axis are whole, one element behind the other
+    (not one element for several), and follow each other in 16-byte steps
+    (16-bit elements)."""
     strides = _axis_strides(shape, stride)
-    return strides[-1] in (0, 1) and all(s % 8 == 0 for s in strides[:-1])
+    return (shape[-1] == 1 or strides[-1] == 1) and all(s % 8 == 0 for s in strides[:-1])
 
 
 def _in_chunks(t: torch.Tensor) -> torch.Tensor:

@@ -496,3 +496,40 @@ def test_caches_beyond_32_bits(dev, L):
     got = ops.window_attention(qn, kc, vc, left=500, right=0)
     ref, tol = refs.window_attention(qn.cpu(), ks.cpu(), vs.cpu(), left=500, right=0)[::2][:2]
     _within(got, ref, tol, "attention")
+
+
+# --------------------------------------------------------------------------
+# views whose channels share an element
+# --------------------------------------------------------------------------
+
+def _shared_channels(t):
+    """Views of t's shape whose channels have stride 0: of its first channel,
+    of a later one, of one element."""
+    return t[..., :1].expand(t.shape), t[..., 8:9].expand(t.shape), t.flatten()[5].expand(t.shape)
+
+
+@pytest.mark.parametrize("L", [2, 70])
+def test_operators_take_channels_that_share_an_element(dev, L):
+    gen = torch.Generator().manual_seed(81)
+    base = {n: _randn(gen, 2, h, s, 64, dtype=BF).to(dev) for n, h, s in (("q", 4, L), ("k", 2, 90), ("v", 2, 90))}
+    lens = torch.tensor([3, 0], dtype=torch.int32, device=dev)
+    for name in base:
+        for view in _shared_channels(base[name]):
+            print(f"shared channels L={L} {name} {tuple(view.stride())}", flush=True)
+            args = {**base, name: view}
+            got = ops.window_attention(**args, left=40, right=0)
+            assert torch.equal(got, ops.window_attention(**{**args, name: view.contiguous()}, left=40, right=0))
+            new = {**{n: base["v" if n == "k" else "k"][:, :, :5].transpose(1, 2) for n in "qkv"},
+                   name: view[:, :2, :2].transpose(1, 2)}
+            new = {n: t[:, :2] for n, t in new.items()}
+            assert new[name].stride(3) == 0
+            caches = [[torch.zeros(2, 2, 9, 64, dtype=BF, device=dev) for _ in range(2)] for _ in range(2)]
+            a = ops.qkv_cache(**new, k_cache=caches[0][0], v_cache=caches[0][1], lens=lens)
+            whole = {n: t.contiguous() for n, t in new.items()}
+            b = ops.qkv_cache(**whole, k_cache=caches[1][0], v_cache=caches[1][1], lens=lens)
+            assert torch.equal(a, b)
+            assert torch.equal(caches[0][0], caches[1][0]) and torch.equal(caches[0][1], caches[1][1])
+            x = view[0, 0]
+            w = base["k"][0, 0]
+            assert torch.equal(ops.linear(x, w), ops.linear(x.contiguous(), w))
+            assert torch.equal(ops.linear(w, x), ops.linear(w, x.contiguous()))

@@ -205,3 +205,38 @@ def test_sizes_beyond_a_launch_are_refused():
         setattr(a, name, 16)
     with pytest.raises(_lib.DfsKernelError, match="too many rows"):
         _lib.call("dfs_window_attention", bytes(a), None)
+
+
+# --------------------------------------------------------------------------
+# channels that share an element
+# --------------------------------------------------------------------------
+
+def _shared_channels(*shape):
+    """Tensors of this shape whose channels (and more axes) have stride 0."""
+    whole = torch.arange(4096, dtype=BF).repeat(8)[:torch.Size(shape).numel()].reshape(shape)
+    return [whole[..., :1].expand(shape), whole[..., 8:9].expand(shape), torch.tensor(3.0, dtype=BF).expand(shape),
+            whole[:1, ..., :1].expand(shape), whole[:, :, :1, :1].expand(shape)]
+
+
+def test_channels_that_share_an_element_are_copied():
+    """The kernels read a row's channels one behind the other: rows whose
+    channels are one element are never read in place."""
+    for t in _shared_channels(2, 2, 9, 64):
+        assert t.stride(3) == 0
+        assert not ops._chunk_rows(t.shape, t.stride()) and not ops._own_rows(t.shape, t.stride())
+        c = ops._in_chunks(t)
+        assert c.is_contiguous() and torch.equal(c, t)
+        for name in ("q", "k", "v"):
+            x = {**{n: (2, 2, 9, 64) for n in "qkv"}}
+            strides = {n: (1152, 576, 64, 1) for n in "qkv"}
+            strides[name] = t.stride()
+            plan = ops._window_plan(x["q"], strides["q"], x["k"], strides["k"], x["v"], strides["v"], (BF, BF, BF),
+                                    None, None, 0, 0, False, False, None)
+            assert not plan[3] and plan[2][-1] == 1  # not in place; out has channels of its own
+            shapes = (*x.values(), (2, 9, 9, 64), (2, 9, 9, 64))
+            dense = ops._contiguous_stride((2, 9, 9, 64))
+            assert not ops._cache_plan(shapes, (*strides.values(), dense, dense), (BF,) * 5, (None, None), None, 1e-6,
+                                       0, False)[1]
+    for shape, stride in (((2, 2, 9, 64), (1152, 576, 64, 1)), ((2, 2, 9, 64), (0, 0, 64, 1)),
+                          ((1, 1, 1, 64), (5, 3, 7, 1)), ((4, 1), (8, 5))):
+        assert ops._chunk_rows(shape, stride)
