@@ -266,20 +266,28 @@ __device__ __forceinline__ void pin_read_ahead() {
   __builtin_amdgcn_sched_group_barrier(kMfma, kAhead, 0);
 }
 
-// Running maximum, in log2 units, of the scores s[0..N) times c; O and l follow
-// it when some row's maximum has grown by more than 2^kSlack (P then stays
-// below 2^kSlack, which costs neither its relative precision nor fp32's range,
-// and most tiles leave O alone).
-constexpr float kSlack = 8.f;
-template <int N, int DCH>
+// A row's reference m, in log2 units: P = 2^(s c - m). It follows the running
+// maximum of the scores s[0..N) times c, less kBelow, and O and l follow it,
+// when some row's maximum has grown by more than 2^kSlack beyond it, so that most
+// tiles leave O alone. bf16 has fp32's exponents: P stays below 2^8, which costs
+// neither its relative precision nor the sums' range. f16 holds 11 bits only down
+// to 2^-14 and nothing below 2^-25: the row's largest P stands at 2^13 to 2^15
+// (65,504 is the largest), so that weights down to 2^-27 of it keep their 11 bits
+// and only those below 2^-38 are lost. (At 1, keys 17 nats below a sink counted
+// 1.44 times and those 17.4 below not at all.) f16 video 16.0 ms, 15.9 at 1.
+template <bool F16>
+struct Reference {
+  static constexpr float kBelow = F16 ? 13.f : 0.f, kSlack = F16 ? 2.f : 8.f;
+};
+template <int N, int DCH, bool F16>
 __device__ __forceinline__ float follow_max(const f32x16* s, float c, float& m, float& l, f32x16* o) {
   float mx = -INFINITY;
 #pragma unroll
   for (int k = 0; k < N; ++k)
 #pragma unroll
     for (int r = 0; r < 16; ++r) mx = fmaxf(mx, s[k][r]);
-  mx = xhalf_max(mx) * c;
-  if (__any(mx > m + kSlack)) {
+  mx = xhalf_max(mx) * c - Reference<F16>::kBelow;
+  if (__any(mx > m + Reference<F16>::kSlack)) {
     const float mn = fmaxf(m, mx);
     const float alpha = exp2_fast(m - (mn == -INFINITY ? 0.f : mn));
     l *= alpha;
@@ -318,8 +326,10 @@ __device__ __forceinline__ void mask32(f32x16& s, int first, int hl, int klo, in
   }
 }
 
+template <bool F16>
 __device__ __forceinline__ float lse_of(float m, float l) {
-  return l == 0.f ? -INFINITY : (m + log2f(l)) * 0.69314718055994531f;
+  constexpr float kBelow = Reference<F16>::kBelow, kUnit = F16 ? 0x1p-13f : 1.f;  // 2^-kBelow
+  return l == 0.f ? -INFINITY : ((m + kBelow) + log2f(l * kUnit)) * 0.69314718055994531f;
 }
 
 // O^T / l of a lane's row: the halves of a lane pair are joined into 8
@@ -426,7 +436,7 @@ __device__ __forceinline__ bool item_of(const WindowParams& p, Item& it) {
 //
 // P is rounded to the operands' 8 or 11 bits (the products take no more), and
 // the row sum adds the rounded values, so that the rounding cancels where one
-// weight dominates; statistics and O are fp32.
+// weight dominates; f16's range is at Reference. Statistics and O are fp32.
 //
 // 75,600 tokens x 40 heads, 10,800 keys a row: 15.0 ms, 1.07 PFLOP/s; matrix
 // cores busy 58% of the cycles at 1.8 GHz, the vector units 43%, which overlap
@@ -502,7 +512,7 @@ __global__ void __launch_bounds__(256, 2) window_tile_kernel(WindowParams p) {
 #pragma unroll
           for (int kb = 0; kb < 4; ++kb) mask32(s[kb], first + kb * 32, hl, klo, khi, p.sinks);
         }
-        const float ref = follow_max<4, DCH>(s, p.scale_log2, m, l, o);
+        const float ref = follow_max<4, DCH, F16>(s, p.scale_log2, m, l, o);
 #pragma unroll
         for (int kb = 0; kb < 4; ++kb) weights32<F16>(s[kb], p.scale_log2, ref, pf + 2 * kb, l);
       }
@@ -536,7 +546,7 @@ __global__ void __launch_bounds__(256, 2) window_tile_kernel(WindowParams p) {
   }
   store_row<D, F16>(p.out + b * p.o_sb + head * p.o_sh + row.i * p.o_sl, o, inv, in, hl);
   if (p.lse && in && hl == 0)
-    p.lse[(static_cast<int64_t>(b) * p.Hq + head) * p.Lq + row.i] = dead ? -INFINITY : lse_of(m, l);
+    p.lse[(static_cast<int64_t>(b) * p.Hq + head) * p.Lq + row.i] = dead ? -INFINITY : lse_of<F16>(m, l);
 }
 
 // At most 32 rows (a token, or a few, of a group's heads) over many keys: a
@@ -591,7 +601,7 @@ __global__ void __launch_bounds__(64, 2) window_few_kernel(WindowParams p) {
       f32x16 s;
       scores<D, F16, T>(kb, qf, l32, hl, &s);
       mask32(s, first, hl, klo, khi, p.sinks);
-      const float ref = follow_max<1, DCH>(&s, p.scale_log2, m, l, o);
+      const float ref = follow_max<1, DCH, F16>(&s, p.scale_log2, m, l, o);
       vec pf[2];
       weights32<F16>(s, p.scale_log2, ref, pf, l);
       vec vf[2][DCH];
@@ -624,7 +634,7 @@ __global__ void __launch_bounds__(64, 2) window_few_kernel(WindowParams p) {
   }
   store_row<D, F16>(p.out + b * p.o_sb + head * p.o_sh + row.i * p.o_sl, o, inv, in, hl);
   if (p.lse && in && hl == 0)
-    p.lse[(static_cast<int64_t>(b) * p.Hq + head) * p.Lq + row.i] = dead ? -INFINITY : lse_of(m, l);
+    p.lse[(static_cast<int64_t>(b) * p.Hq + head) * p.Lq + row.i] = dead ? -INFINITY : lse_of<F16>(m, l);
 }
 
 // Joins the parts of a row: O = sum 2^(m_i - M) O_i over the same sum of l_i.
@@ -704,7 +714,7 @@ __global__ void __launch_bounds__(256) window_join_kernel(WindowParams p) {
   const int head = g * p.group + row.g;
   *reinterpret_cast<uint2*>(p.out + b * p.o_sb + head * p.o_sh + row.i * p.o_sl + sub * 4) =
       make_uint2(pack2<F16>(o[0] * inv, o[1] * inv), pack2<F16>(o[2] * inv, o[3] * inv));
-  if (p.lse && sub == 0) p.lse[(static_cast<int64_t>(b) * p.Hq + head) * p.Lq + row.i] = lse_of(M, l);
+  if (p.lse && sub == 0) p.lse[(static_cast<int64_t>(b) * p.Hq + head) * p.Lq + row.i] = lse_of<F16>(M, l);
 }
 
 // How a call is cut. Slots for two workgroups on each of 256 CUs; the blocks

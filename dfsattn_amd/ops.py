@@ -982,8 +982,11 @@ def window_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, left: Op
     (``qkv_cache``); kv_lens counts every token so far and S must be at least
     sinks + left + L.
 
-    bf16 or f16, D 64 or 128, fp32 softmax; returns out in q's dtype (and
-    storage order) and with ``want_lse`` the fp32 log-sum-exp [B, H, L]. Rows
+    bf16 or f16, D 64 or 128, fp32 scores and statistics; the weights are
+    rounded to the operands' type for the product with v (f16: those below
+    2^-27 of a row's largest lose bits, those below 2^-38 are 0). Returns out
+    in q's dtype (and storage order) and with ``want_lse`` the fp32
+    log-sum-exp [B, H, L]. Rows
     that see no key (rows from q_lens[b] on among them) are 0, their lse -inf.
     Keys behind kv_lens may hold anything; values a query does not see inside
     the sequence must be finite. No backward pass."""

@@ -508,7 +508,9 @@ int dfs_linear(const dfs_linear_args* args, dfs_stream_t stream);
  * Attention with a sliding window and sinks. q [B][q_heads][q_rows][D], k and
  * v [B][kv_heads][slots][D] (q head h reads kv head h / (q_heads / kv_heads)),
  * out like q, with any strides that are multiples of 8 elements; D 64 or 128,
- * bf16 or f16. A sequence of nq = q_lens[b] queries (q_rows without q_lens) and
+ * bf16 or f16. Scores and statistics are fp32; the weights are rounded to the
+ * operands' type for the product with v (in f16 those below 2^-27 of a row's
+ * largest lose bits, those below 2^-38 are 0). A sequence of nq = q_lens[b] queries (q_rows without q_lens) and
  * nk = kv_lens[b] keys (slots without kv_lens; device int32, clamped to the
  * tensors): query i stands at position p = nk - nq + i and sees key j where
  * j < nk, j <= p + right and (j >= p - left or j < sinks); left and right -1:

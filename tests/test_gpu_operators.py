@@ -533,3 +533,29 @@ def test_operators_take_channels_that_share_an_element(dev, L):
             w = base["k"][0, 0]
             assert torch.equal(ops.linear(x, w), ops.linear(x.contiguous(), w))
             assert torch.equal(ops.linear(w, x), ops.linear(w, x.contiguous()))
+
+
+# --------------------------------------------------------------------------
+# weights far below a row's largest
+# --------------------------------------------------------------------------
+
+@pytest.mark.parametrize("dtype", [BF, HF])
+@pytest.mark.parametrize("L,S,D,place", [(1, 4000, 64, 0), (1, 300, 128, 299), (40, 4000, 128, 0), (40, 900, 64, 450)])
+@pytest.mark.parametrize("nats,spread", [(10.0, 0.3), (14.0, 0.3), (17.0, 0.3), (16.0, 0.0), (17.5, 0.0)])
+def test_window_attention_keeps_small_weights(dev, L, S, D, place, nats, spread, dtype):
+    """A key that takes nearly all of every row's weight and whose values are
+    zero (a sink): the output is what the other keys, 10 to 18 nats below it,
+    leave, and the bound is relative to that. f16 holds 11 bits down to 2^-14
+    and the largest weight stands at 2^13 or more, so 18.7 nats below it."""
+    print(f"small weights L={L} S={S} D={D} at {place} {nats} nats spread {spread} {dtype}", flush=True)
+    gen = torch.Generator().manual_seed(L + S)
+    q, k = (_randn(gen, 1, 2, n, D, dtype=dtype, std=spread / math.sqrt(D)) for n in (L, S))
+    v = _randn(gen, 1, 2, S, D, dtype=dtype).abs() + 0.5
+    q[..., 0] = 1
+    k[..., 0] = _randn(gen, 1, 2, S, dtype=dtype, std=spread)
+    k[:, :, place, 0], v[:, :, place] = nats, 0
+    ref, lse_ref, tol, lse_tol = refs.window_attention(q, k, v, scale=1.0)
+    assert 0.9 < float((torch.log(ref.mean()) + nats - math.log(S)).exp()) < 2.0
+    out, lse = ops.window_attention(q.to(dev), k.to(dev), v.to(dev), scale=1.0, want_lse=True)
+    _within(out, ref, tol, "small weights")
+    _within(lse, lse_ref, lse_tol, "their lse")
