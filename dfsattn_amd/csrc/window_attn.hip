@@ -7,6 +7,7 @@
 // Key j lies in slot j of the sequence's rows, or, in a rolling cache of S
 // slots, in slot j < sinks ? j : sinks + (j - sinks) mod (S - sinks).
 #include <algorithm>
+#include <type_traits>
 
 #include "common.h"
 #include "lds_copy.h"
@@ -33,7 +34,9 @@ struct WindowParams {
   int blocks;  // of 128 rows of a (sequence, key head)
   int chunks, whole, split, parts;
   int short_last;  // the heads' last blocks, of few rows, come behind all others
-  float *part_o, *part_ml;  // O [row][D] and (m, l) [row][2] of the parts
+  // Of the parts: O [row][D], (m, l) [row][2] and, where lse is wanted, the sum
+  // for it [row].
+  float *part_o, *part_ml, *part_e;
 };
 
 __device__ __forceinline__ int slot_of(const WindowParams& p, int pos) {
@@ -279,8 +282,8 @@ template <bool F16>
 struct Reference {
   static constexpr float kBelow = F16 ? 13.f : 0.f, kSlack = F16 ? 2.f : 8.f;
 };
-template <int N, int DCH, bool F16>
-__device__ __forceinline__ float follow_max(const f32x16* s, float c, float& m, float& l, f32x16* o) {
+template <int N, int DCH, bool F16, bool LSE>
+__device__ __forceinline__ float follow_max(const f32x16* s, float c, float& m, float& l, float& e, f32x16* o) {
   float mx = -INFINITY;
 #pragma unroll
   for (int k = 0; k < N; ++k)
@@ -291,6 +294,7 @@ __device__ __forceinline__ float follow_max(const f32x16* s, float c, float& m, 
     const float mn = fmaxf(m, mx);
     const float alpha = exp2_fast(m - (mn == -INFINITY ? 0.f : mn));
     l *= alpha;
+    if (LSE) e *= alpha;
 #pragma unroll
     for (int i = 0; i < DCH; ++i)
 #pragma unroll
@@ -301,15 +305,25 @@ __device__ __forceinline__ float follow_max(const f32x16* s, float c, float& m, 
 }
 
 // P = 2^(s c - m) of 32 keys as two PV operands; their rounded values are added
-// to l.
-template <bool F16>
-__device__ __forceinline__ void weights32(const f32x16& s, float c, float m, typename Half<F16>::vec* pf, float& l) {
+// to l, which divides O, and, where the log-sum-exp is wanted, the values as they
+// are to e: there is no rounding above that l's could cancel there (two keys in
+// tiles apart: 3e-3 with l in bf16). It costs instances that have no lse nothing
+// and the others 4% (video 15.05 and 15.7 ms, 32 single tokens 201 and 209 us).
+template <bool F16, bool LSE>
+__device__ __forceinline__ void weights32(const f32x16& s, float c, float m, typename Half<F16>::vec* pf, float& l,
+                                          float& e) {
 #pragma unroll
   for (int h = 0; h < 2; ++h) {
     uint32_t w[4];
 #pragma unroll
     for (int j = 0; j < 4; ++j) {
-      w[j] = pack2<F16>(exp2_fast(fmaf(s[h * 8 + 2 * j], c, -m)), exp2_fast(fmaf(s[h * 8 + 2 * j + 1], c, -m)));
+      if constexpr (LSE) {
+        const float x = exp2_fast(fmaf(s[h * 8 + 2 * j], c, -m)), y = exp2_fast(fmaf(s[h * 8 + 2 * j + 1], c, -m));
+        w[j] = pack2<F16>(x, y);
+        e += x + y;
+      } else {
+        w[j] = pack2<F16>(exp2_fast(fmaf(s[h * 8 + 2 * j], c, -m)), exp2_fast(fmaf(s[h * 8 + 2 * j + 1], c, -m)));
+      }
       l = Half<F16>::sum2(__builtin_bit_cast(typename Half<F16>::pair, w[j]), l);
     }
     pf[h] = __builtin_bit_cast(typename Half<F16>::vec, make_uint4(w[0], w[1], w[2], w[3]));
@@ -327,9 +341,9 @@ __device__ __forceinline__ void mask32(f32x16& s, int first, int hl, int klo, in
 }
 
 template <bool F16>
-__device__ __forceinline__ float lse_of(float m, float l) {
+__device__ __forceinline__ float lse_of(float m, float e) {
   constexpr float kBelow = Reference<F16>::kBelow, kUnit = F16 ? 0x1p-13f : 1.f;  // 2^-kBelow
-  return l == 0.f ? -INFINITY : ((m + kBelow) + log2f(l * kUnit)) * 0.69314718055994531f;
+  return e == 0.f ? -INFINITY : ((m + kBelow) + log2f(e * kUnit)) * 0.69314718055994531f;
 }
 
 // O^T / l of a lane's row: the halves of a lane pair are joined into 8
@@ -352,16 +366,21 @@ __device__ __forceinline__ void store_row(uint16_t* out, const f32x16* o, float 
     }
 }
 
-// A part's O and (m, l) of a lane's row as they are.
-template <int D>
-__device__ __forceinline__ void store_part(float* po, float* pml, const f32x16* o, float m, float l, int hl) {
+// A part's O, (m, l) and e of a lane's row as they are, to row `at` of the parts.
+template <int D, bool LSE>
+__device__ __forceinline__ void store_part(const WindowParams& p, int64_t at, const f32x16* o, float m, float l,
+                                           float e, int hl) {
+  float* const po = p.part_o + at * D;
 #pragma unroll
   for (int dc = 0; dc < D / 32; ++dc)
 #pragma unroll
     for (int g = 0; g < 4; ++g)
       *reinterpret_cast<float4*>(po + dc * 32 + g * 8 + hl * 4) =
           make_float4(o[dc][g * 4], o[dc][g * 4 + 1], o[dc][g * 4 + 2], o[dc][g * 4 + 3]);
-  if (hl == 0) *reinterpret_cast<float2*>(pml) = make_float2(m, l);
+  if (hl == 0) {
+    *reinterpret_cast<float2*>(p.part_ml + at * 2) = make_float2(m, l);
+    if (LSE) p.part_e[at] = e;
+  }
 }
 
 // Rows of a (sequence, key head): query i of query head g of the group is row
@@ -444,7 +463,7 @@ __device__ __forceinline__ bool item_of(const WindowParams& p, Item& it) {
 // half a turn apart over shared tiles (17.5 ms), three workgroups a CU with
 // tiles of 64 keys (27 ms, spills), a reference from a row's first tile without
 // later maxima (15.8 ms), raised wave priority in either phase (no change).
-template <int D, bool F16, bool ROLL>
+template <int D, bool F16, bool ROLL, bool LSE>
 __global__ void __launch_bounds__(256, 2) window_tile_kernel(WindowParams p) {
   constexpr int DCH = D / 32, T = 128;
   typedef KeyTile<D, T, 4> KT;
@@ -474,7 +493,7 @@ __global__ void __launch_bounds__(256, 2) window_tile_kernel(WindowParams p) {
   f32x16 o[DCH];
 #pragma unroll
   for (int i = 0; i < DCH; ++i) o[i] = f32x16{};
-  float m = -INFINITY, l = 0.f;
+  float m = -INFINITY, l = 0.f, e = 0.f;
   if (t0 < t1) {
     const uint16_t* const ks = p.k + b * p.k_sb + g * p.k_sh;
     const uint16_t* const vs = p.v + b * p.v_sb + g * p.v_sh;
@@ -512,9 +531,9 @@ __global__ void __launch_bounds__(256, 2) window_tile_kernel(WindowParams p) {
 #pragma unroll
           for (int kb = 0; kb < 4; ++kb) mask32(s[kb], first + kb * 32, hl, klo, khi, p.sinks);
         }
-        const float ref = follow_max<4, DCH, F16>(s, p.scale_log2, m, l, o);
+        const float ref = follow_max<4, DCH, F16, LSE>(s, p.scale_log2, m, l, e, o);
 #pragma unroll
-        for (int kb = 0; kb < 4; ++kb) weights32<F16>(s[kb], p.scale_log2, ref, pf + 2 * kb, l);
+        for (int kb = 0; kb < 4; ++kb) weights32<F16, LSE>(s[kb], p.scale_log2, ref, pf + 2 * kb, l, e);
       }
       wait_vmcnt<KT::LOADS>();  // V has landed
       block_barrier();
@@ -533,10 +552,11 @@ __global__ void __launch_bounds__(256, 2) window_tile_kernel(WindowParams p) {
     wait_vmcnt_0();  // the trailing copies have landed before the workgroup's LDS is released
   }
   l = xhalf_sum(l);
+  if (LSE) e = xhalf_sum(e);
   const bool dead = row.i >= seq.nq;
   if (it.pieces > 1) {
     const int64_t at = static_cast<int64_t>(it.slot) * 128 + w * 32 + l32;
-    if (in) store_part<D>(p.part_o + at * D, p.part_ml + at * 2, o, dead ? -INFINITY : m, dead ? 0.f : l, hl);
+    if (in) store_part<D, LSE>(p, at, o, dead ? -INFINITY : m, dead ? 0.f : l, e, hl);
     return;
   }
   const float inv = dead || l == 0.f ? 0.f : 1.f / l;
@@ -545,8 +565,10 @@ __global__ void __launch_bounds__(256, 2) window_tile_kernel(WindowParams p) {
     for (int i = 0; i < DCH; ++i) o[i] = f32x16{};
   }
   store_row<D, F16>(p.out + b * p.o_sb + head * p.o_sh + row.i * p.o_sl, o, inv, in, hl);
+  // (asked of p.lse although LSE says it: the compiler orders the copies before
+  // the loop otherwise, video 15.25 ms for 15.05)
   if (p.lse && in && hl == 0)
-    p.lse[(static_cast<int64_t>(b) * p.Hq + head) * p.Lq + row.i] = dead ? -INFINITY : lse_of<F16>(m, l);
+    p.lse[(static_cast<int64_t>(b) * p.Hq + head) * p.Lq + row.i] = dead ? -INFINITY : lse_of<F16>(m, e);
 }
 
 // At most 32 rows (a token, or a few, of a group's heads) over many keys: a
@@ -555,7 +577,7 @@ __global__ void __launch_bounds__(256, 2) window_tile_kernel(WindowParams p) {
 // The keys are dealt over p.parts waves; reading them is all that counts, past
 // the last-level cache with streaming loads (32 sequences x 8 heads x 8,256
 // keys: 210 us, 229 with ordinary ones).
-template <int D, bool F16, bool ROLL, bool STREAM>
+template <int D, bool F16, bool ROLL, bool STREAM, bool LSE>
 __global__ void __launch_bounds__(64, 2) window_few_kernel(WindowParams p) {
   constexpr int DCH = D / 32, T = 32;
   typedef KeyTile<D, T, 1> KT;
@@ -576,7 +598,7 @@ __global__ void __launch_bounds__(64, 2) window_few_kernel(WindowParams p) {
   f32x16 o[DCH];
 #pragma unroll
   for (int i = 0; i < DCH; ++i) o[i] = f32x16{};
-  float m = -INFINITY, l = 0.f;
+  float m = -INFINITY, l = 0.f, e = 0.f;
   if (t0 < t1) {
     const uint16_t* const ks = p.k + b * p.k_sb + g * p.k_sh;
     const uint16_t* const vs = p.v + b * p.v_sb + g * p.v_sh;
@@ -601,9 +623,9 @@ __global__ void __launch_bounds__(64, 2) window_few_kernel(WindowParams p) {
       f32x16 s;
       scores<D, F16, T>(kb, qf, l32, hl, &s);
       mask32(s, first, hl, klo, khi, p.sinks);
-      const float ref = follow_max<1, DCH, F16>(&s, p.scale_log2, m, l, o);
+      const float ref = follow_max<1, DCH, F16, LSE>(&s, p.scale_log2, m, l, e, o);
       vec pf[2];
-      weights32<F16>(s, p.scale_log2, ref, pf, l);
+      weights32<F16, LSE>(s, p.scale_log2, ref, pf, l, e);
       vec vf[2][DCH];
       values32<D, F16>(vb, lane, vf);
 #pragma unroll
@@ -621,10 +643,11 @@ __global__ void __launch_bounds__(64, 2) window_few_kernel(WindowParams p) {
     wait_vmcnt_0();
   }
   l = xhalf_sum(l);
+  if (LSE) e = xhalf_sum(e);
   const bool dead = row.i >= seq.nq;
   if (p.parts > 1) {
     const int64_t at = static_cast<int64_t>(blockIdx.x) * rows + l32;
-    if (in) store_part<D>(p.part_o + at * D, p.part_ml + at * 2, o, dead ? -INFINITY : m, dead ? 0.f : l, hl);
+    if (in) store_part<D, LSE>(p, at, o, dead ? -INFINITY : m, dead ? 0.f : l, e, hl);
     return;
   }
   const float inv = dead || l == 0.f ? 0.f : 1.f / l;
@@ -633,8 +656,8 @@ __global__ void __launch_bounds__(64, 2) window_few_kernel(WindowParams p) {
     for (int i = 0; i < DCH; ++i) o[i] = f32x16{};
   }
   store_row<D, F16>(p.out + b * p.o_sb + head * p.o_sh + row.i * p.o_sl, o, inv, in, hl);
-  if (p.lse && in && hl == 0)
-    p.lse[(static_cast<int64_t>(b) * p.Hq + head) * p.Lq + row.i] = dead ? -INFINITY : lse_of<F16>(m, l);
+  if (LSE && in && hl == 0)
+    p.lse[(static_cast<int64_t>(b) * p.Hq + head) * p.Lq + row.i] = dead ? -INFINITY : lse_of<F16>(m, e);
 }
 
 // Joins the parts of a row: O = sum 2^(m_i - M) O_i over the same sum of l_i.
@@ -646,7 +669,7 @@ template <int D, bool F16, bool FEW, int WAVES>
 __global__ void __launch_bounds__(256) window_join_kernel(WindowParams p) {
   constexpr int LANES = D / 4, GROUPS = 64 * WAVES / LANES;
   __shared__ float4 so[4][LANES];
-  __shared__ float sl[4], sm[4];
+  __shared__ float sl[4], se[4], sm[4];
   const int lane = threadIdx.x & 63, w = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), sub = lane % LANES;
   const int grp = (WAVES == 4 ? static_cast<int>(threadIdx.x) : lane) / LANES;
   const int64_t id = WAVES == 4 ? blockIdx.x : static_cast<int64_t>(blockIdx.x) * 4 + w;
@@ -677,7 +700,7 @@ __global__ void __launch_bounds__(256) window_join_kernel(WindowParams p) {
     M = fmaxf(fmaxf(sm[0], sm[1]), fmaxf(sm[2], sm[3]));
   }
   const float ref = M == -INFINITY ? 0.f : M;
-  float l = 0.f, o[4] = {};
+  float l = 0.f, e = 0.f, o[4] = {};
 #pragma unroll 8
   for (int i = grp; i < p.parts; i += GROUPS) {
     const float2 ml = *reinterpret_cast<const float2*>(p.part_ml + (first + i * step) * 2);
@@ -686,20 +709,23 @@ __global__ void __launch_bounds__(256) window_join_kernel(WindowParams p) {
     const float a = none ? 0.f : exp2_fast(ml.x - ref);
     if (none) v = make_float4(0.f, 0.f, 0.f, 0.f);
     l += a * ml.y;
+    if (p.lse && !none) e += a * p.part_e[first + i * step];
     o[0] += a * v.x; o[1] += a * v.y; o[2] += a * v.z; o[3] += a * v.w;
   }
 #pragma unroll
   for (int off = LANES; off < 64; off *= 2) {
     l += __shfl_xor(l, off, 64);
+    e += __shfl_xor(e, off, 64);
 #pragma unroll
     for (int i = 0; i < 4; ++i) o[i] += __shfl_xor(o[i], off, 64);
   }
   if (WAVES == 4) {
     if (lane < LANES) so[w][sub] = make_float4(o[0], o[1], o[2], o[3]);
-    if (lane == 0) sl[w] = l;
+    if (lane == 0) sl[w] = l, se[w] = e;
     __syncthreads();
     if (threadIdx.x >= LANES) return;
     l = (sl[0] + sl[1]) + (sl[2] + sl[3]);
+    e = (se[0] + se[1]) + (se[2] + se[3]);
     const float4 a = so[0][sub], b = so[1][sub], c = so[2][sub], d = so[3][sub];
     o[0] = (a.x + b.x) + (c.x + d.x);
     o[1] = (a.y + b.y) + (c.y + d.y);
@@ -714,7 +740,7 @@ __global__ void __launch_bounds__(256) window_join_kernel(WindowParams p) {
   const int head = g * p.group + row.g;
   *reinterpret_cast<uint2*>(p.out + b * p.o_sb + head * p.o_sh + row.i * p.o_sl + sub * 4) =
       make_uint2(pack2<F16>(o[0] * inv, o[1] * inv), pack2<F16>(o[2] * inv, o[3] * inv));
-  if (p.lse && sub == 0) p.lse[(static_cast<int64_t>(b) * p.Hq + head) * p.Lq + row.i] = lse_of<F16>(M, l);
+  if (p.lse && sub == 0) p.lse[(static_cast<int64_t>(b) * p.Hq + head) * p.Lq + row.i] = lse_of<F16>(M, e);
 }
 
 // How a call is cut. Slots for two workgroups on each of 256 CUs; the blocks
@@ -772,19 +798,19 @@ int64_t part_rows(const dfs_window_args* a, const WindowParams& p) {
   return p.few ? a->batch * a->kv_heads * p.parts * a->q_rows * p.group : int64_t(8) * p.split * p.parts * 128;
 }
 
-template <int D, bool F16, bool ROLL>
+template <int D, bool F16, bool ROLL, bool LSE>
 void launch(const WindowParams& p, hipStream_t st) {
   const unsigned heads = static_cast<unsigned>(p.B * p.Hkv);
   if (p.few) {
     if (p.stream)
-      window_few_kernel<D, F16, ROLL, true><<<heads * p.parts, 64, 0, st>>>(p);
+      window_few_kernel<D, F16, ROLL, true, LSE><<<heads * p.parts, 64, 0, st>>>(p);
     else
-      window_few_kernel<D, F16, ROLL, false><<<heads * p.parts, 64, 0, st>>>(p);
+      window_few_kernel<D, F16, ROLL, false, LSE><<<heads * p.parts, 64, 0, st>>>(p);
     const int64_t rows = static_cast<int64_t>(heads) * p.Lq * p.group;
     if (p.parts > 1) window_join_kernel<D, F16, true, 4><<<static_cast<unsigned>(rows), 256, 0, st>>>(p);
     return;
   }
-  window_tile_kernel<D, F16, ROLL><<<8u * (p.whole + p.split * p.parts), 256, 0, st>>>(p);
+  window_tile_kernel<D, F16, ROLL, LSE><<<8u * (p.whole + p.split * p.parts), 256, 0, st>>>(p);
   const unsigned cut = static_cast<unsigned>(p.split) * 8 * 128;  // rows of the blocks that were
   if (p.parts > 8)
     window_join_kernel<D, F16, false, 4><<<cut, 256, 0, st>>>(p);
@@ -803,7 +829,7 @@ extern "C" int64_t dfs_window_attention_workspace_size(const dfs_window_args* a)
   }
   WindowParams p{};
   plan(a, p);
-  return part_rows(a, p) * (a->head_dim + 2) * 4;
+  return part_rows(a, p) * (a->head_dim + 3) * 4;
 }
 
 extern "C" int dfs_window_attention(const dfs_window_args* a, dfs_stream_t stream) {
@@ -867,28 +893,29 @@ extern "C" int dfs_window_attention(const dfs_window_args* a, dfs_stream_t strea
   p.rolling = a->rolling != 0;
   p.scale_log2 = static_cast<float>(a->scale * 1.4426950408889634);
   plan(a, p);
-  const int64_t spare = part_rows(a, p), need = spare * (a->head_dim + 2) * 4;
+  const int64_t spare = part_rows(a, p), need = spare * (a->head_dim + 3) * 4;
   DFS_REQUIRE(need == 0 || (a->workspace != nullptr && a->workspace_bytes >= need &&
                             reinterpret_cast<uintptr_t>(a->workspace) % 16 == 0),
               "%s: a 16-byte aligned workspace of %lld bytes is needed", name, (long long)need);
   p.part_o = static_cast<float*>(a->workspace);
   p.part_ml = p.part_o + spare * a->head_dim;
+  p.part_e = p.part_ml + spare * 2;
   // A launch holds fewer than 2^32 threads.
   DFS_REQUIRE((p.whole + static_cast<int64_t>(p.split) * p.parts) * 8 < (1 << 24) &&
                   a->batch * a->kv_heads * p.parts < (1 << 26) && a->q_rows * p.group < kNoLimit,
               "%s: too many rows", name);
   hipStream_t st = reinterpret_cast<hipStream_t>(stream);
   const bool f16 = a->dtype == DFS_DTYPE_F16, roll = p.rolling;
-  if (a->head_dim == 128) {
-    if (f16)
-      roll ? launch<128, true, true>(p, st) : launch<128, true, false>(p, st);
+  auto run = [&](auto wide, auto half, auto ring) {
+    constexpr int D = decltype(wide)::value ? 128 : 64;
+    if (p.lse)
+      launch<D, decltype(half)::value, decltype(ring)::value, true>(p, st);
     else
-      roll ? launch<128, false, true>(p, st) : launch<128, false, false>(p, st);
-  } else {
-    if (f16)
-      roll ? launch<64, true, true>(p, st) : launch<64, true, false>(p, st);
-    else
-      roll ? launch<64, false, true>(p, st) : launch<64, false, false>(p, st);
-  }
+      launch<D, decltype(half)::value, decltype(ring)::value, false>(p, st);
+  };
+  auto with = [](bool b, auto&& f) { b ? f(std::true_type{}) : f(std::false_type{}); };
+  with(a->head_dim == 128, [&](auto wide) {
+    with(f16, [&](auto half) { with(roll, [&](auto ring) { run(wide, half, ring); }); });
+  });
   return check_launch(name);
 }

@@ -559,3 +559,53 @@ def test_window_attention_keeps_small_weights(dev, L, S, D, place, nats, spread,
     out, lse = ops.window_attention(q.to(dev), k.to(dev), v.to(dev), scale=1.0, want_lse=True)
     _within(out, ref, tol, "small weights")
     _within(lse, lse_ref, lse_tol, "their lse")
+
+
+# --------------------------------------------------------------------------
+# the log-sum-exp
+# --------------------------------------------------------------------------
+
+def _fp32_lse_tol(lse_ref, lse_tol, dtype):
+    """operator_refs' bound of the lse without the rounding of the weights to
+    the operands' type, for which rows that see keys have 2 u in it: what the
+    fp32 scores, their sum and its logarithm take."""
+    return lse_tol - 2 * refs.half_step(dtype) * (lse_ref != -math.inf)
+
+
+@pytest.mark.parametrize("dtype", [BF, HF])
+@pytest.mark.parametrize("L,D", [(1, 64), (1, 128), (8, 64), (40, 128), (300, 64)])
+def test_window_attention_lse_is_fp32(dev, L, D, dtype):
+    """Rows that see two keys in tiles apart, the first key and their own,
+    whose score is up to 5 nats higher or lower: the weight of neither is a
+    number of the operands' type."""
+    print(f"lse L={L} D={D} {dtype}", flush=True)
+    gen = torch.Generator().manual_seed(L + D)
+    S, B = 200 + L, 1 if L > 8 else 40
+    q = torch.zeros(B, 2, L, D, dtype=dtype)
+    k, v = torch.zeros(B, 2, S, D, dtype=dtype), _randn(gen, B, 2, S, D, dtype=dtype)
+    q[..., 0] = 1
+    k[:, :, 1:, 0] = (torch.rand(B, 2, S - 1, generator=gen) * 10 - 5).to(dtype)
+    ref, lse_ref, tol, lse_tol = refs.window_attention(q, k, v, left=0, right=0, sinks=1, scale=1.0)
+    out, lse = ops.window_attention(q.to(dev), k.to(dev), v.to(dev), left=0, right=0, sinks=1, scale=1.0, want_lse=True)
+    _within(out, ref, tol, "out")
+    _within(lse, lse_ref, _fp32_lse_tol(lse_ref, lse_tol, dtype), "lse")
+
+
+@pytest.mark.parametrize("B,H,G,L,S,D,dtype,left,right,sinks,q_lens,kv_lens,rolling", ATTENTION)
+def test_window_attention_lse_is_fp32_everywhere(dev, B, H, G, L, S, D, dtype, left, right, sinks, q_lens, kv_lens,
+                                                 rolling):
+    """The same bound over the forms and parts; out does not depend on whether
+    the lse is asked for."""
+    print(f"lse B={B} H={H} G={G} L={L} S={S} D={D} {dtype} left={left} right={right} sinks={sinks} "
+          f"q={q_lens} kv={kv_lens} rolling={rolling}", flush=True)
+    g = torch.Generator().manual_seed(L * S + H + 1)
+    q, k, v = (_randn(g, B, n, s, D, dtype=dtype) for n, s in ((H, L), (G, S), (G, S)))
+    _, lse_ref, _, lse_tol = refs.window_attention(q, k, v, left, right, sinks, q_lens, kv_lens, rolling)
+    lens = [None if t is None else torch.tensor(t, dtype=torch.int32, device=dev) for t in (q_lens, kv_lens)]
+    args = (q.to(dev), k.to(dev), v.to(dev), left, right, sinks, *lens)
+    out, lse = ops.window_attention(*args, rolling=rolling, want_lse=True)
+    assert torch.equal(out, ops.window_attention(*args, rolling=rolling))
+    empty = lse_ref == -math.inf
+    lse = lse.cpu().double()
+    assert torch.equal(lse == -math.inf, empty)
+    _within(lse.masked_fill(empty, 0), lse_ref.masked_fill(empty, 0), _fp32_lse_tol(lse_ref, lse_tol, dtype), "lse")
