@@ -184,7 +184,8 @@ def full_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, mode: str 
     ``operand_dtype`` picks the native kernel's operand precision (f16 by
     default, with every finite bf16 input kept; bf16 for the reference
     kernel's precision class), as ``DFS_Attention.operand_dtype`` does for
-    the sparse path."""
+    the sparse path. Mode "window" multiplies in q's dtype, bf16 weights of 8
+    bits among them, and refuses another one."""
     if mode == "flash":
         if causal:
             raise NotImplementedError("causal attention is not used by the DFS processors")
@@ -194,6 +195,8 @@ def full_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, mode: str 
     if mode == "window":
         if drop_rate or attn_mask is not None or causal:
             raise NotImplementedError("window attention takes its mask from window and sinks alone, without dropout")
+        if operand_dtype not in (None, q.dtype):
+            raise ValueError(f"window attention multiplies in q's dtype {q.dtype}, got operand_dtype {operand_dtype}")
         for cu, total in ((cu_seqlens_q, q.shape[2]), (cu_seqlens_kv, k.shape[2])):
             if cu is not None and (cu.device.type != "cpu" or [int(x) for x in cu.tolist()][:2] != [0, total]):
                 raise NotImplementedError("window attention runs one whole sequence a row; pass host cu_seqlens of it "

@@ -240,3 +240,17 @@ def test_channels_that_share_an_element_are_copied():
     for shape, stride in (((2, 2, 9, 64), (1152, 576, 64, 1)), ((2, 2, 9, 64), (0, 0, 64, 1)),
                           ((1, 1, 1, 64), (5, 3, 7, 1)), ((4, 1), (8, 5))):
         assert ops._chunk_rows(shape, stride)
+
+
+def test_window_mode_refuses_other_operands_than_its_inputs():
+    """mode "window" multiplies in q's dtype: another operand_dtype is refused,
+    not passed over."""
+    from dfsattn_amd.fullattention import full_attention
+
+    for dtype, other in ((BF, torch.float16), (torch.float16, BF)):
+        q = _t(1, 2, 8, 64, dtype=dtype)
+        with pytest.raises(ValueError, match="operand_dtype"):
+            full_attention(q, q, q, mode="window", window=(4, 0), operand_dtype=other)
+        for same in (dtype, None):  # as far as the device
+            with pytest.raises(RuntimeError, match="ROCm GPU"):
+                full_attention(q, q, q, mode="window", window=(4, 0), operand_dtype=same)
