@@ -2,8 +2,9 @@
 
 A layer keeps the keys and values of the tokens so far in a ``StreamCache``
 with a sliding window and sinks: the first tokens (usually the first frame)
-and the newest ones stay, the others' slots are taken again, so a stream of any
-length holds a fixed amount of memory. ``Wan_Stream_Processor`` drives an
+and the newest ones stay, the others' slots are taken again, so a stream holds
+a fixed amount of memory however long it is. It ends where its rotary table
+does, and with its int32 lengths, 2^31 - 256 tokens. ``Wan_Stream_Processor`` drives an
 attention module (the members ``Wan_DFSAttn_Processor2_0`` uses) over such a
 cache: ``linear`` for the projections, ``qkv_cache`` for norms, rotation and
 append, ``window_attention`` over the cache.
@@ -28,6 +29,8 @@ class StreamCache:
     channels, the first ``sinks`` tokens and at least ``left`` tokens before
     a chunk of up to ``chunk`` tokens."""
 
+    MOST = 0x7fffff00  # keys that window_attention counts
+
     def __init__(self, batch: int, heads: int, head_dim: int, left: int, chunk: int, sinks: int = 0, device="cuda",
                  dtype: torch.dtype = torch.bfloat16):
         for name, n in (("batch", batch), ("heads", heads), ("left", left + 1), ("chunk", chunk), ("sinks", sinks + 1)):
@@ -37,7 +40,22 @@ class StreamCache:
         shape = (batch, heads, sinks + left + chunk, head_dim)
         self.k = torch.zeros(shape, dtype=dtype, device=device)
         self.v = torch.zeros(shape, dtype=dtype, device=device)
-        self.lens = torch.zeros(batch, dtype=torch.int32, device=device)  # tokens behind which the chunk stands
+        with torch.inference_mode(False):  # an inference tensor would not count its changes
+            self.lens = torch.zeros(batch, dtype=torch.int32, device=device)  # tokens behind which the chunk stands
+        self._keep(0)
+
+    def _keep(self, position: Optional[int]) -> None:
+        """What lens holds, by the host's count (None: not known, as under a
+        capture, whose replays move lens unseen)."""
+        if self.lens.is_cuda and torch.cuda.is_current_stream_capturing():
+            position = None
+        self._known = (self.lens, self.lens._version, position)
+
+    def _position(self) -> Optional[int]:
+        """The host's count, None where lens was moved otherwise than by
+        ``advance`` and ``reset``."""
+        lens, version, position = self._known
+        return position if self.lens is lens and lens._version == version else None
 
     def attend(self, q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, q_weight: Optional[torch.Tensor] = None,
                k_weight: Optional[torch.Tensor] = None, eps: float = 1e-6,
@@ -47,10 +65,18 @@ class StreamCache:
         attends over them all: q [B, T, H, D], k and v [B, T, G, D] as the
         projections leave them (see ``ops.qkv_cache``), out [B, H, T, D] in
         token-major storage. right: how far a token sees ahead within the
-        chunk (None: all of it, 0: causal)."""
+        chunk (None: all of it, 0: causal). A chunk past the table's last row
+        is refused; where the host does not know the place (lens moved by hand
+        or by a replayed graph), the rows past it are NaN."""
         tokens = q.shape[1]
         if tokens > self.chunk:
             raise ValueError(f"StreamCache: a chunk of {tokens} tokens, made for {self.chunk}")
+        at = self._position()
+        if at is not None and table is not None and at + tokens > table[0].shape[0]:
+            raise ValueError(f"StreamCache: tokens {at} to {at + tokens - 1} of a stream whose rotary table has "
+                             f"{table[0].shape[0]} rows")
+        if at is not None and at + tokens > self.MOST:
+            raise ValueError(f"StreamCache: a stream holds up to 2^31 - 256 tokens, this chunk ends at {at + tokens}")
         q = ops.qkv_cache(q, k, v, self.k, self.v, self.lens, q_weight, k_weight, eps, table, sinks=self.sinks,
                           rolling=True)
         return ops.window_attention(q, self.k, self.v, self.left, right, self.sinks, kv_lens=self.lens + tokens,
@@ -60,10 +86,13 @@ class StreamCache:
         """The chunk's ``tokens`` are final; the next one follows them."""
         if not 0 <= tokens <= self.chunk:
             raise ValueError(f"StreamCache: advance by {tokens} of a chunk of up to {self.chunk} tokens")
+        at = self._position()
         self.lens += tokens
+        self._keep(None if at is None else at + tokens)
 
     def reset(self) -> None:
         self.lens.zero_()
+        self._keep(0)
 
 
 class Wan_Stream_Processor:

@@ -157,3 +157,35 @@ def test_block_with_its_own_ffn(dev):
     a = ops.linear(h, l1.weight, l1.bias, activation="gelu_tanh").cpu()
     ref, tol = refs.linear(a[0], l2.weight.cpu(), l2.bias.cpu(), None, gate[0, 0].cpu(), x[0].cpu())
     assert bool(((got[0].cpu().double() - ref).abs() <= tol).all())
+
+
+@torch.inference_mode()
+def test_stream_past_its_table_is_refused_and_graphs_move_on(dev):
+    """A chunk past the rotary table raises before anything is written; a
+    captured advance, whose replays the host does not see, leaves the place
+    unknown."""
+    dim, heads = 256, 2
+    m = _attention_module(dev, dim, heads, 5)
+    x = torch.randn(1, 8, dim, device=dev).to(BF)
+    freqs = wan_rope_freqs((1, 4, 5), dim // heads).to(dev)
+    cache = StreamCache(1, heads, dim // heads, 8, 8, 0, dev, BF)
+    m.set_processor(Wan_Stream_Processor(cache))
+    for _ in range(2):
+        m(x, None, None, freqs)
+        cache.advance(8)
+    kept = cache.k.clone()
+    with pytest.raises(ValueError, match="table"):
+        m(x, None, None, freqs)  # positions 16 to 23 of 20
+    assert torch.equal(kept, cache.k) and bool(torch.isfinite(m(x[:, :4], None, None, freqs)).all())
+    cache.reset()
+    torch.cuda.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        cache.advance(4)
+    assert cache._position() is None
+    for i in range(1, 4):
+        graph.replay()
+        torch.cuda.synchronize()
+        assert int(cache.lens) == 4 * i
+    cache.reset()
+    assert cache._position() == 0 and int(cache.lens) == 0
