@@ -244,17 +244,32 @@ class WanLikeDiT(nn.Module):
         x = x.permute(0, 2, 4, 6, 1, 3, 5, 7)  # tokens (f, h, w) row-major, channels (c, pf, ph, pw)
         return x.reshape(b, (f // pf) * (h // ph) * (w // pw), c * pf * ph * pw)
 
-    def unpatchify(self, tokens: torch.Tensor) -> torch.Tensor:
-        b = tokens.shape[0]
+    def _frames(self, tokens: int) -> int:
+        """Frames of a latent of so many tokens: the grid's (or those of a rotary
+        table put in its place), or, where every self-attention runs over a
+        stream's cache, a chunk's."""
         _, h, w = self.cfg.grid
-        f = tokens.shape[1] // (h * w)  # the grid's frames, or those of a stream's chunk
+        chunks = all(getattr(b.attn1.processor, "takes_chunks", False) for b in self.blocks)
+        if tokens == 0 or tokens % (h * w) or (not chunks and tokens not in (self.cfg.seq_len, self.rotary_emb.shape[2])):
+            raise ValueError(f"a latent of {tokens} tokens: "
+                             + (f"a stream takes whole frames of {h * w}" if chunks
+                                else f"the model's grid has {self.cfg.seq_len}"))
+        return tokens // (h * w)
+
+    def unpatchify(self, tokens: torch.Tensor, frames: Optional[int] = None) -> torch.Tensor:
+        """[B, tokens, C pf ph pw] to the latent; frames: the grid's by default."""
+        b = tokens.shape[0]
+        f, h, w = self.cfg.grid
+        f = f if frames is None else frames
         pf, ph, pw = self.cfg.patch
         c = self.cfg.in_channels
         x = tokens.reshape(b, f, h, w, c, pf, ph, pw).permute(0, 4, 1, 5, 2, 6, 3, 7)
         return x.reshape(b, c, f * pf, h * ph, w * pw)
 
     def forward(self, latent: torch.Tensor, timestep: torch.Tensor, context: torch.Tensor) -> torch.Tensor:
-        x = self.patch_embedding(self.patchify(latent).to(self.patch_embedding.weight.dtype))
+        x = self.patchify(latent)
+        frames = self._frames(x.shape[1])
+        x = self.patch_embedding(x.to(self.patch_embedding.weight.dtype))
         temb = self.time_embedder(timestep_embedding(timestep, self.cfg.freq_dim))
         tproj = self.time_proj(temb.to(self.time_proj[1].weight.dtype)).unflatten(1, (6, -1))
         ctx = self.text_embedder(context.to(self.text_embedder[0].weight.dtype))
@@ -262,7 +277,7 @@ class WanLikeDiT(nn.Module):
             x = block(x, ctx, tproj, self.rotary_emb)
         shift, scale = (self.scale_shift_table + temb.unsqueeze(1)).chunk(2, dim=1)
         x = (self.norm_out(x.float()) * (1 + scale) + shift).type_as(x)
-        return self.unpatchify(self.proj_out(x))
+        return self.unpatchify(self.proj_out(x), frames)
 
 
 @torch.no_grad()

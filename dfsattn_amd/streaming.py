@@ -100,6 +100,8 @@ class Wan_Stream_Processor:
     states are a chunk's tokens [B, T, C], rotary_emb the complex table of all
     positions (as the model's blocks pass it)."""
 
+    takes_chunks = True  # the tokens need not be the whole table's
+
     def __init__(self, cache: StreamCache, right: Optional[int] = None):
         self.cache = cache
         self.right = right

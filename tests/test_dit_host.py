@@ -55,3 +55,48 @@ def test_tiny_forward_on_cpu_runs_the_torch_path():
     out = dit.denoise_step(model, latent, torch.tensor([500.0]), ctx, neg)
     assert out.shape == latent.shape and bool(torch.isfinite(out).all())
     assert [p.step_idx for p in procs] == [2] * len(procs)  # both CFG passes counted
+
+
+def test_a_latent_of_other_frames_is_refused_outside_a_stream():
+    """unpatchify takes the grid's tokens unless told otherwise; forward takes
+    the rotary table's tokens, or, where every self-attention runs over a
+    stream's cache, whole frames of the grid."""
+    cfg = dit.DIT_CONFIGS["tiny"]
+    model = dit.build_model(cfg, "cpu", torch.float32)
+    latent, ctx, _ = dit.synth_inputs(cfg, "cpu")
+    t = torch.tensor([500.0])
+    frame = cfg.grid[1] * cfg.grid[2]
+    tokens = model.patchify(latent)
+    for n in (frame, 2 * frame, frame + 1):
+        with pytest.raises(RuntimeError):
+            model.unpatchify(tokens[:, :n])
+    assert torch.equal(model.unpatchify(tokens[:, :frame], frames=1), latent[:, :, :1])
+    ran = []
+
+    class Attention:
+        """Self-attention that leaves its input as it is."""
+
+        def __init__(self, takes_chunks):
+            self.takes_chunks = takes_chunks
+
+        def __call__(self, attn, hidden, *args):
+            ran.append(hidden.shape[1])
+            return hidden
+
+    for takes_chunks in (False, True):
+        for _, m in model.attention_modules():
+            m.set_processor(Attention(takes_chunks))
+        with torch.no_grad():
+            assert model(latent, t, ctx).shape == latent.shape
+            ran.clear()
+            if takes_chunks:
+                assert model(latent[:, :, :2], t, ctx).shape == latent[:, :, :2].shape
+            else:
+                with pytest.raises(ValueError, match="tokens"):
+                    model(latent[:, :, :2], t, ctx)
+                assert not ran
+            with pytest.raises(ValueError, match="tokens"):  # half a frame
+                model(latent[:, :, :2, :8], t, ctx)
+    model.blocks[0].attn1.set_processor(Attention(False))  # one of the two
+    with torch.no_grad(), pytest.raises(ValueError, match="tokens"):
+        model(latent[:, :, :2], t, ctx)
