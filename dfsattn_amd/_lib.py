@@ -52,8 +52,10 @@ SIGNATURES = {
     "dfs_adaln_modulate": [_p, _i64, _i64, _i32, _p, _p, _p, _p, _f32, _p, _p],
     "dfs_gated_residual": [_p, _p, _p, _i64, _i64, _i32, _p, _p],
     "dfs_linear_workspace_size": [_i64, _i64, _i64, _i32],
+    "dfs_linear_form": [_i64, _i64, _i64, _i32],
     "dfs_linear": [_p, _p],
     "dfs_window_attention_workspace_size": [_p],
+    "dfs_window_attention_form": [_p],
     "dfs_window_attention": [_p, _p],
     "dfs_qkv_cache": [_p, _p],
 }
@@ -108,7 +110,7 @@ _RESTYPES = {"dfs_last_error": ctypes.c_char_p, "dfs_block_score_topk_workspace_
              "dfs_block_score_topk_split_size": ctypes.c_int64, "dfs_bsa_fwd_workspace_size": ctypes.c_int64,
              "dfs_call_workspace_size": ctypes.c_int64, "dfs_linear_workspace_size": ctypes.c_int64,
              "dfs_window_attention_workspace_size": ctypes.c_int64}
-ABI_VERSION = 6
+ABI_VERSION = 7
 
 _lock = threading.Lock()
 _lib = None

@@ -891,15 +891,20 @@ void launch_tile(const LinearParams& p, bool f16, hipStream_t st) {
   }
 }
 
+// Whether the few-row form reads w past the last-level cache, and whether it
+// takes more waves a workgroup, where there are few of them.
+bool few_stream(int64_t n, int64_t k) { return n * k * 2 > kLastLevelCache; }
+bool few_wide(int64_t n, int64_t k) { return !few_stream(n, k) && (n + 15) / 16 < 256; }
+
 template <bool F16>
 void launch_few(const LinearParams& p, hipStream_t st) {
   const int groups = (p.N + 15) / 16;
-  if (static_cast<int64_t>(p.N) * p.K * 2 > kLastLevelCache)
+  if (few_stream(p.N, p.K))
     linear_few_kernel<4, F16, true><<<groups, 256, 0, st>>>(p);
-  else if (groups >= 256)
-    linear_few_kernel<4, F16, false><<<groups, 256, 0, st>>>(p);
-  else  // more waves a workgroup where there are few
+  else if (few_wide(p.N, p.K))
     linear_few_kernel<8, F16, false><<<groups, 512, 0, st>>>(p);
+  else
+    linear_few_kernel<4, F16, false><<<groups, 256, 0, st>>>(p);
 }
 
 // The rows of x, then those of w, K elements each at any stride, into rows of
@@ -915,7 +920,15 @@ __global__ void __launch_bounds__(256) pad_rows_kernel(LinearParams p, int wide,
 }
 
 // How a product is cut: its form and, for the tiles, the parts of the channels.
-enum Form { kFew, kTileAny, kTile64, kTile64x128, kTile128Deep, kTile128, kTile256 };
+enum Form {
+  kFew = DFS_LINEAR_FEW,
+  kTileAny = DFS_LINEAR_ANY,
+  kTile64 = DFS_LINEAR_64,
+  kTile64x128 = DFS_LINEAR_64X128,
+  kTile128Deep = DFS_LINEAR_128_DEEP,
+  kTile128 = DFS_LINEAR_128,
+  kTile256 = DFS_LINEAR_256
+};
 struct Cut {
   Form form;
   int splits, depth;
@@ -1004,6 +1017,21 @@ extern "C" int64_t dfs_linear_workspace_size(int64_t rows, int64_t n, int64_t k,
     return -1;
   }
   return workspace_bytes_of(cut_of(rows, n, k, aligned != 0), rows, n, k);
+}
+
+extern "C" int dfs_linear_form(int64_t rows, int64_t n, int64_t k, int aligned) {
+  using namespace dfs;
+  if (rows <= 0 || n <= 0 || k <= 0) {
+    set_error("linear: rows=%lld n=%lld k=%lld must be positive", (long long)rows, (long long)n, (long long)k);
+    return -1;
+  }
+  const Cut c = cut_of(rows, n, k, aligned != 0);
+  int form = c.form;
+  if (c.splits > 1) form |= DFS_FORM_PARTS;
+  if (c.pad) form |= DFS_LINEAR_LAID_OUT;
+  if (c.form == kFew && few_stream(n, padded(k))) form |= DFS_FORM_STREAM;
+  if (c.form == kFew && few_wide(n, padded(k))) form |= DFS_LINEAR_WIDE;
+  return form;
 }
 
 extern "C" int dfs_linear(const dfs_linear_args* a, dfs_stream_t stream) {

@@ -832,6 +832,18 @@ extern "C" int64_t dfs_window_attention_workspace_size(const dfs_window_args* a)
   return part_rows(a, p) * (a->head_dim + 3) * 4;
 }
 
+extern "C" int dfs_window_attention_form(const dfs_window_args* a) {
+  using namespace dfs;
+  if (!a || a->batch <= 0 || a->kv_heads <= 0 || a->q_heads < a->kv_heads || a->q_rows <= 0 || a->slots <= 0) {
+    set_error("window_attention: batch, heads, q_rows and slots must be positive");
+    return -1;
+  }
+  WindowParams p{};
+  plan(a, p);
+  return (p.few ? DFS_WINDOW_FEW : DFS_WINDOW_BLOCKS) | (p.parts > 1 ? DFS_FORM_PARTS : 0) |
+         (p.stream ? DFS_FORM_STREAM : 0) | (p.short_last ? DFS_WINDOW_SHORT_LAST : 0);
+}
+
 extern "C" int dfs_window_attention(const dfs_window_args* a, dfs_stream_t stream) {
   using namespace dfs;
   const char* name = "window_attention";

@@ -986,10 +986,12 @@ def window_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, left: Op
     rounded to the operands' type for the product with v (f16: those below
     2^-27 of a row's largest lose bits, those below 2^-38 are 0). Returns out
     in q's dtype (and storage order) and with ``want_lse`` the fp32
-    log-sum-exp [B, H, L]. Rows
-    that see no key (rows from q_lens[b] on among them) are 0, their lse -inf.
-    Keys behind kv_lens may hold anything; values a query does not see inside
-    the sequence must be finite. No backward pass."""
+    log-sum-exp [B, H, L]. Rows that see no key (rows from q_lens[b] on among
+    them), or none with a score above minus infinity, are 0, their lse -inf; a
+    score of plus infinity makes its row NaN. Keys behind kv_lens may hold
+    anything, keys that a query does not see too, but the values inside the
+    sequence must be finite where not every query sees them. No backward
+    pass."""
     entry = "window_attention"
     _refuse_grad(entry, q, k, v, out)
     if out is not None and (out.shape != q.shape or out.dtype != q.dtype or out.data_ptr() % 16

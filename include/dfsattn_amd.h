@@ -42,7 +42,8 @@ const char* dfs_last_error(void);
 /* ABI version; bumped whenever a signature below changes (2: scoring workspace; 3: device cu_seqlens
  * and per-head operand exponents in the attention call, per-head overflow flags and dfs_prepare_fixup;
  * 4: separate query and key tile sizes in preparation and scoring; 5: Q read from the input by
- * the attention kernel, q_perm optional; 6: dfs_linear, dfs_window_attention and dfs_qkv_cache). */
+ * the attention kernel, q_perm optional; 6: dfs_linear, dfs_window_attention and dfs_qkv_cache;
+ * 7: dfs_linear_form and dfs_window_attention_form). */
 int dfs_abi_version(void);
 
 /*
@@ -493,6 +494,21 @@ int dfs_gated_residual(const void* x, const void* y, const float* gate,
  */
 enum { DFS_ACT_NONE = 0, DFS_ACT_GELU_TANH = 1, DFS_ACT_GELU = 2, DFS_ACT_SILU = 3 };
 int64_t dfs_linear_workspace_size(int64_t rows, int64_t n, int64_t k, int aligned);
+/*
+ * Host functions for tests and profiles: the kernel that a call takes, which
+ * goes by its sizes alone. dfs_linear: at most 8 rows; rows on any boundary as
+ * they are; tiles of 64 x 64, 64 outputs by 128 rows, 128 x 128 with three or
+ * two buffers, 256 x 256. dfs_window_attention: a wave with all rows of a key
+ * head, or blocks of 128 rows. Plus flags: the product or the keys are cut into
+ * parts that are joined; w or the keys are read past the last-level cache;
+ * operands are laid out on 16-byte rows first; eight waves instead of four; a
+ * head's last block of few rows comes behind all others. -1: sizes not positive.
+ */
+enum { DFS_LINEAR_FEW = 0, DFS_LINEAR_ANY = 1, DFS_LINEAR_64 = 2, DFS_LINEAR_64X128 = 3, DFS_LINEAR_128_DEEP = 4,
+       DFS_LINEAR_128 = 5, DFS_LINEAR_256 = 6, DFS_WINDOW_FEW = 0, DFS_WINDOW_BLOCKS = 1,
+       DFS_FORM_PARTS = 16, DFS_FORM_STREAM = 32, DFS_LINEAR_LAID_OUT = 64, DFS_LINEAR_WIDE = 128,
+       DFS_WINDOW_SHORT_LAST = 256 };
+int dfs_linear_form(int64_t rows, int64_t n, int64_t k, int aligned);
 typedef struct dfs_linear_args {
   int64_t rows, n, k, dtype, bias_dtype, activation;
   int64_t x_stride, w_stride, residual_stride, out_stride;
@@ -510,14 +526,17 @@ int dfs_linear(const dfs_linear_args* args, dfs_stream_t stream);
  * out like q, with any strides that are multiples of 8 elements; D 64 or 128,
  * bf16 or f16. Scores and statistics are fp32; the weights are rounded to the
  * operands' type for the product with v (in f16 those below 2^-27 of a row's
- * largest lose bits, those below 2^-38 are 0). A sequence of nq = q_lens[b] queries (q_rows without q_lens) and
- * nk = kv_lens[b] keys (slots without kv_lens; device int32, clamped to the
- * tensors): query i stands at position p = nk - nq + i and sees key j where
- * j < nk, j <= p + right and (j >= p - left or j < sinks); left and right -1:
- * no limit. Keys and values behind nk may hold anything; keys that a row does
- * not see too, but values inside the sequence must be finite (their weight of
- * 0 is multiplied). Rows that see no key, rows from nq on among them, are 0 and
- * their lse (fp32 [B][q_heads][q_rows], optional) is -inf.
+ * largest lose bits, those below 2^-38 are 0). A sequence of nq = q_lens[b]
+ * queries (q_rows without q_lens) and nk = kv_lens[b] keys (slots without
+ * kv_lens; device int32, clamped to the tensors): query i stands at position
+ * p = nk - nq + i and sees key j where j < nk, j <= p + right and
+ * (j >= p - left or j < sinks); left and right -1: no limit. Keys and values
+ * behind nk may hold anything; keys that a row does not see too, but values
+ * inside the sequence must be finite where not every row sees them (their weight
+ * of 0 is multiplied). Rows that see no key, rows from nq on among them, or none
+ * with a score above minus infinity, are 0 and their lse (fp32
+ * [B][q_heads][q_rows], optional, from the weights as they are) is -inf; a score
+ * of plus infinity makes its row NaN.
  * rolling: key j lies in slot j < sinks ? j : sinks + (j - sinks) mod
  * (slots - sinks); kv_lens counts all keys ever written and slots - sinks must
  * be at least left + q_rows. The workspace is the caller's,
@@ -539,6 +558,7 @@ typedef struct dfs_window_args {
   void* workspace;
 } dfs_window_args;
 int64_t dfs_window_attention_workspace_size(const dfs_window_args* args);
+int dfs_window_attention_form(const dfs_window_args* args);
 int dfs_window_attention(const dfs_window_args* args, dfs_stream_t stream);
 
 /*
