@@ -787,8 +787,33 @@ def _in_chunks(t: torch.Tensor) -> torch.Tensor:
 
 
 def _own_rows(shape: Shape, stride: Shape) -> bool:
-    """Rows to write to: whole, in 16-byte steps, none of them shared."""
-    return _chunk_rows(shape, stride) and not any(n > 1 and s == 0 for n, s in zip(shape, stride))
+    """Rows to write to: whole, in 16-byte steps, and no element twice (every
+    axis steps past all that the axes of smaller steps reach)."""
+    reach = 1
+    for s, n in sorted((s, n) for n, s in zip(shape, stride) if n > 1):
+        if s < reach:
+            return False
+        reach += (n - 1) * s
+    return _chunk_rows(shape, stride)
+
+
+@functools.lru_cache(maxsize=1024)
+def _share(shape: Shape, a: Shape, b: Shape, shift: int) -> bool:
+    """Whether two tensors of this shape and strides a and b, each with rows
+    of its own, share an element, the second beginning `shift` elements behind
+    the first. With other strides than the first's: whether their ranges do."""
+    a, b = _axis_strides(shape, a), _axis_strides(shape, b)
+    if a != b:
+        return shift < _reach(shape, a) and -shift < _reach(shape, b)
+    axes = sorted((s, n) for n, s in zip(shape, a) if n > 1)
+
+    def reached(d: int, i: int) -> bool:  # d as a sum of steps c s, |c| < n, of the axes before i
+        if i == 0:
+            return d == 0
+        s, n = axes[i - 1]
+        return any(abs(c) < n and reached(d - c * s, i - 1) for c in (d // s, d // s + 1))
+
+    return reached(shift, len(axes))
 
 
 def _row_stride(shape: Shape, stride: Shape) -> Optional[int]:
@@ -1133,8 +1158,8 @@ def qkv_cache(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, k_cache: torch.
     for x, n in zip(at, reach):
         if x < ek and pk < x + n or x < ev and pv < x + n:
             raise ValueError(f"{entry}: a cache overlaps an input")
-    if pk == pv and reach[3]:  # their rows may alternate in one tensor
-        raise ValueError(f"{entry}: k_cache and v_cache are the same memory")
+    if pk < ev and pv < ek and _share(k_cache.shape, k_cache.stride(), v_cache.stride(), (pv - pk) // 2):
+        raise ValueError(f"{entry}: k_cache and v_cache hold the same memory")  # their rows may alternate in one tensor
     _check_lens(entry, "lens", lens, batch)
     if new_lens is not None:
         _check_lens(entry, "new_lens", new_lens, batch)

@@ -254,3 +254,54 @@ def test_window_mode_refuses_other_operands_than_its_inputs():
         for same in (dtype, None):  # as far as the device
             with pytest.raises(RuntimeError, match="ROCm GPU"):
                 full_attention(q, q, q, mode="window", window=(4, 0), operand_dtype=same)
+
+
+# --------------------------------------------------------------------------
+# rows that are written share no memory
+# --------------------------------------------------------------------------
+
+def test_rows_to_write_that_overlap_each_other_are_refused():
+    buf = torch.zeros(200000, dtype=BF)
+    shape = (2, 2, 9, 64)
+    good = [(1152, 576, 64, 1), (1152, 64, 128, 1), (64, 128, 256, 1), (9216, 4608, 512, 1), (1168, 584, 64, 1)]
+    bad = [(1152, 576, 32, 1), (1152, 64, 64, 1), (1152, 512, 64, 1), (576, 576, 64, 1), (8, 576, 64, 1)]
+    for stride in good + bad:
+        view = buf.as_strided(shape, stride)
+        cells = torch.arange(200000).as_strided(shape, stride).flatten()
+        assert (cells.unique().numel() == cells.numel()) == (stride in good)
+        cache = {**CACHE, "k_cache": view}
+        with pytest.raises(RuntimeError if stride in good else ValueError,
+                           match="ROCm GPU" if stride in good else "rows of their own"):
+            ops.qkv_cache(**cache)
+        q = _t(*shape)
+        with pytest.raises(RuntimeError if stride in good else ValueError,
+                           match="ROCm GPU" if stride in good else "rows of its own"):
+            ops.window_attention(q, q, q, out=view)
+
+
+def test_caches_that_overlap_each_other_are_refused():
+    """Their rows may alternate in one tensor, but no element may be both's."""
+    shape = (2, 2, 9, 64)
+    buf = torch.zeros(100000, dtype=BF)
+    cells = torch.arange(100000)
+    rng = torch.Generator().manual_seed(0)
+    orders = [(2304, 1152, 128, 1), (2304, 128, 256, 1), (1152, 576, 64, 1), (4608, 64, 256, 1)]
+    shifts = [0, 8, 64, 128, 512, 576, 1152, 1216, 2304, 2368, 4608, 20000]
+    shifts += (torch.randint(0, 1200, (40,), generator=rng) * 8).tolist()
+    kinds = {True: 0, False: 0}
+    for stride in orders:
+        for shift in shifts:
+            for first, second in ((0, shift), (shift, 0)):
+                k, v = (buf.as_strided(shape, stride, at) for at in (first, second))
+                at = [cells.as_strided(shape, stride, o).flatten() for o in (first, second)]
+                shared = torch.cat(at).unique().numel() < 2 * at[0].numel()
+                kinds[shared] += 1
+                with pytest.raises(ValueError if shared else RuntimeError, match="same memory" if shared else "ROCm GPU"):
+                    ops.qkv_cache(**{**CACHE, "k_cache": k, "v_cache": v})
+    assert min(kinds.values()) > 50
+    # other strides than k's: apart, or refused
+    k = buf.as_strided(shape, orders[0])
+    with pytest.raises(ValueError, match="same memory"):
+        ops.qkv_cache(**{**CACHE, "k_cache": k, "v_cache": buf.as_strided(shape, orders[1], 64)})
+    with pytest.raises(RuntimeError, match="ROCm GPU"):
+        ops.qkv_cache(**{**CACHE, "k_cache": k, "v_cache": buf.as_strided(shape, orders[1], 50000)})
