@@ -860,7 +860,8 @@ extern "C" int dfs_window_attention(const dfs_window_args* a, dfs_stream_t strea
               "%s: sizes too large", name);
   DFS_REQUIRE(a->left >= -1 && a->right >= -1 && a->sinks >= 0, "%s: left and right must be -1 or more, sinks 0 or more",
               name);
-  DFS_REQUIRE(a->scale > 0. && a->scale < 1e30, "%s: scale must be positive and finite", name);
+  // (a scale of 0 in fp32 would make a hidden key's minus infinity NaN)
+  DFS_REQUIRE(a->scale >= 1e-30 && a->scale < 1e30, "%s: scale must lie from 1e-30 to 1e30", name);
   const int64_t strides[12] = {a->q_batch_stride, a->q_head_stride, a->q_row_stride, a->k_batch_stride,
                                a->k_head_stride,  a->k_row_stride,  a->v_batch_stride, a->v_head_stride,
                                a->v_row_stride,   a->out_batch_stride, a->out_head_stride, a->out_row_stride};

@@ -967,8 +967,8 @@ def _window_plan(q_shape: Shape, q_stride: Shape, k_shape: Shape, k_stride: Shap
         raise ValueError(f"{entry}: a rolling cache needs kv_lens, left and at least sinks + left + L slots, got "
                          f"{slots} for sinks={sinks}, left={left}, L={rows}")
     scale = 1.0 / math.sqrt(dim) if scale is None else scale
-    if not 0.0 < scale < 1e30:
-        raise ValueError(f"{entry}: scale must be positive and finite, got {scale}")
+    if not 1e-30 <= scale < 1e30:  # a scale of 0 in fp32 would make a hidden key's minus infinity NaN
+        raise ValueError(f"{entry}: scale must lie from 1e-30 to 1e30, got {scale}")
     if out_stride is None:  # q's storage order, where it leaves no gaps
         dense = _chunk_rows(q_shape, q_stride) and _dense(q_shape, q_stride)
         out_stride = q_stride if dense else _contiguous_stride(q_shape)
@@ -1004,8 +1004,8 @@ def window_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, left: Op
     vectors and are never read back.
 
     ``rolling``: k and v are caches that keep the sinks and the newest tokens
-    (``qkv_cache``); kv_lens counts every token so far and S must be at least
-    sinks + left + L.
+    (``qkv_cache``); kv_lens counts every token so far (up to 2^31 - 256) and S
+    must be at least sinks + left + L.
 
     bf16 or f16, D 64 or 128, fp32 scores and statistics; the weights are
     rounded to the operands' type for the product with v (f16: those below

@@ -539,7 +539,8 @@ int dfs_linear(const dfs_linear_args* args, dfs_stream_t stream);
  * of plus infinity makes its row NaN.
  * rolling: key j lies in slot j < sinks ? j : sinks + (j - sinks) mod
  * (slots - sinks); kv_lens counts all keys ever written and slots - sinks must
- * be at least left + q_rows. The workspace is the caller's,
+ * be at least left + q_rows. kv_lens up to 2^31 - 256; scale from 1e-30 to 1e30.
+ * The workspace is the caller's,
  * dfs_window_attention_workspace_size bytes (0: none).
  */
 typedef struct dfs_window_args {

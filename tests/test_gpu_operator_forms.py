@@ -213,3 +213,13 @@ def test_window_attention_infinite_scores_and_values(dev, L, dtype):
         rest = [i for i in range(L) if i != 2]
         assert bool(torch.isnan(out[:, :, 2]).all())
         _within(out[:, :, rest], ref[:, :, rest], tol[:, :, rest], "beside a query of NaN")
+
+
+@pytest.mark.parametrize("L", [1, 200])
+def test_window_attention_smallest_scale(dev, L):
+    """At 1e-30 every key that a row sees counts the same."""
+    gen = torch.Generator().manual_seed(L)
+    q, k, v = (torch.randn(1, 2, n, 64, generator=gen).to(BF) for n in (L, 300, 300))
+    ref, _, tol, _ = refs.window_attention(q, k, v, 100, 0, 4, scale=1e-30)
+    out = ops.window_attention(q.to(dev), k.to(dev), v.to(dev), 100, 0, 4, scale=1e-30)
+    _within(out, ref, tol, "smallest scale")

@@ -305,3 +305,20 @@ def test_caches_that_overlap_each_other_are_refused():
         ops.qkv_cache(**{**CACHE, "k_cache": k, "v_cache": buf.as_strided(shape, orders[1], 64)})
     with pytest.raises(RuntimeError, match="ROCm GPU"):
         ops.qkv_cache(**{**CACHE, "k_cache": k, "v_cache": buf.as_strided(shape, orders[1], 50000)})
+
+
+def test_scales_that_single_precision_cannot_hold_are_refused():
+    """Below 1e-45 a scale is 0 in fp32, and 0 times a hidden key's minus
+    infinity would be NaN."""
+    for scale in (1e-31, 1e-46, 5e-324, 1e30, float("inf"), -0.125):
+        with pytest.raises(ValueError, match="scale"):
+            ops.window_attention(**ATT, scale=scale)
+        a = _lib.WindowArgs()
+        a.batch = a.q_heads = a.kv_heads = a.q_rows = a.slots = 1
+        a.head_dim, a.left, a.right, a.scale = 64, -1, -1, scale
+        for name in ("q", "k", "v", "out"):
+            setattr(a, name, 16)
+        with pytest.raises(_lib.DfsKernelError, match="scale"):
+            _lib.call("dfs_window_attention", bytes(a), None)
+    with pytest.raises(RuntimeError, match="ROCm GPU"):
+        ops.window_attention(**ATT, scale=1e-30)
