@@ -199,7 +199,8 @@ __device__ __forceinline__ uint4 load_row8(const uint16_t* row, int k, int K) {
 // strides and sizes: rows are loaded into registers, four steps ahead, and
 // stored to one of two LDS buffers from there, one barrier a step. The channels
 // behind the last whole step go first, so that the steps' loads have no edge.
-// 333 x 1,017 x 709: 8.9 us; loads a step ahead, with two barriers: 11.9.
+// 333 x 1,017 x 709, one of many in a graph: 8.8 us, 10.4 with bias, SiLU and
+// residual (11.4 by trace); loads a step ahead, with two barriers, 11.9 for 8.8.
 template <bool F16>
 __global__ void __launch_bounds__(256) linear_any_kernel(LinearParams p) {
   __shared__ __attribute__((aligned(16))) uint16_t ws[2][64 * 64];
@@ -615,9 +616,10 @@ __global__ void __launch_bounds__(256, 2) linear_tile_kernel(LinearParams p) {
 // loaded three pairs before they are read, one barrier that says both that the
 // halves to be read have landed and that those to be loaded were read by all.
 //
-// 75,600 x 13,824 x 5,120 with GELU: 7.97 ms, 1.34 PFLOP/s (the library's
-// product alone 7.1, 1.50); 75,600 x 5,120 x 13,824: 7.56 ms, 1.41 PFLOP/s (6.9,
-// 1.55); 16,384 x 16,384 x 5,120: 1.90 ms, 1.45 PFLOP/s (1.77, 1.55). The matrix
+// 75,600 x 13,824 x 5,120 with GELU: 7.97 to 8.2 ms by the card, 1.3 PFLOP/s (the
+// library's product alone 7.1, 1.50); 75,600 x 5,120 x 13,824: 7.56 to 7.7 ms, 1.4
+// PFLOP/s (6.9 to 7.0, 1.53), 7.86 to 8.0 with bias, gate and residual; 16,384 x
+// 16,384 x 5,120: 1.90 to 1.97 ms, 1.4 PFLOP/s (1.77 to 1.80, 1.54). The matrix
 // cores are busy 79% of the cycles and the clock falls to 1.55 GHz: power is the
 // bound, and a barrier a phase costs 0.5%. A barrier a step of 64 channels with
 // its loads behind it took 10.6 ms, the phases with a branch for the last step's
@@ -938,7 +940,7 @@ struct Cut {
 int64_t big_tiles(int64_t rows, int64_t n) { return (rows + 255) / 256 * ((n + 255) / 256); }
 Cut cut_of(int64_t rows, int64_t n, int64_t k, bool chunks) {
   // Rows on no 16-byte boundary: small products of few steps as they are, the
-  // others laid out anew (us, as they are and anew: 333 by 1,017 x 709 8.9 and
+  // others laid out anew (us in a graph, as they are and anew: 333 by 1,017 x 709 8.9 and
   // 11.3, 100 by 5,119 x 1,001 11.7 and 15.9; 333 by 1,017 x 1,501 13.6 and 14.9,
   // 100 by 1,001 x 2,001 16.6 and 13.6, 64 by 640 x 6,001 35.8 and 18.8).
   if (!chunks && k <= 1024 && rows * n * k < (int64_t(1) << 30)) return Cut{kTileAny, 1, 0, false, 0};

@@ -425,8 +425,8 @@ __device__ __forceinline__ void block_of(const WindowParams& p, int x, int i, in
 // window_join_kernel. Late blocks, which see most keys where left has no limit,
 // are started first; where left has a limit, a head's last block with rows for
 // at most two of its waves comes behind all others and fills places that the
-// last round leaves (40 heads, 1,560 rows by 9,360 keys 358 us, in its place 370;
-// 3,600 by 14,400 963 and 981; without a limit 8 heads x 12,040 458 and 386).
+// last round leaves (40 heads, 1,560 rows by 9,360 keys 291 us, in its place 300;
+// 3,600 by 14,400 938 and 962; without a limit 8 heads x 12,040 458 and 386).
 __device__ __forceinline__ bool item_of(const WindowParams& p, Item& it) {
   const int x = blockIdx.x & 7, j = blockIdx.x >> 3;
   int i = j;
