@@ -225,7 +225,8 @@ class Wan_DFSAttn_Processor2_0:
         if branch == "window":
             hidden_states = full_attention(
                 query, key, value, mode="window", attn_mask=attention_mask, cu_seqlens_q=cu_seqlens_q,
-                cu_seqlens_kv=cu_seqlens_kv, window=self.window, sinks=self.sinks)
+                cu_seqlens_kv=cu_seqlens_kv, operand_dtype=WanDFSAttention.operand_dtype, window=self.window,
+                sinks=self.sinks)
         elif branch == "dfs":
             hidden_states = dfs_attention(
                 query, key, value, step_idx=self.step_idx, skip_steps=self.skip_steps,

@@ -322,3 +322,19 @@ def test_scales_that_single_precision_cannot_hold_are_refused():
             _lib.call("dfs_window_attention", bytes(a), None)
     with pytest.raises(RuntimeError, match="ROCm GPU"):
         ops.window_attention(**ATT, scale=1e-30)
+
+
+def test_window_mode_of_the_processor_passes_its_operand_dtype_on(monkeypatch):
+    """The operand_dtype that is set for the dense path is not dropped in mode
+    "window": it is refused where it is not the inputs' dtype."""
+    from dfsattn_amd import replace_wan
+    from dfsattn_amd.dit import DiTAttention
+
+    attn = DiTAttention(128, 2, 1e-6, device="cpu", dtype=BF)
+    attn.set_processor(replace_wan.Wan_DFSAttn_Processor2_0("window", 0.3, 16, 128, None, 0, [], 12, 12, 0.0, True, False,
+                                                            window=(4, 4)))
+    x = _t(1, 8, 128)
+    for dtype, error in ((torch.float16, ValueError), (BF, RuntimeError), (None, RuntimeError)):
+        monkeypatch.setattr(replace_wan.WanDFSAttention, "operand_dtype", dtype)
+        with pytest.raises(error, match="operand_dtype" if error is ValueError else "ROCm GPU"), torch.no_grad():
+            attn(x)
