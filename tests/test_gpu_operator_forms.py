@@ -223,3 +223,117 @@ def test_window_attention_smallest_scale(dev, L):
     ref, _, tol, _ = refs.window_attention(q, k, v, 100, 0, 4, scale=1e-30)
     out = ops.window_attention(q.to(dev), k.to(dev), v.to(dev), 100, 0, 4, scale=1e-30)
     _within(out, ref, tol, "smallest scale")
+
+
+# --------------------------------------------------------------------------
+# broadcast inputs, a padded batch, graphs side by side
+# --------------------------------------------------------------------------
+
+@pytest.mark.parametrize("m,n,k", [(3, 140, 264), (70, 140, 264), (70, 140, 77), (4185, 1960, 264)])
+def test_linear_broadcast_rows(dev, m, n, k):
+    """x, weight and residual with one row for all (stride 0): the bits of
+    their copies; a residual shared by two batches."""
+    gen = torch.Generator(dev).manual_seed(m)
+    x, w, r = _randn(gen, m, k, dtype=BF), _randn(gen, n, k, dtype=BF), _randn(gen, m, n, dtype=BF)
+    one = [t[:1].expand(t.shape) for t in (x, w, r)]
+    for i in range(3):
+        a = [x, w, r]
+        a[i] = one[i]
+        print(f"broadcast {m} x {n} x {k}: operand {i}", flush=True)
+        got = ops.linear(a[0], a[1], residual=a[2], activation="silu")
+        a[i] = one[i].contiguous()
+        assert torch.equal(got, ops.linear(a[0], a[1], residual=a[2], activation="silu"))
+    both = ops.linear(torch.stack([x, x]), w, residual=r.expand(2, m, n))
+    alone = ops.linear(torch.stack([x, x]), w, residual=torch.stack([r, r]))
+    assert torch.equal(both, alone) and torch.equal(both[0], both[1])
+
+
+@pytest.mark.parametrize("L", [1, 90])
+def test_window_attention_broadcast_axes(dev, L):
+    """Batches, heads and rows that are one in memory: the bits of their copies."""
+    gen = torch.Generator(dev).manual_seed(L)
+    base = {n: _randn(gen, 3, h, s, 64, dtype=BF) for n, h, s in (("q", 4, L), ("k", 2, 200), ("v", 2, 200))}
+    lens = torch.tensor([200, 31, 130], dtype=torch.int32, device=dev)
+    for name, t in base.items():
+        for view in (t[:1].expand(t.shape), t[:, :1].expand(t.shape), t[:, :, :1].expand(t.shape)):
+            print(f"broadcast L={L} {name} {view.stride()}", flush=True)
+            args = {**base, name: view}
+            got = ops.window_attention(**args, left=50, right=0, sinks=2, kv_lens=lens)
+            args[name] = view.contiguous()
+            assert torch.equal(got, ops.window_attention(**args, left=50, right=0, sinks=2, kv_lens=lens))
+
+
+def test_padded_chunks_equal_each_sequence_alone(dev):
+    """Chunks of three lengths in one padded batch, appended to rolling caches
+    and attended with q_lens, against each sequence by itself; what lies behind
+    a sequence's tokens is 0 in out, its slots stay."""
+    gen = torch.Generator(dev).manual_seed(9)
+    B, T, H, G, D, left, sinks = 3, 40, 4, 2, 64, 60, 5
+    S, new, lens = sinks + left + T, [40, 7, 0], [500, 3, 90]
+    q, k, v = (_randn(gen, B, T, n, D, dtype=BF) for n in (H, G, G))
+    caches = [_randn(gen, B, G, S, D, dtype=BF) for _ in range(2)]
+    before = [c.clone() for c in caches]
+    w = torch.rand(D, device=dev, generator=gen) + 0.5
+    ang = torch.rand(600, D // 2, device=dev, generator=gen)
+    table = (torch.cos(ang), torch.sin(ang))
+
+    def run(q, k, v, caches, lens, new):
+        ld, nd = (torch.tensor(t, dtype=torch.int32, device=dev) for t in (lens, new))
+        a = ops.qkv_cache(q, k, v, *caches, ld, w, w, table=table, new_lens=nd, sinks=sinks, rolling=True)
+        return ops.window_attention(a, *caches, left, 0, sinks, q_lens=nd, kv_lens=ld + nd, rolling=True, want_lse=True)
+
+    out, lse = run(q, k, v, caches, lens, new)
+    for b in range(B):
+        n = new[b]
+        assert bool((out[b, :, n:] == 0).all()) and bool((lse[b, :, n:] == -math.inf).all())
+        if n == 0:
+            assert torch.equal(caches[0][b], before[0][b]) and torch.equal(caches[1][b], before[1][b])
+            continue
+        own = [c[b:b + 1].clone() for c in before]
+        alone, alone_lse = run(*(t[b:b + 1, :n] for t in (q, k, v)), own, lens[b:b + 1], [n])
+        assert torch.equal(own[0][0], caches[0][b]) and torch.equal(own[1][0], caches[1][b])
+        # another number of rows may take other tiles, so sums in another order
+        ref, _, tol, _ = refs.window_attention(
+            ops.qkv_cache(*(t[b:b + 1, :n] for t in (q, k, v)), *[c.clone() for c in own],
+                          torch.tensor(lens[b:b + 1], dtype=torch.int32, device=dev), w, w, table=table, sinks=sinks,
+                          rolling=True).cpu(), own[0].cpu(), own[1].cpu(), left, 0, sinks, None, [lens[b] + n], True)
+        _within(out[b:b + 1, :, :n], ref, tol, f"padded sequence {b}")
+        _within(alone, ref, tol, f"sequence {b} alone")
+
+
+def test_two_graphs_with_workspaces_of_their_own(dev):
+    """Two captured calls that cut their work into parts, replayed in turn and
+    on two streams at once: each has its own workspace."""
+    gen = torch.Generator(dev).manual_seed(10)
+    jobs = []
+    for _ in range(2):
+        x, w = _randn(gen, 64, 4096, dtype=BF), _randn(gen, 640, 4096, dtype=BF, std=0.02)
+        q, k, v = (_randn(gen, 1, 2, n, 128, dtype=BF) for n in (130, 2600, 2600))
+        jobs.append((x, w, q, k, v))
+    assert cases.linear_form(64, 640, 4096) & cases.PARTS
+
+    def run(j):
+        return (ops.linear(j[0], j[1], activation="silu"), *ops.window_attention(*j[2:], right=0, want_lse=True))
+
+    for j in jobs:
+        run(j)
+    torch.cuda.synchronize()
+    graphs, outs = [], []
+    for j in jobs:
+        graph = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(graph):
+            outs.append(run(j))
+        graphs.append(graph)
+    streams = [torch.cuda.Stream() for _ in jobs]
+    for i in range(4):
+        for j in jobs:
+            j[0].normal_(generator=gen)
+            j[2].normal_(generator=gen)
+        want = [run(j) for j in jobs]
+        torch.cuda.synchronize()
+        for s, graph in zip(streams, graphs):
+            with torch.cuda.stream(s):
+                graph.replay()
+        torch.cuda.synchronize()
+        for a, b in zip(outs, want):
+            assert all(torch.equal(x, y) for x, y in zip(a, b))
