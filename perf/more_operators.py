@@ -185,7 +185,7 @@ def _hidden(gen, rows, k, dtype):
 
 def _to_codes(x):
     """(codes, scales) of x [rows, k] in fp32 elementary operations. The exponent e of a block is the smallest one
-    with max |x| <= 448 * 2^e; powers of two are made from their bits."""
+    with max |x| <= 448 * 2^e; powers of two are made from their bits. A block's scales of all rows lie together."""
     rows, k = x.shape
     nb = _blocks(k)
     y = x.float()
@@ -198,7 +198,7 @@ def _to_codes(x):
     e = torch.where(top == 0, 0, e).clamp(-127, 127).to(torch.int32)
     inverse = ((127 - e) << 23).view(torch.float32)
     codes = (y * inverse[..., None]).to(torch.float8_e4m3fn).reshape(rows, nb * BLOCK)[:, :k].contiguous()
-    return codes, (e + 127).to(torch.uint8).view(torch.float8_e8m0fnu)
+    return codes, (e + 127).to(torch.uint8).t().contiguous().view(torch.float8_e8m0fnu).t()
 
 
 def _from_codes(codes, scales, dtype=torch.float32):
