@@ -58,6 +58,10 @@ SIGNATURES = {
     "dfs_window_attention_form": [_p],
     "dfs_window_attention": [_p, _p],
     "dfs_qkv_cache": [_p, _p],
+    "dfs_quantize_fp8": [_p, _p],
+    "dfs_linear_fp8_workspace_size": [_i64, _i64, _i64, _i32],
+    "dfs_linear_fp8_form": [_i64, _i64, _i64],
+    "dfs_linear_fp8": [_p, _p],
 }
 
 class CallArgs(ctypes.Structure):
@@ -106,11 +110,28 @@ class CacheArgs(ctypes.Structure):
                           "sin_table", "lens", "new_lens")]
 
 
+class QuantizeFp8Args(ctypes.Structure):
+    """dfs_quantize_fp8_args, field by field."""
+
+    _fields_ = [(n, _i64) for n in ("rows", "k", "dtype", "x_stride", "values_stride", "scales_stride")] + [
+        (n, _p) for n in ("x", "values", "scales")]
+
+
+class LinearFp8Args(ctypes.Structure):
+    """dfs_linear_fp8_args, field by field."""
+
+    _fields_ = [(n, _i64) for n in (
+        "rows", "n", "k", "x_dtype", "dtype", "bias_dtype", "activation", "x_stride", "w_stride", "x_scales_stride",
+        "w_scales_stride", "residual_stride", "out_stride", "out8_stride", "out8_scales_stride", "workspace_bytes")] + [
+        (n, _p) for n in ("x", "w", "x_scales", "w_scales", "bias", "gate", "residual", "out", "out8", "out8_scales",
+                          "workspace")]
+
+
 _RESTYPES = {"dfs_last_error": ctypes.c_char_p, "dfs_block_score_topk_workspace_size": ctypes.c_int64,
              "dfs_block_score_topk_split_size": ctypes.c_int64, "dfs_bsa_fwd_workspace_size": ctypes.c_int64,
              "dfs_call_workspace_size": ctypes.c_int64, "dfs_linear_workspace_size": ctypes.c_int64,
-             "dfs_window_attention_workspace_size": ctypes.c_int64}
-ABI_VERSION = 7
+             "dfs_window_attention_workspace_size": ctypes.c_int64, "dfs_linear_fp8_workspace_size": ctypes.c_int64}
+ABI_VERSION = 8
 
 _lock = threading.Lock()
 _lib = None

@@ -1,0 +1,95 @@
+// Rows of 16-bit values to 8-bit codes with a scale for every 128 channels (the
+// definition is in fp8_block.h).
+#include <algorithm>
+
+#include "fp8_block.h"
+#include "lds_copy.h"
+
+namespace dfs {
+namespace {
+
+template <bool F16>
+__device__ __forceinline__ float to_f32(uint32_t bits) {
+  return F16 ? f16_bits_to_f32(bits) : bf16_bits_to_f32(bits);
+}
+
+struct QuantizeParams {
+  const uint16_t* x;
+  uint8_t *values, *scales;
+  int64_t ldx, ldv, lds;
+  int rows, k, fill, blocks;  // blocks: of a row
+};
+
+// Sixteen lanes a block, eight channels each; x's rows may lie anywhere.
+template <bool F16>
+__global__ void __launch_bounds__(256) quantize_kernel(QuantizeParams p) {
+  const int64_t id = static_cast<int64_t>(blockIdx.x) * 16 + (threadIdx.x >> 4);
+  if (id >= static_cast<int64_t>(p.rows) * p.blocks) return;  // whole groups of sixteen lanes
+  const int row = static_cast<int>(id / p.blocks), block = static_cast<int>(id - static_cast<int64_t>(row) * p.blocks);
+  const int l16 = threadIdx.x & 15, c = block * kScaleBlock + l16 * 8;
+  const uint16_t* const src = p.x + row * p.ldx;
+  uint4 v = make_uint4(0, 0, 0, 0);
+  if (c + 8 <= p.k) {
+    __builtin_memcpy(&v, src + c, 16);
+  } else if (c < p.k) {
+    uint16_t t[8];
+#pragma unroll
+    for (int i = 0; i < 8; ++i) t[i] = src[min(c + i, p.k - 1)];
+#pragma unroll
+    for (int i = 0; i < 8; ++i) t[i] = c + i < p.k ? t[i] : 0;
+    __builtin_memcpy(&v, t, 16);
+  }
+  float f[8], top = 0.f;
+#pragma unroll
+  for (int i = 0; i < 8; ++i) {
+    f[i] = to_f32<F16>(u16_at(v, i));
+    top = fmaxf(top, finite_magnitude(f[i]));
+  }
+  const uint32_t scale = block_scale(max16(top));
+  const uint2 codes = to_codes8(f, inverse_scale(scale));
+  uint8_t* const dst = p.values + row * p.ldv + c;
+  if (c + 8 <= p.fill) {
+    __builtin_memcpy(dst, &codes, 8);
+  } else {
+    uint8_t b[8];
+    __builtin_memcpy(b, &codes, 8);
+#pragma unroll
+    for (int i = 0; i < 8; ++i)
+      if (c + i < p.fill) dst[i] = b[i];
+  }
+  if (l16 == 0) p.scales[block * p.lds + row] = static_cast<uint8_t>(scale);
+}
+
+}  // namespace
+
+void launch_quantize(const uint16_t* x, int64_t rows, int64_t k, int64_t ldx, bool f16, uint8_t* values, int64_t ldv,
+                     int64_t fill, uint8_t* scales, int64_t lds, hipStream_t stream) {
+  QuantizeParams p{x, values, scales, ldx, ldv, lds, static_cast<int>(rows), static_cast<int>(k),
+                   static_cast<int>(fill), static_cast<int>((k + kScaleBlock - 1) / kScaleBlock)};
+  const dim3 grid(static_cast<unsigned>((rows * p.blocks + 15) / 16));
+  if (f16)
+    quantize_kernel<true><<<grid, 256, 0, stream>>>(p);
+  else
+    quantize_kernel<false><<<grid, 256, 0, stream>>>(p);
+}
+
+}  // namespace dfs
+
+extern "C" int dfs_quantize_fp8(const dfs_quantize_fp8_args* a, dfs_stream_t stream) {
+  using namespace dfs;
+  const char* name = "quantize_fp8";
+  DFS_REQUIRE(a != nullptr, "%s: args is NULL", name);
+  DFS_REQUIRE(a->x && a->values && a->scales, "%s: NULL operand", name);
+  const int64_t blocks = (a->k + kScaleBlock - 1) / kScaleBlock;
+  DFS_REQUIRE(a->rows > 0 && a->k > 0 && a->rows < (int64_t(1) << 30) && a->k < (int64_t(1) << 21),
+              "%s: rows=%lld k=%lld must be positive, below 2^30 and 2^21", name, (long long)a->rows, (long long)a->k);
+  DFS_REQUIRE(a->rows * blocks < (int64_t(1) << 28), "%s: too many blocks", name);  // a launch holds 2^32 threads
+  DFS_REQUIRE(a->dtype == DFS_DTYPE_BF16 || a->dtype == DFS_DTYPE_F16, "%s: dtype must be bf16 or f16", name);
+  DFS_REQUIRE(reinterpret_cast<uintptr_t>(a->x) % 2 == 0, "%s: x must be aligned to its elements", name);
+  DFS_REQUIRE(a->x_stride >= 0 && a->values_stride >= a->k && a->scales_stride >= a->rows,
+              "%s: x's stride must not be negative, the results' rows must not overlap", name);
+  launch_quantize(static_cast<const uint16_t*>(a->x), a->rows, a->k, a->x_stride, a->dtype == DFS_DTYPE_F16,
+                  static_cast<uint8_t*>(a->values), a->values_stride, a->k, static_cast<uint8_t*>(a->scales),
+                  a->scales_stride, reinterpret_cast<hipStream_t>(stream));
+  return check_launch(name);
+}

@@ -1183,3 +1183,205 @@ def qkv_cache(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, k_cache: torch.
     block = head + _CACHE_POINTERS.pack(*at, out.data_ptr(), pk, pv, *vectors, lens.data_ptr(), _ptr(new_lens) or 0)
     _call_on(device, "dfs_qkv_cache", block)
     return out
+
+
+# --------------------------------------------------------------------------
+# 8-bit operands and the products of them
+# --------------------------------------------------------------------------
+
+E4M3, E8M0 = torch.float8_e4m3fn, torch.float8_e8m0fnu
+SCALE_BLOCK = 128
+_FP8_X_CODES, _FP8_X_ALIGNED, _FP8_W_ALIGNED, _FP8_OUT_CODES = 1, 2, 4, 8  # DFS_FP8_*
+_E4M3_CODE = 3
+_QUANTIZE_POINTERS = struct.Struct("@3P")
+_LINEAR_FP8_POINTERS = struct.Struct("@11P")
+
+
+def _scale_blocks(k: int) -> int:
+    return -(-k // SCALE_BLOCK)
+
+
+def _empty_scales(like: torch.Tensor, lead: Shape, blocks: int) -> torch.Tensor:
+    """[*lead, blocks] scales whose storage holds a block's scales of all rows one behind the other."""
+    t = torch.empty((blocks, *lead), dtype=E8M0, device=like.device)
+    return t.movedim(0, -1) if lead else t
+
+
+@functools.lru_cache(maxsize=1024)
+def _quantize_plan(shape: Shape, stride: Shape, dtype: torch.dtype):
+    """(argument block up to the pointers, or None where rows do not join, rows) of a ``quantize_fp8`` call."""
+    if dtype not in HALF:
+        raise ValueError(f"quantize_fp8: x must be bf16 or f16, got {dtype}")
+    if len(shape) < 1 or shape[-1] == 0:
+        raise ValueError(f"quantize_fp8: x must be [..., K] with K > 0, got {tuple(shape)}")
+    rows, ld = math.prod(shape[:-1]), _row_stride(shape, stride)
+    if ld is None:
+        return None, rows
+    a = _lib.QuantizeFp8Args()
+    a.rows, a.k, a.dtype, a.x_stride, a.values_stride, a.scales_stride = rows, shape[-1], DTYPE_CODE[dtype], ld, shape[-1], rows
+    return bytes(a)[:_pointers(a, "x")], rows
+
+
+def quantize_fp8(x: torch.Tensor) -> Tuple[torch.Tensor, torch.Tensor]:
+    """x [..., K] (bf16 or f16) as operand of ``linear_fp8``: (codes
+    float8_e4m3fn [..., K], scales float8_e8m0fnu [..., ceil(K / 128)]), x being
+    codes * scales with a scale for each 128 consecutive channels of a row: the
+    smallest power of two (2^-127 at least) that leaves the block's largest
+    finite value within 448, 1 for zeros. Codes are rounded to nearest even,
+    values that are not finite become NaN. The scales are a view of storage
+    that holds a block's scales of all rows together, as ``linear_fp8`` reads
+    them in place. No backward pass."""
+    _refuse_grad("quantize_fp8", x)
+    head, rows = _quantize_plan(x.shape, x.stride(), x.dtype)
+    _one_device(x)
+    if head is None and rows:
+        return quantize_fp8(x.contiguous())
+    values = torch.empty(x.shape, dtype=E4M3, device=x.device)
+    scales = _empty_scales(x, x.shape[:-1], _scale_blocks(x.shape[-1]))
+    if rows:
+        _call_on(x.device, "dfs_quantize_fp8",
+                 head + _QUANTIZE_POINTERS.pack(x.data_ptr(), values.data_ptr(), scales.data_ptr()))
+    return values, scales
+
+
+def _scales_in_place(shape: Shape, stride: Shape) -> Optional[int]:
+    """Block stride of scales [..., blocks] whose rows lie one behind the other; None where they do not."""
+    step = 1
+    for n, s in zip(reversed(shape[:-1]), reversed(stride[:-1])):
+        if n > 1:
+            if s != step:
+                return None
+            step *= n
+    return stride[-1] if shape[-1] > 1 else step
+
+
+def _scales_laid_out(scales: torch.Tensor) -> torch.Tensor:
+    """The same scales with rows one behind the other."""
+    return scales.view(torch.uint8).movedim(-1, 0).contiguous().movedim(0, -1).view(E8M0)
+
+
+@functools.lru_cache(maxsize=1024)
+def _linear_fp8_plan(x_shape: Shape, x_stride: Shape, x_dtype: torch.dtype, w_shape: Shape, w_stride: Shape,
+                     w_dtype: torch.dtype, xs: Optional[Tuple[Shape, Shape, torch.dtype]],
+                     ws: Tuple[Shape, Shape, torch.dtype], out_dtype: Optional[torch.dtype], activation: Optional[str],
+                     bias: Optional[Tuple[Shape, torch.dtype]], residual: Optional[Tuple[Shape, Shape, torch.dtype]],
+                     quantize: bool):
+    """(shape of out, its dtype, what is read in place: x, weight, residual and
+    both scales, and the argument block up to the pointers with its workspace
+    bytes by the alignment of x and weight) of a ``linear_fp8`` call."""
+    entry = "linear_fp8"
+    codes = x_dtype == E4M3
+    if w_dtype != E4M3 or not (codes or x_dtype in HALF):
+        raise ValueError(f"{entry}: weight must be float8_e4m3fn and x that, bf16 or f16, got {w_dtype} and {x_dtype}")
+    if len(x_shape) < 1 or len(w_shape) != 2 or w_shape[1] != x_shape[-1]:
+        raise ValueError(f"{entry}: weight must be [N, K] for x [..., K], got {tuple(w_shape)} and {tuple(x_shape)}")
+    if 0 in w_shape:
+        raise ValueError(f"{entry}: weight {tuple(w_shape)} has no elements")
+    n, k = w_shape
+    blocks = _scale_blocks(k)
+    if ws[2] != E8M0 or tuple(ws[0]) != (n, blocks):
+        raise ValueError(f"{entry}: weight_scales must be float8_e8m0fnu {(n, blocks)}, got {ws[2]} {tuple(ws[0])}")
+    if codes != (xs is not None):
+        raise ValueError(f"{entry}: x_scales go with an x of codes, and only with one")
+    if xs is not None and (xs[2] != E8M0 or tuple(xs[0]) != (*x_shape[:-1], blocks)):
+        raise ValueError(f"{entry}: x_scales must be float8_e8m0fnu {(*x_shape[:-1], blocks)}, got {xs[2]} "
+                         f"{tuple(xs[0])}")
+    dtype = x_dtype if not codes else out_dtype or (residual[2] if residual is not None else torch.bfloat16)
+    if dtype not in HALF or out_dtype not in (None, dtype):
+        raise ValueError(f"{entry}: out_dtype must be bf16 or f16, and that of an x of one of them, got {out_dtype}")
+    if activation not in ACTIVATION_CODE:
+        raise ValueError(f"{entry}: activation must be one of {list(ACTIVATION_CODE)}, got {activation!r}")
+    if bias is not None and (tuple(bias[0]) != (n,) or bias[1] not in (dtype, torch.float32)):
+        raise ValueError(f"{entry}: bias must hold {n} {dtype} or float32 values, got {bias[1]} {tuple(bias[0])}")
+    shape = (*x_shape[:-1], n)
+    if residual is not None and (tuple(residual[0]) != shape or residual[2] != dtype):
+        raise ValueError(f"{entry}: residual must be {dtype} {shape}, got {residual[2]} {tuple(residual[0])}")
+    rows = math.prod(x_shape[:-1])
+    ldx, ldw = _row_stride(x_shape, x_stride), _row_stride(w_shape, w_stride)
+    ldr = 0 if residual is None else _row_stride(residual[0], residual[1])
+    ldxs = 0 if xs is None else _scales_in_place(xs[0], xs[1])
+    ldws = _scales_in_place(ws[0], ws[1])
+    if rows == 0 or None in (ldx, ldw, ldr, ldxs, ldws):
+        return shape, dtype, tuple(t is not None for t in (ldx, ldw, ldr, ldxs, ldws)), None
+    a = _lib.LinearFp8Args()
+    a.rows, a.n, a.k, a.activation, a.dtype = rows, n, k, ACTIVATION_CODE[activation], DTYPE_CODE[dtype]
+    a.x_dtype = _E4M3_CODE if codes else a.dtype
+    a.bias_dtype = 0 if bias is None else DTYPE_CODE[bias[1]]
+    a.x_stride, a.w_stride, a.x_scales_stride, a.w_scales_stride = ldx, ldw, ldxs, ldws
+    a.residual_stride, a.out_stride, a.out8_stride, a.out8_scales_stride = ldr, n, n, rows
+    whole = [k % 16 == 0 and ld % 16 == 0 and ld < 1 << 22 for ld in (ldx, ldw)]
+    blocks_of = []
+    for at in range(4):  # bit 0: x on 16 bytes, bit 1: weight
+        flags = _FP8_OUT_CODES if quantize else 0
+        if codes:
+            flags |= _FP8_X_CODES | (_FP8_X_ALIGNED if whole[0] and at & 1 else 0)
+        if whole[1] and at & 2:
+            flags |= _FP8_W_ALIGNED
+        size = int(_lib.lib().dfs_linear_fp8_workspace_size(rows, n, k, flags))
+        if size < 0:
+            raise _lib.DfsKernelError(_lib.lib().dfs_last_error().decode(errors="replace"))
+        a.workspace_bytes = size
+        blocks_of.append((bytes(a)[:_pointers(a, "x")], size))
+    return shape, dtype, None, blocks_of
+
+
+def linear_fp8(x: torch.Tensor, weight: torch.Tensor, weight_scales: torch.Tensor,
+               x_scales: Optional[torch.Tensor] = None, bias: Optional[torch.Tensor] = None,
+               activation: Optional[str] = None, gate: Optional[torch.Tensor] = None,
+               residual: Optional[torch.Tensor] = None, out: Optional[torch.Tensor] = None,
+               out_dtype: Optional[torch.dtype] = None, quantize: bool = False):
+    """residual + gate * act(x @ weight.T + bias) as ``linear``, on operands of
+    8 bits: weight [N, K] and weight_scales [N, ceil(K / 128)] as
+    ``quantize_fp8`` gives them, x [..., K] the same with x_scales, or bf16 or
+    f16, which is quantised first. Every product is exact and sums are fp32; the
+    result is rounded once, to x's dtype or, for an x of codes, out_dtype
+    (default: the residual's, else bf16). bias in that dtype or fp32, gate N
+    fp32 values. ``quantize``: returns ``quantize_fp8`` of the result, (codes,
+    scales), instead. ``out`` may be the residual itself. Codes whose rows lie
+    off 16-byte boundaries and scales whose rows do not lie one behind the other
+    are copied at each call. No backward pass."""
+    entry = "linear_fp8"
+    _refuse_grad(entry, x, bias, gate, residual, out)
+    if weight_scales is None:
+        raise ValueError(f"{entry}: weight_scales are needed")
+    quantize = bool(quantize)
+    shape, dtype, in_place, blocks = _linear_fp8_plan(
+        x.shape, x.stride(), x.dtype, weight.shape, weight.stride(), weight.dtype,
+        None if x_scales is None else (x_scales.shape, x_scales.stride(), x_scales.dtype),
+        (weight_scales.shape, weight_scales.stride(), weight_scales.dtype), out_dtype, activation,
+        None if bias is None else (bias.shape, bias.dtype),
+        None if residual is None else (residual.shape, residual.stride(), residual.dtype), quantize)
+    if bias is not None and not bias.is_contiguous():
+        bias = bias.contiguous()
+    if gate is not None and not (gate.dim() == 1 and gate.shape[0] == shape[-1] and gate.dtype == torch.float32
+                                 and gate.is_contiguous()):
+        gate = _vec(gate, shape[-1], "linear_fp8: gate")
+    if out is not None and (quantize or tuple(out.shape) != shape or out.dtype != dtype or not out.is_contiguous()):
+        raise ValueError(f"{entry}: out must be contiguous {dtype} {shape}, and goes with no quantize, got {out.dtype} "
+                         f"{tuple(out.shape)}")
+    _one_device(x, weight, weight_scales, x_scales, bias, gate, residual, out)
+    if out is not None:
+        same = residual is not None and residual.data_ptr() == out.data_ptr() and residual.is_contiguous()
+        _refuse_overlap(entry, "out", out, x, weight, weight_scales, x_scales, bias, gate, None if same else residual)
+    if blocks is None and math.prod(shape):
+        x, weight, residual = (t if t is None or whole else t.contiguous()
+                               for t, whole in zip((x, weight, residual), in_place))
+        x_scales, weight_scales = (t if t is None or whole else _scales_laid_out(t)
+                                   for t, whole in zip((x_scales, weight_scales), in_place[3:]))
+        return linear_fp8(x, weight, weight_scales, x_scales, bias, activation, gate, residual, out, out_dtype, quantize)
+    scales = None
+    if quantize:
+        out = torch.empty(shape, dtype=E4M3, device=x.device)
+        scales = _empty_scales(x, shape[:-1], _scale_blocks(shape[-1]))
+    elif out is None:
+        out = torch.empty(shape, dtype=dtype, device=x.device)
+    if blocks is not None:
+        px, pw = x.data_ptr(), weight.data_ptr()
+        head, size = blocks[(px % 16 == 0) + 2 * (pw % 16 == 0)]
+        ws = torch.empty(size, dtype=torch.uint8, device=x.device) if size else None
+        po = out.data_ptr()
+        block = head + _LINEAR_FP8_POINTERS.pack(
+            px, pw, _ptr(x_scales) or 0, weight_scales.data_ptr(), _ptr(bias) or 0, _ptr(gate) or 0,
+            _ptr(residual) or 0, 0 if quantize else po, po if quantize else 0, _ptr(scales) or 0, _ptr(ws) or 0)
+        _call_on(x.device, "dfs_linear_fp8", block)
+    return (out, scales) if quantize else out

@@ -43,7 +43,8 @@ const char* dfs_last_error(void);
  * and per-head operand exponents in the attention call, per-head overflow flags and dfs_prepare_fixup;
  * 4: separate query and key tile sizes in preparation and scoring; 5: Q read from the input by
  * the attention kernel, q_perm optional; 6: dfs_linear, dfs_window_attention and dfs_qkv_cache;
- * 7: dfs_linear_form and dfs_window_attention_form). */
+ * 7: dfs_linear_form and dfs_window_attention_form; 8: dfs_quantize_fp8, dfs_linear_fp8,
+ * dfs_residual_norm and dfs_axial_rope). */
 int dfs_abi_version(void);
 
 /*
@@ -593,6 +594,60 @@ typedef struct dfs_cache_args {
   const int32_t *lens, *new_lens;
 } dfs_cache_args;
 int dfs_qkv_cache(const dfs_cache_args* args, dfs_stream_t stream);
+
+/*
+ * 8-bit operands (no reference code): rows of k 16-bit values as e4m3 codes
+ * and one power of two (e8m0, a byte: exponent + 127) for every 128
+ * consecutive channels of a row, the last block of a row as long as it is.
+ * The exponent e of a block is the smallest with max |x| <= 448 * 2^e over its
+ * finite values, from -127 to 127 (0 for zeros); a code is x * 2^-e rounded to
+ * nearest even, NaN where x is not finite. values [rows][k], row stride
+ * values_stride; scales [ceil(k / 128)][rows], block stride scales_stride (the
+ * products read a block's scales of neighbouring rows together). k below 2^21.
+ */
+typedef struct dfs_quantize_fp8_args {
+  int64_t rows, k, dtype, x_stride, values_stride, scales_stride;
+  const void* x;
+  void *values, *scales;
+} dfs_quantize_fp8_args;
+int dfs_quantize_fp8(const dfs_quantize_fp8_args* args, dfs_stream_t stream);
+
+/*
+ * dfs_linear on 8-bit operands:
+ *   out = residual + gate * act(sum_b sx[b] sw[b] sum_{k in b} x[k] w[k] + bias)
+ * over blocks b of 128 channels. w [n][k] codes with w_scales [ceil(k/128)][n];
+ * x [rows][k] codes with x_scales (x_dtype DFS_DTYPE_E4M3), or bf16 or f16
+ * values that are quantised first (x_scales NULL). out, residual: dtype (bf16
+ * or f16; x_dtype where that is one of them). Sums and epilogue are fp32,
+ * rounded once to dtype. out8 / out8_scales (both or neither): the rounded
+ * result is quantised instead of written, out is NULL then. The
+ * workspace is the caller's, dfs_linear_fp8_workspace_size bytes (0: none),
+ * with `flags` the sum of
+ *   DFS_FP8_X_CODES    x is codes;
+ *   DFS_FP8_X_ALIGNED  x's codes lie on 16-byte boundaries, their stride and k
+ *                      are multiples of 16, the stride below 2^22 (codes are
+ *                      laid out anew otherwise);
+ *   DFS_FP8_W_ALIGNED  the same of w;
+ *   DFS_FP8_OUT_CODES  the result is left as codes.
+ * Out may be the residual itself, but overlap nothing else.
+ */
+enum { DFS_DTYPE_E4M3 = 3 };
+typedef struct dfs_linear_fp8_args {
+  int64_t rows, n, k, x_dtype, dtype, bias_dtype, activation;
+  int64_t x_stride, w_stride, x_scales_stride, w_scales_stride;
+  int64_t residual_stride, out_stride, out8_stride, out8_scales_stride, workspace_bytes;
+  const void *x, *w, *x_scales, *w_scales, *bias;
+  const float* gate;
+  const void* residual;
+  void *out, *out8, *out8_scales, *workspace;
+} dfs_linear_fp8_args;
+enum { DFS_FP8_X_CODES = 1, DFS_FP8_X_ALIGNED = 2, DFS_FP8_W_ALIGNED = 4, DFS_FP8_OUT_CODES = 8 };
+int64_t dfs_linear_fp8_workspace_size(int64_t rows, int64_t n, int64_t k, int flags);
+/* Host function for tests and profiles: the kernel that a call takes, which
+ * goes by its sizes alone: the forms of dfs_linear_form (FEW up to 16 rows),
+ * with DFS_FORM_PARTS and DFS_FORM_STREAM. */
+int dfs_linear_fp8_form(int64_t rows, int64_t n, int64_t k);
+int dfs_linear_fp8(const dfs_linear_fp8_args* args, dfs_stream_t stream);
 
 #ifdef __cplusplus
 }

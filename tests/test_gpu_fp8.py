@@ -1,0 +1,153 @@
+"""GPU parity of ops.quantize_fp8 and ops.linear_fp8 with their 64-bit
+definitions (block_refs)."""
+import math
+
+import pytest
+import torch
+
+import block_refs as refs
+from dfsattn_amd import _lib, ops
+
+pytestmark = pytest.mark.gpu
+BF, HF = torch.bfloat16, torch.float16
+
+
+def _randn(gen, *shape, dtype, std=1.0):
+    return (torch.randn(*shape, generator=gen) * std).to(dtype)
+
+
+def _within(got, ref, tol, what=""):
+    got = got.detach().cpu().double()
+    assert got.shape == ref.shape
+    assert bool(torch.isfinite(got).all()), f"{what}: not finite"
+    off = (got - ref).abs() - tol
+    worst = int(off.argmax())
+    assert float(off.max()) <= 0, (f"{what}: at {worst} got {float(got.flatten()[worst])}, want "
+                                   f"{float(ref.flatten()[worst])} within {float(tol.flatten()[worst])}")
+
+
+def _hidden(gen, rows, k, dtype):
+    """Rows and channels of very different sizes."""
+    x = torch.randn(rows, k, generator=gen) * torch.exp(torch.randn(rows, 1, generator=gen))
+    x[:, ::37] *= 30
+    return x.to(dtype)
+
+
+def _same_codes(got, want):
+    """Codes and scales equal to quantize's 64-bit values, NaN to NaN."""
+    for g, w in zip(got, want):
+        g = g.cpu().double()
+        assert g.shape == w.shape
+        assert torch.equal(torch.isnan(g), torch.isnan(w))
+        assert torch.equal(torch.nan_to_num(g), torch.nan_to_num(w))
+
+
+# --------------------------------------------------------------------------
+# quantize_fp8
+# --------------------------------------------------------------------------
+
+@pytest.mark.parametrize("dtype", [BF, HF])
+@pytest.mark.parametrize("rows,k", [(1, 1), (1, 128), (3, 127), (5, 129), (2, 8), (77, 1001), (300, 640), (9, 5120),
+                                    (1000, 136)])
+def test_quantize_matches_definition(dev, rows, k, dtype):
+    print(f"quantize {rows} x {k} {dtype}", flush=True)
+    g = torch.Generator().manual_seed(rows * 3 + k)
+    x = _hidden(g, rows, k, dtype)
+    _same_codes(ops.quantize_fp8(x.to(dev)), refs.quantize(x))
+
+
+@pytest.mark.parametrize("dtype", [BF, HF])
+def test_quantize_every_value(dev, dtype):
+    """All 2^16 values, each the largest of a block beside smaller ones, each a
+    small one beside a large one, zeros and values that are not finite."""
+    every = torch.arange(1 << 16, dtype=torch.int32).to(torch.int16).view(dtype)
+    alone = torch.zeros(1 << 16, 128, dtype=dtype)
+    alone[:, 5] = every
+    alone[:, 99] = torch.where(torch.isfinite(every), every * 0.37, torch.ones(()).to(dtype))
+    beside = every.view(-1, 128).clone()
+    beside[:, 0] = 1.75
+    for x in (alone, beside, every.view(-1, 256)):
+        print("quantize every value", tuple(x.shape), flush=True)
+        _same_codes(ops.quantize_fp8(x.to(dev)), refs.quantize(x))
+
+
+def test_quantize_views(dev):
+    """Rows inside wider ones at any element, a batch axis, a transposed view, no rows."""
+    g = torch.Generator().manual_seed(0)
+    wide = _hidden(g, 60, 400, BF)
+    for off in (0, 8, 3):
+        x = wide.view(4, 15, 400)[:, :, off:off + 300]
+        got = ops.quantize_fp8(wide.to(dev).view(4, 15, 400)[:, :, off:off + 300])
+        assert got[0].shape == (4, 15, 300) and got[1].shape == (4, 15, 3)
+        _same_codes([t.flatten(0, 1) if t.is_contiguous() else t.reshape(60, -1) for t in
+                     (got[0], got[1].view(torch.uint8).reshape(60, 3).view(torch.float8_e8m0fnu))],
+                    refs.quantize(x.reshape(60, 300)))
+    t = wide.t()
+    _same_codes(ops.quantize_fp8(wide.to(dev).t()), refs.quantize(t))
+    one = ops.quantize_fp8(wide[0].to(dev))
+    assert one[0].shape == (400,) and one[1].shape == (4,)
+    none = ops.quantize_fp8(wide[:0].to(dev))
+    assert none[0].shape == (0, 400) and none[1].shape == (0, 4)
+
+
+# --------------------------------------------------------------------------
+# linear_fp8
+# --------------------------------------------------------------------------
+
+LINEAR = [
+    # M, N, K, dtype, x in codes, bias dtype, act, gate, residual
+    (1, 64, 64, BF, False, BF, None, False, False),
+    (1, 1, 1, BF, True, None, None, False, True),
+    (1, 2048, 1024, BF, False, torch.float32, "silu", False, False),
+    (3, 257, 2500, HF, True, HF, "gelu_tanh", True, True),
+    (2, 200, 8200, BF, False, BF, None, False, False),
+    (16, 640, 256, BF, True, BF, "gelu", False, True),
+    (17, 96, 2048, HF, False, None, None, True, False),
+    (33, 1000, 1032, BF, True, BF, "gelu_tanh", False, False),
+    (64, 520, 4096, BF, False, None, None, False, True),
+    (65, 129, 63, BF, True, BF, "silu", True, True),
+    (100, 128, 65, HF, False, torch.float32, None, False, False),
+    (127, 255, 511, HF, True, HF, "gelu", True, True),
+    (128, 128, 128, BF, False, BF, None, False, False),
+    (200, 384, 640, BF, True, BF, "gelu_tanh", True, True),
+    (256, 256, 64, BF, False, None, None, False, False),
+    (257, 513, 72, HF, True, HF, None, False, True),
+    (300, 1025, 1000, BF, False, BF, "silu", False, False),
+    (513, 1024, 1024, BF, True, BF, "gelu_tanh", False, True),
+    (1000, 776, 136, HF, False, None, None, True, True),
+    (2100, 2056, 192, BF, True, BF, None, True, True),
+    (2049, 2304, 328, HF, False, HF, "gelu_tanh", False, False),
+    (4099, 1100, 70, BF, True, torch.float32, "gelu_tanh", False, True),
+]
+
+
+@pytest.mark.parametrize("m,n,k,dtype,codes,bias,act,gate,residual", LINEAR)
+def test_linear_fp8_matches_definition(dev, m, n, k, dtype, codes, bias, act, gate, residual):
+    print(f"linear_fp8 {m} x {n} x {k} {dtype} codes={codes} bias={bias} act={act} gate={gate} residual={residual}",
+          flush=True)
+    g = torch.Generator().manual_seed(m * 7 + n * 3 + k)
+    x, w = _hidden(g, m, k, dtype), _randn(g, n, k, dtype=dtype, std=2 / math.sqrt(k))
+    xq, wq = refs.quantize(x), refs.quantize(w)
+    b = None if bias is None else _randn(g, n, dtype=bias)
+    gt = torch.randn(n, generator=g) if gate else None
+    r = _randn(g, m, n, dtype=dtype) if residual else None
+    xt, wt = refs.to_tensors(*xq), refs.to_tensors(*wq)
+    ref, tol = refs.linear_fp8(refs.values(*xt), refs.values(*wt), dtype, b, act, gt, r)
+    d = [None if t is None else t.to(dev) for t in (*(xt if codes else (x, None)), *wt, b, gt, r)]
+
+    def call(**kw):
+        return ops.linear_fp8(d[0], d[2], d[3], d[1], bias=d[4], activation=act, gate=d[5], residual=d[6],
+                              out_dtype=dtype, **kw)
+
+    got = call()
+    assert got.dtype == dtype
+    _within(got, ref, tol, "linear_fp8")
+    assert torch.equal(got, call())
+    _same_codes(call(quantize=True), refs.quantize(got.cpu()))
+    # scales whose rows lie one behind the other are read in place: the same
+    d[3] = ops._scales_laid_out(d[3])
+    d[1] = d[1] if d[1] is None else ops._scales_laid_out(d[1])
+    assert torch.equal(got, call())
+    if residual:  # in place of the residual
+        d[6] = call(out=d[6])
+        assert torch.equal(got, d[6])
