@@ -62,6 +62,8 @@ SIGNATURES = {
     "dfs_linear_fp8_workspace_size": [_i64, _i64, _i64, _i32],
     "dfs_linear_fp8_form": [_i64, _i64, _i64],
     "dfs_linear_fp8": [_p, _p],
+    "dfs_residual_norm": [_p, _p],
+    "dfs_axial_rope": [_p, _p],
 }
 
 class CallArgs(ctypes.Structure):
@@ -125,6 +127,31 @@ class LinearFp8Args(ctypes.Structure):
         "w_scales_stride", "residual_stride", "out_stride", "out8_stride", "out8_scales_stride", "workspace_bytes")] + [
         (n, _p) for n in ("x", "w", "x_scales", "w_scales", "bias", "gate", "residual", "out", "out8", "out8_scales",
                           "workspace")]
+
+
+class ResidualNormArgs(ctypes.Structure):
+    """dfs_residual_norm_args, field by field."""
+
+    _fields_ = [(n, _i64) for n in (
+        "rows", "channels", "dtype", "post_norm", "norm", "x_stride", "y_stride", "out_stride", "h_stride",
+        "h8_scales_stride", "gate_rows", "gate_stride", "scale_rows", "scale_stride", "shift_rows", "shift_stride",
+        "post_weight_dtype", "post_bias_dtype", "weight_dtype", "bias_dtype")] + [
+        (n, ctypes.c_double) for n in ("residual_scale", "eps", "post_eps")] + [
+        (n, _p) for n in ("x", "y", "gate", "scale", "shift", "post_weight", "post_bias", "weight", "bias", "out", "h",
+                          "h8", "h8_scales")]
+
+
+class AxialRopeArgs(ctypes.Structure):
+    """dfs_axial_rope_args, field by field."""
+
+    _fields_ = [(n, _i64) for n in (
+        "batch", "tokens", "q_heads", "kv_heads", "head_dim", "dtype", "halves", "axes", "q_weight_dtype", "q_norm_all",
+        "k_weight_dtype", "k_norm_all", "q_batch_stride", "q_token_stride", "q_head_stride", "k_batch_stride",
+        "k_token_stride", "k_head_stride", "q_out_batch_stride", "q_out_token_stride", "q_out_head_stride",
+        "k_out_batch_stride", "k_out_token_stride", "k_out_head_stride", "positions_batch_stride",
+        "positions_token_stride")] + [("pairs", _i64 * 4), ("size", _i64 * 4), ("slope", ctypes.c_double * 4),
+                                      ("turn", ctypes.c_double * 4), ("eps", ctypes.c_double)] + [
+        (n, _p) for n in ("q", "k", "q_out", "k_out", "q_weight", "k_weight", "start", "positions")]
 
 
 _RESTYPES = {"dfs_last_error": ctypes.c_char_p, "dfs_block_score_topk_workspace_size": ctypes.c_int64,

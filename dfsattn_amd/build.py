@@ -18,7 +18,8 @@ INCLUDE = os.path.join(REPO_DIR, "include")
 OUT_DIR = os.path.join(PKG_DIR, "_lib")
 LIB_NAME = "libdfsattn_amd.so"
 SOURCES = ["host.cpp", "call.cpp", "permute.hip", "score_topk.hip", "bsa_fwd.hip", "masks.hip", "norm_rope.hip", "dit_fused.hip",
-           "linear.hip", "window_attn.hip", "qkv_cache.hip", "quantize.hip", "linear_fp8.hip"]
+           "linear.hip", "window_attn.hip", "qkv_cache.hip", "quantize.hip", "linear_fp8.hip",
+           "residual_norm.hip", "axial_rope.hip"]
 ARCH = "gfx950"
 
 

@@ -1385,3 +1385,297 @@ def linear_fp8(x: torch.Tensor, weight: torch.Tensor, weight_scales: torch.Tenso
             _ptr(residual) or 0, 0 if quantize else po, po if quantize else 0, _ptr(scales) or 0, _ptr(ws) or 0)
         _call_on(x.device, "dfs_linear_fp8", block)
     return (out, scales) if quantize else out
+
+
+# --------------------------------------------------------------------------
+# Between the branches of a block, and rotation by several axes
+# --------------------------------------------------------------------------
+
+NORM_CODE = {None: 0, "rms": 1, "layer": 2}
+_NORM_POINTERS = struct.Struct("@13P")
+_ROPE_POINTERS = struct.Struct("@8P")
+Meta = Tuple[Shape, Shape, torch.dtype]  # shape, strides and type of a tensor
+
+
+def _meta(t: Optional[torch.Tensor]) -> Optional[Meta]:
+    return None if t is None else (t.shape, t.stride(), t.dtype)
+
+
+def _vector_groups(entry: str, name: str, t: Meta, x_shape: Shape) -> Tuple[int, Optional[int], Shape]:
+    """Of fp32 vectors [..., C] that broadcast over the rows of x: (consecutive
+    rows of x a vector serves, its vectors' stride or None where it has to be
+    laid out anew, and the shape for that)."""
+    shape, stride, dtype = t
+    n = len(x_shape)
+    full = (1,) * (n - len(shape)) + tuple(shape)
+    if dtype != torch.float32 or len(full) != n or full[-1] != x_shape[-1] or any(
+            a not in (1, b) for a, b in zip(full[:-1], x_shape[:-1])):
+        raise ValueError(f"{entry}: {name} must be float32 vectors that broadcast over {tuple(x_shape)}, got {dtype} "
+                         f"{tuple(shape)}")
+    p = max((i + 1 for i in range(n - 1) if full[i] != 1), default=0)
+    laid_out = (*x_shape[:p], *(1,) * (n - 1 - p), x_shape[-1])
+    rows = math.prod(x_shape[p:-1])
+    if full != laid_out:
+        return rows, None, laid_out
+    return rows, _row_stride(shape, stride), laid_out
+
+
+@functools.lru_cache(maxsize=1024)
+def _norm_plan(x: Meta, y: Optional[Meta], gate: Optional[Meta], scale: Optional[Meta], shift: Optional[Meta],
+               weights: Tuple[Optional[Meta], ...], post_norm: Optional[str], norm: str, residual_scale: float,
+               eps: float, post_eps: float, quantize: bool):
+    """(argument block up to the pointers, or None, and, where there is none:
+    whether x and y are read in place and the shapes that gate, scale and shift
+    are laid out in, None for as they are) of a ``residual_norm`` call."""
+    entry = "residual_norm"
+    shape, _, dtype = x
+    if dtype not in HALF or y is not None and (y[2] != dtype or y[0] != shape):
+        raise ValueError(f"{entry}: x and y must be bf16 or f16 of one shape, got {x} and {y}")
+    if len(shape) < 1 or not 0 < shape[-1] <= 8192:
+        raise ValueError(f"{entry}: x must be [..., C] with C from 1 to 8192, got {tuple(shape)}")
+    if norm not in ("rms", "layer") or post_norm not in NORM_CODE:
+        raise ValueError(f"{entry}: norm must be 'rms' or 'layer', post_norm one of them or None, got {norm!r} and "
+                         f"{post_norm!r}")
+    if y is None and (gate is not None or post_norm is not None or residual_scale != 1.0):
+        raise ValueError(f"{entry}: a gate, norm or residual_scale without y")
+    if post_norm is None and (weights[0] is not None or weights[1] is not None):
+        raise ValueError(f"{entry}: post_weight and post_bias go with a post_norm")
+    if not (eps >= 0.0 and post_eps >= 0.0) or not math.isfinite(residual_scale):
+        raise ValueError(f"{entry}: eps must not be negative and residual_scale finite, got {eps}, {post_eps}, "
+                         f"{residual_scale}")
+    C = shape[-1]
+    a = _lib.ResidualNormArgs()
+    for name, w in zip(("post_weight", "post_bias", "weight", "bias"), weights):
+        if w is None:
+            continue
+        if tuple(w[0]) != (C,) or w[2] not in DTYPE_CODE:
+            raise ValueError(f"{entry}: {name} must be a [{C}] vector of bf16, f16 or float32, got {w[2]} {tuple(w[0])}")
+        setattr(a, f"{name}_dtype", DTYPE_CODE[w[2]])
+    rows = math.prod(shape[:-1])
+    lds = [0 if t is None else _row_stride(t[0], t[1]) for t in (x, y)]
+    anew = [None, None, None]
+    for i, (name, t) in enumerate((("gate", gate), ("scale", scale), ("shift", shift))):
+        if t is None:
+            continue
+        each, stride, laid_out = _vector_groups(entry, name, t, shape)
+        if stride is None:
+            anew[i] = laid_out
+        setattr(a, f"{name}_rows", each)
+        setattr(a, f"{name}_stride", stride or 0)
+    if rows == 0 or None in lds or any(s is not None for s in anew):
+        return None, (lds[0] is not None, lds[1] is not None), anew
+    a.rows, a.channels, a.dtype = rows, C, DTYPE_CODE[dtype]
+    a.post_norm, a.norm = NORM_CODE[post_norm], NORM_CODE[norm]
+    a.x_stride, a.y_stride, a.out_stride, a.h_stride, a.h8_scales_stride = lds[0], lds[1], C, C, rows
+    a.residual_scale, a.eps, a.post_eps = residual_scale, eps, post_eps
+    return bytes(a)[:_pointers(a, "x")], None, None
+
+
+def residual_norm(x: torch.Tensor, y: Optional[torch.Tensor] = None, gate: Optional[torch.Tensor] = None,
+                  residual_scale: float = 1.0, post_norm: Optional[str] = None,
+                  post_weight: Optional[torch.Tensor] = None, post_bias: Optional[torch.Tensor] = None,
+                  post_eps: Optional[float] = None, norm: str = "layer", weight: Optional[torch.Tensor] = None,
+                  bias: Optional[torch.Tensor] = None, scale: Optional[torch.Tensor] = None,
+                  shift: Optional[torch.Tensor] = None, eps: float = 1e-6, out: Optional[torch.Tensor] = None,
+                  quantize: bool = False):
+    """What stands between two branches of a block, in one pass: returns
+
+        r = residual_scale * x + gate * post(y)
+        h = (norm(r) * weight + bias) * (1 + scale) + shift
+
+    in x's dtype (bf16 or f16), h of r as it is rounded. x and y [..., C], C up
+    to 8192; post: no norm (None), "rms" or "layer" with post_weight and
+    post_bias and post_eps (default eps); norm "layer" or "rms". Weights and
+    biases are [C] in bf16, f16 or fp32; gate, scale and shift fp32, one vector
+    [C] or vectors that broadcast over x's leading axes (for each sequence, or
+    each frame of x [B, F, tokens, C]). Computed in fp32 step by step as written:
+    with no post norm r and h equal ``gated_residual`` and ``adaln_modulate``.
+    Without y r is x itself. ``quantize``: returns (r, codes, scales) with
+    ``quantize_fp8`` of h in its place. ``out`` takes r and may be x or y. No
+    backward pass."""
+    entry = "residual_norm"
+    _refuse_grad(entry, x, y, gate, post_weight, post_bias, weight, bias, scale, shift, out)
+    quantize, eps = bool(quantize), float(eps)
+    head, whole, anew = _norm_plan(
+        _meta(x), _meta(y), _meta(gate), _meta(scale), _meta(shift),
+        (_meta(post_weight), _meta(post_bias), _meta(weight), _meta(bias)), post_norm, norm, float(residual_scale), eps,
+        eps if post_eps is None else float(post_eps), quantize)
+    if out is not None and (y is None or out.shape != x.shape or out.dtype != x.dtype or not out.is_contiguous()):
+        raise ValueError(f"{entry}: out must be contiguous {x.dtype} {tuple(x.shape)}, and goes with a y, got {out.dtype} "
+                         f"{tuple(out.shape)}")
+    _one_device(x, y, gate, post_weight, post_bias, weight, bias, scale, shift, out)
+    if out is not None:
+        others = [t for t in (x, y) if not (t.data_ptr() == out.data_ptr() and t.is_contiguous())]
+        _refuse_overlap(entry, "out", out, *others, gate, post_weight, post_bias, weight, bias, scale, shift)
+    if head is None and x.numel():
+        x, y = (t if t is None or ok else t.contiguous() for t, ok in zip((x, y), whole))
+        gate, scale, shift = (t if shape is None else t.expand(shape).contiguous()
+                              for t, shape in zip((gate, scale, shift), anew))
+        return residual_norm(x, y, gate, residual_scale, post_norm, post_weight, post_bias, post_eps, norm, weight, bias,
+                             scale, shift, eps, out, quantize)
+    weights = [t if t is None or t.is_contiguous() else t.contiguous() for t in (post_weight, post_bias, weight, bias)]
+    device = x.device
+    if y is None:
+        r = x
+    else:
+        r = torch.empty(x.shape, dtype=x.dtype, device=device) if out is None else out
+    scales = None
+    if quantize:
+        h = torch.empty(x.shape, dtype=E4M3, device=device)
+        scales = _empty_scales(x, x.shape[:-1], _scale_blocks(x.shape[-1]))
+    else:
+        h = torch.empty(x.shape, dtype=x.dtype, device=device)
+    if head is not None:
+        ph = h.data_ptr()
+        block = head + _NORM_POINTERS.pack(
+            x.data_ptr(), _ptr(y) or 0, _ptr(gate) or 0, _ptr(scale) or 0, _ptr(shift) or 0,
+            *(_ptr(t) or 0 for t in weights), 0 if y is None else r.data_ptr(), 0 if quantize else ph,
+            ph if quantize else 0, _ptr(scales) or 0)
+        _call_on(device, "dfs_residual_norm", block)
+    return (r, h, scales) if quantize else (r, h)
+
+
+@dataclass(frozen=True)
+class RotaryAxes:
+    """Rotary positions of several axes: axis a (time, height, width, say) has
+    the next ``sections[a]`` channels of a head of ``head_dim``, pair i of its n
+    channels turns by speed_a * theta_a^(-2i/n) radians a position; channels
+    behind the sections are not rotated. ``theta`` and ``speeds`` are one number
+    for all axes or one for each. ``layout`` "pairs": a pair is two neighbouring
+    channels; "halves": channel p and p + head_dim/2, the sections taken over
+    the pairs."""
+
+    head_dim: int
+    sections: Tuple[int, ...]
+    theta: object = 10000.0
+    layout: str = "pairs"
+    speeds: object = 1.0
+
+    def __post_init__(self):
+        for name in ("theta", "speeds"):
+            v = getattr(self, name)
+            v = tuple(float(x) for x in v) if isinstance(v, (tuple, list)) else (float(v),) * len(self.sections)
+            object.__setattr__(self, name, v)
+        object.__setattr__(self, "sections", tuple(int(n) for n in self.sections))
+        object.__setattr__(self, "head_dim", int(self.head_dim))
+        n = len(self.sections)
+        if not 1 <= n <= 4 or any(c < 0 or c % 2 for c in self.sections) or sum(self.sections) > self.head_dim:
+            raise ValueError(f"RotaryAxes: 1 to 4 sections of even numbers of channels, {self.head_dim} together at "
+                             f"most, got {self.sections}")
+        if self.head_dim < 8 or self.head_dim > 512 or self.head_dim % 8:
+            raise ValueError(f"RotaryAxes: head_dim {self.head_dim} must be a multiple of 8 up to 512")
+        if len(self.theta) != n or len(self.speeds) != n or any(
+                not (0.0 < t < math.inf) for t in self.theta) or any(not math.isfinite(v) for v in self.speeds):
+            raise ValueError(f"RotaryAxes: a positive theta and a finite speed for each axis, got {self.theta} and "
+                             f"{self.speeds}")
+        if self.layout not in ("pairs", "halves"):
+            raise ValueError(f"RotaryAxes: layout must be 'pairs' or 'halves', got {self.layout!r}")
+
+
+@functools.lru_cache(maxsize=1024)
+def _rope_plan(q: Meta, k: Optional[Meta], axes: RotaryAxes, grid: Optional[Tuple[int, ...]],
+               positions: Optional[Meta], weights: Tuple[Optional[Tuple[Shape, torch.dtype]], ...], eps: float):
+    """(argument block up to the pointers, whether q and k are read in place) of an ``axial_rope`` call."""
+    entry = "axial_rope"
+    shape, _, dtype = q
+    if dtype not in HALF or k is not None and k[2] != dtype:
+        raise ValueError(f"{entry}: q and k must both be bf16 or f16, got {dtype}{'' if k is None else f' and {k[2]}'}")
+    if len(shape) != 4 or k is not None and (len(k[0]) != 4 or k[0][:2] != shape[:2] or k[0][3] != shape[3]):
+        raise ValueError(f"{entry}: q must be [B, T, H, D] and k [B, T, G, D], got {tuple(shape)}"
+                         f"{'' if k is None else f' and {tuple(k[0])}'}")
+    B, T, H, D = shape
+    G = 0 if k is None else k[0][2]
+    if D != axes.head_dim:
+        raise ValueError(f"{entry}: heads of {D} channels, axes for {axes.head_dim}")
+    lanes = 1 << max(D // 8 - 1, 0).bit_length()
+    if H == 0 or (k is not None and G == 0) or -(-max(H, G) // (64 // lanes)) > 16:
+        raise ValueError(f"{entry}: {max(H, G)} heads of {D} channels (supported: 1 to {16 * (64 // lanes)})")
+    if not eps >= 0.0:
+        raise ValueError(f"{entry}: eps must not be negative, got {eps}")
+    n = len(axes.sections)
+    if (grid is None) == (positions is None):
+        raise ValueError(f"{entry}: pass a grid or positions")
+    a = _lib.AxialRopeArgs()
+    if grid is not None:
+        if len(grid) != n - 1 or any(not 0 < s < 1 << 30 for s in grid):
+            raise ValueError(f"{entry}: grid must hold the positive sizes of the {n - 1} axes behind the first, got {grid}")
+        for i, s in enumerate(grid):
+            a.size[i + 1] = s
+    else:
+        p_shape, p_stride, p_dtype = positions
+        if p_dtype != torch.int32 or tuple(p_shape) not in ((T, n), (1, T, n), (B, T, n)) or n > 1 and p_stride[-1] != 1:
+            raise ValueError(f"{entry}: positions must be int32 [T, {n}] or [B, T, {n}] for T={T} and B={B} with contiguous "
+                             f"axes, got {p_dtype} {tuple(p_shape)}")
+        a.positions_batch_stride = p_stride[0] if len(p_shape) == 3 and p_shape[0] > 1 else 0
+        a.positions_token_stride = p_stride[-2] if T > 1 else 0
+    a.batch, a.tokens, a.q_heads, a.kv_heads, a.head_dim, a.dtype = B, T, H, G, D, DTYPE_CODE[dtype]
+    a.halves, a.axes, a.eps = int(axes.layout == "halves"), n, eps
+    for i, (c, theta, speed) in enumerate(zip(axes.sections, axes.theta, axes.speeds)):
+        a.pairs[i] = c // 2
+        a.slope[i] = -2.0 / c * math.log2(theta) if c else 0.0
+        a.turn[i] = speed / (2 * math.pi)
+    for side, w, count in (("q", weights[0], H), ("k", weights[1], G)):
+        if w is None:
+            continue
+        if count == 0 or len(w[0]) != 1 or w[0][0] not in (D, count * D) or w[1] not in DTYPE_CODE:
+            raise ValueError(f"{entry}: {side}_weight must be a [{D}] or [{count * D}] vector, got {w[1]} {tuple(w[0])}")
+        setattr(a, f"{side}_weight_dtype", DTYPE_CODE[w[1]])
+        setattr(a, f"{side}_norm_all", int(w[0][0] != D))
+    for side, t, heads in (("q", q, H), ("k", k, G)):
+        if t is None:
+            continue
+        sb, st, sh, _ = _axis_strides(t[0], t[1])
+        setattr(a, f"{side}_batch_stride", sb)
+        setattr(a, f"{side}_token_stride", st)
+        setattr(a, f"{side}_head_stride", sh)
+        setattr(a, f"{side}_out_batch_stride", T * heads * D)
+        setattr(a, f"{side}_out_token_stride", heads * D)
+        setattr(a, f"{side}_out_head_stride", D)
+    in_place = _chunk_rows(q[0], q[1]) and (k is None or _chunk_rows(k[0], k[1]))
+    return bytes(a)[:_pointers(a, "q")], in_place
+
+
+def axial_rope(q: torch.Tensor, k: Optional[torch.Tensor], axes: RotaryAxes, grid: Optional[Sequence[int]] = None,
+               start: Optional[torch.Tensor] = None, positions: Optional[torch.Tensor] = None,
+               q_weight: Optional[torch.Tensor] = None, k_weight: Optional[torch.Tensor] = None, eps: float = 1e-6):
+    """The heads of q [B, T, H, D] and k [B, T, G, D] (None: q alone)
+    RMS-normalised (weight [D]: each by itself; weight [H * D] or [G * D]: all
+    together; None: not at all) and rotated by positions of several ``axes``, in
+    fp32 and rounded once: new q and k as [B, H, T, D] and [B, G, T, D] views of
+    token-major storage, as the attentions read them. For bf16 and f16.
+
+    A token's positions: with ``grid``, the sizes of the axes behind the first
+    (height and width of a video's frames), its place in row-major order, token t
+    of sequence b being number start[b] + t (start: device int32 counts, not
+    negative, read on the device; None: 0); or ``positions``, device int32 [T, A]
+    or [B, T, A], of either sign. No table is read, so a stream has no end but
+    its int32 counts: angles are taken in 64 bits. No backward pass."""
+    entry = "axial_rope"
+    _refuse_grad(entry, q, k, q_weight, k_weight)
+    if not isinstance(axes, RotaryAxes):
+        raise ValueError(f"{entry}: axes must be RotaryAxes, got {type(axes).__name__}")
+    if k is None and k_weight is not None:
+        raise ValueError(f"{entry}: a k_weight without k")
+    head, in_place = _rope_plan(
+        _meta(q), _meta(k), axes, None if grid is None else tuple(int(s) for s in grid), _meta(positions),
+        (None if q_weight is None else (q_weight.shape, q_weight.dtype),
+         None if k_weight is None else (k_weight.shape, k_weight.dtype)), float(eps))
+    B, T, H, D = q.shape
+    if start is not None:
+        if grid is None:
+            raise ValueError(f"{entry}: start goes with a grid")
+        _check_lens(entry, "start", start, B)
+    _one_device(q, k, start, positions, q_weight, k_weight)
+    outs = [None if t is None else t.new_empty_strided((B, t.shape[2], T, D), (T * t.shape[2] * D, D, t.shape[2] * D, 1))
+            for t in (q, k)]
+    if B == 0 or T == 0:
+        return tuple(outs)
+    pq, pk = q.data_ptr(), _ptr(k) or 0
+    if not (in_place and (pq | pk) % 16 == 0):
+        return axial_rope(_in_chunks(q), None if k is None else _in_chunks(k), axes, grid, start, positions, q_weight,
+                          k_weight, eps)
+    q_weight, k_weight = (t if t is None or t.is_contiguous() else t.contiguous() for t in (q_weight, k_weight))
+    block = head + _ROPE_POINTERS.pack(pq, pk, outs[0].data_ptr(), _ptr(outs[1]) or 0, _ptr(q_weight) or 0,
+                                       _ptr(k_weight) or 0, _ptr(start) or 0, _ptr(positions) or 0)
+    _call_on(q.device, "dfs_axial_rope", block)
+    return tuple(outs)

@@ -649,6 +649,67 @@ int64_t dfs_linear_fp8_workspace_size(int64_t rows, int64_t n, int64_t k, int fl
 int dfs_linear_fp8_form(int64_t rows, int64_t n, int64_t k);
 int dfs_linear_fp8(const dfs_linear_fp8_args* args, dfs_stream_t stream);
 
+/*
+ * Between two branches of a transformer block (no reference code):
+ *   r = a x + g P(y)                        rounded to dtype,
+ *   h = (N(r) weight + bias) (1 + s) + t    of the rounded r
+ * x, y, out (r) and h: [rows][channels] bf16 or f16 (row strides in elements).
+ * P: post_norm none, RMS or layer norm over the channels with its optional
+ * weight and bias; N: RMS or layer norm; weights and biases [channels], bf16,
+ * f16 or fp32. gate g, scale s and shift t are optional (NULL), fp32, a vector
+ * of `channels` values for each *_rows consecutive rows (a divisor of rows),
+ * *_stride elements apart. Without y (out NULL) h is of x itself. h8 and
+ * h8_scales instead of h: dfs_quantize_fp8 of the rounded h. Statistics and
+ * steps are fp32, each product and sum rounded in the order written. out may be
+ * x or y. channels up to 8192.
+ */
+enum { DFS_NORM_NONE = 0, DFS_NORM_RMS = 1, DFS_NORM_LAYER = 2 };
+typedef struct dfs_residual_norm_args {
+  int64_t rows, channels, dtype, post_norm, norm;
+  int64_t x_stride, y_stride, out_stride, h_stride, h8_scales_stride;
+  int64_t gate_rows, gate_stride, scale_rows, scale_stride, shift_rows, shift_stride;
+  int64_t post_weight_dtype, post_bias_dtype, weight_dtype, bias_dtype;
+  double residual_scale, eps, post_eps;
+  const void *x, *y;
+  const float *gate, *scale, *shift;
+  const void *post_weight, *post_bias, *weight, *bias;
+  void *out, *h, *h8, *h8_scales;
+} dfs_residual_norm_args;
+int dfs_residual_norm(const dfs_residual_norm_args* args, dfs_stream_t stream);
+
+/*
+ * RMS norm of the heads of q [B][T][q_heads][head_dim] and k (NULL: q alone)
+ * and their rotation by positions of up to four axes (no reference code). Axis
+ * a has the next pairs[a] pairs of a head's channels; its pair i turns by
+ * turn[a] * 2^(slope[a] * i) of a whole turn a position; pairs behind the axes'
+ * are not turned. Pairs are neighbouring channels, or with `halves` channel p
+ * and p + head_dim / 2. A token's positions are positions [B][T][axes] (int32,
+ * strides for batch and token, axes contiguous), or, with NULL, the places of
+ * its number start[b] + t (start int32, not negative, NULL: 0) in a row-major
+ * grid whose axes behind the first have size[a]. Norms as in dfs_qkv_cache
+ * (*_norm_all 0: each head by itself), computed in fp32, rounded once.
+ * head_dim a multiple of 8 up to 512, heads times the next power of two of
+ * head_dim up to 8192, strides multiples of 8, operands on 16 bytes; q_out may be
+ * q, k_out k.
+ */
+typedef struct dfs_axial_rope_args {
+  int64_t batch, tokens, q_heads, kv_heads, head_dim, dtype, halves, axes;
+  int64_t q_weight_dtype, q_norm_all, k_weight_dtype, k_norm_all;
+  int64_t q_batch_stride, q_token_stride, q_head_stride;
+  int64_t k_batch_stride, k_token_stride, k_head_stride;
+  int64_t q_out_batch_stride, q_out_token_stride, q_out_head_stride;
+  int64_t k_out_batch_stride, k_out_token_stride, k_out_head_stride;
+  int64_t positions_batch_stride, positions_token_stride;
+  int64_t pairs[4], size[4];
+  double slope[4], turn[4];
+  double eps;
+  const void *q, *k;
+  void *q_out, *k_out;
+  const void *q_weight, *k_weight;
+  const int32_t *start, *positions;
+} dfs_axial_rope_args;
+int dfs_axial_rope(const dfs_axial_rope_args* args, dfs_stream_t stream);
+
 #ifdef __cplusplus
 }
 #endif

@@ -73,3 +73,95 @@ def linear_fp8(x, w, dtype, bias=None, act=None, gate=None, residual=None):
     lost = 1.13 * 7 * 2.0 ** -13 * (eights(x) @ eights(w).t())  # 1.13: the activations' slopes
     err = err + (lost if gate is None else lost * gate.double().abs())
     return y, err + half_step(dtype) * (y.abs() + err) + 2.0 ** -25
+
+
+def _normalise(x, kind, weight, bias, eps):
+    """(value, bound) of a norm of x (64 bits, exact): a sum of C terms in fp32 is
+    off by C F of their magnitudes, so the mean by C F of the mean magnitude and
+    the mean square by relative 2 C F (its terms by 2 F more and by what the
+    mean is off); root, quotient and the steps behind them by F each."""
+    C = x.shape[-1]
+    mean = x.mean(-1, keepdim=True) if kind == "layer" else torch.zeros_like(x[..., :1])
+    off = (C + 2) * F * x.abs().mean(-1, keepdim=True) if kind == "layer" else 0.0
+    d = x - mean
+    var = d.square().mean(-1, keepdim=True)
+    var_off = (C + 4) * F * var + 2 * off * d.abs().mean(-1, keepdim=True) + off * off
+    rstd = 1 / torch.sqrt(var + eps)
+    y = d * rstd
+    # relative: half of the variance's error (2 of it near the end of its range), and a few steps
+    rel = torch.clamp(2 * var_off * rstd * rstd, max=1e6) + 8 * F
+    err = y.abs() * rel + (off + F * d.abs()) * rstd
+    if weight is not None:
+        y, err = y * weight.double(), (err + F * y.abs()) * weight.double().abs()
+    if bias is not None:
+        y = y + bias.double()
+        err = err + F * (y.abs() + bias.double().abs())
+    return y, err
+
+
+def residual(x, y, gate=None, residual_scale=1.0, post_norm=None, post_weight=None, post_bias=None, eps=1e-6):
+    """(r, bound): y, its gate and the sum with the scaled x in fp32, one rounding."""
+    a = float(torch.tensor(residual_scale, dtype=torch.float32))
+    yd, err = y.double(), torch.zeros(y.shape, dtype=torch.float64)
+    if post_norm is not None:
+        yd, err = _normalise(yd, post_norm, post_weight, post_bias, eps)
+    if gate is not None:
+        yd, err = yd * gate.double(), (err + F * yd.abs()) * gate.double().abs()
+    xd = x.double() * a
+    r = xd + yd
+    err = err + F * (xd.abs() + 2 * r.abs() + yd.abs())
+    return r, err + half_step(x.dtype) * (r.abs() + err) + 2.0 ** -25
+
+
+def norm_of(r, norm="layer", weight=None, bias=None, scale=None, shift=None, eps=1e-6):
+    """(h, bound) of r as it is stored."""
+    h, err = _normalise(r.double(), norm, weight, bias, eps)
+    if scale is not None:
+        s = 1 + scale.double()
+        h, err = h * s, (err + 2 * F * h.abs()) * s.abs() + 2 * F * h.abs()
+    if shift is not None:
+        h = h + shift.double()
+        err = err + F * (h.abs() + shift.double().abs())
+    return h, err + half_step(r.dtype) * (h.abs() + err) + 2.0 ** -25
+
+
+def grid_positions(start, tokens, grid):
+    """[B, T, A] places of tokens start[b] + t in a row-major grid."""
+    at = torch.tensor(start)[:, None] + torch.arange(tokens)[None]
+    places = []
+    for n in reversed(grid):
+        places.append(at % n)
+        at = at // n
+    return torch.stack([at, *reversed(places)], -1)
+
+
+def axial_rope(x, positions, sections, theta, layout, weight=None, eps=1e-6, speeds=None):
+    """([B, H, T, D] value, bound) of x [B, T, H, D] at positions [B, T, A]. The
+    norm is off as in operator_refs.qkv_cache; an angle in 64 bits by relative
+    2^-50, and what is left of it behind whole turns, in fp32 turns of at most a
+    half, by 2^-26 turns = 2^-23.3 radians, its sine and cosine by 2 F more; the
+    products and their sum by 3 F of the magnitudes."""
+    B, T, H, D = x.shape
+    y = x.double()
+    if weight is not None:
+        flat = y if weight.numel() == D else y.flatten(2)
+        y = (flat / torch.sqrt(flat.square().mean(-1, keepdim=True) + eps) * weight.double()).reshape(x.shape)
+    C = 0 if weight is None else weight.numel()
+    angle, far = torch.zeros(B, T, D // 2, dtype=torch.float64), torch.zeros(B, T, D // 2, dtype=torch.float64)
+    at = 0
+    for a, n in enumerate(sections):
+        f = (1.0 if speeds is None else speeds[a]) * theta[a] ** (-torch.arange(0, n, 2, dtype=torch.float64) / n) \
+            if n else torch.zeros(0, dtype=torch.float64)
+        angle[..., at:at + n // 2] = positions[..., a].double()[..., None] * f
+        at += n // 2
+    far = angle.abs() * 2.0 ** -50
+    c, s = torch.cos(angle)[:, :, None], torch.sin(angle)[:, :, None]
+    i0, i1 = (slice(0, D // 2), slice(D // 2, D)) if layout == "halves" else (slice(0, D, 2), slice(1, D, 2))
+    a, b = y[..., i0], y[..., i1]
+    z, mag = torch.empty_like(y), torch.empty_like(y)
+    z[..., i0], z[..., i1] = a * c - b * s, b * c + a * s
+    big = a.abs() + b.abs()
+    turn_off = far[:, :, None] + 2.0 ** -23 + 2 * F
+    err = big * ((C + 16) * F + turn_off)
+    mag[..., i0] = mag[..., i1] = err
+    return (z.transpose(1, 2), (mag + half_step(x.dtype) * (z.abs() + mag) + 2.0 ** -25).transpose(1, 2))
