@@ -23,9 +23,14 @@ struct Fp8Params : Epilogue {
   int64_t ldx, ldw, ldxs, ldws;
   int K, kb;
   // The channels of a tile are cut into `splits` parts of `depth` (a multiple of
-  // 256); a part's sums go to part [split][M][ceil(N / 8) * 8] in fp32.
-  int splits, depth;
+  // 256); a part's sums go to part [split][M][ceil(N / 8) * 8] in fp32. Of the
+  // 256 x 256 tiles the first `whole` are not cut, the others' sums go to part
+  // [split][tile][256][256].
+  int splits, depth, whole;
   float* part;
+  // 256 x 256 tiles: the result as codes and scales [ceil(N / 128)][M], or NULL.
+  uint8_t *out8, *out8_scales;
+  int64_t ldo8, ldos;
 };
 
 typedef int i32x4 __attribute__((ext_vector_type(4)));
@@ -324,6 +329,314 @@ __global__ void __launch_bounds__(256, 2) fp8_tile_kernel(Fp8Params p) {
   });
 }
 
+// Eight outputs n.. of row m, finished and rounded, as they are stored.
+template <bool F16, int ACT>
+__device__ __forceinline__ uint4 finished8(const Epilogue& p, int m, int n, const float* z, const float* bias,
+                                           const float* gate) {
+  float y[8];
+#pragma unroll
+  for (int i = 0; i < 8; ++i) {
+    y[i] = activate<ACT>(z[i] + bias[i]);
+    if (p.gate) y[i] *= gate[i];
+    if (p.residual && m < p.M && n + i < p.N) y[i] += Half<F16>::to_f32(p.residual[m * p.ldr + n + i]);
+    if (n + i >= p.N) y[i] = 0.f;
+  }
+  return make_uint4(Half<F16>::pack(y[0], y[1]), Half<F16>::pack(y[2], y[3]), Half<F16>::pack(y[4], y[5]),
+                    Half<F16>::pack(y[6], y[7]));
+}
+template <bool F16>
+__device__ __forceinline__ float magnitude8(const uint4& v) {
+  float top = 0.f;
+#pragma unroll
+  for (int i = 0; i < 8; ++i) top = fmaxf(top, finite_magnitude(Half<F16>::to_f32(u16_at(v, i))));
+  return top;
+}
+// Codes of eight rounded outputs n.. of row m under a scale.
+template <bool F16>
+__device__ __forceinline__ void store_codes8(const Fp8Params& p, int m, int n, const uint4& v, uint32_t scale) {
+  if (m >= p.M || n >= p.N) return;
+  float f[8];
+#pragma unroll
+  for (int i = 0; i < 8; ++i) f[i] = Half<F16>::to_f32(u16_at(v, i));
+  const uint2 codes = to_codes8(f, inverse_scale(scale));
+  uint8_t* const dst = p.out8 + m * p.ldo8 + n;
+  if (n + 8 <= p.N) {
+    __builtin_memcpy(dst, &codes, 8);
+  } else {
+    uint8_t b[8];
+    __builtin_memcpy(b, &codes, 8);
+#pragma unroll
+    for (int i = 0; i < 8; ++i)
+      if (n + i < p.N) dst[i] = b[i];
+  }
+}
+
+// 256 x 256 outputs a workgroup, four waves of 128 x 128, 128 channels a step, in
+// the order of the 16-bit products' large tiles: each operand's slice of a step
+// is two halves of 128 rows, a step is four phases of one quadrant each, eight
+// products of K = 64:
+//   (A0, B0) (A1, B0) (A1, B1) (A0, B1)
+// A phase reads one half into registers for the next (A1, B1, then the next
+// step's B0 and A0: the registers just left), and loads a half read in the pair
+// of phases before, two steps on; one barrier a pair says both that the halves to
+// be read have landed and that those to be loaded were read by all.
+//
+// Row l of the 32 of tile 2 h + i of a wave (half h) is its row 4 l + 2 h + i of
+// 128, of x as of w: so the scales of a lane's four rows are four neighbouring
+// bytes, one load a step and operand, of which the matrix instruction picks its
+// tile's, and a lane ends with 16 consecutive outputs, tile by tile.
+template <bool F16, int ACT>
+__global__ void __launch_bounds__(256, 1) fp8_big_kernel(Fp8Params p) {
+  __shared__ __attribute__((aligned(16))) uint8_t a00[128 * 128], a01[128 * 128], a10[128 * 128], a11[128 * 128];
+  __shared__ __attribute__((aligned(16))) uint8_t b00[128 * 128], b01[128 * 128], b10[128 * 128], b11[128 * 128];
+  __shared__ __attribute__((aligned(16))) float stage[4 * 2048];
+  const int lane = threadIdx.x & 63, w = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  const int l32 = lane & 31, hl = lane >> 5;
+  const int mt = (p.M + 255) / 256, nt = (p.N + 255) / 256, cut = mt * nt - p.whole;
+  const bool in_parts = static_cast<int>(blockIdx.x) >= p.whole;
+  const int split = in_parts ? (static_cast<int>(blockIdx.x) - p.whole) / cut : 0, from = split * p.depth;
+  const int K = in_parts ? min(p.K - from, p.depth) : p.K, id = blockIdx.x - split * cut;
+  int tm, tn;
+  tile_of(id, mt, nt, tm, tn);
+  const int n0 = tn * 256, m0 = tm * 256;
+  // Rows past the matrix lie past the buffers' records and come as zeros. The
+  // whole offset is the lane's: the check against the records subtracts a scalar
+  // part from them, which could be more than they are.
+  auto slice = [&](const uint8_t* base, int64_t ld, int at, int rows) {
+    const int64_t records = (min(rows - at, 256) - 1) * ld + p.K - from;
+    return make_rsrc(base + at * ld + from, static_cast<uint32_t>(records));
+  };
+  const auto wrs = slice(p.w, p.ldw, n0, p.N), xrs = slice(p.x, p.ldx, m0, p.M);
+  // This lane's chunk of step 0 in load j of half h is row r8 * 4 + 2 h + (j & 1)
+  // of wave row j >> 1: the lane's own part of its byte offset is r8 * 4 rows.
+  const int r8 = w * 8 + (lane >> 3), c8 = (lane & 7) ^ (r8 >> 1 & 7);
+  uint32_t wv = static_cast<uint32_t>(r8 * 4) * static_cast<uint32_t>(p.ldw) + c8 * 16;
+  uint32_t xv = static_cast<uint32_t>(r8 * 4) * static_cast<uint32_t>(p.ldx) + c8 * 16;
+  const int ldw = static_cast<int>(p.ldw), ldx = static_cast<int>(p.ldx);
+  const int steps = (K + 255) >> 8 << 1;  // an even number: the last may be all zeros
+  // The last steps' chunks past K (tail) come as zeros, without a memory access.
+  auto load = [&](auto tail, __amdgpu_buffer_rsrc_t rs, uint32_t v, int ld, int t, int h, uint8_t* buf) {
+    if (tail.value && c8 * 16 >= K - t * 128) v = kOutside;
+#pragma unroll
+    for (int j = 0; j < 4; ++j)
+      load_lds16(rs, buf + (j * 4 + w) * 1024, v + (t * 128 + ((j >> 1) * 128 + 2 * h + (j & 1)) * ld), 0);
+  };
+  auto load_w = [&](auto tail, int t, int h, uint8_t* buf) { load(tail, wrs, wv, ldw, t, h, buf); };
+  auto load_x = [&](auto tail, int t, int h, uint8_t* buf) { load(tail, xrs, xv, ldx, t, h, buf); };
+  const int wn = w & 1, wm = w >> 1;
+  // Scales of this lane's rows, four a load (rows past the matrix: the last four).
+  const uint32_t wsv = min(n0 + wn * 128 + l32 * 4, (p.N - 1) & ~3), xsv = min(m0 + wm * 128 + l32 * 4, (p.M - 1) & ~3);
+  auto load_scales = [&](int t, uint32_t& sw, uint32_t& sx) {
+    const int b = min((from >> 7) + t, p.kb - 1);
+    sw = *reinterpret_cast<const uint32_t*>(p.ws + b * p.ldws + wsv);
+    sx = *reinterpret_cast<const uint32_t*>(p.xs + b * p.ldxs + xsv);
+  };
+  const int arow = (wn * 64 + l32) * 128, brow = (wm * 64 + l32) * 128, f = l32 >> 1 & 7;
+  f32x16 acc[4][4];
+#pragma unroll
+  for (int i = 0; i < 4; ++i)
+#pragma unroll
+    for (int j = 0; j < 4; ++j) acc[i][j] = f32x16{};
+  typedef i32x8 Frag[4];  // [64 channels][tile]
+  auto read = [&](const uint8_t* row, Frag& v) {
+#pragma unroll
+    for (int u = 0; u < 2; ++u)
+#pragma unroll
+      for (int i = 0; i < 2; ++i) {
+        const int c = (4 * u + hl) ^ f;
+        v[2 * u + i] = join(chunk_at(row + i * 4096 + c * 16), chunk_at(row + i * 4096 + (c ^ 2) * 16));
+      }
+  };
+  // One quadrant: halves HA of w and HB of x.
+  auto quadrant = [&](auto ha, auto hb, const Frag& a, const Frag& b, uint32_t sw, uint32_t sx) {
+    constexpr int HA = decltype(ha)::value, HB = decltype(hb)::value;
+#pragma unroll
+    for (int u = 0; u < 2; ++u) {
+      f32x16 &c00 = acc[2 * HA][2 * HB], &c10 = acc[2 * HA + 1][2 * HB];
+      f32x16 &c01 = acc[2 * HA][2 * HB + 1], &c11 = acc[2 * HA + 1][2 * HB + 1];
+      const i32x8 &a0 = a[2 * u], &a1 = a[2 * u + 1], &b0 = b[2 * u], &b1 = b[2 * u + 1];
+      const int s = static_cast<int>(sw), x = static_cast<int>(sx);
+      c00 = __builtin_amdgcn_mfma_scale_f32_32x32x64_f8f6f4(a0, b0, c00, 0, 0, 2 * HA, s, 2 * HB, x);
+      c10 = __builtin_amdgcn_mfma_scale_f32_32x32x64_f8f6f4(a1, b0, c10, 0, 0, 2 * HA + 1, s, 2 * HB, x);
+      c01 = __builtin_amdgcn_mfma_scale_f32_32x32x64_f8f6f4(a0, b1, c01, 0, 0, 2 * HA, s, 2 * HB + 1, x);
+      c11 = __builtin_amdgcn_mfma_scale_f32_32x32x64_f8f6f4(a1, b1, c11, 0, 0, 2 * HA + 1, s, 2 * HB + 1, x);
+    }
+    constexpr int kMfma = 0x008, kDsRead = 0x100, kVmem = 0x020;
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      __builtin_amdgcn_sched_group_barrier(kMfma, 1, 0);
+      __builtin_amdgcn_sched_group_barrier(kDsRead, 2, 0);
+    }
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      __builtin_amdgcn_sched_group_barrier(kMfma, 1, 0);
+      __builtin_amdgcn_sched_group_barrier(kVmem, 1, 0);
+    }
+    __builtin_amdgcn_sched_barrier(0);
+  };
+  auto landed = [&] {  // the halves loaded three pairs of phases ago; two pairs' loads, and scales, are behind them
+    wait_vmcnt<16>();
+    block_barrier();
+  };
+  Frag fa0, fa1, fb0, fb1;
+  uint32_t sw0, sx0, sw1, sx1;
+  // One step with its A0 in c0, the other A registers c1; ends with the next
+  // step's A0 in c1. *c: this step's buffers, *n: the next step's.
+  constexpr std::true_type may_end{};
+  constexpr std::false_type whole{};
+  constexpr std::integral_constant<int, 0> h0{};
+  constexpr std::integral_constant<int, 1> h1{};
+  auto step = [&](auto tail, int t, Frag& c0, Frag& c1, uint32_t& sw, uint32_t& sx, uint8_t* a0c, uint8_t* a1c,
+                  uint8_t* b0c, uint8_t* b1c, uint8_t* a0n, uint8_t* b0n) {
+    landed();
+    read(a1c + arow, c1);
+    load_x(tail, t + 2, 0, b0c);
+    quadrant(h0, h0, c0, fb0, sw, sx);
+    read(b1c + brow, fb1);
+    load_w(tail, t + 2, 0, a0c);
+    quadrant(h1, h0, c1, fb0, sw, sx);
+    landed();
+    read(b0n + brow, fb0);
+    load_w(tail, t + 2, 1, a1c);
+    quadrant(h1, h1, c1, fb1, sw, sx);
+    read(a0n + arow, c1);
+    load_x(tail, t + 2, 1, b1c);
+    quadrant(h0, h1, c0, fb1, sw, sx);
+    load_scales(t + 2, sw, sx);
+  };
+  load_scales(0, sw0, sx0);
+  load_scales(1, sw1, sx1);
+  load_x(may_end, 0, 0, b00);
+  load_w(may_end, 0, 0, a00);
+  load_w(may_end, 0, 1, a10);
+  load_x(may_end, 0, 1, b10);
+  load_x(may_end, 1, 0, b01);
+  load_w(may_end, 1, 0, a01);
+  load_w(may_end, 1, 1, a11);
+  load_x(may_end, 1, 1, b11);
+  wait_vmcnt<24>();
+  block_barrier();
+  read(b00 + brow, fb0);
+  read(a00 + arow, fa0);
+  int t = 0;
+  for (; (t + 4) * 128 <= K; t += 2) {  // nothing past K is loaded
+    step(whole, t, fa0, fa1, sw0, sx0, a00, a10, b00, b10, a01, b01);
+    step(whole, t + 1, fa1, fa0, sw1, sx1, a01, a11, b01, b11, a00, b00);
+  }
+#pragma unroll 1
+  for (; t < steps; t += 2) {
+    step(may_end, t, fa0, fa1, sw0, sx0, a00, a10, b00, b10, a01, b01);
+    step(may_end, t + 1, fa1, fa0, sw1, sx1, a01, a11, b01, b11, a00, b00);
+  }
+  wait_vmcnt_0();  // the trailing loads have landed before the workgroup's LDS is released
+  // The sums stay in the accumulation registers to here: otherwise the compiler
+  // moves some of them between the files in every step.
+#pragma unroll
+  for (int i = 0; i < 4; ++i)
+#pragma unroll
+    for (int j = 0; j < 4; ++j) asm volatile("" : "+a"(acc[i][j]));
+  // The sums go through LDS, 32 rows x 64 outputs at a time, in the wave's own
+  // part of it: whole rows of 128 bytes leave (and come, for the residual). Row r
+  // of tile j is 4 r + j of the wave's 128.
+  float* const st = stage + w * 2048;
+  const bool inside = m0 + 256 <= p.M && n0 + 256 <= p.N;
+  float* const part = p.part + static_cast<int64_t>(split * cut + id - p.whole) * 65536;  // of a tile in parts
+  const int nw = n0 + wn * 128 + (lane & 7) * 8, mw = m0 + wm * 128 + (lane >> 3) * 4;
+  float bias[2][8], gate[2][8];
+#pragma unroll
+  for (int gp = 0; gp < 2; ++gp) load_columns8(p, nw + gp * 64, bias[gp], gate[gp]);
+  auto to_stage = [&](auto tile, auto half) {  // outputs gp * 64 .. + 63 of tile j's rows
+    constexpr int j = decltype(tile)::value, gp = decltype(half)::value;
+#pragma unroll
+    for (int g = 0; g < 2; ++g)
+#pragma unroll
+      for (int e = 0; e < 4; ++e) {  // outputs g * 32 + hl * 16 + 4 e .. + 3 of row l32
+        constexpr int kFirst = gp * 8;
+        const int r = kFirst + g * 4 + e;
+        *reinterpret_cast<float4*>(st + l32 * 64 + ((g * 8 + hl * 4 + e) ^ (l32 & 15)) * 4) =
+            make_float4(acc[0][j][r], acc[1][j][r], acc[2][j][r], acc[3][j][r]);
+      }
+  };
+  auto from_stage = [&](int i, float* z) {  // outputs (lane & 7) * 8 .. + 7 of row i * 8 + (lane >> 3)
+    const int r = i * 8 + (lane >> 3), c = (lane & 7) * 2;
+    const float4 lo = *reinterpret_cast<const float4*>(st + r * 64 + (c ^ (r & 15)) * 4);
+    const float4 hi = *reinterpret_cast<const float4*>(st + r * 64 + ((c + 1) ^ (r & 15)) * 4);
+    z[0] = lo.x; z[1] = lo.y; z[2] = lo.z; z[3] = lo.w;
+    z[4] = hi.x; z[5] = hi.y; z[6] = hi.z; z[7] = hi.w;
+  };
+  constexpr std::integral_constant<int, 2> h2{};
+  constexpr std::integral_constant<int, 3> h3{};
+  auto each_tile = [&](auto&& f) {
+    f(h0);
+    f(h1);
+    f(h2);
+    f(h3);
+  };
+  auto each_half = [&](auto&& f) {
+    f(h0);
+    f(h1);
+  };
+  if (in_parts) {
+    each_tile([&](auto j) {
+      each_half([&](auto gp) {
+        to_stage(j, gp);
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+          float z[8];
+          from_stage(i, z);
+          float* const at = part + (mw + i * 32 + decltype(j)::value - m0) * 256 + nw + decltype(gp)::value * 64 - n0;
+          *reinterpret_cast<float4*>(at) = make_float4(z[0], z[1], z[2], z[3]);
+          *reinterpret_cast<float4*>(at + 4) = make_float4(z[4], z[5], z[6], z[7]);
+        }
+      });
+    });
+  } else if (p.out8) {  // a scale's 128 outputs are the wave's: eight lanes, twice
+    each_tile([&](auto j) {
+      uint4 y[2][4];
+      each_half([&](auto gp) {
+        constexpr int GP = decltype(gp)::value;
+        to_stage(j, gp);
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+          float z[8];
+          from_stage(i, z);
+          y[GP][i] = finished8<F16, ACT>(p, mw + i * 32 + decltype(j)::value, nw + GP * 64, z, bias[GP], gate[GP]);
+        }
+      });
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        const int m = mw + i * 32 + decltype(j)::value;
+        const uint32_t scale = block_scale(max8(fmaxf(magnitude8<F16>(y[0][i]), magnitude8<F16>(y[1][i]))));
+        store_codes8<F16>(p, m, nw, y[0][i], scale);
+        store_codes8<F16>(p, m, nw + 64, y[1][i], scale);
+        if ((lane & 7) == 0 && m < p.M && nw < p.N) p.out8_scales[(nw >> 7) * p.ldos + m] = static_cast<uint8_t>(scale);
+      }
+    });
+  } else {
+    each_tile([&](auto j) {
+      each_half([&](auto gp) {
+        constexpr int GP = decltype(gp)::value;
+        to_stage(j, gp);
+        if (inside) {
+#pragma unroll
+          for (int i = 0; i < 4; ++i) {
+            float z[8];
+            from_stage(i, z);
+            finish8_wide<F16, ACT>(p, mw + i * 32 + decltype(j)::value, nw + GP * 64, z, bias[GP], gate[GP]);
+          }
+        } else {
+#pragma unroll 1
+          for (int i = 0; i < 4; ++i) {
+            float z[8];
+            from_stage(i, z);
+            finish8_edge<F16, ACT>(p, mw + i * 32 + decltype(j)::value, nw + GP * 64, z, bias[GP], gate[GP]);
+          }
+        }
+      });
+    });
+  }
+}
+
 // Joins the parts of a cut product, in their order, and finishes: a thread has
 // eight outputs.
 template <bool F16>
@@ -343,6 +656,40 @@ __global__ void __launch_bounds__(256) fp8_join_kernel(Fp8Params p) {
   float bias[8], gate[8];
   load_columns8(p, n, bias, gate);
   with_activation(p.act, [&](auto act) { finish8<F16, decltype(act)::value>(p, m, n, z, bias, gate); });
+}
+
+// The same for the 256 x 256 tiles in parts, 32 workgroups a tile.
+template <bool F16>
+__global__ void __launch_bounds__(256) fp8_join_big_kernel(Fp8Params p) {
+  const int mt = (p.M + 255) / 256, nt = (p.N + 255) / 256, cut = mt * nt - p.whole;
+  const int tile = blockIdx.x >> 5, row = (blockIdx.x & 31) * 8 + (threadIdx.x >> 5), col = (threadIdx.x & 31) * 8;
+  int tm, tn;
+  tile_of(p.whole + tile, mt, nt, tm, tn);
+  const int m = tm * 256 + row, n = tn * 256 + col;
+  float z[8] = {};
+  for (int i = 0; i < p.splits; ++i) {
+    const float* const src = p.part + static_cast<int64_t>(i * cut + tile) * 65536 + row * 256 + col;
+    const float4 a = *reinterpret_cast<const float4*>(src), b = *reinterpret_cast<const float4*>(src + 4);
+    z[0] += a.x; z[1] += a.y; z[2] += a.z; z[3] += a.w;
+    z[4] += b.x; z[5] += b.y; z[6] += b.z; z[7] += b.w;
+  }
+  float bias[8], gate[8];
+  load_columns8(p, n, bias, gate);
+  with_activation(p.act, [&](auto act) {
+    constexpr int ACT = decltype(act)::value;
+    if (!p.out8) return finish8<F16, ACT>(p, m, n, z, bias, gate);
+    const uint4 y = finished8<F16, ACT>(p, m, n, z, bias, gate);  // a scale's outputs are sixteen lanes'
+    const uint32_t scale = block_scale(max16(magnitude8<F16>(y)));
+    store_codes8<F16>(p, m, n, y, scale);
+    if ((threadIdx.x & 15) == 0 && m < p.M && n < p.N) p.out8_scales[(n >> 7) * p.ldos + m] = static_cast<uint8_t>(scale);
+  });
+}
+
+// Scale bytes [blocks][rows] at any stride into ones of stride `wide`, a multiple
+// of 4, zeros behind the rows.
+__global__ void __launch_bounds__(256) pad_scales_kernel(const uint8_t* src, int64_t ld, int rows, int wide, uint8_t* dst) {
+  const int r = blockIdx.x * 256 + threadIdx.x;
+  if (r < wide) dst[static_cast<int64_t>(blockIdx.y) * wide + r] = r < rows ? src[blockIdx.y * ld + r] : 0;
 }
 
 // Rows of k codes at any address and stride into rows of `wide` on 16-byte
@@ -405,14 +752,17 @@ enum Form {
   kTile64 = DFS_LINEAR_64,
   kTile64x128 = DFS_LINEAR_64X128,
   kTile128Deep = DFS_LINEAR_128_DEEP,
-  kTile128 = DFS_LINEAR_128
+  kTile128 = DFS_LINEAR_128,
+  kTile256 = DFS_LINEAR_256
 };
 struct Cut {
   Form form;
   int splits, depth;
+  int64_t whole;  // 256 x 256 tiles that are not cut
 };
+int64_t big_tiles(int64_t rows, int64_t n) { return (rows + 255) / 256 * ((n + 255) / 256); }
 Cut cut_of(int64_t rows, int64_t n, int64_t k) {
-  if (rows <= 16) return Cut{kFew, 1, 0};
+  if (rows <= 16) return Cut{kFew, 1, 0, 0};
   // The tiles and parts with the least time by what each takes on an idle CU and
   // beside others, a step of 128 channels of a workgroup in us, and by writing
   // and joining the parts' sums at 3 TB/s behind 5 us.
@@ -421,11 +771,12 @@ Cut cut_of(int64_t rows, int64_t n, int64_t k) {
     int m, n, most;  // most: parts
     bool single;     // one workgroup a CU
     double alone, beside;
-  } kinds[4] = {{kTile64, 64, 64, 8, false, 0.26, 0.25},
+  } kinds[5] = {{kTile64, 64, 64, 8, false, 0.26, 0.25},
                 {kTile64x128, 128, 64, 4, false, 0.36, 0.375},
                 {kTile128Deep, 128, 128, 2, true, 0.55, 0.55},
-                {kTile128, 128, 128, 4, false, 0.72, 0.57}};
-  Cut best{kTile64, 1, 0};
+                {kTile128, 128, 128, 4, false, 0.72, 0.57},
+                {kTile256, 256, 256, 1, true, 1.15, 1.4}};
+  Cut best{kTile64, 1, 0, 0};
   double least = 1e30;
   for (const auto& f : kinds)
     for (int s = 1; s <= f.most; s *= 2) {
@@ -438,28 +789,51 @@ Cut cut_of(int64_t rows, int64_t n, int64_t k) {
       if (parts > 1) us += 5.0 + 8e-6 / 3.0 * static_cast<double>(parts * rows * n);
       if (us < least) {
         least = us;
-        best = Cut{f.form, static_cast<int>(parts), static_cast<int>(depth)};
+        best = Cut{f.form, static_cast<int>(parts), static_cast<int>(depth), 0};
       }
     }
+  // The 256 x 256 tiles behind the last full round of 256 in parts, which
+  // together fill it.
+  const int64_t tiles = big_tiles(rows, n), whole = tiles / 256 * 256, rest = tiles - whole, steps = (k + 127) / 128;
+  best.whole = best.form == kTile256 ? tiles : 0;
+  for (int64_t s = 2; rest > 0 && rest * s <= 256; ++s) {
+    const int64_t depth = ((k + s - 1) / s + 255) / 256 * 256, parts = (k + depth - 1) / depth;
+    if (depth < 1024) break;
+    const double us = 1.4 * static_cast<double>(steps * (whole / 256) + depth / 128) + 10.0 +
+                      8e-6 / 3.0 * static_cast<double>(parts * rest * 65536);
+    if (parts == s && us < least) {
+      least = us;
+      best = Cut{kTile256, static_cast<int>(parts), static_cast<int>(depth), whole};
+    }
+  }
   return best;
 }
 
-// The workspace: the parts' sums, x's codes and scales (where x comes in 16
-// bits, or its codes off 16-byte rows), w's codes (off 16-byte rows), and the
-// rounded result where it is left as codes. Each begins on 16 bytes.
 int64_t up16(int64_t n) { return (n + 15) / 16 * 16; }
+int64_t up4(int64_t n) { return (n + 3) / 4 * 4; }
+int64_t part_bytes(const Cut& c, int64_t rows, int64_t n) {
+  if (c.splits <= 1) return 0;
+  return c.form == kTile256 ? c.splits * (big_tiles(rows, n) - c.whole) * 65536 * 4
+                            : c.splits * rows * ((n + 7) / 8 * 8) * 4;
+}
+// The workspace: the parts' sums, x's codes (where x comes in 16 bits, or its
+// codes off 16-byte rows) and scales (where x comes in 16 bits, or for the
+// 256 x 256 tiles, which read four scales at once, off 4-byte boundaries), w's
+// the same, and the rounded result where it is left as codes but the form does
+// not make them. Each begins on 16 bytes.
 struct Workspace {
-  int64_t part, x, xs, w, y, total;  // offsets
+  int64_t part, x, xs, w, ws, y, total;  // offsets
 };
 Workspace workspace_of(const Cut& c, int64_t rows, int64_t n, int64_t k, int flags) {
   const int64_t kb = (k + kScaleBlock - 1) / kScaleBlock;
-  const bool codes = flags & DFS_FP8_X_CODES;
+  const bool codes = flags & DFS_FP8_X_CODES, big = c.form == kTile256;
   Workspace s{};
-  s.x = s.part + (c.splits > 1 ? c.splits * rows * ((n + 7) / 8 * 8) * 4 : 0);
+  s.x = s.part + part_bytes(c, rows, n);
   s.xs = s.x + (codes && (flags & DFS_FP8_X_ALIGNED) ? 0 : rows * up16(k));
-  s.w = s.xs + (codes ? 0 : up16(rows * kb));
-  s.y = s.w + (flags & DFS_FP8_W_ALIGNED ? 0 : n * up16(k));
-  s.total = s.y + (flags & DFS_FP8_OUT_CODES ? up16(rows * n * 2) : 0);
+  s.w = s.xs + (!codes || (big && !(flags & DFS_FP8_XS_ALIGNED)) ? up16(up4(rows) * kb) : 0);
+  s.ws = s.w + (flags & DFS_FP8_W_ALIGNED ? 0 : n * up16(k));
+  s.y = s.ws + (big && !(flags & DFS_FP8_WS_ALIGNED) ? up16(up4(n) * kb) : 0);
+  s.total = s.y + (flags & DFS_FP8_OUT_CODES && !big ? up16(rows * n * 2) : 0);
   return s;
 }
 
@@ -524,12 +898,17 @@ extern "C" int dfs_linear_fp8(const dfs_linear_fp8_args* a, dfs_stream_t stream)
   int flags = (codes ? DFS_FP8_X_CODES : 0) | (out8 ? DFS_FP8_OUT_CODES : 0);
   if (codes && in_place(a->x, a->x_stride)) flags |= DFS_FP8_X_ALIGNED;
   if (in_place(a->w, a->w_stride)) flags |= DFS_FP8_W_ALIGNED;
+  auto in_fours = [&](const void* q, int64_t count, int64_t stride) {
+    return addr(q) % 4 == 0 && count % 4 == 0 && stride % 4 == 0;
+  };
+  if (codes && in_fours(a->x_scales, rows, a->x_scales_stride)) flags |= DFS_FP8_XS_ALIGNED;
+  if (in_fours(a->w_scales, n, a->w_scales_stride)) flags |= DFS_FP8_WS_ALIGNED;
   const Cut cut = cut_of(rows, n, k);
   const Workspace at = workspace_of(cut, rows, n, k, flags);
   DFS_REQUIRE(at.total == 0 || (a->workspace != nullptr && a->workspace_bytes >= at.total && addr(a->workspace) % 16 == 0),
               "%s: a 16-byte aligned workspace of %lld bytes is needed", name, (long long)at.total);
   // A launch holds fewer than 2^32 threads.
-  DFS_REQUIRE(((rows + 63) / 64) * ((n + 63) / 64) * cut.splits < (1 << 24) && (cut.form != kFew || n < (1 << 27)) &&
+  DFS_REQUIRE(((rows + 63) / 64) * ((n + 63) / 64) * cut.splits < (1 << 24) && kb < 65536 && (cut.form != kFew || n < (1 << 27)) &&
                   rows * kb < (1 << 28) && (!out8 || rows * nb < (1 << 28)),
               "%s: too many outputs", name);
   char* const ws = static_cast<char*>(a->workspace);
@@ -558,8 +937,8 @@ extern "C" int dfs_linear_fp8(const dfs_linear_fp8_args* a, dfs_stream_t stream)
   if (!codes) {
     uint8_t *const xq = reinterpret_cast<uint8_t*>(ws + at.x), *const xsq = reinterpret_cast<uint8_t*>(ws + at.xs);
     p.ldx = wide;
-    p.ldxs = rows;
-    launch_quantize(static_cast<const uint16_t*>(a->x), rows, k, a->x_stride, f16, xq, wide, wide, xsq, rows, st);
+    p.ldxs = up4(rows);
+    launch_quantize(static_cast<const uint16_t*>(a->x), rows, k, a->x_stride, f16, xq, wide, wide, xsq, p.ldxs, st);
     p.x = xq;
     p.xs = xsq;
   } else if (!(flags & DFS_FP8_X_ALIGNED)) {
@@ -569,6 +948,21 @@ extern "C" int dfs_linear_fp8(const dfs_linear_fp8_args* a, dfs_stream_t stream)
   if (!(flags & DFS_FP8_W_ALIGNED)) {
     p.w = lay_out(p.w, p.ldw, n, at.w);
     p.ldw = wide;
+  }
+  auto fours = [&](const uint8_t* src, int64_t ld, int64_t count, int64_t offset) {
+    uint8_t* const dst = reinterpret_cast<uint8_t*>(ws + offset);
+    const dim3 grid(static_cast<unsigned>((up4(count) + 255) / 256), static_cast<unsigned>(kb));
+    pad_scales_kernel<<<grid, 256, 0, st>>>(src, ld, static_cast<int>(count), static_cast<int>(up4(count)), dst);
+    return dst;
+  };
+  const bool big = cut.form == kTile256;
+  if (big && codes && !(flags & DFS_FP8_XS_ALIGNED)) {
+    p.xs = fours(p.xs, p.ldxs, rows, at.xs);
+    p.ldxs = up4(rows);
+  }
+  if (big && !(flags & DFS_FP8_WS_ALIGNED)) {
+    p.ws = fours(p.ws, p.ldws, n, at.ws);
+    p.ldws = up4(n);
   }
   p.K = static_cast<int>(wide);  // zeros behind the k
   p.bias = a->bias;
@@ -581,7 +975,14 @@ extern "C" int dfs_linear_fp8(const dfs_linear_fp8_args* a, dfs_stream_t stream)
   p.ldo = out8 ? n : a->out_stride;
   p.splits = cut.splits;
   p.depth = cut.depth;
+  p.whole = static_cast<int>(cut.whole);
   p.part = reinterpret_cast<float*>(ws + at.part);
+  if (big && out8) {
+    p.out8 = static_cast<uint8_t*>(a->out8);
+    p.out8_scales = static_cast<uint8_t*>(a->out8_scales);
+    p.ldo8 = a->out8_stride;
+    p.ldos = a->out8_scales_stride;
+  }
   switch (cut.form) {
     case kFew:
       f16 ? launch_few<true>(p, st) : launch_few<false>(p, st);
@@ -598,8 +999,23 @@ extern "C" int dfs_linear_fp8(const dfs_linear_fp8_args* a, dfs_stream_t stream)
     case kTile128:
       launch_tile<2, 2, 2, 2, 2>(p, f16, st);
       break;
+    case kTile256: {
+      const int64_t rest = big_tiles(rows, n) - cut.whole;
+      const dim3 grid(static_cast<unsigned>(cut.whole + rest * cut.splits));
+      with_activation(p.act, [&](auto act) {
+        if (f16)
+          fp8_big_kernel<true, decltype(act)::value><<<grid, 256, 0, st>>>(p);
+        else
+          fp8_big_kernel<false, decltype(act)::value><<<grid, 256, 0, st>>>(p);
+      });
+      if (rest > 0) {
+        const dim3 join(static_cast<unsigned>(rest * 32));
+        f16 ? fp8_join_big_kernel<true><<<join, 256, 0, st>>>(p) : fp8_join_big_kernel<false><<<join, 256, 0, st>>>(p);
+      }
+      break;
+    }
   }
-  if (out8)
+  if (out8 && !big)
     launch_quantize(p.out, rows, n, n, f16, static_cast<uint8_t*>(a->out8), a->out8_stride, n,
                     static_cast<uint8_t*>(a->out8_scales), a->out8_scales_stride, st);
   return check_launch(name);

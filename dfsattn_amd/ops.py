@@ -1191,7 +1191,8 @@ def qkv_cache(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, k_cache: torch.
 
 E4M3, E8M0 = torch.float8_e4m3fn, torch.float8_e8m0fnu
 SCALE_BLOCK = 128
-_FP8_X_CODES, _FP8_X_ALIGNED, _FP8_W_ALIGNED, _FP8_OUT_CODES = 1, 2, 4, 8  # DFS_FP8_*
+_FP8_X_CODES, _FP8_X_ALIGNED, _FP8_W_ALIGNED, _FP8_OUT_CODES, _FP8_XS_ALIGNED, _FP8_WS_ALIGNED = (
+    1, 2, 4, 8, 16, 32)  # DFS_FP8_*
 _E4M3_CODE = 3
 _QUANTIZE_POINTERS = struct.Struct("@3P")
 _LINEAR_FP8_POINTERS = struct.Struct("@11P")
@@ -1268,7 +1269,7 @@ def _linear_fp8_plan(x_shape: Shape, x_stride: Shape, x_dtype: torch.dtype, w_sh
                      quantize: bool):
     """(shape of out, its dtype, what is read in place: x, weight, residual and
     both scales, and the argument block up to the pointers with its workspace
-    bytes by the alignment of x and weight) of a ``linear_fp8`` call."""
+    bytes by the alignment of x, weight and their scales) of a ``linear_fp8`` call."""
     entry = "linear_fp8"
     codes = x_dtype == E4M3
     if w_dtype != E4M3 or not (codes or x_dtype in HALF):
@@ -1310,13 +1311,17 @@ def _linear_fp8_plan(x_shape: Shape, x_stride: Shape, x_dtype: torch.dtype, w_sh
     a.x_stride, a.w_stride, a.x_scales_stride, a.w_scales_stride = ldx, ldw, ldxs, ldws
     a.residual_stride, a.out_stride, a.out8_stride, a.out8_scales_stride = ldr, n, n, rows
     whole = [k % 16 == 0 and ld % 16 == 0 and ld < 1 << 22 for ld in (ldx, ldw)]
+    fours = [count % 4 == 0 and ld % 4 == 0 for count, ld in ((rows, ldxs), (n, ldws))]
     blocks_of = []
-    for at in range(4):  # bit 0: x on 16 bytes, bit 1: weight
+    for at in range(16):  # bits: x and weight on 16 bytes, their scales on 4
         flags = _FP8_OUT_CODES if quantize else 0
         if codes:
-            flags |= _FP8_X_CODES | (_FP8_X_ALIGNED if whole[0] and at & 1 else 0)
+            flags |= (_FP8_X_CODES | (_FP8_X_ALIGNED if whole[0] and at & 1 else 0)
+                      | (_FP8_XS_ALIGNED if fours[0] and at & 4 else 0))
         if whole[1] and at & 2:
             flags |= _FP8_W_ALIGNED
+        if fours[1] and at & 8:
+            flags |= _FP8_WS_ALIGNED
         size = int(_lib.lib().dfs_linear_fp8_workspace_size(rows, n, k, flags))
         if size < 0:
             raise _lib.DfsKernelError(_lib.lib().dfs_last_error().decode(errors="replace"))
@@ -1376,12 +1381,12 @@ def linear_fp8(x: torch.Tensor, weight: torch.Tensor, weight_scales: torch.Tenso
     elif out is None:
         out = torch.empty(shape, dtype=dtype, device=x.device)
     if blocks is not None:
-        px, pw = x.data_ptr(), weight.data_ptr()
-        head, size = blocks[(px % 16 == 0) + 2 * (pw % 16 == 0)]
+        px, pw, pxs, pws = x.data_ptr(), weight.data_ptr(), _ptr(x_scales) or 0, weight_scales.data_ptr()
+        head, size = blocks[(px % 16 == 0) + 2 * (pw % 16 == 0) + 4 * (pxs % 4 == 0) + 8 * (pws % 4 == 0)]
         ws = torch.empty(size, dtype=torch.uint8, device=x.device) if size else None
         po = out.data_ptr()
         block = head + _LINEAR_FP8_POINTERS.pack(
-            px, pw, _ptr(x_scales) or 0, weight_scales.data_ptr(), _ptr(bias) or 0, _ptr(gate) or 0,
+            px, pw, pxs, pws, _ptr(bias) or 0, _ptr(gate) or 0,
             _ptr(residual) or 0, 0 if quantize else po, po if quantize else 0, _ptr(scales) or 0, _ptr(ws) or 0)
         _call_on(x.device, "dfs_linear_fp8", block)
     return (out, scales) if quantize else out

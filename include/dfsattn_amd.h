@@ -628,7 +628,11 @@ int dfs_quantize_fp8(const dfs_quantize_fp8_args* args, dfs_stream_t stream);
  *                      are multiples of 16, the stride below 2^22 (codes are
  *                      laid out anew otherwise);
  *   DFS_FP8_W_ALIGNED  the same of w;
- *   DFS_FP8_OUT_CODES  the result is left as codes.
+ *   DFS_FP8_OUT_CODES  the result is left as codes;
+ *   DFS_FP8_XS_ALIGNED x's scales lie on 4-byte boundaries, their stride and
+ *                      rows are multiples of 4 (the largest tiles read them in
+ *                      place then, and copy others first);
+ *   DFS_FP8_WS_ALIGNED the same of w's scales, and n.
  * Out may be the residual itself, but overlap nothing else.
  */
 enum { DFS_DTYPE_E4M3 = 3 };
@@ -641,7 +645,8 @@ typedef struct dfs_linear_fp8_args {
   const void* residual;
   void *out, *out8, *out8_scales, *workspace;
 } dfs_linear_fp8_args;
-enum { DFS_FP8_X_CODES = 1, DFS_FP8_X_ALIGNED = 2, DFS_FP8_W_ALIGNED = 4, DFS_FP8_OUT_CODES = 8 };
+enum { DFS_FP8_X_CODES = 1, DFS_FP8_X_ALIGNED = 2, DFS_FP8_W_ALIGNED = 4, DFS_FP8_OUT_CODES = 8,
+       DFS_FP8_XS_ALIGNED = 16, DFS_FP8_WS_ALIGNED = 32 };
 int64_t dfs_linear_fp8_workspace_size(int64_t rows, int64_t n, int64_t k, int flags);
 /* Host function for tests and profiles: the kernel that a call takes, which
  * goes by its sizes alone: the forms of dfs_linear_form (FEW up to 16 rows),

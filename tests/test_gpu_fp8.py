@@ -151,3 +151,32 @@ def test_linear_fp8_matches_definition(dev, m, n, k, dtype, codes, bias, act, ga
     if residual:  # in place of the residual
         d[6] = call(out=d[6])
         assert torch.equal(got, d[6])
+
+
+@pytest.mark.parametrize("m,n,k,codes,act", [(4200, 4200, 3000, False, "gelu_tanh"), (2560, 6500, 4104, True, None),
+                                             (4185, 1953, 264, True, "silu"), (4099, 5003, 200, False, "gelu"),
+                                             (4000, 4001, 2057, True, None), (8200, 8200, 128, False, None)])
+def test_linear_fp8_large_tiles(dev, m, n, k, codes, act):
+    """256 x 256 tiles, whole and behind the last full round in parts; rows and
+    outputs picked all over the result."""
+    print(f"linear_fp8 {m} x {n} x {k} codes={codes} {act}", flush=True)
+    gen = torch.Generator().manual_seed(m + n + k)
+    x, w = _hidden(gen, m, k, BF), _randn(gen, n, k, dtype=BF, std=2 / math.sqrt(k))
+    b, gate, r = _randn(gen, n, dtype=BF), torch.randn(n, generator=gen), _randn(gen, m, n, dtype=BF)
+    xt, wt = refs.to_tensors(*refs.quantize(x)), refs.to_tensors(*refs.quantize(w))
+    d = [None if t is None else t.to(dev) for t in (*(xt if codes else (x, None)), *wt, b, gate, r)]
+
+    def call(**kw):
+        return ops.linear_fp8(d[0], d[2], d[3], d[1], bias=d[4], activation=act, gate=d[5], residual=d[6], **kw)
+
+    got = call()
+    assert torch.equal(got, call())
+    rows, cols = torch.arange(0, m, 13), torch.arange(0, n, 11)
+    rows[-1], cols[-1] = m - 1, n - 1
+    ref, tol = refs.linear_fp8(refs.values(*xt)[rows], refs.values(*wt)[cols], BF, b[cols], act, gate[cols],
+                               r[rows][:, cols])
+    _within(got.cpu()[rows][:, cols], ref, tol, "large tiles")
+    for a, b in zip(call(quantize=True), ops.quantize_fp8(got)):
+        assert torch.equal(a.view(torch.uint8), b.view(torch.uint8))
+    d[3], d[1] = ops._scales_laid_out(d[3]), d[1] if d[1] is None else ops._scales_laid_out(d[1])
+    assert torch.equal(got, call())
