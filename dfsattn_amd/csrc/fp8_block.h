@@ -51,17 +51,76 @@ __device__ __forceinline__ uint2 to_codes8(const float* v, float inverse) {
 }
 
 template <int CTRL>
-__device__ __forceinline__ float dpp_max(float v) {
-  return fmaxf(v, __int_as_float(__builtin_amdgcn_update_dpp(0, __float_as_int(v), CTRL, 0xF, 0xF, true)));
+__device__ __forceinline__ uint32_t dpp_max(uint32_t v) {
+  return max(v, static_cast<uint32_t>(__builtin_amdgcn_update_dpp(0, static_cast<int>(v), CTRL, 0xF, 0xF, true)));
 }
-// Largest over aligned groups of eight or sixteen lanes, in each of them
-// (values not negative).
-__device__ __forceinline__ float max8(float v) {
-  v = dpp_max<0xB1>(v);  // quad_perm [1, 0, 3, 2]
-  v = dpp_max<0x4E>(v);  // quad_perm [2, 3, 0, 1]
-  return dpp_max<0x141>(v);  // row_half_mirror
+// Largest over aligned groups of 8 or 16 lanes, in each of them.
+template <int LANES>
+__device__ __forceinline__ uint32_t group_max(uint32_t v) {
+  static_assert(LANES == 8 || LANES == 16, "half a row of lanes or a whole one");
+  v = dpp_max<0xB1>(v);   // quad_perm [1, 0, 3, 2]
+  v = dpp_max<0x4E>(v);   // quad_perm [2, 3, 0, 1]
+  v = dpp_max<0x141>(v);  // row_half_mirror
+  return LANES == 16 ? dpp_max<0x140>(v) : v;  // row_mirror
 }
-__device__ __forceinline__ float max16(float v) { return dpp_max<0x140>(max8(v)); }  // row_mirror
+
+// The largest magnitude of eight 16-bit values, as its bits: both types order
+// as integers.
+__device__ __forceinline__ uint32_t top_bits8(const uint4& v) {
+  typedef unsigned short u16x2 __attribute__((ext_vector_type(2)));
+  auto mag = [](uint32_t w) { return __builtin_bit_cast(u16x2, w & 0x7fff7fffu); };
+  const u16x2 m = __builtin_elementwise_max(__builtin_elementwise_max(mag(v.x), mag(v.y)),
+                                            __builtin_elementwise_max(mag(v.z), mag(v.w)));
+  return max(static_cast<uint32_t>(m.x), static_cast<uint32_t>(m.y));
+}
+
+// A block of 128 values held by LANES neighbouring lanes, eight in each of the
+// N vectors of a lane (zeros where the row has ended): its scale byte and codes.
+// Magnitudes are compared as integers and the conversion takes pairs of 16-bit
+// values with the scale, one instruction each for two values. Blocks with values
+// that are not finite, and those with the smallest scale, whose float is no
+// normal number, go the long way.
+template <bool F16, int LANES, int N>
+__device__ __forceinline__ uint32_t encode(const uint4 (&v)[N], uint2 (&codes)[N]) {
+  static_assert(LANES * N == 16, "a block has 128 values");
+  typedef __bf16 bf16x2 __attribute__((ext_vector_type(2)));
+  typedef _Float16 f16x2 __attribute__((ext_vector_type(2)));
+  typedef short s16x2 __attribute__((ext_vector_type(2)));
+  uint32_t top = 0;
+#pragma unroll
+  for (int k = 0; k < N; ++k) top = max(top, top_bits8(v[k]));
+  top = group_max<LANES>(top);
+  uint32_t scale = block_scale(F16 ? f16_bits_to_f32(top) : bf16_bits_to_f32(top));
+  if (top < (F16 ? 0x7c00u : 0x7f80u) && scale > 0) {
+    const float s = __uint_as_float(scale << 23);
+    auto pair = [&](uint32_t lo, uint32_t hi) {
+      s16x2 r = {0, 0};
+      if constexpr (F16) {
+        r = __builtin_amdgcn_cvt_scalef32_pk_fp8_f16(r, __builtin_bit_cast(f16x2, lo), s, false);
+        r = __builtin_amdgcn_cvt_scalef32_pk_fp8_f16(r, __builtin_bit_cast(f16x2, hi), s, true);
+      } else {
+        r = __builtin_amdgcn_cvt_scalef32_pk_fp8_bf16(r, __builtin_bit_cast(bf16x2, lo), s, false);
+        r = __builtin_amdgcn_cvt_scalef32_pk_fp8_bf16(r, __builtin_bit_cast(bf16x2, hi), s, true);
+      }
+      return __builtin_bit_cast(uint32_t, r);
+    };
+#pragma unroll
+    for (int k = 0; k < N; ++k) codes[k] = make_uint2(pair(v[k].x, v[k].y), pair(v[k].z, v[k].w));
+    return scale;
+  }
+  float f[N][8], most = 0.f;
+#pragma unroll
+  for (int k = 0; k < N; ++k)
+#pragma unroll
+    for (int i = 0; i < 8; ++i) {
+      f[k][i] = F16 ? f16_bits_to_f32(u16_at(v[k], i)) : bf16_bits_to_f32(u16_at(v[k], i));
+      most = fmaxf(most, finite_magnitude(f[k][i]));
+    }
+  scale = block_scale(__uint_as_float(group_max<LANES>(__float_as_uint(most))));
+#pragma unroll
+  for (int k = 0; k < N; ++k) codes[k] = to_codes8(f[k], inverse_scale(scale));
+  return scale;
+}
 
 }  // namespace
 

@@ -329,38 +329,53 @@ __global__ void __launch_bounds__(256, 2) fp8_tile_kernel(Fp8Params p) {
   });
 }
 
-// Eight outputs n.. of row m, finished and rounded, as they are stored.
-template <bool F16, int ACT>
+// activate, with the tanh form's exponent as z (c0 + c1 z^2): two steps fewer.
+template <int ACT>
+__device__ __forceinline__ float activate_short(float z) {
+  if constexpr (ACT == kActGeluTanh)  // c0 = -2 sqrt(2 / pi) log2(e), c1 = 0.044715 c0
+    return z * __builtin_amdgcn_rcpf(1.f + exp2_fast(z * __builtin_fmaf(-0.10294324f, z * z, -2.3022082f)));
+  else
+    return activate<ACT>(z);
+}
+
+// Eight outputs n.. of row m, finished and rounded, as they are stored; zeros
+// past the matrix (INSIDE: there are none).
+template <bool F16, int ACT, bool INSIDE>
 __device__ __forceinline__ uint4 finished8(const Epilogue& p, int m, int n, const float* z, const float* bias,
                                            const float* gate) {
   float y[8];
 #pragma unroll
-  for (int i = 0; i < 8; ++i) {
-    y[i] = activate<ACT>(z[i] + bias[i]);
-    if (p.gate) y[i] *= gate[i];
-    if (p.residual && m < p.M && n + i < p.N) y[i] += Half<F16>::to_f32(p.residual[m * p.ldr + n + i]);
-    if (n + i >= p.N) y[i] = 0.f;
+  for (int i = 0; i < 8; ++i) y[i] = activate_short<ACT>(z[i] + bias[i]);
+  if (p.gate) {
+#pragma unroll
+    for (int i = 0; i < 8; ++i) y[i] *= gate[i];
+  }
+  if (p.residual) {
+    if (INSIDE || (m < p.M && n + 8 <= p.N)) {
+      uint4 rv;
+      __builtin_memcpy(&rv, p.residual + m * p.ldr + n, 16);
+#pragma unroll
+      for (int i = 0; i < 8; ++i) y[i] += Half<F16>::to_f32(u16_at(rv, i));
+    } else {
+#pragma unroll
+      for (int i = 0; i < 8; ++i)
+        if (m < p.M && n + i < p.N) y[i] += Half<F16>::to_f32(p.residual[m * p.ldr + n + i]);
+    }
+  }
+  if constexpr (!INSIDE) {
+#pragma unroll
+    for (int i = 0; i < 8; ++i)
+      if (m >= p.M || n + i >= p.N) y[i] = 0.f;
   }
   return make_uint4(Half<F16>::pack(y[0], y[1]), Half<F16>::pack(y[2], y[3]), Half<F16>::pack(y[4], y[5]),
                     Half<F16>::pack(y[6], y[7]));
 }
-template <bool F16>
-__device__ __forceinline__ float magnitude8(const uint4& v) {
-  float top = 0.f;
-#pragma unroll
-  for (int i = 0; i < 8; ++i) top = fmaxf(top, finite_magnitude(Half<F16>::to_f32(u16_at(v, i))));
-  return top;
-}
-// Codes of eight rounded outputs n.. of row m under a scale.
-template <bool F16>
-__device__ __forceinline__ void store_codes8(const Fp8Params& p, int m, int n, const uint4& v, uint32_t scale) {
-  if (m >= p.M || n >= p.N) return;
-  float f[8];
-#pragma unroll
-  for (int i = 0; i < 8; ++i) f[i] = Half<F16>::to_f32(u16_at(v, i));
-  const uint2 codes = to_codes8(f, inverse_scale(scale));
+// Codes of eight outputs n.. of row m.
+template <bool INSIDE>
+__device__ __forceinline__ void store_codes8(const Fp8Params& p, int m, int n, const uint2& codes) {
+  if (!INSIDE && (m >= p.M || n >= p.N)) return;
   uint8_t* const dst = p.out8 + m * p.ldo8 + n;
-  if (n + 8 <= p.N) {
+  if (INSIDE || n + 8 <= p.N) {
     __builtin_memcpy(dst, &codes, 8);
   } else {
     uint8_t b[8];
@@ -591,27 +606,36 @@ __global__ void __launch_bounds__(256, 1) fp8_big_kernel(Fp8Params p) {
       });
     });
   } else if (p.out8) {  // a scale's 128 outputs are the wave's: eight lanes, twice
-    each_tile([&](auto j) {
-      uint4 y[2][4];
-      each_half([&](auto gp) {
-        constexpr int GP = decltype(gp)::value;
-        to_stage(j, gp);
+    auto quantized = [&](auto in) {
+      constexpr bool INSIDE = decltype(in)::value;
+      each_tile([&](auto j) {
+        uint4 y[4][2];
+        each_half([&](auto gp) {
+          constexpr int GP = decltype(gp)::value;
+          to_stage(j, gp);
+#pragma unroll
+          for (int i = 0; i < 4; ++i) {
+            float z[8];
+            from_stage(i, z);
+            y[i][GP] = finished8<F16, ACT, INSIDE>(p, mw + i * 32 + decltype(j)::value, nw + GP * 64, z, bias[GP], gate[GP]);
+          }
+        });
 #pragma unroll
         for (int i = 0; i < 4; ++i) {
-          float z[8];
-          from_stage(i, z);
-          y[GP][i] = finished8<F16, ACT>(p, mw + i * 32 + decltype(j)::value, nw + GP * 64, z, bias[GP], gate[GP]);
+          const int m = mw + i * 32 + decltype(j)::value;
+          uint2 codes[2];
+          const uint32_t scale = encode<F16, 8, 2>(y[i], codes);
+          store_codes8<INSIDE>(p, m, nw, codes[0]);
+          store_codes8<INSIDE>(p, m, nw + 64, codes[1]);
+          if ((lane & 7) == 0 && (INSIDE || (m < p.M && nw < p.N)))
+            p.out8_scales[(nw >> 7) * p.ldos + m] = static_cast<uint8_t>(scale);
         }
       });
-#pragma unroll
-      for (int i = 0; i < 4; ++i) {
-        const int m = mw + i * 32 + decltype(j)::value;
-        const uint32_t scale = block_scale(max8(fmaxf(magnitude8<F16>(y[0][i]), magnitude8<F16>(y[1][i]))));
-        store_codes8<F16>(p, m, nw, y[0][i], scale);
-        store_codes8<F16>(p, m, nw + 64, y[1][i], scale);
-        if ((lane & 7) == 0 && m < p.M && nw < p.N) p.out8_scales[(nw >> 7) * p.ldos + m] = static_cast<uint8_t>(scale);
-      }
-    });
+    };
+    if (inside)
+      quantized(std::true_type{});
+    else
+      quantized(std::false_type{});
   } else {
     each_tile([&](auto j) {
       each_half([&](auto gp) {
@@ -678,9 +702,10 @@ __global__ void __launch_bounds__(256) fp8_join_big_kernel(Fp8Params p) {
   with_activation(p.act, [&](auto act) {
     constexpr int ACT = decltype(act)::value;
     if (!p.out8) return finish8<F16, ACT>(p, m, n, z, bias, gate);
-    const uint4 y = finished8<F16, ACT>(p, m, n, z, bias, gate);  // a scale's outputs are sixteen lanes'
-    const uint32_t scale = block_scale(max16(magnitude8<F16>(y)));
-    store_codes8<F16>(p, m, n, y, scale);
+    const uint4 y[1] = {finished8<F16, ACT, false>(p, m, n, z, bias, gate)};  // a scale's outputs are sixteen lanes'
+    uint2 codes[1];
+    const uint32_t scale = encode<F16, 16, 1>(y, codes);
+    store_codes8<false>(p, m, n, codes[0]);
     if ((threadIdx.x & 15) == 0 && m < p.M && n < p.N) p.out8_scales[(n >> 7) * p.ldos + m] = static_cast<uint8_t>(scale);
   });
 }

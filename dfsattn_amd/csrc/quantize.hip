@@ -8,11 +8,6 @@
 namespace dfs {
 namespace {
 
-template <bool F16>
-__device__ __forceinline__ float to_f32(uint32_t bits) {
-  return F16 ? f16_bits_to_f32(bits) : bf16_bits_to_f32(bits);
-}
-
 struct QuantizeParams {
   const uint16_t* x;
   uint8_t *values, *scales;
@@ -39,14 +34,10 @@ __global__ void __launch_bounds__(256) quantize_kernel(QuantizeParams p) {
     for (int i = 0; i < 8; ++i) t[i] = c + i < p.k ? t[i] : 0;
     __builtin_memcpy(&v, t, 16);
   }
-  float f[8], top = 0.f;
-#pragma unroll
-  for (int i = 0; i < 8; ++i) {
-    f[i] = to_f32<F16>(u16_at(v, i));
-    top = fmaxf(top, finite_magnitude(f[i]));
-  }
-  const uint32_t scale = block_scale(max16(top));
-  const uint2 codes = to_codes8(f, inverse_scale(scale));
+  const uint4 values[1] = {v};
+  uint2 code[1];
+  const uint32_t scale = encode<F16, 16, 1>(values, code);
+  const uint2 codes = code[0];
   uint8_t* const dst = p.values + row * p.ldv + c;
   if (c + 8 <= p.fill) {
     __builtin_memcpy(dst, &codes, 8);

@@ -258,22 +258,18 @@ __global__ void __launch_bounds__(256) residual_norm_kernel(NormParams p) {
           if (scale) y = y * (1.0f + sc[i + t]);
           if (shift) y = y + sh[i + t];
           r[t] = from_f32<F16>(y);
+          if (EDGE && e + i + t >= C) r[t] = 0;
         }
         packed[i / 2] = r[0] | r[1] << 16;
       }
       const uint4 out = make_uint4(packed[0], packed[1], packed[2], packed[3]);
       const int row = row0 + q;
       if (p.h8) {  // a scale's 128 channels are sixteen lanes'
-        float f[8], top = 0.f;
-#pragma unroll
-        for (int i = 0; i < 8; ++i) {
-          f[i] = to_f32<F16>(u16_at(out, i));
-          if (e + i < C) top = fmaxf(top, finite_magnitude(f[i]));
-        }
-        const uint32_t byte = block_scale(max16(top));
-        const uint2 codes = to_codes8(f, inverse_scale(byte));
+        const uint4 values[1] = {e < C ? out : make_uint4(0, 0, 0, 0)};
+        uint2 codes[1];
+        const uint32_t byte = encode<F16, 16, 1>(values, codes);
         if (e < C && row < p.rows) {
-          store8_u8<EDGE>(p.h8 + row * p.ldh, e, C, codes);
+          store8_u8<EDGE>(p.h8 + row * p.ldh, e, C, codes[0]);
           if ((lane & 15) == 0) p.h8_scales[(e >> 7) * p.lds + row] = static_cast<uint8_t>(byte);
         }
       } else if (e < C && row < p.rows) {
