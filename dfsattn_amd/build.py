@@ -17,9 +17,10 @@ CSRC = os.path.join(PKG_DIR, "csrc")
 INCLUDE = os.path.join(REPO_DIR, "include")
 OUT_DIR = os.path.join(PKG_DIR, "_lib")
 LIB_NAME = "libdfsattn_amd.so"
-SOURCES = ["host.cpp", "call.cpp", "permute.hip", "score_topk.hip", "bsa_fwd.hip", "masks.hip", "norm_rope.hip", "dit_fused.hip",
-           "linear.hip", "window_attn.hip", "qkv_cache.hip", "quantize.hip", "linear_fp8.hip",
-           "residual_norm.hip", "axial_rope.hip"]
+SOURCES = ["host.cpp", "call.cpp", "linear_fp8_large_bf16.hip", "linear_fp8_large_f16.hip", "residual_norm.hip",
+           "residual_norm_f16.hip", "axial_rope.hip", "linear_fp8.hip", "linear.hip", "norm_rope.hip", "permute.hip",
+           "score_topk.hip", "bsa_fwd.hip", "masks.hip", "dit_fused.hip", "window_attn.hip", "qkv_cache.hip",
+           "quantize.hip"]
 ARCH = "gfx950"
 
 

@@ -66,16 +66,40 @@ __device__ __forceinline__ float group_sum(float v, int lanes) {
   return v;
 }
 
-__device__ __forceinline__ float weight_at(const void* w, int dtype, int e) {
-  if (dtype == DFS_DTYPE_F32) return static_cast<const float*>(w)[e];
-  const uint32_t b = static_cast<const uint16_t*>(w)[e];
-  return dtype == DFS_DTYPE_BF16 ? bf16_bits_to_f32(b) : f16_bits_to_f32(b);
+typedef unsigned int u32x2_t __attribute__((ext_vector_type(2)));
+template <bool STREAM>
+__device__ __forceinline__ uint2 load_half(const uint16_t* p) {
+  const u32x2_t* const q = reinterpret_cast<const u32x2_t*>(p);
+  const u32x2_t t = STREAM ? __builtin_nontemporal_load(q) : *q;
+  return make_uint2(t.x, t.y);
+}
+template <bool STREAM>
+__device__ __forceinline__ void store_half(uint16_t* p, const uint2& v) {
+  const u32x2_t t = {v.x, v.y};
+  u32x2_t* const q = reinterpret_cast<u32x2_t*>(p);
+  if constexpr (STREAM)
+    __builtin_nontemporal_store(t, q);
+  else
+    *q = t;
+}
+
+// Four weights from element e on, a multiple of 4, in fp32.
+__device__ __forceinline__ void load_weight4(const void* w, int dtype, int e, float* out) {
+  if (dtype == DFS_DTYPE_F32) {
+    __builtin_memcpy(out, static_cast<const float*>(w) + e, 16);
+    return;
+  }
+  uint16_t t[4];
+  __builtin_memcpy(t, static_cast<const uint16_t*>(w) + e, 8);
+#pragma unroll
+  for (int i = 0; i < 4; ++i) out[i] = dtype == DFS_DTYPE_BF16 ? bf16_bits_to_f32(t[i]) : f16_bits_to_f32(t[i]);
 }
 
 // One wave per token and tensor (grid y). Lane l of a head's has its pairs
 // 4 l .. 4 l + 3: eight neighbouring channels, or four of either half. Values
 // i and pair(i): HALVES 4 + i, else 2 i and 2 i + 1.
-template <int NCH, bool F16, bool HALVES>
+// STREAM: for tensors beyond the last-level cache.
+template <int NCH, bool F16, bool HALVES, bool STREAM>
 __global__ void __launch_bounds__(256) axial_rope_kernel(RopeParams p) {
   __shared__ __attribute__((aligned(16))) float table[4][2][256];  // cosines, sines of a wave's token
   const int lane = threadIdx.x & 63, w = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), n = blockIdx.y;
@@ -93,11 +117,10 @@ __global__ void __launch_bounds__(256) axial_rope_kernel(RopeParams p) {
     v[j] = make_uint4(0, 0, 0, 0);
     if (working && h < H) {
       if constexpr (HALVES) {
-        const uint2 lo = *reinterpret_cast<const uint2*>(src + h * p.x_sh[n] + c0);
-        const uint2 hi = *reinterpret_cast<const uint2*>(src + h * p.x_sh[n] + c1);
+        const uint2 lo = load_half<STREAM>(src + h * p.x_sh[n] + c0), hi = load_half<STREAM>(src + h * p.x_sh[n] + c1);
         v[j] = make_uint4(lo.x, lo.y, hi.x, hi.y);
       } else {
-        v[j] = *reinterpret_cast<const uint4*>(src + h * p.x_sh[n] + c0);
+        v[j] = load_chunk<STREAM>(reinterpret_cast<const uint4*>(src + h * p.x_sh[n] + c0));
       }
     }
   }
@@ -160,15 +183,17 @@ __global__ void __launch_bounds__(256) axial_rope_kernel(RopeParams p) {
     rstd[j] = ss;
     all += ss;
   }
-  float wt[8];
+  float wt[8] = {};
   if (weight) {
     if (w_all) {
       const float r = 1.f / sqrtf(group_sum(all, 64) / static_cast<float>(H * D) + p.eps);
 #pragma unroll
       for (int j = 0; j < NCH; ++j) rstd[j] = r;
     } else {
-#pragma unroll
-      for (int i = 0; i < 8; ++i) wt[i] = working ? weight_at(weight, w_dtype, (i < 4 ? c0 + i : c1 + i - 4)) : 0.f;
+      if (working) {
+        load_weight4(weight, w_dtype, c0, wt);
+        load_weight4(weight, w_dtype, c1, wt + 4);
+      }
 #pragma unroll
       for (int j = 0; j < NCH; ++j) rstd[j] = 1.f / sqrtf(group_sum(rstd[j], lanes) / static_cast<float>(D) + p.eps);
     }
@@ -183,8 +208,8 @@ __global__ void __launch_bounds__(256) axial_rope_kernel(RopeParams p) {
     for (int i = 0; i < 8; ++i) y[i] = to_f32<F16>(u16_at(v[j], i));
     if (weight) {
       if (w_all) {
-#pragma unroll
-        for (int i = 0; i < 8; ++i) wt[i] = weight_at(weight, w_dtype, h * D + (i < 4 ? c0 + i : c1 + i - 4));
+        load_weight4(weight, w_dtype, h * D + c0, wt);
+        load_weight4(weight, w_dtype, h * D + c1, wt + 4);
       }
 #pragma unroll
       for (int i = 0; i < 8; ++i) y[i] = y[i] * rstd[j] * wt[i];
@@ -198,22 +223,27 @@ __global__ void __launch_bounds__(256) axial_rope_kernel(RopeParams p) {
     }
     const uint4 o = make_uint4(r[0] | r[1] << 16, r[2] | r[3] << 16, r[4] | r[5] << 16, r[6] | r[7] << 16);
     if constexpr (HALVES) {
-      *reinterpret_cast<uint2*>(dst + h * p.o_sh[n] + c0) = make_uint2(o.x, o.y);
-      *reinterpret_cast<uint2*>(dst + h * p.o_sh[n] + c1) = make_uint2(o.z, o.w);
+      store_half<STREAM>(dst + h * p.o_sh[n] + c0, make_uint2(o.x, o.y));
+      store_half<STREAM>(dst + h * p.o_sh[n] + c1, make_uint2(o.z, o.w));
     } else {
-      *reinterpret_cast<uint4*>(dst + h * p.o_sh[n] + c0) = o;
+      store_chunk<STREAM>(reinterpret_cast<uint4*>(dst + h * p.o_sh[n] + c0), o);
     }
   }
 }
 
+template <int NCH, bool STREAM>
+void launch_as(const RopeParams& p, bool f16, bool halves, dim3 grid, hipStream_t st) {
+  if (halves)
+    f16 ? axial_rope_kernel<NCH, true, true, STREAM><<<grid, 256, 0, st>>>(p)
+        : axial_rope_kernel<NCH, false, true, STREAM><<<grid, 256, 0, st>>>(p);
+  else
+    f16 ? axial_rope_kernel<NCH, true, false, STREAM><<<grid, 256, 0, st>>>(p)
+        : axial_rope_kernel<NCH, false, false, STREAM><<<grid, 256, 0, st>>>(p);
+}
 template <int NCH>
 void launch(const RopeParams& p, bool f16, bool halves, dim3 grid, hipStream_t st) {
-  if (halves)
-    f16 ? axial_rope_kernel<NCH, true, true><<<grid, 256, 0, st>>>(p)
-        : axial_rope_kernel<NCH, false, true><<<grid, 256, 0, st>>>(p);
-  else
-    f16 ? axial_rope_kernel<NCH, true, false><<<grid, 256, 0, st>>>(p)
-        : axial_rope_kernel<NCH, false, false><<<grid, 256, 0, st>>>(p);
+  const int64_t bytes = int64_t(4) * p.B * p.T * (p.heads[0] + p.heads[1]) * p.D;
+  bytes > kLastLevelCache / 4 ? launch_as<NCH, true>(p, f16, halves, grid, st) : launch_as<NCH, false>(p, f16, halves, grid, st);
 }
 
 }  // namespace
