@@ -13,7 +13,7 @@ namespace {
 
 constexpr uint32_t kOutside = 0x80000000u;  // byte offset past every buffer's records
 
-enum Activation { kActNone = 0, kActGeluTanh = 1, kActGelu = 2, kActSilu = 3 };
+enum Activation { kActNone = 0, kActGeluTanh = 1, kActGelu = 2, kActSilu = 3, kActGeluTanhShort = 4 };
 
 struct Epilogue {
   int M, N;
@@ -70,6 +70,10 @@ __device__ __forceinline__ float activate(float z) {
   if constexpr (ACT == kActGeluTanh) {
     const float u = 1.5957691216057308f * (z + 0.044715f * z * z * z);
     return z * __builtin_amdgcn_rcpf(1.f + exp2_fast(-1.4426950408889634f * u));
+  } else if constexpr (ACT == kActGeluTanhShort) {
+    // The tanh form with its exponent as z (c0 + c1 z^2), two steps fewer:
+    // c0 = -2 sqrt(2 / pi) log2(e), c1 = 0.044715 c0.
+    return z * __builtin_amdgcn_rcpf(1.f + exp2_fast(z * __builtin_fmaf(-0.10294324f, z * z, -2.3022082f)));
   } else if constexpr (ACT == kActGelu) {
     return 0.5f * z * erfcf(-0.70710678118654752f * z);
   } else if constexpr (ACT == kActSilu) {

@@ -25,7 +25,7 @@ __device__ __forceinline__ void finish16(const Epilogue& p, int n0, const float*
   float z = 0.f;
   for (int v = 0; v < waves; ++v) z += sums[v * 256 + ((n16 >> 2) * 16 + m) * 4 + (n16 & 3)];
   z += bias_at(p, n);
-  with_activation(p.act, [&](auto act) { z = activate<decltype(act)::value>(z); });
+  with_fp8_activation(p.act, [&](auto act) { z = activate<decltype(act)::value>(z); });
   if (p.gate) z *= p.gate[n];
   if (p.residual) z += Half<F16>::to_f32(p.residual[m * p.ldr + n]);
   p.out[m * p.ldo + n] = static_cast<uint16_t>(Half<F16>::from_f32(z));
@@ -284,7 +284,7 @@ __global__ void __launch_bounds__(256, 2) fp8_tile_kernel(Fp8Params p) {
         }
     return;
   }
-  with_activation(p.act, [&](auto act) {
+  with_fp8_activation(p.act, [&](auto act) {
     if constexpr (NI == 1) {
 #pragma unroll
       for (int g = 0; g < 2; ++g) {
@@ -342,7 +342,7 @@ __global__ void __launch_bounds__(256) fp8_join_kernel(Fp8Params p) {
   }
   float bias[8], gate[8];
   load_columns8(p, n, bias, gate);
-  with_activation(p.act, [&](auto act) { finish8<F16, decltype(act)::value>(p, m, n, z, bias, gate); });
+  with_fp8_activation(p.act, [&](auto act) { finish8<F16, decltype(act)::value>(p, m, n, z, bias, gate); });
 }
 
 // Scale bytes [blocks][rows] at any stride into ones of stride `wide`, a multiple

@@ -8,15 +8,6 @@
 namespace dfs {
 namespace {
 
-// activate, with the tanh form's exponent as z (c0 + c1 z^2): two steps fewer.
-template <int ACT>
-__device__ __forceinline__ float activate_short(float z) {
-  if constexpr (ACT == kActGeluTanh)  // c0 = -2 sqrt(2 / pi) log2(e), c1 = 0.044715 c0
-    return z * __builtin_amdgcn_rcpf(1.f + exp2_fast(z * __builtin_fmaf(-0.10294324f, z * z, -2.3022082f)));
-  else
-    return activate<ACT>(z);
-}
-
 // Eight outputs n.. of row m, finished and rounded, as they are stored; zeros
 // past the matrix (INSIDE: there are none).
 template <bool F16, int ACT, bool INSIDE>
@@ -24,7 +15,7 @@ __device__ __forceinline__ uint4 finished8(const Epilogue& p, int m, int n, cons
                                            const float* gate) {
   float y[8];
 #pragma unroll
-  for (int i = 0; i < 8; ++i) y[i] = activate_short<ACT>(z[i] + bias[i]);
+  for (int i = 0; i < 8; ++i) y[i] = activate<ACT>(z[i] + bias[i]);
   if (p.gate) {
 #pragma unroll
     for (int i = 0; i < 8; ++i) y[i] *= gate[i];
@@ -358,7 +349,7 @@ __global__ void __launch_bounds__(256) fp8_join_big_kernel(Fp8Params p) {
   }
   float bias[8], gate[8];
   load_columns8(p, n, bias, gate);
-  with_activation(p.act, [&](auto act) {
+  with_fp8_activation(p.act, [&](auto act) {
     constexpr int ACT = decltype(act)::value;
     if (!p.out8) return finish8<F16, ACT>(p, m, n, z, bias, gate);
     const uint4 y[1] = {finished8<F16, ACT, false>(p, m, n, z, bias, gate)};  // a scale's outputs are sixteen lanes'
@@ -372,7 +363,7 @@ __global__ void __launch_bounds__(256) fp8_join_big_kernel(Fp8Params p) {
 template <bool F16>
 void run_fp8_large(const Fp8Params& p, int64_t rest, hipStream_t st) {
   const dim3 grid(static_cast<unsigned>(p.whole + rest * p.splits));
-  with_activation(p.act, [&](auto act) { fp8_big_kernel<F16, decltype(act)::value><<<grid, 256, 0, st>>>(p); });
+  with_fp8_activation(p.act, [&](auto act) { fp8_big_kernel<F16, decltype(act)::value><<<grid, 256, 0, st>>>(p); });
   if (rest > 0) fp8_join_big_kernel<F16><<<dim3(static_cast<unsigned>(rest * 32)), 256, 0, st>>>(p);
 }
 

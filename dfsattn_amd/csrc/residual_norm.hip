@@ -16,6 +16,7 @@ extern "C" int dfs_residual_norm(const dfs_residual_norm_args* a, dfs_stream_t s
   DFS_REQUIRE(rows > 0 && rows < (int64_t(1) << 26) && C > 0 && C <= 512 * kMaxChunks,
               "%s: rows=%lld channels=%lld must be positive, below 2^26 and up to %d", name, (long long)rows,
               (long long)C, 512 * kMaxChunks);
+  DFS_REQUIRE(C % 8 == 0 || rows < (int64_t(1) << 24), "%s: too many rows of %lld channels", name, (long long)C);
   DFS_REQUIRE(a->dtype == DFS_DTYPE_BF16 || a->dtype == DFS_DTYPE_F16, "%s: dtype must be bf16 or f16", name);
   DFS_REQUIRE(a->norm == DFS_NORM_RMS || a->norm == DFS_NORM_LAYER, "%s: norm code %lld is not supported", name,
               (long long)a->norm);

@@ -26,6 +26,8 @@ import torch
 import torch.nn as nn
 import torch.nn.functional as F
 
+from .fp8 import Fp8Linear
+
 
 @dataclass(frozen=True)
 class DiTConfig:
@@ -165,7 +167,8 @@ class DiTBlock(nn.Module):
         self.scale_shift_table = nn.Parameter(torch.zeros(1, 6, d, **f32))
 
     # On the GPU the layer norms with their modulation and the gated residuals
-    # run as one fused pass each (dfs_adaln_modulate, dfs_gated_residual)
+    # run as one fused pass each (dfs_adaln_modulate, dfs_gated_residual, and
+    # between two branches both in one, dfs_residual_norm)
     # instead of torch's chain of dtype copies and broadcast ops, and the FFN's
     # GELU runs in the first GEMM's epilogue (hipBLASLt, through torch's
     # _addmm_activation: 8.2 -> 7.5 ms per call at 75,600 x 5,120 x 13,824; the
@@ -185,24 +188,40 @@ class DiTBlock(nn.Module):
         a = ops.linear(h, lin1.weight, lin1.bias, activation="gelu_tanh")
         return ops.linear(a, lin2.weight, lin2.bias, gate=gate, residual=x)
 
+    def _ffn_fp8(self, x: torch.Tensor, a: torch.Tensor, scale: torch.Tensor, shift: torch.Tensor,
+                 gate: torch.Tensor) -> torch.Tensor:
+        """The residual of a, the norm and the feed-forward products on 8-bit
+        operands, each left by the operator before it."""
+        from . import ops
+
+        x, codes, scales = ops.residual_norm(x, a, scale=scale, shift=shift, eps=self.norm3.eps, quantize=True)
+        codes, scales = self.ffn[0](codes, scales, activation="gelu_tanh", out_dtype=x.dtype, quantize=True)
+        return self.ffn[2](codes, scales, gate=gate, residual=x, out_dtype=x.dtype)
+
     def _ffn_fused(self, h: torch.Tensor) -> torch.Tensor:
         lin1, act, lin2 = self.ffn
-        if lin1.bias is None or not hasattr(torch, "_addmm_activation"):
+        if not isinstance(lin1, nn.Linear) or lin1.bias is None or not hasattr(torch, "_addmm_activation"):
             return self.ffn(h)
         a = torch._addmm_activation(lin1.bias, h.reshape(-1, h.shape[-1]), lin1.weight.t(), use_gelu=True)
         return lin2(a).reshape(*h.shape[:-1], -1)
 
     def forward(self, x: torch.Tensor, context: torch.Tensor, temb: torch.Tensor,
-                rotary_emb: torch.Tensor) -> torch.Tensor:
+                rotary_emb) -> torch.Tensor:
         shift_msa, scale_msa, gate_msa, c_shift, c_scale, c_gate = (self.scale_shift_table + temb.float()).chunk(6, 1)
         if self.fused_elementwise and x.is_cuda and x.shape[0] == 1:
             from . import ops
 
             h = ops.adaln_modulate(x, self.norm1.eps, scale=scale_msa, shift=shift_msa)
-            x = ops.gated_residual(x, self.attn1(h, None, None, rotary_emb), gate_msa)
-            h = ops.adaln_modulate(x, self.norm2.eps, weight=self.norm2.weight.float(), bias=self.norm2.bias.float())
-            x = x + self.attn2(h, context)
-            h = ops.adaln_modulate(x, self.norm3.eps, scale=c_scale, shift=c_shift)
+            # a branch's residual and the norm before the next one in one pass
+            a = self.attn1(h, None, None, rotary_emb)
+            with torch.no_grad():
+                x, h = ops.residual_norm(x, a, gate_msa, weight=self.norm2.weight, bias=self.norm2.bias,
+                                         eps=self.norm2.eps)
+            a = self.attn2(h, context)
+            if isinstance(self.ffn[0], Fp8Linear) and isinstance(self.ffn[2], Fp8Linear):
+                return self._ffn_fp8(x, a, c_scale, c_shift, c_gate)
+            with torch.no_grad():
+                x, h = ops.residual_norm(x, a, scale=c_scale, shift=c_shift, eps=self.norm3.eps)
             if self.native_ffn:
                 return self._ffn_native(h, x, c_gate)
             return ops.gated_residual(x, self._ffn_fused(h), c_gate)
@@ -234,6 +253,17 @@ class WanLikeDiT(nn.Module):
         self.scale_shift_table = nn.Parameter(torch.zeros(1, 2, d, **f32))
         self.register_buffer("rotary_emb", wan_rope_freqs(cfg.grid, cfg.head_dim, cfg.theta).to(device),
                              persistent=False)
+        self.rotary_axes = None  # a GridRotary in the place of the table
+
+    def use_rotary_axes(self, on: bool = True) -> None:
+        """Has the processors make the rotary angles from the tokens' places on
+        the grid (``ops.axial_rope``) instead of reading them from the table."""
+        from .ops import GridRotary, RotaryAxes
+
+        d = self.cfg.head_dim
+        side = 2 * (d // 6)
+        axes = RotaryAxes(d, (d - 2 * side, side, side), self.cfg.theta)
+        self.rotary_axes = GridRotary(axes, tuple(self.cfg.grid[1:])) if on else None
 
     def attention_modules(self) -> List[Tuple[str, DiTAttention]]:
         """(name, module) in the order diffusers' attn_processors lists them."""
@@ -275,8 +305,9 @@ class WanLikeDiT(nn.Module):
         temb = self.time_embedder(timestep_embedding(timestep, self.cfg.freq_dim))
         tproj = self.time_proj(temb.to(self.time_proj[1].weight.dtype)).unflatten(1, (6, -1))
         ctx = self.text_embedder(context.to(self.text_embedder[0].weight.dtype))
+        rotary = self.rotary_emb if self.rotary_axes is None else self.rotary_axes
         for block in self.blocks:
-            x = block(x, ctx, tproj, self.rotary_emb)
+            x = block(x, ctx, tproj, rotary)
         shift, scale = (self.scale_shift_table + temb.unsqueeze(1)).chunk(2, dim=1)
         x = (self.norm_out(x.float()) * (1 + scale) + shift).type_as(x)
         return self.unpatchify(self.proj_out(x), frames)

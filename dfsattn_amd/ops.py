@@ -1577,6 +1577,32 @@ class RotaryAxes:
             raise ValueError(f"RotaryAxes: layout must be 'pairs' or 'halves', got {self.layout!r}")
 
 
+@dataclass(frozen=True)
+class GridRotary:
+    """Rotary positions of a video's tokens in row-major order: ``axes`` over
+    frames of ``grid`` (height, width) tokens. Passed to the processors in the
+    place of a table of frequencies."""
+
+    axes: RotaryAxes
+    grid: Tuple[int, ...]
+
+    def table(self, tokens: int, device=None) -> torch.Tensor:
+        """complex128 [1, 1, tokens, head_dim/2]: the table that it stands for
+        (layout "pairs"; channels behind the sections are not rotated)."""
+        if self.axes.layout != "pairs":
+            raise ValueError("GridRotary: a table is of neighbouring pairs")
+        at, places = torch.arange(tokens, dtype=torch.int64, device=device), []
+        for n in reversed(self.grid):
+            places.append(at % n)
+            at = at // n
+        angles = [p.double()[:, None] * (v * t ** (-torch.arange(0, c, 2, dtype=torch.float64, device=device) / max(c, 1)))
+                  for p, c, t, v in zip((at, *reversed(places)), self.axes.sections, self.axes.theta, self.axes.speeds)]
+        rest = self.axes.head_dim // 2 - sum(self.axes.sections) // 2
+        angles.append(torch.zeros((tokens, rest), dtype=torch.float64, device=device))
+        angle = torch.cat(angles, -1)
+        return torch.polar(torch.ones_like(angle), angle)[None, None]
+
+
 @functools.lru_cache(maxsize=1024)
 def _rope_plan(q: Meta, k: Optional[Meta], axes: RotaryAxes, grid: Optional[Tuple[int, ...]],
                positions: Optional[Meta], weights: Tuple[Optional[Tuple[Shape, torch.dtype]], ...], eps: float):

@@ -29,6 +29,7 @@ import torch.nn.functional as F
 from .attention_wan import DFS_Attention as WanDFSAttention
 from .attention_wan import dfs_attention
 from .fullattention import full_attention
+from .ops import GridRotary
 
 
 def apply_rotary_emb_complex(x: torch.Tensor, freqs: torch.Tensor) -> torch.Tensor:
@@ -85,12 +86,23 @@ def fused_qkv_heads(attn, query: torch.Tensor, key: torch.Tensor, value: torch.T
     the library's fused kernel (one pass per tensor, the three tensors of a
     self-attention in one launch). ``token_major``: views of [B, L, H, D]
     storage instead of new head-major tensors where that launch applies (the
-    library's attention reads them in place)."""
-    from .ops import norm_rope_heads, qkv_heads, qkv_heads_fusable
+    library's attention reads them in place). ``rotary_emb``: a complex table,
+    or a ``GridRotary``, whose angles are made from the tokens' places instead
+    of read (``ops.axial_rope``)."""
+    from .ops import axial_rope, norm_rope_heads, qkv_heads, qkv_heads_fusable
 
     heads = attn.heads
     wq, eq = _norm_args(attn.norm_q, query.shape[-1], query)
     wk, ek = _norm_args(attn.norm_k, key.shape[-1], key)
+    if isinstance(rotary_emb, GridRotary):
+        q, k, v = (t.unflatten(2, (heads, -1)) for t in (query, key, value))
+        axes, grid = rotary_emb.axes, rotary_emb.grid
+        if eq == ek:
+            q, k = axial_rope(q, k, axes, grid, q_weight=wq, k_weight=wk, eps=eq)
+        else:
+            q, k = (axial_rope(t, None, axes, grid, q_weight=w, eps=e)[0] for t, w, e in ((q, wq, eq), (k, wk, ek)))
+        v = v.transpose(1, 2)
+        return (q, k, v) if token_major else (q.contiguous(), k.contiguous(), v.contiguous())
     if qkv_heads_fusable(query, key, value):
         # self-attention: one launch, the complex table read as it is
         table = None
@@ -197,6 +209,8 @@ class Wan_DFSAttn_Processor2_0:
             key = key.unflatten(2, (attn.heads, -1)).transpose(1, 2).contiguous()
             value = value.unflatten(2, (attn.heads, -1)).transpose(1, 2).contiguous()
             if rotary_emb is not None:
+                if isinstance(rotary_emb, GridRotary):
+                    rotary_emb = rotary_emb.table(query.shape[2], query.device)
                 query = apply_rotary_emb_complex(query, rotary_emb)
                 key = apply_rotary_emb_complex(key, rotary_emb)
 

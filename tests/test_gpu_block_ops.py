@@ -166,3 +166,168 @@ def test_axial_rope_matches_definition(dev, B, T, H, G, D, dtype, sections, thet
     if positions is not None:  # one set of positions for every sequence
         both = ops.axial_rope(d[0], d[1], axes, q_weight=d[2], k_weight=d[3], positions=d[4][0])
         _within(both[0], *refs.axial_rope(q, places[:1].expand(B, T, n), sections, (theta,) * n, layout, wq), "shared")
+
+
+def test_residual_norm_rows_that_are_not_finite(dev):
+    """A NaN or infinity in a row stays in it; rows of one value, whose layer
+    norm is that of zeros; a channel count of every remainder by eight."""
+    for C in (64, 65, 71, 2500, 2503):
+        print(f"residual_norm not finite C={C}", flush=True)
+        g = torch.Generator().manual_seed(C)
+        x, y = _randn(g, 9, C, dtype=BF).to(dev), _randn(g, 9, C, dtype=BF).to(dev)
+        whole = ops.residual_norm(x, y, norm="layer")
+        x[2, C - 1], y[5, 0] = math.inf, math.nan
+        got = ops.residual_norm(x, y, norm="layer")
+        keep = [0, 1, 3, 4, 6, 7, 8]
+        for a, b in zip(got, whole):
+            assert torch.equal(a[keep], b[keep])
+        assert bool(torch.isnan(got[1][[2, 5]]).all())
+        r, codes, scales = ops.residual_norm(x, y, norm="layer", quantize=True)
+        assert bool(torch.isnan(codes[[2, 5]].float()).all())
+        flat = torch.full((3, C), 2.0, dtype=BF, device=dev)
+        assert bool((ops.residual_norm(flat, flat)[1] == 0).all())
+
+
+def test_residual_norm_views(dev):
+    """Rows inside wider ones at any element, vectors cut from one tensor or
+    expanded, what surrounds out stays, no rows."""
+    g = torch.Generator().manual_seed(4)
+    for C, off in ((512, 8), (512, 3), (77, 1)):
+        print(f"residual_norm views C={C} offset={off}", flush=True)
+        x, y = _randn(g, 2, 5, C + 16, dtype=BF), _randn(g, 2, 5, C + 16, dtype=BF)
+        both = _randn(g, 2, 3, C)
+        xs, ys = x.to(dev)[..., off:off + C], y.to(dev)[..., off:off + C]
+        gate, scale, shift = both.to(dev).chunk(3, 1)
+        room = torch.full((10 * C + 512,), 7.0, dtype=BF, device=dev)
+        out = room[256:256 + 10 * C].view(2, 5, C)
+        r, h = ops.residual_norm(xs, ys, gate, scale=scale, shift=shift, out=out)
+        assert r is out and bool((room[:256] == 7).all()) and bool((room[256 + 10 * C:] == 7).all())
+        want = ops.residual_norm(xs.contiguous(), ys.contiguous(), gate.contiguous(), scale=scale.contiguous(),
+                                 shift=shift.contiguous())
+        assert torch.equal(r, want[0]) and torch.equal(h, want[1])
+        _within(r, *refs.residual(x[..., off:off + C], y[..., off:off + C], both[:, :1]), "r")
+        one = ops.residual_norm(xs, ys, gate[:1].expand(2, 1, C))
+        assert torch.equal(one[0][0], want[0][0])
+        t = ops.residual_norm(xs.transpose(0, 1), ys.transpose(0, 1), gate.transpose(0, 1))
+        assert torch.equal(t[0].transpose(0, 1), want[0])
+    empty = ops.residual_norm(torch.zeros(0, 64, dtype=BF, device=dev), torch.zeros(0, 64, dtype=BF, device=dev), quantize=True)
+    assert [tuple(e.shape) for e in empty] == [(0, 64), (0, 64), (0, 1)]
+
+
+def test_axial_rope_views_and_far_positions(dev):
+    """Heads inside wider rows on and off 16-byte boundaries, head-major storage;
+    positions at the ends of int32."""
+    g = torch.Generator().manual_seed(6)
+    axes = ops.RotaryAxes(64, (24, 20, 20), 1e4)
+    x = _randn(g, 2, 7, 3, 80, dtype=BF)
+    places = torch.tensor([[[2 ** 31 - 1 - i, -2 ** 31 + i, 12345 * i] for i in range(7)]] * 2)
+    pos = places.to(torch.int32).to(dev)
+    for off in (0, 8, 3):
+        print(f"axial_rope views offset={off}", flush=True)
+        xd = x.to(dev)[..., off:off + 64]
+        got = ops.axial_rope(xd, xd, axes, positions=pos)
+        _within(got[0], *refs.axial_rope(x[..., off:off + 64], places, (24, 20, 20), (1e4,) * 3, "pairs"), "far")
+        assert torch.equal(got[0], got[1])
+        major = xd.transpose(1, 2).contiguous().transpose(1, 2)
+        assert torch.equal(ops.axial_rope(major, None, axes, positions=pos)[0], got[0])
+        wide = torch.zeros(2, 7, 9, dtype=torch.int32, device=dev)
+        wide[..., 4:7] = pos
+        assert torch.equal(ops.axial_rope(xd, None, axes, positions=wide[..., 4:7])[0], got[0])
+    assert ops.axial_rope(xd[:, :0], xd[:, :0], axes, grid=(2, 2))[0].shape == (2, 3, 0, 64)
+
+
+def test_block_operators_beyond_32_bits(dev):
+    rows = 430000
+    print("residual_norm 430,000 x 5,120", flush=True)
+    g = torch.Generator().manual_seed(8)
+    x, y = torch.zeros(rows, 5120, dtype=BF, device=dev), torch.zeros(rows, 5120, dtype=BF, device=dev)
+    x[-2:], y[-2:] = _randn(g, 2, 5120, dtype=BF).to(dev), _randn(g, 2, 5120, dtype=BF).to(dev)
+    gate = _randn(g, 5120).to(dev)
+    for q in (False, True):
+        got, want = ops.residual_norm(x, y, gate, quantize=q), ops.residual_norm(x[-2:], y[-2:], gate, quantize=q)
+        for a, b in zip(got, want):
+            assert torch.equal(a[-2:].view(torch.uint8), b.view(torch.uint8))
+    del got, y
+    print("axial_rope 430,000 x 40 x 128", flush=True)
+    axes = ops.RotaryAxes(128, (44, 42, 42))
+    got = ops.axial_rope(x.view(1, rows, 40, 128), None, axes, grid=(45, 80))[0]
+    start = torch.tensor([rows - 2], dtype=torch.int32, device=dev)
+    want = ops.axial_rope(x[-2:].view(1, 2, 40, 128), None, axes, grid=(45, 80), start=start)[0]
+    assert torch.equal(got[:, :, -2:], want)
+
+
+def _calls(dev, seed):
+    """A run of the operators as a block uses them, on inputs of its own."""
+    g = torch.Generator().manual_seed(seed)
+    rows, C, F = 300, 640, 1100
+    x, y = _randn(g, rows, C, dtype=BF).to(dev), _randn(g, rows, C, dtype=BF).to(dev)
+    gate, scale, shift = (_randn(g, C).to(dev) for _ in range(3))
+    w1, w2 = (ops.quantize_fp8(_randn(g, *s, dtype=BF, std=0.05).to(dev)) for s in ((F, C), (C, F)))
+    b1, b2 = _randn(g, F, dtype=BF).to(dev), _randn(g, C, dtype=BF).to(dev)
+    axes = ops.RotaryAxes(128, (44, 42, 42))
+    start = torch.tensor([7], dtype=torch.int32, device=dev)
+
+    def run():
+        r, codes, scales = ops.residual_norm(x, y, gate, scale=scale, shift=shift, quantize=True)
+        codes, scales = ops.linear_fp8(codes, *w1, scales, bias=b1, activation="gelu_tanh", quantize=True, out_dtype=BF)
+        o = ops.linear_fp8(codes, *w2, scales, bias=b2, gate=gate, residual=r)
+        p = ops.linear_fp8(o, *w1)
+        q, k = ops.axial_rope(o.view(1, rows, 5, 128), r.view(1, rows, 5, 128), axes, grid=(5, 6), start=start)
+        return r, codes.view(torch.uint8), scales.view(torch.uint8), o, p, q, k
+
+    return run, x, start
+
+
+def test_block_operators_on_another_stream_and_in_threads(dev):
+    import threading
+
+    runs = [_calls(dev, seed)[0] for seed in (1, 2)]
+    want = [run() for run in runs]
+    torch.cuda.synchronize()
+    s = torch.cuda.Stream()
+    s.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(s):
+        got = runs[0]()
+    s.synchronize()
+    assert all(torch.equal(a, b) for a, b in zip(got, want[0]))
+    bad = []
+
+    def work(i):
+        stream = torch.cuda.Stream()
+        with torch.cuda.stream(stream):
+            for _ in range(20):
+                if not all(torch.equal(a, b) for a, b in zip(runs[i](), want[i])):
+                    bad.append(i)
+        stream.synchronize()
+
+    threads = [threading.Thread(target=work, args=(i,)) for i in range(2)]
+    for t in threads:
+        t.start()
+    for t in threads:
+        t.join()
+    assert not bad
+
+
+def test_block_operators_in_graphs(dev):
+    """Two captured runs, replayed by turns and at once with new inputs between."""
+    made = [_calls(dev, seed) for seed in (3, 4)]
+    graphs, outs = [], []
+    for run, _, _ in made:
+        run()
+        torch.cuda.synchronize()
+        g = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(g):
+            outs.append(run())
+        graphs.append(g)
+    streams = [torch.cuda.Stream() for _ in graphs]
+    for turn in range(4):
+        for i, (run, x, start) in enumerate(made):
+            x.copy_(torch.randn(x.shape, generator=torch.Generator().manual_seed(10 * turn + i)).to(BF))
+            start.fill_(1000 * turn + i)
+        torch.cuda.synchronize()
+        for g, s in zip(graphs, streams):
+            with torch.cuda.stream(s):
+                g.replay()
+        torch.cuda.synchronize()
+        for (run, _, _), got in zip(made, outs):
+            assert all(torch.equal(a, b) for a, b in zip(got, run()))

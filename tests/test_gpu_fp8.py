@@ -6,7 +6,8 @@ import pytest
 import torch
 
 import block_refs as refs
-from dfsattn_amd import _lib, ops
+from dfsattn_amd import ops
+from test_block_ops_host import FORMS, form
 
 pytestmark = pytest.mark.gpu
 BF, HF = torch.bfloat16, torch.float16
@@ -180,3 +181,113 @@ def test_linear_fp8_large_tiles(dev, m, n, k, codes, act):
         assert torch.equal(a.view(torch.uint8), b.view(torch.uint8))
     d[3], d[1] = ops._scales_laid_out(d[3]), d[1] if d[1] is None else ops._scales_laid_out(d[1])
     assert torch.equal(got, call())
+
+
+@pytest.mark.parametrize("dtype", [BF, HF])
+@pytest.mark.parametrize("m,n,k,want", FORMS)
+def test_linear_fp8_forms(dev, m, n, k, want, dtype):
+    """Every kernel that sizes can choose, both types, all steps of the epilogue;
+    x in codes and in 16 bits, the result in both; what surrounds out stays."""
+    print(f"linear_fp8 form {want}: {m} x {n} x {k} {dtype}", flush=True)
+    assert form(m, n, k) == want
+    g = torch.Generator().manual_seed(m + 3 * n + k)
+    x, w = _hidden(g, m, k, dtype), _randn(g, n, k, dtype=dtype, std=2 / math.sqrt(k))
+    b, gate, r = _randn(g, n, dtype=dtype), torch.randn(n, generator=g), _randn(g, m, n, dtype=dtype)
+    xt, wt = refs.to_tensors(*refs.quantize(x)), refs.to_tensors(*refs.quantize(w))
+    rows, cols = torch.arange(0, m, max(1, m // 150)), torch.arange(0, n, max(1, n // 150))
+    rows[-1], cols[-1] = m - 1, n - 1
+    ref, tol = refs.linear_fp8(refs.values(*xt)[rows], refs.values(*wt)[cols], dtype, b[cols], "gelu_tanh", gate[cols],
+                               r[rows][:, cols])
+    d = [t.to(dev) for t in (x, *xt, *wt, b, gate, r)]
+    room = torch.full((m * n + 512,), 7.0, dtype=dtype, device=dev)
+    out = room[256:256 + m * n].view(m, n)
+    for at, scales in ((d[1], d[2]), (d[0], None)):
+        got = ops.linear_fp8(at, d[3], d[4], scales, bias=d[5], activation="gelu_tanh", gate=d[6], residual=d[7],
+                             out_dtype=dtype, out=out)
+        _within(got.cpu()[rows][:, cols], ref, tol, "form")
+        assert bool((room[:256] == 7).all()) and bool((room[256 + m * n:] == 7).all())
+        codes = ops.linear_fp8(at, d[3], d[4], scales, bias=d[5], activation="gelu_tanh", gate=d[6], residual=d[7],
+                               out_dtype=dtype, quantize=True)
+        for a, b_ in zip(codes, ops.quantize_fp8(got)):
+            assert torch.equal(a.view(torch.uint8), b_.view(torch.uint8))
+
+
+@pytest.mark.parametrize("m,n,k", [(2, 100, 300), (40, 200, 700), (300, 520, 1000), (913, 7811, 224)])
+def test_linear_fp8_infinities_and_nan_stay_in_their_rows(dev, m, n, k):
+    """Values of x that are not finite make their row NaN, others what they are
+    without them; a NaN scale of w its output."""
+    print(f"linear_fp8 not finite {m} x {n} x {k}", flush=True)
+    g = torch.Generator().manual_seed(m)
+    x, w = _hidden(g, m, k, BF), _randn(g, n, k, dtype=BF)
+    wt = [t.to(dev) for t in refs.to_tensors(*refs.quantize(w))]
+    whole = ops.linear_fp8(x.to(dev), *wt)
+    x[0, 5], x[m - 1, k - 1] = math.inf, math.nan
+    keep = torch.ones(m, dtype=torch.bool)
+    keep[[0, m - 1]] = False
+    got = ops.linear_fp8(x.to(dev), *wt)
+    assert bool(torch.isnan(got[[0, m - 1]]).all())
+    assert torch.equal(got[keep], whole[keep])
+    bad = wt[1].view(torch.uint8).clone()
+    bad[3, 0] = 255
+    got = ops.linear_fp8(x.to(dev), wt[0], bad.view(torch.float8_e8m0fnu))
+    others = torch.arange(n) != 3
+    assert bool(torch.isnan(got[:, 3]).all()) and torch.equal(got[keep][:, others], whole[keep][:, others])
+
+
+@pytest.mark.parametrize("m", [1, 5, 40, 130, 700])
+def test_linear_fp8_strided_rows_and_batches(dev, m):
+    """Codes inside wider rows on and off 16-byte boundaries, a batch axis, scales
+    of any strides, a residual that is a transposed view."""
+    g = torch.Generator().manual_seed(m)
+    k, n = 272, 136
+    x, w, r = _hidden(g, 2 * m, k, BF), _randn(g, n, k, dtype=BF, std=0.1), _randn(g, n, 2, m, dtype=BF)
+    (xc, xs), (wc, ws) = refs.to_tensors(*refs.quantize(x)), refs.to_tensors(*refs.quantize(w))
+    ref, tol = refs.linear_fp8(refs.values(xc, xs), refs.values(wc, ws), BF, None, None, None,
+                               r.permute(1, 2, 0).reshape(-1, n))
+    rd = r.to(dev).permute(1, 2, 0)
+    for off in (0, 16, 3):
+        print(f"linear_fp8 strided m={m} offset={off}", flush=True)
+
+        def inside(t, pad):
+            wide = torch.zeros((*t.shape[:-1], t.shape[-1] + pad), dtype=torch.uint8)
+            wide[..., off:off + t.shape[-1]] = t.view(torch.uint8)
+            return wide.to(dev)[..., off:off + t.shape[-1]].view(t.dtype)
+
+        got = ops.linear_fp8(inside(xc.view(2, m, k), 48), inside(wc, 32), inside(ws, 25), inside(xs.view(2, m, -1), 27),
+                             residual=rd)
+        assert got.shape == (2, m, n)
+        _within(got.reshape(-1, n), ref, tol, "strided")
+        half = torch.zeros(2, m, k + 24, dtype=BF)
+        half[:, :, off:off + k] = x.view(2, m, k)
+        assert torch.equal(got, ops.linear_fp8(half.to(dev)[:, :, off:off + k], wc.to(dev), ws.to(dev), residual=rd))
+
+
+def test_linear_fp8_empty_and_one(dev):
+    w = ops.quantize_fp8(torch.ones(8, 16, dtype=BF, device=dev))
+    assert ops.linear_fp8(torch.zeros(0, 16, dtype=BF, device=dev), *w).shape == (0, 8)
+    codes, scales = ops.linear_fp8(torch.zeros(0, 16, dtype=BF, device=dev), *w, quantize=True)
+    assert codes.shape == (0, 8) and scales.shape == (0, 1)
+    one = ops.linear_fp8(torch.ones(16, dtype=BF, device=dev), *w)
+    assert one.shape == (8,) and bool((one == 16).all())
+    codes, scales = ops.linear_fp8(torch.ones(16, dtype=BF, device=dev), *w, quantize=True)
+    assert codes.shape == (8,) and scales.shape == (1,)
+
+
+def test_fp8_offsets_beyond_32_bits(dev):
+    """More than 2^31 elements of x to quantise, and of outputs."""
+    print("quantize 430,000 x 5,120", flush=True)
+    x = torch.zeros(430000, 5120, dtype=BF, device=dev)
+    x[-3:] = torch.randn(3, 5120, generator=torch.Generator().manual_seed(0)).to(BF).to(dev)
+    codes, scales = ops.quantize_fp8(x)
+    _same_codes((codes[-3:], scales[-3:]), refs.quantize(x[-3:].cpu()))
+    del x, codes, scales
+    print("linear_fp8 160,000 x 13,824 x 128", flush=True)
+    g = torch.Generator().manual_seed(1)
+    x, w = _randn(g, 160000, 128, dtype=BF), _randn(g, 13824, 128, dtype=BF, std=0.1)
+    wt = [t.to(dev) for t in refs.to_tensors(*refs.quantize(w))]
+    got = ops.linear_fp8(x.to(dev), *wt)
+    alone = ops.linear_fp8(x[-5:].to(dev), *wt)
+    ref, tol = refs.linear_fp8(refs.values(*refs.to_tensors(*refs.quantize(x[-5:]))),
+                               refs.values(*(t.cpu() for t in wt)), BF)
+    _within(got[-5:], ref, tol, "last rows")
+    _within(alone, ref, tol, "alone")
