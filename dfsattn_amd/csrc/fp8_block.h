@@ -74,6 +74,27 @@ __device__ __forceinline__ uint32_t top_bits8(const uint4& v) {
   return max(static_cast<uint32_t>(m.x), static_cast<uint32_t>(m.y));
 }
 
+// Eight codes of finite 16-bit values under a scale byte of 1 at least.
+template <bool F16>
+__device__ __forceinline__ uint2 to_codes8_scaled(const uint4& v, uint32_t scale) {
+  typedef __bf16 bf16x2 __attribute__((ext_vector_type(2)));
+  typedef _Float16 f16x2 __attribute__((ext_vector_type(2)));
+  typedef short s16x2 __attribute__((ext_vector_type(2)));
+  const float s = __uint_as_float(scale << 23);
+  auto pair = [&](uint32_t lo, uint32_t hi) {
+    s16x2 r = {0, 0};
+    if constexpr (F16) {
+      r = __builtin_amdgcn_cvt_scalef32_pk_fp8_f16(r, __builtin_bit_cast(f16x2, lo), s, false);
+      r = __builtin_amdgcn_cvt_scalef32_pk_fp8_f16(r, __builtin_bit_cast(f16x2, hi), s, true);
+    } else {
+      r = __builtin_amdgcn_cvt_scalef32_pk_fp8_bf16(r, __builtin_bit_cast(bf16x2, lo), s, false);
+      r = __builtin_amdgcn_cvt_scalef32_pk_fp8_bf16(r, __builtin_bit_cast(bf16x2, hi), s, true);
+    }
+    return __builtin_bit_cast(uint32_t, r);
+  };
+  return make_uint2(pair(v.x, v.y), pair(v.z, v.w));
+}
+
 // A block of 128 values held by LANES neighbouring lanes, eight in each of the
 // N vectors of a lane (zeros where the row has ended): its scale byte and codes.
 // Magnitudes are compared as integers and the conversion takes pairs of 16-bit
@@ -83,29 +104,14 @@ __device__ __forceinline__ uint32_t top_bits8(const uint4& v) {
 template <bool F16, int LANES, int N>
 __device__ __forceinline__ uint32_t encode(const uint4 (&v)[N], uint2 (&codes)[N]) {
   static_assert(LANES * N == 16, "a block has 128 values");
-  typedef __bf16 bf16x2 __attribute__((ext_vector_type(2)));
-  typedef _Float16 f16x2 __attribute__((ext_vector_type(2)));
-  typedef short s16x2 __attribute__((ext_vector_type(2)));
   uint32_t top = 0;
 #pragma unroll
   for (int k = 0; k < N; ++k) top = max(top, top_bits8(v[k]));
   top = group_max<LANES>(top);
   uint32_t scale = block_scale(F16 ? f16_bits_to_f32(top) : bf16_bits_to_f32(top));
   if (top < (F16 ? 0x7c00u : 0x7f80u) && scale > 0) {
-    const float s = __uint_as_float(scale << 23);
-    auto pair = [&](uint32_t lo, uint32_t hi) {
-      s16x2 r = {0, 0};
-      if constexpr (F16) {
-        r = __builtin_amdgcn_cvt_scalef32_pk_fp8_f16(r, __builtin_bit_cast(f16x2, lo), s, false);
-        r = __builtin_amdgcn_cvt_scalef32_pk_fp8_f16(r, __builtin_bit_cast(f16x2, hi), s, true);
-      } else {
-        r = __builtin_amdgcn_cvt_scalef32_pk_fp8_bf16(r, __builtin_bit_cast(bf16x2, lo), s, false);
-        r = __builtin_amdgcn_cvt_scalef32_pk_fp8_bf16(r, __builtin_bit_cast(bf16x2, hi), s, true);
-      }
-      return __builtin_bit_cast(uint32_t, r);
-    };
 #pragma unroll
-    for (int k = 0; k < N; ++k) codes[k] = make_uint2(pair(v[k].x, v[k].y), pair(v[k].z, v[k].w));
+    for (int k = 0; k < N; ++k) codes[k] = to_codes8_scaled<F16>(v[k], scale);
     return scale;
   }
   float f[N][8], most = 0.f;

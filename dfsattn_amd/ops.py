@@ -716,7 +716,7 @@ Shape = Tuple[int, ...]
 
 def _refuse_grad(entry: str, *tensors: Optional[torch.Tensor]) -> None:
     """These operators have no backward pass: a graph would lose it silently."""
-    if torch.is_grad_enabled() and any([t is not None and t.requires_grad for t in tensors]):
+    if torch.is_grad_enabled() and any([t.requires_grad for t in tensors if t is not None]):
         raise RuntimeError(f"{entry} has no backward pass: call it under torch.no_grad() or inference_mode()")
 
 
@@ -1202,25 +1202,26 @@ def _scale_blocks(k: int) -> int:
     return -(-k // SCALE_BLOCK)
 
 
-def _empty_scales(like: torch.Tensor, lead: Shape, blocks: int) -> torch.Tensor:
-    """[*lead, blocks] scales whose storage holds a block's scales of all rows one behind the other."""
-    t = torch.empty((blocks, *lead), dtype=E8M0, device=like.device)
-    return t.movedim(0, -1) if lead else t
+def _scales_layout(lead: Shape, k: int) -> Tuple[Shape, Shape]:
+    """Shape and strides of scales [*lead, blocks] whose storage holds a block's
+    scales of all rows one behind the other."""
+    return (*lead, _scale_blocks(k)), (*_contiguous_stride(lead), math.prod(lead))
 
 
 @functools.lru_cache(maxsize=1024)
 def _quantize_plan(shape: Shape, stride: Shape, dtype: torch.dtype):
-    """(argument block up to the pointers, or None where rows do not join, rows) of a ``quantize_fp8`` call."""
+    """(argument block up to the pointers, or None where rows do not join or
+    there are none, shape and strides of the scales) of a ``quantize_fp8`` call."""
     if dtype not in HALF:
         raise ValueError(f"quantize_fp8: x must be bf16 or f16, got {dtype}")
     if len(shape) < 1 or shape[-1] == 0:
         raise ValueError(f"quantize_fp8: x must be [..., K] with K > 0, got {tuple(shape)}")
-    rows, ld = math.prod(shape[:-1]), _row_stride(shape, stride)
-    if ld is None:
-        return None, rows
+    rows, ld, layout = math.prod(shape[:-1]), _row_stride(shape, stride), _scales_layout(shape[:-1], shape[-1])
+    if ld is None or rows == 0:
+        return None, layout
     a = _lib.QuantizeFp8Args()
     a.rows, a.k, a.dtype, a.x_stride, a.values_stride, a.scales_stride = rows, shape[-1], DTYPE_CODE[dtype], ld, shape[-1], rows
-    return bytes(a)[:_pointers(a, "x")], rows
+    return bytes(a)[:_pointers(a, "x")], layout
 
 
 def quantize_fp8(x: torch.Tensor) -> Tuple[torch.Tensor, torch.Tensor]:
@@ -1233,13 +1234,13 @@ def quantize_fp8(x: torch.Tensor) -> Tuple[torch.Tensor, torch.Tensor]:
     that holds a block's scales of all rows together, as ``linear_fp8`` reads
     them in place. No backward pass."""
     _refuse_grad("quantize_fp8", x)
-    head, rows = _quantize_plan(x.shape, x.stride(), x.dtype)
+    head, layout = _quantize_plan(x.shape, x.stride(), x.dtype)
     _one_device(x)
-    if head is None and rows:
+    if head is None and x.numel():
         return quantize_fp8(x.contiguous())
-    values = torch.empty(x.shape, dtype=E4M3, device=x.device)
-    scales = _empty_scales(x, x.shape[:-1], _scale_blocks(x.shape[-1]))
-    if rows:
+    values = torch.empty_like(x, dtype=E4M3, memory_format=torch.contiguous_format)
+    scales = x.new_empty_strided(*layout, dtype=E8M0)
+    if head is not None:
         _call_on(x.device, "dfs_quantize_fp8",
                  head + _QUANTIZE_POINTERS.pack(x.data_ptr(), values.data_ptr(), scales.data_ptr()))
     return values, scales
@@ -1267,8 +1268,8 @@ def _linear_fp8_plan(x_shape: Shape, x_stride: Shape, x_dtype: torch.dtype, w_sh
                      ws: Tuple[Shape, Shape, torch.dtype], out_dtype: Optional[torch.dtype], activation: Optional[str],
                      bias: Optional[Tuple[Shape, torch.dtype]], residual: Optional[Tuple[Shape, Shape, torch.dtype]],
                      quantize: bool):
-    """(shape of out, its dtype, what is read in place: x, weight, residual and
-    both scales, and the argument block up to the pointers with its workspace
+    """(shape of out, its dtype, shape and strides of its scales, what is read in
+    place: x, weight, residual and both scales, and the argument block up to the pointers with its workspace
     bytes by the alignment of x, weight and their scales) of a ``linear_fp8`` call."""
     entry = "linear_fp8"
     codes = x_dtype == E4M3
@@ -1303,7 +1304,7 @@ def _linear_fp8_plan(x_shape: Shape, x_stride: Shape, x_dtype: torch.dtype, w_sh
     ldxs = 0 if xs is None else _scales_in_place(xs[0], xs[1])
     ldws = _scales_in_place(ws[0], ws[1])
     if rows == 0 or None in (ldx, ldw, ldr, ldxs, ldws):
-        return shape, dtype, tuple(t is not None for t in (ldx, ldw, ldr, ldxs, ldws)), None
+        return shape, dtype, _scales_layout(shape[:-1], n), tuple(t is not None for t in (ldx, ldw, ldr, ldxs, ldws)), None
     a = _lib.LinearFp8Args()
     a.rows, a.n, a.k, a.activation, a.dtype = rows, n, k, ACTIVATION_CODE[activation], DTYPE_CODE[dtype]
     a.x_dtype = _E4M3_CODE if codes else a.dtype
@@ -1327,7 +1328,7 @@ def _linear_fp8_plan(x_shape: Shape, x_stride: Shape, x_dtype: torch.dtype, w_sh
             raise _lib.DfsKernelError(_lib.lib().dfs_last_error().decode(errors="replace"))
         a.workspace_bytes = size
         blocks_of.append((bytes(a)[:_pointers(a, "x")], size))
-    return shape, dtype, None, blocks_of
+    return shape, dtype, _scales_layout(shape[:-1], n), None, blocks_of
 
 
 def linear_fp8(x: torch.Tensor, weight: torch.Tensor, weight_scales: torch.Tensor,
@@ -1350,7 +1351,7 @@ def linear_fp8(x: torch.Tensor, weight: torch.Tensor, weight_scales: torch.Tenso
     if weight_scales is None:
         raise ValueError(f"{entry}: weight_scales are needed")
     quantize = bool(quantize)
-    shape, dtype, in_place, blocks = _linear_fp8_plan(
+    shape, dtype, layout, in_place, blocks = _linear_fp8_plan(
         x.shape, x.stride(), x.dtype, weight.shape, weight.stride(), weight.dtype,
         None if x_scales is None else (x_scales.shape, x_scales.stride(), x_scales.dtype),
         (weight_scales.shape, weight_scales.stride(), weight_scales.dtype), out_dtype, activation,
@@ -1376,14 +1377,14 @@ def linear_fp8(x: torch.Tensor, weight: torch.Tensor, weight_scales: torch.Tenso
         return linear_fp8(x, weight, weight_scales, x_scales, bias, activation, gate, residual, out, out_dtype, quantize)
     scales = None
     if quantize:
-        out = torch.empty(shape, dtype=E4M3, device=x.device)
-        scales = _empty_scales(x, shape[:-1], _scale_blocks(shape[-1]))
+        out = x.new_empty(shape, dtype=E4M3)
+        scales = x.new_empty_strided(*layout, dtype=E8M0)
     elif out is None:
-        out = torch.empty(shape, dtype=dtype, device=x.device)
+        out = x.new_empty(shape, dtype=dtype)
     if blocks is not None:
         px, pw, pxs, pws = x.data_ptr(), weight.data_ptr(), _ptr(x_scales) or 0, weight_scales.data_ptr()
         head, size = blocks[(px % 16 == 0) + 2 * (pw % 16 == 0) + 4 * (pxs % 4 == 0) + 8 * (pws % 4 == 0)]
-        ws = torch.empty(size, dtype=torch.uint8, device=x.device) if size else None
+        ws = x.new_empty(size, dtype=torch.uint8) if size else None
         po = out.data_ptr()
         block = head + _LINEAR_FP8_POINTERS.pack(
             px, pw, pxs, pws, _ptr(bias) or 0, _ptr(gate) or 0,
@@ -1428,10 +1429,11 @@ def _vector_groups(entry: str, name: str, t: Meta, x_shape: Shape) -> Tuple[int,
 @functools.lru_cache(maxsize=1024)
 def _norm_plan(x: Meta, y: Optional[Meta], gate: Optional[Meta], scale: Optional[Meta], shift: Optional[Meta],
                weights: Tuple[Optional[Meta], ...], post_norm: Optional[str], norm: str, residual_scale: float,
-               eps: float, post_eps: float, quantize: bool):
-    """(argument block up to the pointers, or None, and, where there is none:
-    whether x and y are read in place and the shapes that gate, scale and shift
-    are laid out in, None for as they are) of a ``residual_norm`` call."""
+               eps: float, post_eps: float):
+    """(argument block up to the pointers, or None, shape and strides of the
+    scales, and, where there is no block: whether x and y are read in place and
+    the shapes that gate, scale and shift are laid out in, None for as they are)
+    of a ``residual_norm`` call. weights: post_weight, post_bias, weight, bias."""
     entry = "residual_norm"
     shape, _, dtype = x
     if dtype not in HALF or y is not None and (y[2] != dtype or y[0] != shape):
@@ -1456,7 +1458,7 @@ def _norm_plan(x: Meta, y: Optional[Meta], gate: Optional[Meta], scale: Optional
         if tuple(w[0]) != (C,) or w[2] not in DTYPE_CODE:
             raise ValueError(f"{entry}: {name} must be a [{C}] vector of bf16, f16 or float32, got {w[2]} {tuple(w[0])}")
         setattr(a, f"{name}_dtype", DTYPE_CODE[w[2]])
-    rows = math.prod(shape[:-1])
+    rows, layout = math.prod(shape[:-1]), _scales_layout(shape[:-1], C)
     lds = [0 if t is None else _row_stride(t[0], t[1]) for t in (x, y)]
     anew = [None, None, None]
     for i, (name, t) in enumerate((("gate", gate), ("scale", scale), ("shift", shift))):
@@ -1468,12 +1470,12 @@ def _norm_plan(x: Meta, y: Optional[Meta], gate: Optional[Meta], scale: Optional
         setattr(a, f"{name}_rows", each)
         setattr(a, f"{name}_stride", stride or 0)
     if rows == 0 or None in lds or any(s is not None for s in anew):
-        return None, (lds[0] is not None, lds[1] is not None), anew
+        return None, layout, (lds[0] is not None, lds[1] is not None), anew
     a.rows, a.channels, a.dtype = rows, C, DTYPE_CODE[dtype]
     a.post_norm, a.norm = NORM_CODE[post_norm], NORM_CODE[norm]
     a.x_stride, a.y_stride, a.out_stride, a.h_stride, a.h8_scales_stride = lds[0], lds[1], C, C, rows
     a.residual_scale, a.eps, a.post_eps = residual_scale, eps, post_eps
-    return bytes(a)[:_pointers(a, "x")], None, None
+    return bytes(a)[:_pointers(a, "x")], layout, None, None
 
 
 def residual_norm(x: torch.Tensor, y: Optional[torch.Tensor] = None, gate: Optional[torch.Tensor] = None,
@@ -1500,11 +1502,11 @@ def residual_norm(x: torch.Tensor, y: Optional[torch.Tensor] = None, gate: Optio
     backward pass."""
     entry = "residual_norm"
     _refuse_grad(entry, x, y, gate, post_weight, post_bias, weight, bias, scale, shift, out)
-    quantize, eps = bool(quantize), float(eps)
-    head, whole, anew = _norm_plan(
+    eps = float(eps)
+    head, layout, whole, anew = _norm_plan(
         _meta(x), _meta(y), _meta(gate), _meta(scale), _meta(shift),
         (_meta(post_weight), _meta(post_bias), _meta(weight), _meta(bias)), post_norm, norm, float(residual_scale), eps,
-        eps if post_eps is None else float(post_eps), quantize)
+        eps if post_eps is None else float(post_eps))
     if out is not None and (y is None or out.shape != x.shape or out.dtype != x.dtype or not out.is_contiguous()):
         raise ValueError(f"{entry}: out must be contiguous {x.dtype} {tuple(x.shape)}, and goes with a y, got {out.dtype} "
                          f"{tuple(out.shape)}")
@@ -1519,24 +1521,21 @@ def residual_norm(x: torch.Tensor, y: Optional[torch.Tensor] = None, gate: Optio
         return residual_norm(x, y, gate, residual_scale, post_norm, post_weight, post_bias, post_eps, norm, weight, bias,
                              scale, shift, eps, out, quantize)
     weights = [t if t is None or t.is_contiguous() else t.contiguous() for t in (post_weight, post_bias, weight, bias)]
-    device = x.device
-    if y is None:
-        r = x
-    else:
-        r = torch.empty(x.shape, dtype=x.dtype, device=device) if out is None else out
-    scales = None
+    r, scales = x if y is None else out, None
+    if r is None:
+        r = torch.empty_like(x, memory_format=torch.contiguous_format)
     if quantize:
-        h = torch.empty(x.shape, dtype=E4M3, device=device)
-        scales = _empty_scales(x, x.shape[:-1], _scale_blocks(x.shape[-1]))
+        h = torch.empty_like(x, dtype=E4M3, memory_format=torch.contiguous_format)
+        scales = x.new_empty_strided(*layout, dtype=E8M0)
     else:
-        h = torch.empty(x.shape, dtype=x.dtype, device=device)
+        h = torch.empty_like(x, memory_format=torch.contiguous_format)
     if head is not None:
         ph = h.data_ptr()
         block = head + _NORM_POINTERS.pack(
             x.data_ptr(), _ptr(y) or 0, _ptr(gate) or 0, _ptr(scale) or 0, _ptr(shift) or 0,
             *(_ptr(t) or 0 for t in weights), 0 if y is None else r.data_ptr(), 0 if quantize else ph,
             ph if quantize else 0, _ptr(scales) or 0)
-        _call_on(device, "dfs_residual_norm", block)
+        _call_on(x.device, "dfs_residual_norm", block)
     return (r, h, scales) if quantize else (r, h)
 
 
@@ -1557,24 +1556,30 @@ class RotaryAxes:
     speeds: object = 1.0
 
     def __post_init__(self):
-        for name in ("theta", "speeds"):
-            v = getattr(self, name)
-            v = tuple(float(x) for x in v) if isinstance(v, (tuple, list)) else (float(v),) * len(self.sections)
-            object.__setattr__(self, name, v)
-        object.__setattr__(self, "sections", tuple(int(n) for n in self.sections))
-        object.__setattr__(self, "head_dim", int(self.head_dim))
-        n = len(self.sections)
-        if not 1 <= n <= 4 or any(c < 0 or c % 2 for c in self.sections) or sum(self.sections) > self.head_dim:
-            raise ValueError(f"RotaryAxes: 1 to 4 sections of even numbers of channels, {self.head_dim} together at "
-                             f"most, got {self.sections}")
-        if self.head_dim < 8 or self.head_dim > 512 or self.head_dim % 8:
-            raise ValueError(f"RotaryAxes: head_dim {self.head_dim} must be a multiple of 8 up to 512")
-        if len(self.theta) != n or len(self.speeds) != n or any(
-                not (0.0 < t < math.inf) for t in self.theta) or any(not math.isfinite(v) for v in self.speeds):
-            raise ValueError(f"RotaryAxes: a positive theta and a finite speed for each axis, got {self.theta} and "
-                             f"{self.speeds}")
-        if self.layout not in ("pairs", "halves"):
-            raise ValueError(f"RotaryAxes: layout must be 'pairs' or 'halves', got {self.layout!r}")
+        self.__dict__.update(_axes_fields(int(self.head_dim), tuple([int(n) for n in self.sections]),
+                                          _one_or_each(self.theta), str(self.layout), _one_or_each(self.speeds)))
+
+
+def _one_or_each(v):
+    return tuple([float(x) for x in v]) if isinstance(v, (tuple, list)) else float(v)
+
+
+@functools.lru_cache(maxsize=256)
+def _axes_fields(head_dim: int, sections: Tuple[int, ...], theta, layout: str, speeds) -> Dict[str, object]:
+    """The checked fields of ``RotaryAxes``, theta and speeds one number for each axis."""
+    n = len(sections)
+    theta, speeds = (v if isinstance(v, tuple) else (v,) * n for v in (theta, speeds))
+    if not 1 <= n <= 4 or any(c < 0 or c % 2 for c in sections) or sum(sections) > head_dim:
+        raise ValueError(f"RotaryAxes: 1 to 4 sections of even numbers of channels, {head_dim} together at most, got "
+                         f"{sections}")
+    if head_dim < 8 or head_dim > 512 or head_dim % 8:
+        raise ValueError(f"RotaryAxes: head_dim {head_dim} must be a multiple of 8 up to 512")
+    if len(theta) != n or len(speeds) != n or any(not (0.0 < t < math.inf) for t in theta) or any(
+            not math.isfinite(v) for v in speeds):
+        raise ValueError(f"RotaryAxes: a positive theta and a finite speed for each axis, got {theta} and {speeds}")
+    if layout not in ("pairs", "halves"):
+        raise ValueError(f"RotaryAxes: layout must be 'pairs' or 'halves', got {layout!r}")
+    return {"head_dim": head_dim, "sections": sections, "theta": theta, "layout": layout, "speeds": speeds}
 
 
 @dataclass(frozen=True)
@@ -1697,8 +1702,7 @@ def axial_rope(q: torch.Tensor, k: Optional[torch.Tensor], axes: RotaryAxes, gri
             raise ValueError(f"{entry}: start goes with a grid")
         _check_lens(entry, "start", start, B)
     _one_device(q, k, start, positions, q_weight, k_weight)
-    outs = [None if t is None else t.new_empty_strided((B, t.shape[2], T, D), (T * t.shape[2] * D, D, t.shape[2] * D, 1))
-            for t in (q, k)]
+    outs = [None if t is None else t.new_empty((B, T, t.shape[2], D)).transpose(1, 2) for t in (q, k)]
     if B == 0 or T == 0:
         return tuple(outs)
     pq, pk = q.data_ptr(), _ptr(k) or 0
