@@ -32,8 +32,6 @@ void run_fp8_large_f16(const Fp8Params& p, int64_t rest, hipStream_t stream);
 namespace {
 
 typedef int i32x8 __attribute__((ext_vector_type(8)));
-
-
 typedef int i32x4 __attribute__((ext_vector_type(4)));
 __device__ __forceinline__ i32x4 chunk_at(const uint8_t* p) { return *reinterpret_cast<const i32x4*>(p); }
 __device__ __forceinline__ i32x8 join(i32x4 lo, i32x4 hi) {
@@ -49,11 +47,12 @@ __device__ __forceinline__ f32x4 mfma16(i32x8 a, i32x8 b, f32x4 c, uint32_t sa, 
                                                           static_cast<int>(sb));
 }
 
-// with_activation, the tanh form of GELU in its short form: these products take
-// half the time, so their epilogues count for twice as much.
+// with_activation with GELU in its short forms: these products take half the
+// time, so their epilogues count for twice as much.
 template <typename F>
 __host__ __device__ __forceinline__ void with_fp8_activation(int act, F&& f) {
   if (act == kActGeluTanh) return f(std::integral_constant<int, kActGeluTanhShort>{});
+  if (act == kActGelu) return f(std::integral_constant<int, kActGeluShort>{});
   with_activation(act, f);
 }
 
