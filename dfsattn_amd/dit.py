@@ -222,7 +222,7 @@ class DiTBlock(nn.Module):
                 return self._ffn_fp8(x, a, c_scale, c_shift, c_gate)
             with torch.no_grad():
                 x, h = ops.residual_norm(x, a, scale=c_scale, shift=c_shift, eps=self.norm3.eps)
-            if self.native_ffn:
+            if self.native_ffn and not any(isinstance(layer, Fp8Linear) for layer in self.ffn):
                 return self._ffn_native(h, x, c_gate)
             return ops.gated_residual(x, self._ffn_fused(h), c_gate)
         h = (self.norm1(x.float()) * (1 + scale_msa) + shift_msa).type_as(x)

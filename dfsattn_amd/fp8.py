@@ -22,21 +22,28 @@ from . import ops
 
 class Fp8Linear(nn.Module):
     """x @ weight.T + bias on 8-bit operands, in x's type (bf16 or f16). Codes and
-    scales are kept as bytes, so that casts of the module leave them alone."""
+    scales are kept as bytes, so that casts of the module leave them alone;
+    ``dtype``, that of the layer it stands for, follows them."""
 
-    def __init__(self, codes: torch.Tensor, scales: torch.Tensor, bias: Optional[torch.Tensor] = None):
+    def __init__(self, codes: torch.Tensor, scales: torch.Tensor, bias: Optional[torch.Tensor] = None,
+                 dtype: torch.dtype = torch.bfloat16):
         super().__init__()
         self.out_features, self.in_features = codes.shape
         self.register_buffer("codes", codes.view(torch.uint8))
         self.register_buffer("scales", scales.view(torch.uint8))
         self.register_buffer("bias", bias)
+        self.register_buffer("_like", torch.empty(0, dtype=dtype, device=codes.device), persistent=False)
+
+    @property
+    def dtype(self) -> torch.dtype:
+        return self._like.dtype
 
     @classmethod
     @torch.no_grad()
     def from_linear(cls, layer: nn.Linear) -> "Fp8Linear":
         """Of an nn.Linear with bf16 or f16 weights on the GPU."""
         bias = None if layer.bias is None else layer.bias.detach().clone()
-        return cls(*ops.quantize_fp8(layer.weight.detach()), bias)
+        return cls(*ops.quantize_fp8(layer.weight.detach()), bias, layer.weight.dtype)
 
     def forward(self, x: torch.Tensor, x_scales: Optional[torch.Tensor] = None, **options):
         """``options``: those of ``ops.linear_fp8``."""

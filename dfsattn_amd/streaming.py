@@ -151,8 +151,9 @@ def install_stream_processors(model, left: int, chunk: int, sinks: int = 0, righ
         if "attn2" in name:
             module.set_processor(Wan_DFSAttn_Processor2_0("full", 0.0, 16, 128, None, i, [], 0, 1, 0.0, False, True))
             continue
-        weight = module.to_k.bias if isinstance(module.to_k, Fp8Linear) else module.to_k.weight  # of the caches' type
+        to_k = module.to_k
+        weight, dtype = (to_k.codes, to_k.dtype) if isinstance(to_k, Fp8Linear) else (to_k.weight, to_k.weight.dtype)
         caches.append(StreamCache(batch, module.heads, weight.shape[0] // module.heads, left, chunk, sinks,
-                                  weight.device, weight.dtype))
+                                  weight.device, dtype))
         module.set_processor(Wan_Stream_Processor(caches[-1], right))
     return caches

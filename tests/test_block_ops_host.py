@@ -208,3 +208,9 @@ def test_every_form_of_linear_fp8_has_a_case():
     for sizes in ((0, 1, 1), (1, -1, 1), (1, 1, 0), (1, 1, 1 << 21)):
         assert form(*sizes) == -1
         assert _lib.lib().dfs_linear_fp8_workspace_size(*sizes, 0) == -1
+
+
+def test_fp8_linear_knows_its_layers_type():
+    layer = fp8.Fp8Linear(_t(8, 200, dtype=E4), _t(8, 2, dtype=E8), None, HF)
+    assert layer.dtype == HF and layer.to(torch.bfloat16).dtype == torch.bfloat16
+    assert set(layer.state_dict()) == {"codes", "scales"}

@@ -175,3 +175,34 @@ def test_model_streams_on_8_bit_layers_with_rotary_axes(dev):
         assert out.shape == frame.shape and bool(torch.isfinite(out).all())
         for c in caches:
             c.advance(h * w)
+
+
+@torch.no_grad()
+def test_stream_on_8_bit_layers_without_biases(dev):
+    """The caches are of the layers' type, which no bias tells."""
+    model = build_model(DIT_CONFIGS["tiny"], dev, torch.float16)
+    for block in model.blocks:
+        for name in ("to_q", "to_k", "to_v"):
+            getattr(block.attn1, name).bias = None
+    install_fp8(model)
+    f, h, w = model.cfg.grid
+    caches = install_stream_processors(model, left=h * w, chunk=h * w)
+    assert all(c.k.dtype == torch.float16 and c.k.device == dev for c in caches)
+    latent, ctx, _ = synth_inputs(model.cfg, dev)
+    out = model(latent[:, :, :1], torch.tensor([500.0], device=dev), ctx)
+    assert bool(torch.isfinite(out).all())
+
+
+@torch.no_grad()
+@pytest.mark.parametrize("which", [(0,), (2,), (0, 2)])
+def test_ffn_with_8_bit_layers_and_the_native_products(dev, which):
+    """native_ffn asks for the 16-bit products of both layers: a block with an
+    8-bit one runs its layers as they are."""
+    model = _model(dev)
+    block = model.blocks[0]
+    for i in which:
+        block.ffn[i] = Fp8Linear.from_linear(block.ffn[i])
+    x, ctx, temb = _block_inputs(dev, model)
+    want = block(x, ctx, temb, model.rotary_emb)
+    block.native_ffn = True
+    assert torch.equal(block(x, ctx, temb, model.rotary_emb), want)
