@@ -618,8 +618,10 @@ int dfs_quantize_fp8(const dfs_quantize_fp8_args* args, dfs_stream_t stream);
  * over blocks b of 128 channels. w [n][k] codes with w_scales [ceil(k/128)][n];
  * x [rows][k] codes with x_scales (x_dtype DFS_DTYPE_E4M3), or bf16 or f16
  * values that are quantised first (x_scales NULL). out, residual: dtype (bf16
- * or f16; x_dtype where that is one of them). Sums and epilogue are fp32,
- * rounded once to dtype. out8 / out8_scales (both or neither): the rounded
+ * or f16; x_dtype where that is one of them). The matrix instructions add the
+ * products of eight consecutive channels cut, towards zero, to a multiple of
+ * 2^-13 of the largest one's power of two; all other sums and the epilogue are
+ * fp32, rounded once to dtype. out8 / out8_scales (both or neither): the rounded
  * result is quantised instead of written, out is NULL then. The
  * workspace is the caller's, dfs_linear_fp8_workspace_size bytes (0: none),
  * with `flags` the sum of
@@ -649,8 +651,8 @@ enum { DFS_FP8_X_CODES = 1, DFS_FP8_X_ALIGNED = 2, DFS_FP8_W_ALIGNED = 4, DFS_FP
        DFS_FP8_XS_ALIGNED = 16, DFS_FP8_WS_ALIGNED = 32 };
 int64_t dfs_linear_fp8_workspace_size(int64_t rows, int64_t n, int64_t k, int flags);
 /* Host function for tests and profiles: the kernel that a call takes, which
- * goes by its sizes alone: the forms of dfs_linear_form (FEW up to 16 rows),
- * with DFS_FORM_PARTS and DFS_FORM_STREAM. */
+ * goes by its sizes alone: the forms of dfs_linear_form (FEW for 16 rows at
+ * most), with DFS_FORM_PARTS and DFS_FORM_STREAM. */
 int dfs_linear_fp8_form(int64_t rows, int64_t n, int64_t k);
 int dfs_linear_fp8(const dfs_linear_fp8_args* args, dfs_stream_t stream);
 

@@ -178,6 +178,8 @@ FORMS = [
     (16, 1003, 520, FEW | WIDE),
     (5, 4105, 264, FEW),
     (3, 16411, 16520, FEW | STREAM),
+    (9, 20011, 520, T64),
+    (13, 16411, 12008, T64 | PARTS),
     (77, 331, 328, T64),
     (33, 523, 4104, T64 | PARTS),
     (129, 7615, 168, T64X128),
