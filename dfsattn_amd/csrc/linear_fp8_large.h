@@ -74,9 +74,9 @@ __device__ __forceinline__ void store_codes8(const Fp8Params& p, int m, int n, c
 // 75,600 rows by 5,120 x 13,824 with bias, gate and residual 4.1 ms (2.6 PFLOP/s,
 // matrix cores busy 71% of the cycles at 1.63 GHz, no LDS bank conflicts): bound
 // by power, as the 16-bit products are; 128 x 128 tiles took 6.5. By 13,824 x 5,120
-// with GELU and the result quantised 4.6 (busy 62%): the epilogue is a seventh of
-// it and runs alone, since a workgroup fills a CU; written as 16 bits and
-// quantised by a pass of its own 5.3.
+// with bias 4.05, with GELU's tanh form 4.26 and its erf form 4.66 (an epilogue
+// runs alone, since a workgroup fills a CU), with the first and the result
+// quantised 4.29; a pass of its own for that took 1.1 more.
 template <bool F16, int ACT>
 __global__ void __launch_bounds__(256, 1) fp8_big_kernel(Fp8Params p) {
   __shared__ __attribute__((aligned(16))) uint8_t a00[128 * 128], a01[128 * 128], a10[128 * 128], a11[128 * 128];
