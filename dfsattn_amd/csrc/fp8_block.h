@@ -11,9 +11,19 @@
 #include "common.h"
 
 namespace dfs {
-namespace {
 
 constexpr int kScaleBlock = 128;
+
+// Rows of k codes at any address and stride, laid out in rows of `wide` on 16-byte
+// boundaries, zeros behind the k.
+struct PadCodes {
+  const uint8_t* src;
+  int64_t ld, rows;
+  int k, wide;
+  uint8_t* dst;
+};
+
+namespace {
 
 // e + 127 of a block whose largest finite magnitude is `top`. Its bits give it:
 // top = 1.m * 2^p <= 1.75 * 2^8 * 2^e. fp32 subnormals have p = -127 here: they
@@ -128,12 +138,39 @@ __device__ __forceinline__ uint32_t encode(const uint4 (&v)[N], uint2 (&codes)[N
   return scale;
 }
 
+// By a workgroup of 256, number `group` of `groups`: sixteen codes a thread.
+__device__ __forceinline__ void pad_codes(const PadCodes& p, int64_t group, int64_t groups) {
+  const int chunks = p.wide / 16;
+  for (int64_t id = group * 256 + threadIdx.x; id < p.rows * chunks; id += groups * 256) {
+    const int64_t r = id / chunks;
+    const int c = static_cast<int>(id - r * chunks) * 16;
+    const uint8_t* const s = p.src + r * p.ld;
+    uint4 v;
+    if (c + 16 <= p.k) {
+      __builtin_memcpy(&v, s + c, 16);
+    } else {
+      uint8_t t[16];
+#pragma unroll
+      for (int i = 0; i < 16; ++i) t[i] = s[min(c + i, p.k - 1)];
+#pragma unroll
+      for (int i = 0; i < 16; ++i) t[i] = c + i < p.k ? t[i] : 0;
+      __builtin_memcpy(&v, t, 16);
+    }
+    *reinterpret_cast<uint4*>(p.dst + r * p.wide + c) = v;
+  }
+}
+inline unsigned pad_groups(const PadCodes& p) {
+  const int64_t groups = (p.rows * (p.wide / 16) + 255) / 256;
+  return static_cast<unsigned>(groups < (1 << 20) ? groups : 1 << 20);
+}
+
 }  // namespace
 
 // Enqueues the quantisation of `rows` rows of k 16-bit values (row strides in
 // elements) into codes (row stride ldv bytes, zeros from k up to `fill`) and
-// scale bytes (block stride lds, the rows of a block one behind the other).
+// scale bytes (block stride lds, the rows of a block one behind the other), and in
+// the same launch of the codes of `also`, where there are any.
 void launch_quantize(const uint16_t* x, int64_t rows, int64_t k, int64_t ldx, bool f16, uint8_t* values, int64_t ldv,
-                     int64_t fill, uint8_t* scales, int64_t lds, hipStream_t stream);
+                     int64_t fill, uint8_t* scales, int64_t lds, hipStream_t stream, const PadCodes* also = nullptr);
 
 }  // namespace dfs

@@ -359,28 +359,7 @@ __global__ void __launch_bounds__(256) pad_scales_kernel(const uint8_t* src, int
   if (r < wide) dst[static_cast<int64_t>(blockIdx.y) * wide + r] = r < rows ? src[blockIdx.y * ld + r] : 0;
 }
 
-// Rows of k codes at any address and stride into rows of `wide` on 16-byte
-// boundaries, zeros behind the k: sixteen codes a thread, a row a grid row.
-__global__ void __launch_bounds__(256) pad_codes_kernel(const uint8_t* src, int64_t ld, int rows, int k, int wide,
-                                                        uint8_t* dst) {
-  const int c = (blockIdx.x * 256 + threadIdx.x) * 16;
-  if (c >= wide) return;
-  for (int r = blockIdx.y; r < rows; r += gridDim.y) {
-    const uint8_t* const s = src + r * ld + c;
-    uint4 v = make_uint4(0, 0, 0, 0);
-    if (c + 16 <= k) {
-      __builtin_memcpy(&v, s, 16);
-    } else {
-      uint8_t t[16];
-#pragma unroll
-      for (int i = 0; i < 16; ++i) t[i] = src[r * ld + min(c + i, k - 1)];
-#pragma unroll
-      for (int i = 0; i < 16; ++i) t[i] = c + i < k ? t[i] : 0;
-      __builtin_memcpy(&v, t, 16);
-    }
-    *reinterpret_cast<uint4*>(dst + static_cast<int64_t>(r) * wide + c) = v;
-  }
-}
+__global__ void __launch_bounds__(256) pad_codes_kernel(PadCodes p) { pad_codes(p, blockIdx.x, gridDim.x); }
 
 template <int NI, int MI, int WN, int WM, int NS>
 void launch_tile(const Fp8Params& p, bool f16, hipStream_t st) {
@@ -587,9 +566,10 @@ extern "C" int dfs_linear_fp8(const dfs_linear_fp8_args* a, dfs_stream_t stream)
   const Workspace at = workspace_of(cut, rows, n, k, flags);
   DFS_REQUIRE(at.total == 0 || (a->workspace != nullptr && a->workspace_bytes >= at.total && addr(a->workspace) % 16 == 0),
               "%s: a 16-byte aligned workspace of %lld bytes is needed", name, (long long)at.total);
-  // A launch holds fewer than 2^32 threads.
+  // A launch holds fewer than 2^32 threads (x's quantisation, that of w's rows laid
+  // out beside it among them).
   DFS_REQUIRE(((rows + 63) / 64) * ((n + 63) / 64) * cut.splits < (1 << 24) && kb < 65536 && (cut.form != kFew || n < (1 << 27)) &&
-                  rows * kb < (1 << 28) && (!out8 || rows * nb < (1 << 28)),
+                  rows * kb < (1 << 28) - (codes ? 0 : 1 << 24) && (!out8 || rows * nb < (1 << 28)),
               "%s: too many outputs", name);
   char* const ws = static_cast<char*>(a->workspace);
   hipStream_t st = reinterpret_cast<hipStream_t>(stream);
@@ -607,26 +587,28 @@ extern "C" int dfs_linear_fp8(const dfs_linear_fp8_args* a, dfs_stream_t stream)
   p.ldw = a->w_stride;
   p.ldws = a->w_scales_stride;
   const int64_t wide = up16(k);
-  auto lay_out = [&](const uint8_t* src, int64_t ld, int64_t count, int64_t offset) {
-    uint8_t* const dst = reinterpret_cast<uint8_t*>(ws + offset);
-    const dim3 grid(static_cast<unsigned>((wide + 4095) / 4096), static_cast<unsigned>(std::min<int64_t>(count, 65535)));
-    pad_codes_kernel<<<grid, 256, 0, st>>>(src, ld, static_cast<int>(count), static_cast<int>(k), static_cast<int>(wide),
-                                           dst);
-    return dst;
+  auto codes_of = [&](const uint8_t* src, int64_t ld, int64_t count, int64_t offset) {
+    return PadCodes{src, ld, count, static_cast<int>(k), static_cast<int>(wide), reinterpret_cast<uint8_t*>(ws + offset)};
   };
-  if (!codes) {
+  const PadCodes w_codes = codes_of(p.w, p.ldw, n, at.w);
+  const bool pad_w = !(flags & DFS_FP8_W_ALIGNED);
+  if (!codes) {  // w's codes in the same launch
     uint8_t *const xq = reinterpret_cast<uint8_t*>(ws + at.x), *const xsq = reinterpret_cast<uint8_t*>(ws + at.xs);
     p.ldx = wide;
     p.ldxs = up4(rows);
-    launch_quantize(static_cast<const uint16_t*>(a->x), rows, k, a->x_stride, f16, xq, wide, wide, xsq, p.ldxs, st);
+    launch_quantize(static_cast<const uint16_t*>(a->x), rows, k, a->x_stride, f16, xq, wide, wide, xsq, p.ldxs, st,
+                    pad_w ? &w_codes : nullptr);
     p.x = xq;
     p.xs = xsq;
   } else if (!(flags & DFS_FP8_X_ALIGNED)) {
-    p.x = lay_out(p.x, p.ldx, rows, at.x);
+    const PadCodes x_codes = codes_of(p.x, p.ldx, rows, at.x);
+    pad_codes_kernel<<<pad_groups(x_codes), 256, 0, st>>>(x_codes);
+    p.x = x_codes.dst;
     p.ldx = wide;
   }
-  if (!(flags & DFS_FP8_W_ALIGNED)) {
-    p.w = lay_out(p.w, p.ldw, n, at.w);
+  if (pad_w) {
+    if (codes) pad_codes_kernel<<<pad_groups(w_codes), 256, 0, st>>>(w_codes);
+    p.w = w_codes.dst;
     p.ldw = wide;
   }
   auto fours = [&](const uint8_t* src, int64_t ld, int64_t count, int64_t offset) {

@@ -21,7 +21,7 @@ struct QuantizeParams {
 // values' bits as integers and pairs are converted with their scale by one
 // instruction; in fp32, value by value, it was 204.
 template <bool F16>
-__global__ void __launch_bounds__(256) quantize_kernel(QuantizeParams p) {
+__device__ __forceinline__ void quantize_group(const QuantizeParams& p) {
   const int64_t id = static_cast<int64_t>(blockIdx.x) * 16 + (threadIdx.x >> 4);
   if (id >= static_cast<int64_t>(p.rows) * p.blocks) return;  // whole groups of sixteen lanes
   const int row = static_cast<int>(id / p.blocks), block = static_cast<int>(id - static_cast<int64_t>(row) * p.blocks);
@@ -55,13 +55,37 @@ __global__ void __launch_bounds__(256) quantize_kernel(QuantizeParams p) {
   if (l16 == 0) p.scales[block * p.lds + row] = static_cast<uint8_t>(scale);
 }
 
+template <bool F16>
+__global__ void __launch_bounds__(256) quantize_kernel(QuantizeParams p) {
+  quantize_group<F16>(p);
+}
+// With codes to be laid out by the workgroups behind those of the values: a
+// launch less where a product needs both (333 rows by 1,017 x 709 in f16 16.4 us with
+// two, 13.2 with one).
+template <bool F16>
+__global__ void __launch_bounds__(256) quantize_pad_kernel(QuantizeParams p, int groups, PadCodes codes) {
+  const int group = static_cast<int>(blockIdx.x);
+  if (group < groups)
+    quantize_group<F16>(p);
+  else
+    pad_codes(codes, group - groups, static_cast<int>(gridDim.x) - groups);
+}
+
 }  // namespace
 
 void launch_quantize(const uint16_t* x, int64_t rows, int64_t k, int64_t ldx, bool f16, uint8_t* values, int64_t ldv,
-                     int64_t fill, uint8_t* scales, int64_t lds, hipStream_t stream) {
+                     int64_t fill, uint8_t* scales, int64_t lds, hipStream_t stream, const PadCodes* also) {
   QuantizeParams p{x, values, scales, ldx, ldv, lds, static_cast<int>(rows), static_cast<int>(k),
                    static_cast<int>(fill), static_cast<int>((k + kScaleBlock - 1) / kScaleBlock)};
-  const dim3 grid(static_cast<unsigned>((rows * p.blocks + 15) / 16));
+  const int groups = static_cast<int>((rows * p.blocks + 15) / 16);
+  if (also) {
+    const int more = static_cast<int>(pad_groups(*also));
+    const dim3 grid(static_cast<unsigned>(groups) + static_cast<unsigned>(more));
+    f16 ? quantize_pad_kernel<true><<<grid, 256, 0, stream>>>(p, groups, *also)
+        : quantize_pad_kernel<false><<<grid, 256, 0, stream>>>(p, groups, *also);
+    return;
+  }
+  const dim3 grid(static_cast<unsigned>(groups));
   if (f16)
     quantize_kernel<true><<<grid, 256, 0, stream>>>(p);
   else

@@ -1560,6 +1560,10 @@ class RotaryAxes:
     def __post_init__(self):
         self.__dict__.update(_axes_fields(int(self.head_dim), tuple([int(n) for n in self.sections]),
                                           _one_or_each(self.theta), str(self.layout), _one_or_each(self.speeds)))
+        self.__dict__["_hash"] = hash((self.head_dim, self.sections, self.theta, self.layout == "pairs", self.speeds))
+
+    def __hash__(self) -> int:  # taken once: every call looks its plan up by it
+        return self._hash  # of numbers alone, so that it holds in other processes
 
 
 def _one_or_each(v):
@@ -1704,7 +1708,8 @@ def axial_rope(q: torch.Tensor, k: Optional[torch.Tensor], axes: RotaryAxes, gri
             raise ValueError(f"{entry}: start goes with a grid")
         _check_lens(entry, "start", start, B)
     _one_device(q, k, start, positions, q_weight, k_weight)
-    outs = [None if t is None else t.new_empty((B, T, t.shape[2], D)).transpose(1, 2) for t in (q, k)]
+    outs = [None if t is None else t.new_empty_strided((B, t.shape[2], T, D), (T * t.shape[2] * D, D, t.shape[2] * D, 1))
+            for t in (q, k)]
     if B == 0 or T == 0:
         return tuple(outs)
     pq, pk = q.data_ptr(), _ptr(k) or 0

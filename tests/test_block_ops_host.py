@@ -1,6 +1,9 @@
 """What ops.quantize_fp8, ops.linear_fp8, ops.residual_norm and ops.axial_rope
 refuse, before any device is touched, and the sizes that reach each kernel of
 linear_fp8."""
+import copy
+import dataclasses
+import pickle
 import random
 
 import pytest
@@ -216,3 +219,11 @@ def test_fp8_linear_knows_its_layers_type():
     layer = fp8.Fp8Linear(_t(8, 200, dtype=E4), _t(8, 2, dtype=E8), None, HF)
     assert layer.dtype == HF and layer.to(torch.bfloat16).dtype == torch.bfloat16
     assert set(layer.state_dict()) == {"codes", "scales"}
+
+
+def test_rotary_axes_are_keys_by_value():
+    a, b = (ops.RotaryAxes(128, n, 1e4, "halves", 2) for n in ((44, 42, 42), [44, 42, 42]))
+    copies = (b, copy.deepcopy(a), pickle.loads(pickle.dumps(a)), dataclasses.replace(a))
+    assert all(a == c and hash(a) == hash(c) for c in copies)
+    for other in (ops.RotaryAxes(128, (44, 42, 42), 1e4, "pairs", 2), dataclasses.replace(a, theta=1e3)):
+        assert a != other and {a: 1}.get(other) is None
