@@ -13,8 +13,9 @@ extern "C" int dfs_residual_norm(const dfs_residual_norm_args* a, dfs_stream_t s
   DFS_REQUIRE(a->x && (a->y == nullptr) == (a->out == nullptr) && (a->h != nullptr) != (a->h8 != nullptr) &&
                   (a->h8 == nullptr) == (a->h8_scales == nullptr),
               "%s: x and h, or h8 with its scales, must be non-NULL, and y and out go together", name);
-  DFS_REQUIRE(rows > 0 && rows < (int64_t(1) << 26) && C > 0 && C <= 512 * kMaxChunks,
-              "%s: rows=%lld channels=%lld must be positive, below 2^26 and up to %d", name, (long long)rows,
+  // A launch holds fewer than 2^32 threads: 2^24 - 1 workgroups, of four rows each.
+  DFS_REQUIRE(rows > 0 && rows <= (int64_t(1) << 26) - 4 && C > 0 && C <= 512 * kMaxChunks,
+              "%s: rows=%lld channels=%lld must be positive, up to 2^26 - 4 and up to %d", name, (long long)rows,
               (long long)C, 512 * kMaxChunks);
   DFS_REQUIRE(C % 8 == 0 || rows < (int64_t(1) << 24), "%s: too many rows of %lld channels", name, (long long)C);
   DFS_REQUIRE(a->dtype == DFS_DTYPE_BF16 || a->dtype == DFS_DTYPE_F16, "%s: dtype must be bf16 or f16", name);

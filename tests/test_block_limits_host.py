@@ -1,0 +1,25 @@
+"""Sizes past what a launch holds (fewer than 2^32 threads) are refused by the C
+entries before they launch. The pointers are never read: only refused calls are
+made here."""
+import pytest
+
+from dfsattn_amd import _lib
+
+AT = 1 << 20  # an address for operands that nothing reads
+
+
+def _call(entry, args, *names, **fields):
+    a = args()
+    for name in names:
+        setattr(a, name, AT)
+    for name, v in fields.items():
+        setattr(a, name, v)
+    _lib.call(entry, bytes(a), 0)
+
+
+@pytest.mark.parametrize("rows,channels", [((1 << 26) - 3, 8), ((1 << 26) - 1, 64), (1 << 26, 8), (1 << 24, 9)])
+def test_residual_norm_rows(rows, channels):
+    """Four rows a workgroup of 256 threads, or one where a row ends inside a chunk."""
+    with pytest.raises(_lib.DfsKernelError, match="rows"):
+        _call("dfs_residual_norm", _lib.ResidualNormArgs, "x", "h", rows=rows, channels=channels, dtype=0, norm=1,
+              x_stride=channels, h_stride=channels)
