@@ -102,7 +102,8 @@ extern "C" int dfs_quantize_fp8(const dfs_quantize_fp8_args* a, dfs_stream_t str
   const int64_t blocks = (a->k + kScaleBlock - 1) / kScaleBlock;
   DFS_REQUIRE(a->rows > 0 && a->k > 0 && a->rows < (int64_t(1) << 30) && a->k < (int64_t(1) << 21),
               "%s: rows=%lld k=%lld must be positive, below 2^30 and 2^21", name, (long long)a->rows, (long long)a->k);
-  DFS_REQUIRE(a->rows * blocks < (int64_t(1) << 28), "%s: too many blocks", name);  // a launch holds 2^32 threads
+  // A launch holds fewer than 2^32 threads: 2^24 - 1 workgroups, of sixteen blocks each.
+  DFS_REQUIRE(a->rows * blocks <= (int64_t(1) << 28) - 16, "%s: too many blocks", name);
   DFS_REQUIRE(a->dtype == DFS_DTYPE_BF16 || a->dtype == DFS_DTYPE_F16, "%s: dtype must be bf16 or f16", name);
   DFS_REQUIRE(reinterpret_cast<uintptr_t>(a->x) % 2 == 0, "%s: x must be aligned to its elements", name);
   DFS_REQUIRE(a->x_stride >= 0 && a->values_stride >= a->k && a->scales_stride >= a->rows,

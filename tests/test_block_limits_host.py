@@ -23,3 +23,11 @@ def test_residual_norm_rows(rows, channels):
     with pytest.raises(_lib.DfsKernelError, match="rows"):
         _call("dfs_residual_norm", _lib.ResidualNormArgs, "x", "h", rows=rows, channels=channels, dtype=0, norm=1,
               x_stride=channels, h_stride=channels)
+
+
+@pytest.mark.parametrize("rows,k", [((1 << 28) - 15, 128), ((1 << 28) - 1, 5), (1 << 28, 1), ((1 << 25) - 1, 1025)])
+def test_quantize_fp8_blocks(rows, k):
+    """Sixteen blocks of 128 channels a workgroup."""
+    with pytest.raises(_lib.DfsKernelError, match="too many blocks"):
+        _call("dfs_quantize_fp8", _lib.QuantizeFp8Args, "x", "values", "scales", rows=rows, k=k, dtype=0, x_stride=k,
+              values_stride=k, scales_stride=rows)
