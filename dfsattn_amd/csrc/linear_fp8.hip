@@ -566,11 +566,15 @@ extern "C" int dfs_linear_fp8(const dfs_linear_fp8_args* a, dfs_stream_t stream)
   const Workspace at = workspace_of(cut, rows, n, k, flags);
   DFS_REQUIRE(at.total == 0 || (a->workspace != nullptr && a->workspace_bytes >= at.total && addr(a->workspace) % 16 == 0),
               "%s: a 16-byte aligned workspace of %lld bytes is needed", name, (long long)at.total);
-  // A launch holds fewer than 2^32 threads (x's quantisation, that of w's rows laid
-  // out beside it among them).
+  // A launch holds fewer than 2^32 threads: 2^24 - 1 workgroups of x's quantisation
+  // (with that of w's rows laid out beside it) and of the result's.
+  const PadCodes w_codes{static_cast<const uint8_t*>(a->w), a->w_stride, n, static_cast<int>(k), static_cast<int>(up16(k)),
+                         static_cast<uint8_t*>(a->workspace) + at.w};
+  const bool pad_w = !(flags & DFS_FP8_W_ALIGNED);
+  const int64_t x_groups = codes ? 0 : (rows * kb + 15) / 16 + (pad_w ? pad_groups(w_codes) : 0);
   DFS_REQUIRE(((rows + 63) / 64) * ((n + 63) / 64) * cut.splits < (1 << 24) && kb < 65536 && (cut.form != kFew || n < (1 << 27)) &&
-                  rows * kb < (1 << 28) - (codes ? 0 : 1 << 24) && (!out8 || rows * nb < (1 << 28)),
-              "%s: too many outputs", name);
+                  rows * kb < (1 << 28) && x_groups < (1 << 24) && (!out8 || rows * nb <= (1 << 28) - 16),
+              "%s: too many outputs, or rows by channels", name);
   char* const ws = static_cast<char*>(a->workspace);
   hipStream_t st = reinterpret_cast<hipStream_t>(stream);
   const bool f16 = a->dtype == DFS_DTYPE_F16;
@@ -587,11 +591,6 @@ extern "C" int dfs_linear_fp8(const dfs_linear_fp8_args* a, dfs_stream_t stream)
   p.ldw = a->w_stride;
   p.ldws = a->w_scales_stride;
   const int64_t wide = up16(k);
-  auto codes_of = [&](const uint8_t* src, int64_t ld, int64_t count, int64_t offset) {
-    return PadCodes{src, ld, count, static_cast<int>(k), static_cast<int>(wide), reinterpret_cast<uint8_t*>(ws + offset)};
-  };
-  const PadCodes w_codes = codes_of(p.w, p.ldw, n, at.w);
-  const bool pad_w = !(flags & DFS_FP8_W_ALIGNED);
   if (!codes) {  // w's codes in the same launch
     uint8_t *const xq = reinterpret_cast<uint8_t*>(ws + at.x), *const xsq = reinterpret_cast<uint8_t*>(ws + at.xs);
     p.ldx = wide;
@@ -601,7 +600,7 @@ extern "C" int dfs_linear_fp8(const dfs_linear_fp8_args* a, dfs_stream_t stream)
     p.x = xq;
     p.xs = xsq;
   } else if (!(flags & DFS_FP8_X_ALIGNED)) {
-    const PadCodes x_codes = codes_of(p.x, p.ldx, rows, at.x);
+    const PadCodes x_codes{p.x, p.ldx, rows, w_codes.k, w_codes.wide, reinterpret_cast<uint8_t*>(ws + at.x)};
     pad_codes_kernel<<<pad_groups(x_codes), 256, 0, st>>>(x_codes);
     p.x = x_codes.dst;
     p.ldx = wide;

@@ -31,3 +31,18 @@ def test_quantize_fp8_blocks(rows, k):
     with pytest.raises(_lib.DfsKernelError, match="too many blocks"):
         _call("dfs_quantize_fp8", _lib.QuantizeFp8Args, "x", "values", "scales", rows=rows, k=k, dtype=0, x_stride=k,
               values_stride=k, scales_stride=rows)
+
+
+@pytest.mark.parametrize("rows,n,k,codes,out8", [
+    ((1 << 28) - 15, 8, 128, False, False),     # x in 16 bits
+    (227745, 30391, 141313, False, False),      # x in 16 bits, w's codes laid out anew in the same launch
+    ((1 << 27) - 7, 130, 16, False, True),      # the result as codes
+    ((1 << 27) - 7, 130, 16, True, True),
+])
+def test_linear_fp8_blocks(rows, n, k, codes, out8):
+    """Sixteen blocks of 128 channels a workgroup, of x and of the result."""
+    names = (("x_scales",) if codes else ()) + (("out8", "out8_scales") if out8 else ("out",))
+    with pytest.raises(_lib.DfsKernelError, match="too many"):
+        _call("dfs_linear_fp8", _lib.LinearFp8Args, "x", "w", "w_scales", "workspace", *names, rows=rows, n=n, k=k,
+              x_dtype=3 if codes else 0, dtype=0, x_stride=k, w_stride=k, x_scales_stride=rows, w_scales_stride=n,
+              out_stride=n, out8_stride=n, out8_scales_stride=rows, workspace_bytes=1 << 62)
