@@ -11,7 +11,7 @@ import functools
 import math
 import struct
 from dataclasses import dataclass
-from typing import Dict, Optional, Sequence, Tuple
+from typing import Dict, List, Optional, Sequence, Tuple
 
 import torch
 
@@ -1602,6 +1602,21 @@ class GridRotary:
         (layout "pairs"; channels behind the sections are not rotated)."""
         if self.axes.layout != "pairs":
             raise ValueError("GridRotary: a table is of neighbouring pairs")
+        return self._turns(tokens, device)
+
+    def rotate(self, *heads: torch.Tensor) -> List[torch.Tensor]:
+        """Heads [B, H, tokens, head_dim], each rotated by its tokens' places in
+        torch: in 64 bits, rounded once to its type. Either layout."""
+        halves, turns = self.axes.layout == "halves", self._turns(max(x.shape[-2] for x in heads), heads[0].device)
+        out = []
+        for x in heads:
+            y = x.double()
+            y = (y.unflatten(-1, (2, -1)).transpose(-1, -2) if halves else y.unflatten(-1, (-1, 2))).contiguous()
+            z = torch.view_as_real(torch.view_as_complex(y) * turns[:, :, :x.shape[-2]])
+            out.append((z.transpose(-1, -2) if halves else z).flatten(-2).type_as(x))
+        return out
+
+    def _turns(self, tokens: int, device) -> torch.Tensor:
         at, places = torch.arange(tokens, dtype=torch.int64, device=device), []
         for n in reversed(self.grid):
             places.append(at % n)

@@ -208,9 +208,9 @@ class Wan_DFSAttn_Processor2_0:
             query = query.unflatten(2, (attn.heads, -1)).transpose(1, 2).contiguous()
             key = key.unflatten(2, (attn.heads, -1)).transpose(1, 2).contiguous()
             value = value.unflatten(2, (attn.heads, -1)).transpose(1, 2).contiguous()
-            if rotary_emb is not None:
-                if isinstance(rotary_emb, GridRotary):
-                    rotary_emb = rotary_emb.table(query.shape[2], query.device)
+            if isinstance(rotary_emb, GridRotary):
+                query, key = rotary_emb.rotate(query, key)
+            elif rotary_emb is not None:
                 query = apply_rotary_emb_complex(query, rotary_emb)
                 key = apply_rotary_emb_complex(key, rotary_emb)
 
