@@ -1629,6 +1629,12 @@ class GridRotary:
         return torch.polar(torch.ones_like(angle), angle)[None, None]
 
 
+def axial_rope_heads(head_dim: int) -> int:
+    """How many heads ``axial_rope`` takes: heads times the next power of two of head_dim up to 8192."""
+    lanes = 1 << max(head_dim // 8 - 1, 0).bit_length()
+    return 16 * (64 // lanes) if head_dim <= 512 else 0
+
+
 @functools.lru_cache(maxsize=1024)
 def _rope_plan(q: Meta, k: Optional[Meta], axes: RotaryAxes, grid: Optional[Tuple[int, ...]],
                positions: Optional[Meta], weights: Tuple[Optional[Tuple[Shape, torch.dtype]], ...], eps: float):
@@ -1644,9 +1650,8 @@ def _rope_plan(q: Meta, k: Optional[Meta], axes: RotaryAxes, grid: Optional[Tupl
     G = 0 if k is None else k[0][2]
     if D != axes.head_dim:
         raise ValueError(f"{entry}: heads of {D} channels, axes for {axes.head_dim}")
-    lanes = 1 << max(D // 8 - 1, 0).bit_length()
-    if H == 0 or (k is not None and G == 0) or -(-max(H, G) // (64 // lanes)) > 16:
-        raise ValueError(f"{entry}: {max(H, G)} heads of {D} channels (supported: 1 to {16 * (64 // lanes)})")
+    if H == 0 or (k is not None and G == 0) or max(H, G) > axial_rope_heads(D):
+        raise ValueError(f"{entry}: {max(H, G)} heads of {D} channels (supported: 1 to {axial_rope_heads(D)})")
     if not eps >= 0.0:
         raise ValueError(f"{entry}: eps must not be negative, got {eps}")
     n = len(axes.sections)

@@ -88,10 +88,16 @@ def fused_qkv_heads(attn, query: torch.Tensor, key: torch.Tensor, value: torch.T
     storage instead of new head-major tensors where that launch applies (the
     library's attention reads them in place). ``rotary_emb``: a complex table,
     or a ``GridRotary``, whose angles are made from the tokens' places instead
-    of read (``ops.axial_rope``)."""
-    from .ops import axial_rope, norm_rope_heads, qkv_heads, qkv_heads_fusable
+    of read (``ops.axial_rope``; heads that it does not take are rotated by the
+    table that it stands for, or, in halves, in torch)."""
+    from .ops import axial_rope, axial_rope_heads, norm_rope_heads, qkv_heads, qkv_heads_fusable
 
     heads = attn.heads
+    if isinstance(rotary_emb, GridRotary) and heads > axial_rope_heads(query.shape[-1] // heads):
+        if rotary_emb.axes.layout == "halves":
+            q, k, v = fused_qkv_heads(attn, query, key, value, None)
+            return (*rotary_emb.rotate(q, k), v)
+        rotary_emb = rotary_emb.table(query.shape[1], query.device)
     wq, eq = _norm_args(attn.norm_q, query.shape[-1], query)
     wk, ek = _norm_args(attn.norm_k, key.shape[-1], key)
     if isinstance(rotary_emb, GridRotary):
