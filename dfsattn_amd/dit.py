@@ -152,6 +152,21 @@ class DiTAttention(nn.Module):
         return self.processor(self, hidden_states, encoder_hidden_states, attention_mask, rotary_emb)
 
 
+class _NoBackward(torch.autograd.Function):
+    """Hands on what was computed without a graph, in the graph's name (``of``
+    wants gradients): a backward pass raises here instead of ending silently."""
+
+    @staticmethod
+    def forward(ctx, out: torch.Tensor, of: torch.Tensor) -> torch.Tensor:
+        ctx.mark_dirty(out)
+        return out
+
+    @staticmethod
+    def backward(ctx, grad):
+        raise RuntimeError("DiTBlock: its fused passes have no backward: run it under torch.no_grad() or inference_mode(), "
+                           "or freeze it where gradients end before it")
+
+
 class DiTBlock(nn.Module):
     def __init__(self, cfg: DiTConfig, **fk):
         super().__init__()
@@ -172,7 +187,9 @@ class DiTBlock(nn.Module):
     # instead of torch's chain of dtype copies and broadcast ops, and the FFN's
     # GELU runs in the first GEMM's epilogue (hipBLASLt, through torch's
     # _addmm_activation: 8.2 -> 7.5 ms per call at 75,600 x 5,120 x 13,824; the
-    # activation is applied before the bf16 rounding instead of after it).
+    # activation is applied before the bf16 rounding instead of after it). These
+    # passes have no backward: the block runs with gradients enabled all the
+    # same, and a backward pass that reaches its result raises.
     fused_elementwise: bool = True
     # The FFN's products with their GELU and their gated residual in this
     # library's kernel (ops.linear, fused path only): one pass less over the
@@ -205,26 +222,35 @@ class DiTBlock(nn.Module):
         a = torch._addmm_activation(lin1.bias, h.reshape(-1, h.shape[-1]), lin1.weight.t(), use_gelu=True)
         return lin2(a).reshape(*h.shape[:-1], -1)
 
+    def _forward_fused(self, x: torch.Tensor, context: torch.Tensor, modulation: torch.Tensor,
+                       rotary_emb) -> torch.Tensor:
+        from . import ops
+
+        shift_msa, scale_msa, gate_msa, c_shift, c_scale, c_gate = modulation.chunk(6, 1)
+        h = ops.adaln_modulate(x, self.norm1.eps, scale=scale_msa, shift=shift_msa)
+        # a branch's residual and the norm before the next one in one pass
+        a = self.attn1(h, None, None, rotary_emb)
+        x, h = ops.residual_norm(x, a, gate_msa, weight=self.norm2.weight, bias=self.norm2.bias, eps=self.norm2.eps)
+        a = self.attn2(h, context)
+        if isinstance(self.ffn[0], Fp8Linear) and isinstance(self.ffn[2], Fp8Linear):
+            return self._ffn_fp8(x, a, c_scale, c_shift, c_gate)
+        x, h = ops.residual_norm(x, a, scale=c_scale, shift=c_shift, eps=self.norm3.eps)
+        if self.native_ffn and not any(isinstance(layer, Fp8Linear) for layer in self.ffn):
+            return self._ffn_native(h, x, c_gate)
+        return ops.gated_residual(x, self._ffn_fused(h), c_gate)
+
     def forward(self, x: torch.Tensor, context: torch.Tensor, temb: torch.Tensor,
                 rotary_emb) -> torch.Tensor:
-        shift_msa, scale_msa, gate_msa, c_shift, c_scale, c_gate = (self.scale_shift_table + temb.float()).chunk(6, 1)
+        modulation = self.scale_shift_table + temb.float()
+        shift_msa, scale_msa, gate_msa, c_shift, c_scale, c_gate = modulation.chunk(6, 1)
         if self.fused_elementwise and x.is_cuda and x.shape[0] == 1:
-            from . import ops
-
-            h = ops.adaln_modulate(x, self.norm1.eps, scale=scale_msa, shift=shift_msa)
-            # a branch's residual and the norm before the next one in one pass
-            a = self.attn1(h, None, None, rotary_emb)
             with torch.no_grad():
-                x, h = ops.residual_norm(x, a, gate_msa, weight=self.norm2.weight, bias=self.norm2.bias,
-                                         eps=self.norm2.eps)
-            a = self.attn2(h, context)
-            if isinstance(self.ffn[0], Fp8Linear) and isinstance(self.ffn[2], Fp8Linear):
-                return self._ffn_fp8(x, a, c_scale, c_shift, c_gate)
-            with torch.no_grad():
-                x, h = ops.residual_norm(x, a, scale=c_scale, shift=c_shift, eps=self.norm3.eps)
-            if self.native_ffn and not any(isinstance(layer, Fp8Linear) for layer in self.ffn):
-                return self._ffn_native(h, x, c_gate)
-            return ops.gated_residual(x, self._ffn_fused(h), c_gate)
+                out = self._forward_fused(x, context, modulation, rotary_emb)
+            if torch.is_grad_enabled():
+                for t in (modulation, x, context, *self.parameters()):
+                    if t.requires_grad:
+                        return _NoBackward.apply(out, t)
+            return out
         h = (self.norm1(x.float()) * (1 + scale_msa) + shift_msa).type_as(x)
         x = (x.float() + self.attn1(h, None, None, rotary_emb) * gate_msa).type_as(x)
         h = self.norm2(x.float()).type_as(x)
