@@ -1517,11 +1517,12 @@ def residual_norm(x: torch.Tensor, y: Optional[torch.Tensor] = None, gate: Optio
         others = [t for t in (x, y) if not (t.data_ptr() == out.data_ptr() and t.is_contiguous())]
         _refuse_overlap(entry, "out", out, *others, gate, post_weight, post_bias, weight, bias, scale, shift)
     if head is None and x.numel():
-        x, y = (t if t is None or ok else t.contiguous() for t, ok in zip((x, y), whole))
+        rows, y = (t if t is None or ok else t.contiguous() for t, ok in zip((x, y), whole))
         gate, scale, shift = (t if shape is None else t.expand(shape).contiguous()
                               for t, shape in zip((gate, scale, shift), anew))
-        return residual_norm(x, y, gate, residual_scale, post_norm, post_weight, post_bias, post_eps, norm, weight, bias,
-                             scale, shift, eps, out, quantize)
+        results = residual_norm(rows, y, gate, residual_scale, post_norm, post_weight, post_bias, post_eps, norm, weight,
+                                bias, scale, shift, eps, out, quantize)
+        return (x, *results[1:]) if y is None else results
     weights = [t if t is None or t.is_contiguous() else t.contiguous() for t in (post_weight, post_bias, weight, bias)]
     r, scales = x if y is None else out, None
     if r is None:
