@@ -1,6 +1,9 @@
 // The C entry of residual_norm.h and its bf16 kernels.
 #include "residual_norm.h"
 
+#include <cfloat>
+#include <cmath>
+
 namespace dfs {
 void run_residual_norm_bf16(const NormParams& p, hipStream_t stream) { run<false>(p, stream); }
 }  // namespace dfs
@@ -26,6 +29,8 @@ extern "C" int dfs_residual_norm(const dfs_residual_norm_args* a, dfs_stream_t s
   DFS_REQUIRE(a->y || (!a->gate && a->post_norm == DFS_NORM_NONE), "%s: a gate or norm of y without it", name);
   DFS_REQUIRE(a->post_norm != DFS_NORM_NONE || (!a->post_weight && !a->post_bias), "%s: a weight without its norm", name);
   DFS_REQUIRE(a->eps >= 0. && a->post_eps >= 0., "%s: eps must not be negative", name);
+  DFS_REQUIRE(a->eps <= FLT_MAX && a->post_eps <= FLT_MAX && (!a->y || std::fabs(a->residual_scale) <= FLT_MAX),
+              "%s: eps and the residual's scale must be in fp32's range", name);
   DFS_REQUIRE(a->x_stride >= 0 && a->y_stride >= 0 && (!a->out || a->out_stride >= C) && a->h_stride >= C &&
                   (!a->h8 || a->h8_scales_stride >= rows),
               "%s: strides must not be negative, the results' rows must not overlap", name);

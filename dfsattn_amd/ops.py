@@ -1400,6 +1400,7 @@ def linear_fp8(x: torch.Tensor, weight: torch.Tensor, weight_scales: torch.Tenso
 # --------------------------------------------------------------------------
 
 NORM_CODE = {None: 0, "rms": 1, "layer": 2}
+FP32_MAX = torch.finfo(torch.float32).max
 _NORM_POINTERS = struct.Struct("@13P")
 _ROPE_POINTERS = struct.Struct("@8P")
 Meta = Tuple[Shape, Shape, torch.dtype]  # shape, strides and type of a tensor
@@ -1449,9 +1450,9 @@ def _norm_plan(x: Meta, y: Optional[Meta], gate: Optional[Meta], scale: Optional
         raise ValueError(f"{entry}: a gate, norm or residual_scale without y")
     if post_norm is None and (weights[0] is not None or weights[1] is not None):
         raise ValueError(f"{entry}: post_weight and post_bias go with a post_norm")
-    if not (eps >= 0.0 and post_eps >= 0.0) or not math.isfinite(residual_scale):
-        raise ValueError(f"{entry}: eps must not be negative and residual_scale finite, got {eps}, {post_eps}, "
-                         f"{residual_scale}")
+    if not (0.0 <= eps <= FP32_MAX and 0.0 <= post_eps <= FP32_MAX and abs(residual_scale) <= FP32_MAX):
+        raise ValueError(f"{entry}: eps must not be negative, and it and residual_scale in fp32's range, got {eps}, "
+                         f"{post_eps}, {residual_scale}")
     C = shape[-1]
     a = _lib.ResidualNormArgs()
     for name, w in zip(("post_weight", "post_bias", "weight", "bias"), weights):

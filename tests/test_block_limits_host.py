@@ -2,8 +2,9 @@
 entries before they launch. The pointers are never read: only refused calls are
 made here."""
 import pytest
+import torch
 
-from dfsattn_amd import _lib
+from dfsattn_amd import _lib, ops
 
 AT = 1 << 20  # an address for operands that nothing reads
 
@@ -46,3 +47,16 @@ def test_linear_fp8_blocks(rows, n, k, codes, out8):
         _call("dfs_linear_fp8", _lib.LinearFp8Args, "x", "w", "w_scales", "workspace", *names, rows=rows, n=n, k=k,
               x_dtype=3 if codes else 0, dtype=0, x_stride=k, w_stride=k, x_scales_stride=rows, w_scales_stride=n,
               out_stride=n, out8_stride=n, out8_scales_stride=rows, workspace_bytes=1 << 62)
+
+
+@pytest.mark.parametrize("change", [{"residual_scale": 1e39}, {"residual_scale": -3.5e38}, {"eps": 1e39}, {"eps": float("inf")},
+                                    {"post_norm": "rms", "post_eps": 4e38}])
+def test_residual_norm_takes_fp32_numbers(change):
+    """Options are fp32 in the kernel: past its range 1e39 * 0 was not a number."""
+    x = torch.zeros(2, 16, dtype=torch.bfloat16)
+    with pytest.raises(ValueError, match="fp32"):
+        ops.residual_norm(x, x, **change)
+    names = {"x": AT, "y": AT, "out": AT, "h": AT, "rows": 2, "channels": 16, "norm": 1, "x_stride": 16, "y_stride": 16,
+             "out_stride": 16, "h_stride": 16, "residual_scale": 1.0}
+    with pytest.raises(_lib.DfsKernelError, match="fp32"):
+        _call("dfs_residual_norm", _lib.ResidualNormArgs, **{**names, **change, "post_norm": int("post_norm" in change)})
