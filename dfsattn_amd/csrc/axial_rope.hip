@@ -11,6 +11,8 @@
 // and serve all its heads. f and the angle are 64 bits, in turns, so that the
 // whole turns of a far position leave nothing behind: what is left of one goes
 // to fp32's sine and cosine.
+#include <cfloat>
+
 #include "common.h"
 #include "lds_copy.h"
 
@@ -264,7 +266,7 @@ extern "C" int dfs_axial_rope(const dfs_axial_rope_args* a, dfs_stream_t stream)
               "%s: head_dim %lld must be a multiple of 8 up to 512", name, (long long)a->head_dim);
   DFS_REQUIRE(a->dtype == DFS_DTYPE_BF16 || a->dtype == DFS_DTYPE_F16, "%s: dtype must be bf16 or f16", name);
   DFS_REQUIRE(a->axes >= 1 && a->axes <= kMaxAxes, "%s: 1 to %d axes", name, kMaxAxes);
-  DFS_REQUIRE(a->eps >= 0., "%s: eps must not be negative", name);
+  DFS_REQUIRE(a->eps >= 0. && a->eps <= FLT_MAX, "%s: eps must not be negative and in fp32's range", name);
   RopeParams p{};
   while ((int64_t(8) << p.log2l) < a->head_dim) ++p.log2l;
   const int64_t heads = a->k && a->kv_heads > a->q_heads ? a->kv_heads : a->q_heads;

@@ -1654,8 +1654,8 @@ def _rope_plan(q: Meta, k: Optional[Meta], axes: RotaryAxes, grid: Optional[Tupl
         raise ValueError(f"{entry}: heads of {D} channels, axes for {axes.head_dim}")
     if H == 0 or (k is not None and G == 0) or max(H, G) > axial_rope_heads(D):
         raise ValueError(f"{entry}: {max(H, G)} heads of {D} channels (supported: 1 to {axial_rope_heads(D)})")
-    if not eps >= 0.0:
-        raise ValueError(f"{entry}: eps must not be negative, got {eps}")
+    if not 0.0 <= eps <= FP32_MAX:
+        raise ValueError(f"{entry}: eps must not be negative and in fp32's range, got {eps}")
     n = len(axes.sections)
     if (grid is None) == (positions is None):
         raise ValueError(f"{entry}: pass a grid or positions")

@@ -60,3 +60,12 @@ def test_residual_norm_takes_fp32_numbers(change):
              "out_stride": 16, "h_stride": 16, "residual_scale": 1.0}
     with pytest.raises(_lib.DfsKernelError, match="fp32"):
         _call("dfs_residual_norm", _lib.ResidualNormArgs, **{**names, **change, "post_norm": int("post_norm" in change)})
+
+
+@pytest.mark.parametrize("eps", [1e39, float("inf")])
+def test_axial_rope_takes_fp32_eps(eps):
+    q = torch.zeros(1, 2, 1, 8, dtype=torch.bfloat16)
+    with pytest.raises(ValueError, match="fp32"):
+        ops.axial_rope(q, None, ops.RotaryAxes(8, (8,)), (), eps=eps)
+    with pytest.raises(_lib.DfsKernelError, match="fp32"):
+        _call("dfs_axial_rope", _lib.AxialRopeArgs, "q", "q_out", batch=1, tokens=2, q_heads=1, head_dim=8, axes=1, eps=eps)
