@@ -1590,6 +1590,12 @@ def _axes_fields(head_dim: int, sections: Tuple[int, ...], theta, layout: str, s
     return {"head_dim": head_dim, "sections": sections, "theta": theta, "layout": layout, "speeds": speeds}
 
 
+def _check_grid(entry: str, axes: RotaryAxes, grid: Tuple[int, ...]) -> None:
+    n = len(axes.sections)
+    if len(grid) != n - 1 or any(not 0 < s < 1 << 30 for s in grid):
+        raise ValueError(f"{entry}: grid must hold the positive sizes of the {n - 1} axes behind the first, got {grid}")
+
+
 @dataclass(frozen=True)
 class GridRotary:
     """Rotary positions of a video's tokens in row-major order: ``axes`` over
@@ -1598,6 +1604,9 @@ class GridRotary:
 
     axes: RotaryAxes
     grid: Tuple[int, ...]
+
+    def __post_init__(self):
+        _check_grid("GridRotary", self.axes, tuple(self.grid))
 
     def table(self, tokens: int, device=None) -> torch.Tensor:
         """complex128 [1, 1, tokens, head_dim/2]: the table that it stands for
@@ -1661,8 +1670,7 @@ def _rope_plan(q: Meta, k: Optional[Meta], axes: RotaryAxes, grid: Optional[Tupl
         raise ValueError(f"{entry}: pass a grid or positions")
     a = _lib.AxialRopeArgs()
     if grid is not None:
-        if len(grid) != n - 1 or any(not 0 < s < 1 << 30 for s in grid):
-            raise ValueError(f"{entry}: grid must hold the positive sizes of the {n - 1} axes behind the first, got {grid}")
+        _check_grid(entry, axes, grid)
         for i, s in enumerate(grid):
             a.size[i + 1] = s
     else:

@@ -69,3 +69,11 @@ def test_axial_rope_takes_fp32_eps(eps):
         ops.axial_rope(q, None, ops.RotaryAxes(8, (8,)), (), eps=eps)
     with pytest.raises(_lib.DfsKernelError, match="fp32"):
         _call("dfs_axial_rope", _lib.AxialRopeArgs, "q", "q_out", batch=1, tokens=2, q_heads=1, head_dim=8, axes=1, eps=eps)
+
+
+@pytest.mark.parametrize("grid", [(), (4,), (2, 3, 4), (0, 4), (4, -1), (1 << 30, 4)])
+def test_grid_rotary_refuses_another_grid(grid):
+    """A grid of the axes behind the first, as ops.axial_rope takes it: tables of
+    others put the wrong places to the axes."""
+    with pytest.raises(ValueError, match="grid"):
+        ops.GridRotary(ops.RotaryAxes(64, (24, 20, 20)), grid)
