@@ -215,7 +215,8 @@ __global__ void __launch_bounds__(256, 2) fp8_tile_kernel(Fp8Params p) {
   // Loads keep their order over a fence (neither moves over it), within a stretch
   // between two they may not: so a step's data and the scales of another lie in
   // stretches of their own, taking turns from the beginning on, and a wait can
-  // count what is behind the data it needs.
+  // count what is behind the data it needs: DATA and SCALES instructions a step, to
+  // which the built code is held by tests/test_waits_host.py.
   auto fence = [] {
     asm volatile("" ::: "memory");
     __builtin_amdgcn_sched_barrier(0);
