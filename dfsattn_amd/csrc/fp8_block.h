@@ -3,8 +3,10 @@
 // e the smallest integer with max |x_i| <= 448 * 2^e over the block's finite
 // values, from -127 to 127, and 0 for a block of zeros; values that are not
 // finite become NaN, e4m3's only other. The scale is held as e + 127 in a byte
-// (e8m0). With a power of two the division is exact, a code's relative error
-// (2^-4 at most) is what any other scale would leave, and the matrix
+// (e8m0). A code is off by 2^-4 of its value at most, or, for values below 2^-6 *
+// 2^e, whose codes are subnormal, by 2^-10 * 2^e: what lies below that beside one
+// large channel becomes zero. With a power of two the division is exact, the error
+// of normal codes is what any other scale would leave, and the matrix
 // instructions apply it by themselves.
 #pragma once
 

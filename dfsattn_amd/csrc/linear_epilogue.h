@@ -77,7 +77,8 @@ __device__ __forceinline__ float activate(float z) {
   } else if constexpr (ACT == kActGeluShort) {
     // erfc(a / sqrt(2)) = t 2^(p(t) - a^2 / ln 4), t = 1 / (1 + a / sqrt(8)),
     // for a = |z|, with p fitted to erfc on a up to 17 (relative 8e-7; with the
-    // exponent's roundings below 2^-16). z erfc(-z / sqrt(2)) / 2 is z or 0 less
+    // exponent's roundings 2^-18.4 for z above -8, 2^-16.9 below, where bf16's
+    // rounding is 2^-8 and f16's 2^-11). z erfc(-z / sqrt(2)) / 2 is z or 0 less
     // a / 2 times that; past a of 14 it is 0, and the factor stays finite.
     const float a = __builtin_fabsf(z), t = __builtin_amdgcn_rcpf(__builtin_fmaf(0.35355339f, a, 1.f));
     float p = -0.27580905f;

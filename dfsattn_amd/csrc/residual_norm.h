@@ -269,7 +269,10 @@ __global__ void __launch_bounds__(256) residual_norm_kernel(NormParams p) {
 }
 
 // Rows that end inside a chunk: a workgroup a row, chunk t + 256 k for thread t,
-// with the row's last chunk taken value by value. Its sums meet in LDS.
+// with the row's last chunk taken value by value. Its sums meet in LDS, up to four
+// times a row behind a barrier each, which is what bounds it: 75,600 x 5,119 with
+// gate, scale and shift 1,112 us where 5,120 takes 551, 75,600 x 333 (42 threads at
+// work) 219 where 336 takes 55; 4,680 x 5,119 59 and 45.
 __device__ __forceinline__ uint4 part8_u16(const uint16_t* row, int e, int C) {
   if (e + 8 <= C) return load8_u16<false>(row, e);
   uint16_t t[8];

@@ -7,8 +7,10 @@ from the operator before (``DiTBlock`` runs its feed-forward products that way:
 the norm before them and the first product leave their results as operands).
 ``install_fp8`` puts such layers into a ``WanLikeDiT``.
 
-A weight takes half the memory; a code is off by 2^-4 of its value at most, so
-layers differ from their 16-bit originals by a few percent of an output's size.
+A weight takes half the memory; a code is off by 2^-4 of its value at most, or, for
+values below 2^-6 of their block's scale (whose largest value is at most 448 of it),
+by 2^-10 of the scale, so layers differ from their 16-bit originals by a few percent
+of an output's size.
 """
 from __future__ import annotations
 

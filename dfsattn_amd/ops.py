@@ -1346,8 +1346,8 @@ def linear_fp8(x: torch.Tensor, weight: torch.Tensor, weight_scales: torch.Tenso
     residual's, else bf16). bias in that dtype or fp32, gate N
     fp32 values. ``quantize``: returns ``quantize_fp8`` of the result, (codes,
     scales), instead. ``out`` may be the residual itself. Codes whose rows lie
-    off 16-byte boundaries and scales whose rows do not lie one behind the other
-    are copied at each call. No backward pass."""
+    off 16-byte boundaries or whose K is no multiple of 16, and scales whose rows do
+    not lie one behind the other, are copied at each call. No backward pass."""
     entry = "linear_fp8"
     _refuse_grad(entry, x, bias, gate, residual, out)
     if weight_scales is None:
@@ -1714,7 +1714,8 @@ def axial_rope(q: torch.Tensor, k: Optional[torch.Tensor], axes: RotaryAxes, gri
     RMS-normalised (weight [D]: each by itself; weight [H * D] or [G * D]: all
     together; None: not at all) and rotated by positions of several ``axes``, in
     fp32 and rounded once: new q and k as [B, H, T, D] and [B, G, T, D] views of
-    token-major storage, as the attentions read them. For bf16 and f16.
+    token-major storage, as the attentions read them. For bf16 and f16, up to
+    ``axial_rope_heads(D)`` heads.
 
     A token's positions: with ``grid``, the sizes of the axes behind the first
     (height and width of a video's frames), its place in row-major order, token t

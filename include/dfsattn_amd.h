@@ -603,7 +603,8 @@ int dfs_qkv_cache(const dfs_cache_args* args, dfs_stream_t stream);
  * finite values, from -127 to 127 (0 for zeros); a code is x * 2^-e rounded to
  * nearest even, NaN where x is not finite. values [rows][k], row stride
  * values_stride; scales [ceil(k / 128)][rows], block stride scales_stride (the
- * products read a block's scales of neighbouring rows together). k below 2^21.
+ * products read a block's scales of neighbouring rows together). k below 2^21,
+ * rows times blocks up to 2^28 - 16.
  */
 typedef struct dfs_quantize_fp8_args {
   int64_t rows, k, dtype, x_stride, values_stride, scales_stride;
@@ -667,8 +668,9 @@ int dfs_linear_fp8(const dfs_linear_fp8_args* args, dfs_stream_t stream);
  * of `channels` values for each *_rows consecutive rows (a divisor of rows),
  * *_stride elements apart. Without y (out NULL) h is of x itself. h8 and
  * h8_scales instead of h: dfs_quantize_fp8 of the rounded h. Statistics and
- * steps are fp32, each product and sum rounded in the order written. out may be
- * x or y. channels up to 8192.
+ * steps are fp32, each product and sum rounded in the order written; eps and
+ * residual_scale are fp32 numbers. out may be x or y. channels up to 8192, rows up to
+ * 2^26 - 4 (2^24 - 1 where channels are no multiple of 8).
  */
 enum { DFS_NORM_NONE = 0, DFS_NORM_RMS = 1, DFS_NORM_LAYER = 2 };
 typedef struct dfs_residual_norm_args {
