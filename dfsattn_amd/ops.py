@@ -1618,6 +1618,8 @@ class GridRotary:
     def rotate(self, *heads: torch.Tensor) -> List[torch.Tensor]:
         """Heads [B, H, tokens, head_dim], each rotated by its tokens' places in
         torch: in 64 bits, rounded once to its type. Either layout."""
+        if any(x.shape[-1] != self.axes.head_dim for x in heads):
+            raise ValueError(f"GridRotary: heads of {self.axes.head_dim} channels, got {[x.shape[-1] for x in heads]}")
         halves, turns = self.axes.layout == "halves", self._turns(max(x.shape[-2] for x in heads), heads[0].device)
         out = []
         for x in heads:

@@ -42,3 +42,17 @@ def test_processor_without_the_kernel_rotates_by_places(monkeypatch, layout):
             want, tol = _expected(norm(layer(x)).unflatten(2, (H, D)), rotary)
             assert seen[name].dtype == x.dtype and bool(((seen[name].double() - want).abs() <= tol).all())
         assert torch.equal(seen["v"], attn.to_v(x).unflatten(2, (H, D)).transpose(1, 2))
+
+
+@pytest.mark.parametrize("layout", ["pairs", "halves"])
+def test_rotate_keeps_types_and_refuses_other_heads(layout):
+    rotary = ops.GridRotary(_axes(layout), GRID)
+    g = torch.Generator().manual_seed(2)
+    for dtype in (torch.bfloat16, torch.float16, torch.float32):
+        x = torch.randn(2, L, H, D, generator=g).to(dtype)
+        got, short = rotary.rotate(x.transpose(1, 2), x[:, :7].transpose(1, 2))
+        want, tol = _expected(x, rotary)
+        assert got.dtype == dtype and bool(((got.double() - want).abs() <= tol).all())
+        assert torch.equal(short, got[:, :, :7])
+    with pytest.raises(ValueError, match="channels"):
+        rotary.rotate(torch.zeros(1, H, L, D + 8))
